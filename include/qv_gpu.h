@@ -285,6 +285,89 @@ qv_status qv_ivfpq_filter_bitmap(const qv_ivfpq* index, const qv_filter* filter,
                                  uint64_t** device_bitmap);
 qv_status qv_device_free(int device, void* ptr);
 
+/* ---- embedding tables and linear adapters ---------------------------------------------------------
+ * The trainable front of an index (no counterpart in the reference): the table whose rows become
+ * the stored vectors or the queries, and the linear map applied to them before an add or a search.
+ * All pointers are device pointers on `device`; matrices are row-major with a row stride counted in
+ * elements (at least the row's length when there is more than one row); results must not overlap
+ * inputs. The work is enqueued on `stream` as it is given (NULL: CUDA's default stream itself), with
+ * no host synchronization and no device allocation, so the calls can be captured into a CUDA graph;
+ * temporaries live in the caller's workspace (256-byte aligned, not shared with work that may run
+ * at the same time), whose size the *_workspace functions tell. Sums are float32 in a fixed order,
+ * rounded once to the result's type; equal calls give equal bits. */
+enum { QV_DTYPE_F32 = 0, QV_DTYPE_F16 = 1, QV_DTYPE_BF16 = 2 };
+enum { QV_ID_I32 = 0, QV_ID_I64 = 1 };
+enum { QV_ACT_NONE = 0, QV_ACT_RELU = 1, QV_ACT_GELU = 2, QV_ACT_GELU_TANH = 3, QV_ACT_SILU = 4 };
+
+/* out[i] = scale * table[ids[i]] for n ids. A negative id (an unfilled result slot) gives a row of
+ * zeros; an id of `rows` or more gives a row of NaN. */
+qv_status qv_embedding_lookup_device(int device, uint32_t dtype, const void* table, size_t rows,
+                                     size_t dim, size_t table_stride, uint32_t id_type,
+                                     const void* ids, size_t n, float scale, void* out,
+                                     size_t out_stride, void* stream);
+/* The gradient of the lookup: grad[r] = scale * sum of upstream[i] over ids[i] == r, for every row
+ * r of the table (zeros where no id points); ids outside [0, rows) take none. The sums run in the
+ * order of i. */
+qv_status qv_embedding_grad_workspace(size_t n, size_t rows, size_t dim, size_t* bytes);
+qv_status qv_embedding_grad_device(int device, uint32_t dtype, const void* upstream,
+                                   size_t upstream_stride, uint32_t id_type, const void* ids,
+                                   size_t n, size_t rows, size_t dim, float scale, void* grad,
+                                   size_t grad_stride, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+/* qv_embedding_lookup_device on a Flat index's stored float32 rows (as qv_flat_rows reports them,
+ * normalized for cosine), by row number. */
+qv_status qv_flat_lookup_device(const qv_flat* index, uint32_t id_type, const void* ids, size_t n,
+                                float scale, float* out, size_t out_stride, void* stream);
+
+/* out = activation(x weight^T + bias) + residual: x m x k, weight n x k, out m x n. bias (n) and
+ * residual (m x n; residual_stride 0 adds one row to every row) may be NULL. preact (may be NULL)
+ * receives x weight^T + bias, which the gradient of an activation needs. out_dtype is dtype or
+ * QV_DTYPE_F32; everything else has dtype. Infinite float32 inputs may give NaN where the sum is
+ * infinite (their products run on parts of the values). */
+typedef struct qv_linear {
+  uint32_t dtype, out_dtype, activation;
+  size_t m, n, k;
+  const void* x;
+  size_t x_stride;
+  const void* weight;
+  size_t weight_stride;
+  const void* bias;
+  const void* residual;
+  size_t residual_stride;
+  void* out;
+  size_t out_stride;
+  void* preact;
+  size_t preact_stride;
+} qv_linear;
+qv_status qv_linear_workspace(int device, const qv_linear* args, size_t* bytes);
+qv_status qv_linear_device(int device, const qv_linear* args, void* workspace,
+                           size_t workspace_bytes, void* stream);
+/* The gradients of qv_linear for grad = d(loss)/d(out), m x n in dtype: with
+ * dz = grad * activation'(preact), dx = dz weight, dweight = dz^T x, dbias = the column sums of dz
+ * (the residual's gradient is grad itself). Outputs that are NULL are not computed, inputs that no
+ * output needs may be NULL (preact: QV_ACT_NONE; weight: no dx; x: no dweight). 16-bit dz is
+ * rounded once to dtype before the products; dbias sums the unrounded values. */
+typedef struct qv_linear_grad {
+  uint32_t dtype, activation;
+  size_t m, n, k;
+  const void* grad;
+  size_t grad_stride;
+  const void* x;
+  size_t x_stride;
+  const void* weight;
+  size_t weight_stride;
+  const void* preact;
+  size_t preact_stride;
+  void* dx;
+  size_t dx_stride;
+  void* dweight;
+  size_t dweight_stride;
+  void* dbias;
+} qv_linear_grad;
+qv_status qv_linear_grad_workspace(int device, const qv_linear_grad* args, size_t* bytes);
+qv_status qv_linear_grad_device(int device, const qv_linear_grad* args, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
 /* ---- shard merge ---------------------------------------------------------------------------------
  * k-way merge of per-shard results: parts x nq x k (distance, key, label) triples, each row sorted
  * by (distance, key), into nq x k sorted by (distance, key). Device pointers on `device`. Replaces

@@ -91,6 +91,15 @@ def _result_arrays(nq: int, k: int):
     return np.empty((nq, k), np.uint64), np.empty((nq, k), np.float32)
 
 
+def _adapted(adapter, vectors, stream):
+    """adapter(vectors) on the stream an add or a search uses (a raw handle, or PyTorch's)."""
+    import torch
+    if not stream:
+        return adapter(vectors)
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=vectors.device)):
+        return adapter(vectors)
+
+
 class FlatIndex:
     """Exact brute-force index on one GPU (reference: include/quiver/flat_index.h)."""
 
@@ -125,10 +134,13 @@ class FlatIndex:
         """Sizes the GPU row storage for n rows at once (no counterpart in the reference)."""
         check(lib().qv_flat_reserve(self._h, int(n)))
 
-    def add_device(self, vectors, labels=None, stream=None) -> None:
+    def add_device(self, vectors, labels=None, stream=None, *, adapter=None) -> None:
         """Appends rows already in GPU memory: ``vectors`` a contiguous float32 CUDA tensor
         [n, dim] on this index's device, ``labels`` None or a contiguous int64 CUDA tensor [n];
-        the same checks and results as :meth:`add` (no counterpart in the reference)."""
+        the same checks and results as :meth:`add` (no counterpart in the reference). With an
+        ``adapter`` (:class:`quiver_b200.embed.Adapter`) the rows are ``adapter(vectors)``."""
+        if adapter is not None:
+            vectors = _adapted(adapter, vectors, stream)
         if vectors.dim() != 2 or vectors.shape[1] != self.dim or not vectors.is_contiguous():
             raise ValueError(f"expected a contiguous [n, {self.dim}] tensor")
         n = int(vectors.shape[0])
@@ -139,6 +151,44 @@ class FlatIndex:
             lp = labels.data_ptr()
         check(lib().qv_flat_add_device(self._h, vectors.data_ptr(), n, lp,
                                        C.c_void_p(stream) if stream else None))
+
+    def search_device(self, queries, k: int = 10, *, adapter=None):
+        """k-NN search of queries in GPU memory on PyTorch's current stream, without waiting for
+        it: ``queries`` a float32 CUDA tensor [nq, dim] on this index's device, or vectors that
+        ``adapter`` (:class:`quiver_b200.embed.Adapter`) turns into them. Returns CUDA tensors
+        (distances float32 [nq, k], labels int64 [nq, k]; no counterpart in the reference)."""
+        import torch
+        q = queries if adapter is None else _adapted(adapter, queries, None)
+        if q.dim() != 2 or q.shape[1] != self.dim or q.dtype != torch.float32 or not q.is_cuda:
+            raise ValueError(f"expected a float32 CUDA tensor [nq, {self.dim}]")
+        if k <= 0:
+            raise ValueError("k must be positive")
+        q = q.contiguous()
+        nq = int(q.shape[0])
+        dists = torch.empty((nq, int(k)), dtype=torch.float32, device=q.device)
+        labels = torch.empty((nq, int(k)), dtype=torch.int64, device=q.device)
+        st = torch.cuda.current_stream(q.device).cuda_stream
+        check(lib().qv_flat_search_device(self._h, q.data_ptr(), nq, int(k), None,
+                                          labels.data_ptr(), dists.data_ptr(), None,
+                                          C.c_void_p(st)))
+        return dists, labels
+
+    def lookup_device(self, rows, scale: float = 1.0):
+        """Stored vectors by row number, times ``scale``, on PyTorch's current stream: ``rows`` an
+        int32 or int64 CUDA tensor of any shape on this index's device; returns float32
+        ``[*rows.shape, dim]``. A negative number (an unfilled result slot) gives zeros, one past
+        the last row NaN (no counterpart in the reference; :meth:`rows` copies to the host)."""
+        import torch
+        codes = {torch.int32: 0, torch.int64: 1}
+        if not rows.is_cuda or rows.dtype not in codes:
+            raise ValueError("expected an int32 or int64 CUDA tensor of row numbers")
+        r = rows.contiguous()
+        dim = self.dim
+        out = torch.empty(tuple(rows.shape) + (dim,), dtype=torch.float32, device=rows.device)
+        st = torch.cuda.current_stream(rows.device).cuda_stream
+        check(lib().qv_flat_lookup_device(self._h, codes[rows.dtype], r.data_ptr(), r.numel(),
+                                          float(scale), out.data_ptr(), dim, C.c_void_p(st)))
+        return out
 
     def search(self, queries: ArrayLike, k: int = 10, filter: Optional[ArrayLike] = None,
                num_threads: int = 0) -> Tuple[np.ndarray, np.ndarray]:

@@ -41,8 +41,30 @@ class qv_search_stats(C.Structure):
                 ("dominant_work_is_bytes", C.c_uint32), ("dominant_kernel", C.c_char * 64)]
 
 
+class qv_linear(C.Structure):
+    _fields_ = [("dtype", C.c_uint32), ("out_dtype", C.c_uint32), ("activation", C.c_uint32),
+                ("m", C.c_size_t), ("n", C.c_size_t), ("k", C.c_size_t),
+                ("x", C.c_void_p), ("x_stride", C.c_size_t),
+                ("weight", C.c_void_p), ("weight_stride", C.c_size_t),
+                ("bias", C.c_void_p), ("residual", C.c_void_p), ("residual_stride", C.c_size_t),
+                ("out", C.c_void_p), ("out_stride", C.c_size_t),
+                ("preact", C.c_void_p), ("preact_stride", C.c_size_t)]
+
+
+class qv_linear_grad(C.Structure):
+    _fields_ = [("dtype", C.c_uint32), ("activation", C.c_uint32),
+                ("m", C.c_size_t), ("n", C.c_size_t), ("k", C.c_size_t),
+                ("grad", C.c_void_p), ("grad_stride", C.c_size_t),
+                ("x", C.c_void_p), ("x_stride", C.c_size_t),
+                ("weight", C.c_void_p), ("weight_stride", C.c_size_t),
+                ("preact", C.c_void_p), ("preact_stride", C.c_size_t),
+                ("dx", C.c_void_p), ("dx_stride", C.c_size_t),
+                ("dweight", C.c_void_p), ("dweight_stride", C.c_size_t), ("dbias", C.c_void_p)]
+
+
 # (name, restype, argtypes); every function returns qv_status unless stated.
 _vp, _sz, _u32, _u64, _int = C.c_void_p, C.c_size_t, C.c_uint32, C.c_uint64, C.c_int
+_f32 = C.c_float
 _PP = C.POINTER(C.c_void_p)
 _SIGNATURES = {
     "qv_last_error": (C.c_char_p, []),
@@ -98,6 +120,16 @@ _SIGNATURES = {
     "qv_hnsw_store_sq8_params": (_int, [_vp, _vp, _vp]),
     "qv_hnsw_store_search": (_int, [_vp, _vp, _sz, _sz, _vp, _vp, _vp]),
     "qv_hnsw_store_search_device": (_int, [_vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _vp]),
+    "qv_embedding_lookup_device": (_int, [_int, _u32, _vp, _sz, _sz, _sz, _u32, _vp, _sz, _f32, _vp,
+                                          _sz, _vp]),
+    "qv_embedding_grad_workspace": (_int, [_sz, _sz, _sz, C.POINTER(_sz)]),
+    "qv_embedding_grad_device": (_int, [_int, _u32, _vp, _sz, _u32, _vp, _sz, _sz, _sz, _f32, _vp,
+                                        _sz, _vp, _sz, _vp]),
+    "qv_flat_lookup_device": (_int, [_vp, _u32, _vp, _sz, _f32, _vp, _sz, _vp]),
+    "qv_linear_workspace": (_int, [_int, C.POINTER(qv_linear), C.POINTER(_sz)]),
+    "qv_linear_device": (_int, [_int, C.POINTER(qv_linear), _vp, _sz, _vp]),
+    "qv_linear_grad_workspace": (_int, [_int, C.POINTER(qv_linear_grad), C.POINTER(_sz)]),
+    "qv_linear_grad_device": (_int, [_int, C.POINTER(qv_linear_grad), _vp, _sz, _vp]),
     "qv_merge_topk_device": (_int, [_int, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "qv_select_topk_device": (_int, [_int, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
 }

@@ -737,6 +737,18 @@ qv_status qv_flat_rows(const qv_flat* index, size_t first, size_t count, float* 
   });
 }
 
+qv_status qv_flat_lookup_device(const qv_flat* index, uint32_t id_type, const void* ids, size_t n,
+                                float scale, float* out, size_t out_stride, void* stream) {
+  return guarded([&] {
+    QV_REQUIRE(index != nullptr, "null index");
+    std::shared_lock lock(index->mu);
+    const FlatState& s = index->s;
+    DeviceScope scope(s.device);
+    embedding_lookup(QV_DTYPE_F32, s.x.get(), s.n, s.dim, s.dim, id_type, ids, n, scale, out,
+                     out_stride, static_cast<cudaStream_t>(stream));
+  });
+}
+
 qv_status qv_flat_filter_bitmap(const qv_flat* index, const qv_filter* filter,
                                 uint64_t** device_bitmap) {
   return guarded([&] {

@@ -1,0 +1,954 @@
+// Linear adapters: y = act(x W^T + bias) + residual, and its gradients
+//   dz = dy * act'(z),  dx = dz W,  dW = dz^T x,  db = sum over rows of dz     (z = x W^T + bias).
+//
+// The three products run in one tensor-core kernel, product_kernel: D[m][n] = sum_k A[m][k] B[n][k]
+// with either operand stored along k or across it, so that no operand is transposed in memory.
+// 16-bit operands are multiplied as they are. A float32 operand is split into three bfloat16
+// planes whose sum it is (8 + 8 + 8 bits of mantissa), and the product is the sum of the six
+// plane products that reach float32's last bit. Batches of a few rows (single queries) take a
+// kernel that reads the weights once with plain loads.
+#include <algorithm>
+#include <mutex>
+
+#include "embed.cuh"
+#include "linear.cuh"
+#include "tc_common.cuh"
+
+namespace qv {
+namespace {
+
+using dev::Pack;
+
+// ---- packing: operands TMA cannot read in place, and float32 as three bfloat16 planes ------------
+
+// x as a sum of three bfloat16: each is the rounded remainder of the ones before, and the last
+// remainder has at most 8 bits left, so that the sum is x itself. The largest finite values round
+// to infinity in the first plane and are cut there instead; infinity and NaN stay in the first.
+__device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
+  p[0] = __float2bfloat16_rn(x);
+  p[1] = p[2] = __float2bfloat16_rn(0.0f);
+  if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) return;
+  if (__hisinf(p[0])) p[0] = __float2bfloat16_rz(x);
+  const float r = x - __bfloat162float(p[0]);
+  p[1] = __float2bfloat16_rn(r);
+  p[2] = __float2bfloat16_rn(r - __bfloat162float(p[1]));
+}
+
+__device__ __forceinline__ void put_operand(float x, float, __nv_bfloat16* dst, size_t plane,
+                                            size_t at) {
+  __nv_bfloat16 p[3];
+  split3(x, p);
+  dst[at] = p[0];
+  dst[plane + at] = p[1];
+  dst[2 * plane + at] = p[2];
+}
+template <class T>
+__device__ __forceinline__ void put_operand(float x, T, T* dst, size_t, size_t at) {
+  dst[at] = dev::from_f32<T>(x);
+}
+// The element type the tensor core multiplies for values of type T.
+template <class T>
+struct Operand {
+  using type = T;
+};
+template <>
+struct Operand<float> {
+  using type = __nv_bfloat16;
+};
+
+template <class T>
+__global__ void __launch_bounds__(256)
+    pack_kernel(const T* __restrict__ src, size_t rows, uint32_t cols, int64_t stride,
+                typename Operand<T>::type* __restrict__ dst, uint32_t ld) {
+  const size_t plane = rows * ld;
+  for (size_t r = blockIdx.x; r < rows; r += gridDim.x)
+    for (uint32_t c = threadIdx.x + blockIdx.y * 256; c < cols; c += 256 * gridDim.y)
+      put_operand(dev::to_f32<T>(src[static_cast<int64_t>(r) * stride + c]), T{}, dst, plane,
+                  r * ld + c);
+}
+
+// ---- the product kernel -----------------------------------------------------------------------------
+
+constexpr int kBM = 128, kBK = 64;
+constexpr int kEpilogueWarps = 8;
+constexpr int kProductThreads = 128 + 32 * kEpilogueWarps;  // producer, MMA, 2 idle, epilogue
+
+template <int kBN>
+struct Tile {
+  static constexpr int kABytes = kBM * kBK * 2;
+  static constexpr int kBBytes = kBN * kBK * 2;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = kBN == 256 ? 4 : (kBN == 128 ? 6 : 8);
+  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + 1024 + 256;
+};
+
+// Plane pairs of a float32 product, smallest terms first.
+__constant__ int8_t kPairA[6] = {2, 0, 1, 1, 0, 0};
+__constant__ int8_t kPairB[6] = {0, 2, 1, 0, 1, 0};
+
+struct ProductArgs {
+  int64_t m, n, k;
+  int pairs;              // plane pairs: 1, or 6 for float32
+  int k_blocks;           // 64-wide blocks of k
+  int tiles_m, tiles_n, splits, blocks_per_split;
+  uint32_t idesc;
+  uint32_t a_mn, b_mn;    // operand stored across k (MN-major)
+  Epilogue ep;
+  float* partial;         // splits > 1: [split][m][n] float32 sums, joined afterwards
+  long long wait_cycles;
+  uint64_t drain_ns;
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                            int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+// 128-byte swizzled operand tiles. Along k: 64-element rows, 8-row groups 1024 bytes apart.
+// Across k: [64 k][64 m-or-n] blocks of 8 KB (the leading offset), 8-k groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t across) {
+  return (static_cast<uint64_t>(addr >> 4) & 0x3FFFull) |
+         (static_cast<uint64_t>(across ? 8192 >> 4 : 1) << 16) | (64ull << 32) | (1ull << 46) |
+         (2ull << 61);
+}
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                        uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+template <class T, int kBN>
+__global__ void __launch_bounds__(kProductThreads, 1)
+    product_kernel(const __grid_constant__ CUtensorMap map_a,
+                   const __grid_constant__ CUtensorMap map_b, const ProductArgs a) {
+  using S = Tile<kBN>;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* tiles = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + S::kStages * S::kStageBytes);
+  // full[stage], empty[stage], acc_full[2], acc_empty[2], drain
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  __shared__ int s_consumed;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto bar = [&](int i) { return tc::smem_u32(bars + i); };
+  constexpr int FULL = 0, EMPTY = S::kStages, ACC_FULL = 2 * S::kStages, ACC_EMPTY = ACC_FULL + 2,
+                DRAIN = ACC_EMPTY + 2;
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    s_consumed = 0;
+    for (int s = 0; s < S::kStages; ++s) {
+      tc::mbar_init(bar(FULL + s), 1);
+      tc::mbar_init(bar(EMPTY + s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      tc::mbar_init(bar(ACC_FULL + b), 1);
+      tc::mbar_init(bar(ACC_EMPTY + b), kEpilogueWarps);
+    }
+    tc::mbar_init(bar(DRAIN), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     tc::smem_u32(&s_tmem)),
+                 "r"(2 * kBN));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  volatile int* abort_flag = &s_abort;
+  int err_sink = 0;  // mbar_wait's error word: an abort shows in the output (NaN)
+  auto wait = [&](uint32_t b, uint32_t parity) {
+    if (tc::mbar_test(b, parity)) return true;
+    const long long t0 = clock64();
+    for (;;) {
+      if (tc::mbar_sleep_test(b, parity)) return true;
+      if (*abort_flag) return false;
+      if (clock64() - t0 > a.wait_cycles) {
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  };
+  (void)err_sink;
+  const int units = a.tiles_m * a.tiles_n * a.splits;
+  // Unit u: split u / (tiles), tile row / column of the rest, columns fastest (a wave's CTAs share
+  // rows of A and all of B in L2).
+  auto coords = [&](int u, int& split, int& tm, int& tn) {
+    const int per = a.tiles_m * a.tiles_n;
+    split = u / per;
+    const int t = u - split * per;
+    tm = t / a.tiles_n;
+    tn = t - tm * a.tiles_n;
+  };
+  auto block_range = [&](int split, int& b0, int& b1) {
+    b0 = split * a.blocks_per_split;
+    b1 = min(a.k_blocks, b0 + a.blocks_per_split);
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int issued = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        int split, tm, tn, b0, b1;
+        coords(u, split, tm, tn);
+        block_range(split, b0, b1);
+        for (int p = 0; p < a.pairs && ok; ++p) {
+          const int pa = a.pairs == 1 ? 0 : kPairA[p], pb = a.pairs == 1 ? 0 : kPairB[p];
+          for (int kb = b0; kb < b1; ++kb) {
+            const int s = issued % S::kStages;
+            if (!wait(bar(EMPTY + s), ((issued / S::kStages) & 1) ^ 1)) {
+              ok = false;
+              break;
+            }
+            tc::mbar_expect_tx(bar(FULL + s), S::kStageBytes);
+            const uint32_t da = tc::smem_u32(tiles + s * S::kStageBytes);
+            const uint32_t db = da + S::kABytes;
+            if (a.a_mn) {
+              for (int c = 0; c < kBM / 64; ++c)
+                tma_load_3d(da + c * 8192, &map_a, tm * kBM + c * 64, kb * kBK, pa, bar(FULL + s));
+            } else {
+              tma_load_3d(da, &map_a, kb * kBK, tm * kBM, pa, bar(FULL + s));
+            }
+            if (a.b_mn) {
+              for (int c = 0; c < kBN / 64; ++c)
+                tma_load_3d(db + c * 8192, &map_b, tn * kBN + c * 64, kb * kBK, pb, bar(FULL + s));
+            } else {
+              tma_load_3d(db, &map_b, kb * kBK, tn * kBN, pb, bar(FULL + s));
+            }
+            ++issued;
+          }
+        }
+      }
+      if (*abort_flag) {  // wait (bounded) for the copies that the MMA warp did not consume
+        const uint64_t t0 = tc::gtimer();
+        for (int f = s_consumed; f < issued; ++f)
+          while (!tc::mbar_test(bar(FULL + f % S::kStages), (f / S::kStages) & 1) &&
+                 tc::gtimer() - t0 < a.drain_ns) {
+          }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int taken = 0, t = 0;
+      bool ok = true;
+      const uint32_t a_step = a.a_mn ? 2048 >> 4 : 32 >> 4, b_step = a.b_mn ? 2048 >> 4 : 32 >> 4;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++t) {
+        int split, tm, tn, b0, b1;
+        coords(u, split, tm, tn);
+        block_range(split, b0, b1);
+        const int slot = t & 1;
+        if (!wait(bar(ACC_EMPTY + slot), ((t >> 1) & 1) ^ 1)) break;
+        tc::tc_fence_after();
+        const uint32_t d = tmem + slot * kBN;
+        const int blocks = (b1 - b0) * a.pairs;
+        for (int i = 0; i < blocks; ++i) {
+          const int s = taken % S::kStages;
+          if (!wait(bar(FULL + s), (taken / S::kStages) & 1)) {
+            ok = false;
+            break;
+          }
+          s_consumed = ++taken;
+          tc::tc_fence_after();
+          const uint32_t da = tc::smem_u32(tiles + s * S::kStageBytes);
+          const uint64_t ad = operand_desc(da, a.a_mn);
+          const uint64_t bd = operand_desc(da + S::kABytes, a.b_mn);
+#pragma unroll
+          for (int q = 0; q < kBK / 16; ++q)
+            mma_f16(d, ad + q * a_step, bd + q * b_step, a.idesc, (i | q) != 0);
+          tc::umma_commit(bar(EMPTY + s));
+        }
+        if (!ok) break;
+        tc::umma_commit(bar(ACC_FULL + slot));
+      }
+      if (*abort_flag) {  // wait (bounded) for the MMAs in flight before their memory goes
+        tc::umma_commit(bar(DRAIN));
+        const uint64_t t0 = tc::gtimer();
+        while (!tc::mbar_test(bar(DRAIN), 0) && tc::gtimer() - t0 < a.drain_ns) {
+        }
+      }
+    }
+  } else if (warp >= 4) {
+    const int quarter = warp & 3;            // TMEM lanes this warp may read
+    const int half = (warp - 4) >> 2;        // which columns of each 64 it takes
+    int t = 0;
+    for (int u = blockIdx.x; u < units; u += gridDim.x, ++t) {
+      int split, tm, tn;
+      coords(u, split, tm, tn);
+      const int slot = t & 1;
+      const bool ok = wait(bar(ACC_FULL + slot), (t >> 1) & 1);
+      __syncwarp();
+      tc::tc_fence_after();
+      const int64_t row = static_cast<int64_t>(tm) * kBM + quarter * 32 + lane;
+#pragma unroll 1
+      for (int c = half * 32; c < kBN; c += 64) {
+        const int64_t col = static_cast<int64_t>(tn) * kBN + c;
+        if (col >= a.n) break;
+        uint32_t r[32];
+        if (ok) {
+          tmem_ld32(tmem + slot * kBN + c + (static_cast<uint32_t>(quarter * 32) << 16), r);
+        } else {  // the pipeline gave up: the tile is written as NaN
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = 0x7fc00000u;
+        }
+        if (row < a.m) {
+          float v[16];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[h * 16 + j]);
+            const int left = static_cast<int>(min(static_cast<int64_t>(16), a.n - col - h * 16));
+            if (left <= 0) break;
+            if (a.splits > 1) {
+              float* p = a.partial + (static_cast<int64_t>(split) * a.m + row) * a.n + col + h * 16;
+              put16<float>(p, v, left, (a.n & 3) == 0 ? 16 : 4);
+            } else {
+              finish16<T>(a.ep, row, col + h * 16, v, left);
+            }
+          }
+        }
+        __syncwarp();
+      }
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(bar(ACC_EMPTY + slot));
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc::tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(2 * kBN));
+  }
+}
+
+// Joins the splits of k in their order and finishes the elements.
+template <class T>
+__global__ void __launch_bounds__(256)
+    join_splits_kernel(const float* __restrict__ partial, int splits, int64_t m, int64_t n,
+                       Epilogue ep) {
+  const int64_t per_row = (n + 15) / 16;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < m * per_row; i += gridDim.x * 256ll) {
+    const int64_t row = i / per_row, col = (i - row * per_row) * 16;
+    const int left = static_cast<int>(min(static_cast<int64_t>(16), n - col));
+    float v[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+    for (int s = 0; s < splits; ++s) {
+      const float* p = partial + (static_cast<int64_t>(s) * m + row) * n + col;
+      float x[16];
+      get16<float>(p, x, left, (n & 3) == 0 ? 16 : 4);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] += x[j];
+    }
+    finish16<T>(ep, row, col, v, left);
+  }
+}
+
+// ---- few rows: every weight read once with plain loads -------------------------------------------
+
+// One warp per output column for up to kRows rows of x: lanes stride over k, float32 sums.
+template <class T, int kRows, int kV>
+__global__ void __launch_bounds__(128)
+    few_rows_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ w,
+                    int64_t w_stride, int m, int64_t n, int64_t k, Epilogue ep) {
+  const int lane = threadIdx.x & 31;
+  const int64_t col = (blockIdx.x * 128ll + threadIdx.x) >> 5;
+  if (col >= n) return;
+  const T* wr = w + col * w_stride;
+  float acc[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) acc[r] = 0.0f;
+#pragma unroll 4
+  for (int64_t c = lane * kV; c < k; c += 32 * kV) {
+    const Pack<T, kV> a = dev::load_pack<T, kV>(wr + c);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      if (r < m) {
+        const Pack<T, kV> b = dev::load_pack<T, kV>(x + r * x_stride + c);
+#pragma unroll
+        for (int j = 0; j < kV; ++j)
+          acc[r] = fmaf(dev::to_f32<T>(a.v[j]), dev::to_f32<T>(b.v[j]), acc[r]);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) acc[r] += __shfl_xor_sync(dev::kFull, acc[r], d);
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r)
+    if (r < m && lane == r) finish1<T>(ep, r, col, acc[r]);
+}
+
+// ---- dz and the bias gradient ----------------------------------------------------------------------
+
+// dz = dy * act'(z), rounded to the operand type (float32: three planes), and float32 column sums
+// of the unrounded dz over this block's rows. Threads walk down columns; blocks are row ranges.
+template <class T, bool kStore>
+__global__ void __launch_bounds__(256)
+    dz_kernel(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ z,
+              int64_t z_stride, int act, int64_t m, int64_t n, int64_t rows_per_block,
+              typename Operand<T>::type* __restrict__ dz, int64_t ld, float* __restrict__ sums) {
+  const int64_t col = blockIdx.y * 256ll + threadIdx.x;
+  if (col >= n) return;
+  const int64_t r0 = blockIdx.x * rows_per_block, r1 = min(m, r0 + rows_per_block);
+  float s = 0.0f;
+  for (int64_t r = r0; r < r1; ++r) {
+    float g = dev::to_f32<T>(dy[r * dy_stride + col]);
+    // rounded before the sum in both variants, so that dbias does not depend on which runs
+    if (act != QV_ACT_NONE) g = __fmul_rn(g, act_grad<T>(act, dev::to_f32<T>(z[r * z_stride + col])));
+    s += g;
+    if (kStore) put_operand(g, T{}, dz, static_cast<size_t>(m * ld), static_cast<size_t>(r * ld + col));
+  }
+  if (sums != nullptr) sums[blockIdx.x * n + col] = s;
+}
+
+template <class T>
+__global__ void __launch_bounds__(256)
+    join_sums_kernel(const float* __restrict__ sums, int64_t blocks, int64_t n, T* __restrict__ db) {
+  const int64_t col = blockIdx.x * 256ll + threadIdx.x;
+  if (col >= n) return;
+  float s = 0.0f;
+  for (int64_t b = 0; b < blocks; ++b) s += sums[b * n + col];
+  db[col] = dev::from_f32<T>(s);
+}
+
+// ---- host side ----------------------------------------------------------------------------------------
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                              const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static EncodeFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeFn>(p);
+  });
+  if (fn == nullptr) fail(QV_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  return fn;
+}
+
+// A stored operand: `outer` rows of `inner` elements, ld apart, `planes` copies plane_stride apart.
+struct Stored {
+  const void* p = nullptr;
+  int64_t inner = 0, outer = 0, ld = 0;
+  int planes = 1;
+  bool bf16 = true;
+};
+
+CUtensorMap operand_map(const Stored& s, uint32_t box_outer) {
+  CUtensorMap m;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(s.inner), static_cast<cuuint64_t>(s.outer),
+                              static_cast<cuuint64_t>(s.planes)};
+  // A single row may have any stride; the map wants one that holds it.
+  const int64_t ld = s.outer > 1 ? s.ld : (s.inner + 7) / 8 * 8;
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld * 2),
+                                 static_cast<cuuint64_t>(ld * s.outer * 2)};
+  const cuuint32_t box[3] = {64, box_outer, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = encode_fn()(
+      &m, s.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+      const_cast<void*>(s.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) fail(QV_ERR_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string(r));
+  return m;
+}
+
+struct ProductPlan {
+  int bn = 128, splits = 1, blocks_per_split = 1, k_blocks = 1;
+  size_t partial_bytes = 0;
+};
+
+// Tile width and split of k with the least estimated time. In cycles: a 64-wide block of k takes
+// the larger of the MMAs and the copies into shared memory, a tile's results about 12 cycles a
+// column, and the splits are written, read and joined in a launch of their own.
+ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int pairs, int sms) {
+  ProductPlan best;
+  double best_t = 1e300;
+  const int64_t kb = std::max<int64_t>(1, static_cast<int64_t>(ceil_div(k, kBK)));
+  for (int bn : {64, 128, 256}) {
+    const double tiles = static_cast<double>(ceil_div(m, kBM)) * ceil_div(n, bn);
+    const double per_block = bn == 256 ? 560 : (bn == 128 ? 330 : 230);
+    for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+      if (s > 1 && (s > kb || tiles * s > 2.0 * sms)) break;
+      const int64_t per = static_cast<int64_t>(ceil_div(kb, s));
+      const int64_t used = static_cast<int64_t>(ceil_div(kb, per));
+      const double waves = std::ceil(tiles * used / sms);
+      double t = waves * per * pairs * per_block + 12.0 * bn + 1500;
+      if (used > 1) t += 4000 + 8.0 * m * n * used / 3000.0;
+      if (t < best_t) {
+        best_t = t;
+        best.bn = bn;
+        best.splits = static_cast<int>(used);
+        best.blocks_per_split = static_cast<int>(per);
+        best.k_blocks = static_cast<int>(kb);
+      }
+    }
+  }
+  best.partial_bytes =
+      best.splits > 1 ? static_cast<size_t>(best.splits) * m * n * sizeof(float) : 0;
+  return best;
+}
+
+template <class T, int kBN>
+void launch_product(const ProductArgs& a, const Stored& A, const Stored& B, int sms,
+                    cudaStream_t st) {
+  const CUtensorMap ma = operand_map(A, a.a_mn ? kBK : kBM);
+  const CUtensorMap mb = operand_map(B, a.b_mn ? kBK : kBN);
+  static std::once_flag once[16];
+  int device = 0;
+  QV_CUDA(cudaGetDevice(&device));
+  std::call_once(once[device & 15], [&] {
+    QV_CUDA(cudaFuncSetAttribute(product_kernel<T, kBN>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(Tile<kBN>::kSmem)));
+  });
+  const int units = a.tiles_m * a.tiles_n * a.splits;
+  product_kernel<T, kBN>
+      <<<std::min(units, sms), kProductThreads, Tile<kBN>::kSmem, st>>>(ma, mb, a);
+  check_launch("product_kernel");
+}
+
+// D[m][n] = sum_k A B, finished by `ep`. a_mn / b_mn: the operand is stored with m (n) inner.
+template <class T>
+void product(const Stored& A, bool a_mn, const Stored& B, bool b_mn, int64_t m, int64_t n,
+             int64_t k, const Epilogue& ep, const ProductPlan& plan, void* partial, int sms,
+             cudaStream_t st) {
+  ProductArgs a{};
+  a.m = m;
+  a.n = n;
+  a.k = k;
+  a.pairs = std::is_same_v<T, float> ? 6 : 1;
+  a.k_blocks = plan.k_blocks;
+  a.tiles_m = static_cast<int>(ceil_div(m, kBM));
+  a.tiles_n = static_cast<int>(ceil_div(n, plan.bn));
+  a.splits = plan.splits;
+  a.blocks_per_split = plan.blocks_per_split;
+  const uint32_t fmt = A.bf16 ? 1 : 0;
+  a.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(a_mn) << 15) |
+            (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(plan.bn >> 3) << 17) |
+            (static_cast<uint32_t>(kBM >> 4) << 24);
+  a.a_mn = a_mn;
+  a.b_mn = b_mn;
+  a.ep = ep;
+  a.partial = static_cast<float*>(partial);
+  a.wait_cycles = tc::wait_limit_cycles();
+  a.drain_ns = tc::drain_limit_ns();
+  if (plan.bn == 256)
+    launch_product<T, 256>(a, A, B, sms, st);
+  else if (plan.bn == 128)
+    launch_product<T, 128>(a, A, B, sms, st);
+  else
+    launch_product<T, 64>(a, A, B, sms, st);
+  if (plan.splits > 1) {
+    const size_t items = static_cast<size_t>(m) * ceil_div(n, 16);
+    join_splits_kernel<T>
+        <<<static_cast<unsigned>(std::min<size_t>(ceil_div(items, 256), 148 * 16)), 256, 0, st>>>(
+            a.partial, plan.splits, m, n, ep);
+    check_launch("join_splits_kernel");
+  }
+}
+
+// Whether TMA can read 16-bit rows in place: 16-byte aligned rows.
+bool in_place(uint32_t dtype, const void* p, size_t rows, size_t stride) {
+  return dtype != QV_DTYPE_F32 && reinterpret_cast<uintptr_t>(p) % 16 == 0 &&
+         (rows <= 1 || (stride * 2) % 16 == 0);
+}
+size_t packed_ld(size_t cols) { return (cols + 7) / 8 * 8; }
+size_t packed_bytes(uint32_t dtype, size_t rows, size_t cols) {
+  return (rows * packed_ld(cols) * 2 * (dtype == QV_DTYPE_F32 ? 3 : 1) + 255) / 256 * 256;
+}
+
+template <class T>
+Stored pack_rows(const void* src, size_t rows, size_t cols, size_t stride, void* dst,
+                 cudaStream_t st) {
+  Stored s;
+  s.p = dst;
+  s.inner = static_cast<int64_t>(cols);
+  s.outer = static_cast<int64_t>(rows);
+  s.ld = static_cast<int64_t>(packed_ld(cols));
+  s.planes = std::is_same_v<T, float> ? 3 : 1;
+  s.bf16 = !std::is_same_v<T, __half>;
+  pack_kernel<T><<<dim3(static_cast<unsigned>(std::min<size_t>(rows, 148 * 32)),
+                        static_cast<unsigned>(std::min<size_t>(ceil_div(cols, 256), 64))),
+                   256, 0, st>>>(static_cast<const T*>(src), rows, static_cast<uint32_t>(cols),
+                                 static_cast<int64_t>(stride),
+                                 static_cast<typename Operand<T>::type*>(dst),
+                                 static_cast<uint32_t>(s.ld));
+  check_launch("pack_kernel");
+  return s;
+}
+template <class T>
+Stored stored_rows(uint32_t dtype, const void* src, size_t rows, size_t cols, size_t stride,
+                   unsigned char*& ws, cudaStream_t st) {
+  if (in_place(dtype, src, rows, stride)) {
+    Stored s;
+    s.p = src;
+    s.inner = static_cast<int64_t>(cols);
+    s.outer = static_cast<int64_t>(rows);
+    s.ld = static_cast<int64_t>(stride);
+    s.bf16 = dtype == QV_DTYPE_BF16;
+    return s;
+  }
+  void* dst = ws;
+  ws += packed_bytes(dtype, rows, cols);
+  return pack_rows<T>(src, rows, cols, stride, dst, st);
+}
+
+constexpr size_t kMaxFewRows = 8;
+constexpr size_t kMaxDim = 65536;
+constexpr size_t kMaxLinearRows = (size_t{1} << 31) - 256;
+
+template <class F>
+void by_type(uint32_t dtype, F&& f) {
+  if (dtype == QV_DTYPE_F32)
+    f(float{});
+  else if (dtype == QV_DTYPE_F16)
+    f(__half{});
+  else
+    f(__nv_bfloat16{});
+}
+
+void check_matrix(const char* what, uint32_t dtype, const void* p, size_t rows, size_t cols,
+                  size_t stride) {
+  QV_REQUIRE(p != nullptr || rows == 0, std::string("null ") + what);
+  QV_REQUIRE(reinterpret_cast<uintptr_t>(p) % dtype_size(dtype) == 0,
+             std::string(what) + " is not aligned to its element type");
+  QV_REQUIRE(stride >= cols || rows <= 1, std::string(what) + ": row stride below its columns");
+  QV_REQUIRE(stride < (size_t{1} << 36), std::string(what) + ": row stride too large");
+}
+
+void check_linear(const qv_linear& l) {
+  check_dtype(l.dtype);
+  QV_REQUIRE(l.activation <= QV_ACT_SILU, "unknown activation");
+  QV_REQUIRE(l.k >= 1 && l.k <= kMaxDim && l.n >= 1 && l.n <= kMaxDim,
+             "dimensions must be between 1 and 65536");
+  QV_REQUIRE(l.m <= kMaxLinearRows, "too many rows");
+  QV_REQUIRE(l.out_dtype == l.dtype || l.out_dtype == QV_DTYPE_F32,
+             "results have the inputs' type or float32");
+  if (l.m == 0) return;
+  check_matrix("x", l.dtype, l.x, l.m, l.k, l.x_stride);
+  check_matrix("weight", l.dtype, l.weight, l.n, l.k, l.weight_stride);
+  check_matrix("out", l.out_dtype, l.out, l.m, l.n, l.out_stride);
+  if (l.bias != nullptr) check_matrix("bias", l.dtype, l.bias, 1, l.n, l.n);
+  if (l.residual != nullptr) {
+    // Stride 0 adds one row to every row of the result.
+    check_matrix("residual", l.dtype, l.residual, l.residual_stride == 0 ? 1 : l.m, l.n,
+                 l.residual_stride);
+  }
+  if (l.preact != nullptr) check_matrix("preact", l.dtype, l.preact, l.m, l.n, l.preact_stride);
+}
+
+Epilogue epilogue_of(const qv_linear& l) {
+  Epilogue e{};
+  e.act = static_cast<int>(l.activation);
+  e.bias = l.bias;
+  e.residual = l.residual;
+  e.residual_stride = static_cast<int64_t>(l.residual_stride);
+  e.out = l.out;
+  e.out_stride = static_cast<int64_t>(l.out_stride);
+  e.out_f32 = l.out_dtype == QV_DTYPE_F32;
+  e.preact = l.preact;
+  e.preact_stride = static_cast<int64_t>(l.preact_stride);
+  e.set_aligns(dtype_size(l.dtype));
+  return e;
+}
+
+struct LinearPlan {
+  bool few = false;
+  ProductPlan product;
+  size_t bytes = 0;
+};
+LinearPlan linear_plan(const qv_linear& l, int sms) {
+  LinearPlan p;
+  p.few = l.m <= kMaxFewRows;
+  if (p.few || l.m == 0) return p;
+  p.product = plan_product(l.m, l.n, l.k, l.dtype == QV_DTYPE_F32 ? 6 : 1, sms);
+  if (!in_place(l.dtype, l.x, l.m, l.x_stride)) p.bytes += packed_bytes(l.dtype, l.m, l.k);
+  if (!in_place(l.dtype, l.weight, l.n, l.weight_stride))
+    p.bytes += packed_bytes(l.dtype, l.n, l.k);
+  p.bytes += p.product.partial_bytes;
+  return p;
+}
+
+template <class T, int kRows>
+void launch_few(const qv_linear& l, const Epilogue& ep, cudaStream_t st) {
+  const size_t e = sizeof(T);
+  const int align = common_align({reinterpret_cast<uintptr_t>(l.x),
+                                  reinterpret_cast<uintptr_t>(l.weight),
+                                  l.m > 1 ? l.x_stride * e : 0, l.n > 1 ? l.weight_stride * e : 0,
+                                  l.k * e});
+  const unsigned blocks = static_cast<unsigned>(ceil_div(l.n, 4));
+  auto go = [&](auto v) {
+    constexpr int kV = decltype(v)::value;
+    few_rows_kernel<T, kRows, kV><<<blocks, 128, 0, st>>>(
+        static_cast<const T*>(l.x), static_cast<int64_t>(l.x_stride),
+        static_cast<const T*>(l.weight), static_cast<int64_t>(l.weight_stride),
+        static_cast<int>(l.m), static_cast<int64_t>(l.n), static_cast<int64_t>(l.k), ep);
+  };
+  if (align == 16)
+    go(std::integral_constant<int, 16 / sizeof(T)>{});
+  else if (align == 8)
+    go(std::integral_constant<int, 8 / sizeof(T)>{});
+  else
+    go(std::integral_constant<int, 1>{});
+  check_launch("few_rows_kernel");
+}
+
+}  // namespace
+
+size_t linear_workspace(const qv_linear& l, int sms) {
+  check_linear(l);
+  return linear_plan(l, sms).bytes;
+}
+
+void linear_forward(const qv_linear& l, void* workspace, size_t workspace_bytes, int sms,
+                    cudaStream_t st) {
+  check_linear(l);
+  if (l.m == 0) return;
+  const LinearPlan p = linear_plan(l, sms);
+  QV_REQUIRE(p.bytes == 0 || (workspace != nullptr && workspace_bytes >= p.bytes),
+             "workspace too small: qv_linear_workspace tells the size");
+  QV_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0 || p.bytes == 0,
+             "workspace must be 256-byte aligned");
+  const Epilogue ep = epilogue_of(l);
+  by_type(l.dtype, [&](auto t) {
+    using T = decltype(t);
+    if (p.few) {
+      if (l.m == 1)
+        launch_few<T, 1>(l, ep, st);
+      else if (l.m <= 4)
+        launch_few<T, 4>(l, ep, st);
+      else
+        launch_few<T, 8>(l, ep, st);
+      return;
+    }
+    unsigned char* ws = static_cast<unsigned char*>(workspace);
+    const Stored x = stored_rows<T>(l.dtype, l.x, l.m, l.k, l.x_stride, ws, st);
+    const Stored w = stored_rows<T>(l.dtype, l.weight, l.n, l.k, l.weight_stride, ws, st);
+    product<T>(x, false, w, false, l.m, l.n, l.k, ep, p.product, ws, sms, st);
+  });
+}
+
+// ---- gradients -------------------------------------------------------------------------------------
+
+namespace {
+
+void check_linear_grad(const qv_linear_grad& g) {
+  check_dtype(g.dtype);
+  QV_REQUIRE(g.activation <= QV_ACT_SILU, "unknown activation");
+  QV_REQUIRE(g.k >= 1 && g.k <= kMaxDim && g.n >= 1 && g.n <= kMaxDim,
+             "dimensions must be between 1 and 65536");
+  QV_REQUIRE(g.m <= kMaxLinearRows, "too many rows");
+  if (g.dweight != nullptr)
+    check_matrix("dweight", g.dtype, g.dweight, g.n, g.k, g.dweight_stride);
+  if (g.dbias != nullptr) check_matrix("dbias", g.dtype, g.dbias, 1, g.n, g.n);
+  if (g.m == 0) return;
+  check_matrix("grad", g.dtype, g.grad, g.m, g.n, g.grad_stride);
+  if (g.activation != QV_ACT_NONE)
+    check_matrix("preact", g.dtype, g.preact, g.m, g.n, g.preact_stride);
+  if (g.dx != nullptr) {
+    check_matrix("weight", g.dtype, g.weight, g.n, g.k, g.weight_stride);
+    check_matrix("dx", g.dtype, g.dx, g.m, g.k, g.dx_stride);
+  }
+  if (g.dweight != nullptr) check_matrix("x", g.dtype, g.x, g.m, g.k, g.x_stride);
+}
+
+struct GradLayout {
+  bool store_dz = false;      // dz is not the caller's gradient itself
+  size_t row_blocks = 0;      // row ranges of the column sums
+  int64_t rows_per_block = 0;
+  ProductPlan dx, dw;
+  size_t off_dz = 0, off_sums = 0, off_packed = 0, off_partial = 0, bytes = 0;
+};
+GradLayout grad_layout(const qv_linear_grad& g, int sms) {
+  GradLayout L;
+  if (g.m == 0) return L;
+  const int pairs = g.dtype == QV_DTYPE_F32 ? 6 : 1;
+  const bool products = g.dx != nullptr || g.dweight != nullptr;
+  L.store_dz = products && (g.activation != QV_ACT_NONE ||
+                            !in_place(g.dtype, g.grad, g.m, g.grad_stride));
+  const size_t col_blocks = ceil_div(g.n, 256);
+  L.row_blocks = std::min<size_t>(ceil_div(g.m, 8), std::max<size_t>(1, sms * 8 / col_blocks));
+  L.rows_per_block = static_cast<int64_t>(ceil_div(g.m, L.row_blocks));
+  L.row_blocks = ceil_div(g.m, L.rows_per_block);
+  size_t o = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = o;
+    o += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  L.off_dz = take(L.store_dz ? packed_bytes(g.dtype, g.m, g.n) : 0);
+  L.off_sums = take(g.dbias != nullptr ? L.row_blocks * g.n * sizeof(float) : 0);
+  L.off_packed = o;
+  if (g.dx != nullptr) {
+    L.dx = plan_product(g.m, g.k, g.n, pairs, sms);
+    if (!in_place(g.dtype, g.weight, g.n, g.weight_stride)) take(packed_bytes(g.dtype, g.n, g.k));
+  }
+  if (g.dweight != nullptr) {
+    L.dw = plan_product(g.n, g.k, g.m, pairs, sms);
+    if (!in_place(g.dtype, g.x, g.m, g.x_stride)) take(packed_bytes(g.dtype, g.m, g.k));
+  }
+  L.off_partial = take(std::max(L.dx.partial_bytes, L.dw.partial_bytes));
+  L.bytes = o;
+  return L;
+}
+
+}  // namespace
+
+size_t linear_grad_workspace(const qv_linear_grad& g, int sms) {
+  check_linear_grad(g);
+  return grad_layout(g, sms).bytes;
+}
+
+void linear_grad(const qv_linear_grad& g, void* workspace, size_t workspace_bytes, int sms,
+                 cudaStream_t st) {
+  check_linear_grad(g);
+  const size_t e = dtype_size(g.dtype);
+  if (g.m == 0) {  // no rows: the sums over them are zero
+    if (g.dweight != nullptr)
+      QV_CUDA(cudaMemset2DAsync(g.dweight, std::max(g.dweight_stride, g.k) * e, 0, g.k * e, g.n,
+                                st));
+    if (g.dbias != nullptr) QV_CUDA(cudaMemsetAsync(g.dbias, 0, g.n * e, st));
+    return;
+  }
+  const GradLayout L = grad_layout(g, sms);
+  QV_REQUIRE(L.bytes == 0 || (workspace != nullptr && workspace_bytes >= L.bytes),
+             "workspace too small: qv_linear_grad_workspace tells the size");
+  QV_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0 || L.bytes == 0,
+             "workspace must be 256-byte aligned");
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  by_type(g.dtype, [&](auto t) {
+    using T = decltype(t);
+    using O = typename Operand<T>::type;
+    const int64_t m = g.m, n = g.n, k = g.k;
+    float* sums = g.dbias != nullptr ? reinterpret_cast<float*>(ws + L.off_sums) : nullptr;
+    Stored dz;
+    dz.inner = n;
+    dz.outer = m;
+    dz.bf16 = g.dtype != QV_DTYPE_F16;
+    if (L.store_dz || sums != nullptr) {
+      const dim3 grid(static_cast<unsigned>(L.row_blocks),
+                      static_cast<unsigned>(ceil_div(g.n, 256)));
+      O* store = reinterpret_cast<O*>(ws + L.off_dz);
+      const int64_t ld = static_cast<int64_t>(packed_ld(g.n));
+      if (L.store_dz)
+        dz_kernel<T, true><<<grid, 256, 0, st>>>(
+            static_cast<const T*>(g.grad), g.grad_stride, static_cast<const T*>(g.preact),
+            g.preact_stride, static_cast<int>(g.activation), m, n, L.rows_per_block, store, ld,
+            sums);
+      else
+        dz_kernel<T, false><<<grid, 256, 0, st>>>(
+            static_cast<const T*>(g.grad), g.grad_stride, static_cast<const T*>(g.preact),
+            g.preact_stride, static_cast<int>(g.activation), m, n, L.rows_per_block, store, ld,
+            sums);
+      check_launch("dz_kernel");
+    }
+    if (L.store_dz) {
+      dz.p = ws + L.off_dz;
+      dz.ld = static_cast<int64_t>(packed_ld(g.n));
+      dz.planes = std::is_same_v<T, float> ? 3 : 1;
+    } else {
+      dz.p = g.grad;
+      dz.ld = static_cast<int64_t>(g.grad_stride);
+    }
+    if (sums != nullptr) {
+      join_sums_kernel<T><<<static_cast<unsigned>(ceil_div(g.n, 256)), 256, 0, st>>>(
+          sums, static_cast<int64_t>(L.row_blocks), n, static_cast<T*>(g.dbias));
+      check_launch("join_sums_kernel");
+    }
+    unsigned char* packed = ws + L.off_packed;
+    if (g.dx != nullptr) {
+      const Stored w = stored_rows<T>(g.dtype, g.weight, g.n, g.k, g.weight_stride, packed, st);
+      Epilogue ep{};
+      ep.out = g.dx;
+      ep.out_stride = static_cast<int64_t>(g.dx_stride);
+      ep.out_f32 = g.dtype == QV_DTYPE_F32;
+      ep.set_aligns(e);
+      product<T>(dz, false, w, true, m, k, n, ep, L.dx, ws + L.off_partial, sms, st);
+    }
+    if (g.dweight != nullptr) {
+      const Stored x = stored_rows<T>(g.dtype, g.x, g.m, g.k, g.x_stride, packed, st);
+      Epilogue ep{};
+      ep.out = g.dweight;
+      ep.out_stride = static_cast<int64_t>(g.dweight_stride);
+      ep.out_f32 = g.dtype == QV_DTYPE_F32;
+      ep.set_aligns(e);
+      product<T>(dz, true, x, true, n, k, m, ep, L.dw, ws + L.off_partial, sms, st);
+    }
+  });
+}
+
+}  // namespace qv
+
+extern "C" {
+
+qv_status qv_linear_workspace(int device, const qv_linear* args, size_t* bytes) {
+  return qv::guarded([&] {
+    QV_REQUIRE(args != nullptr && bytes != nullptr, "null argument");
+    *bytes = qv::linear_workspace(*args, qv::sm_count(device));
+  });
+}
+
+qv_status qv_linear_device(int device, const qv_linear* args, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  return qv::guarded([&] {
+    QV_REQUIRE(args != nullptr, "null argument");
+    qv::DeviceScope scope(device);
+    qv::linear_forward(*args, workspace, workspace_bytes, qv::sm_count(device),
+                       static_cast<cudaStream_t>(stream));
+  });
+}
+
+qv_status qv_linear_grad_workspace(int device, const qv_linear_grad* args, size_t* bytes) {
+  return qv::guarded([&] {
+    QV_REQUIRE(args != nullptr && bytes != nullptr, "null argument");
+    *bytes = qv::linear_grad_workspace(*args, qv::sm_count(device));
+  });
+}
+
+qv_status qv_linear_grad_device(int device, const qv_linear_grad* args, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  return qv::guarded([&] {
+    QV_REQUIRE(args != nullptr, "null argument");
+    qv::DeviceScope scope(device);
+    qv::linear_grad(*args, workspace, workspace_bytes, qv::sm_count(device),
+                    static_cast<cudaStream_t>(stream));
+  });
+}
+
+}  // extern "C"

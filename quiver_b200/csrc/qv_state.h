@@ -215,6 +215,12 @@ void ivf_candidates(const IvfState& s, const float* d_queries, size_t nq, size_t
 void ivf_refine(const IvfState& s, const float* d_queries, size_t nq, size_t keep,
                 const uint64_t* d_keys, float* d_exact, cudaStream_t st);
 
+// ---- embedding tables and linear adapters (embed.cu, linear.cu) ---------------------------------
+// The operators behind the C ABI's entry points of the same names; they check their arguments.
+void embedding_lookup(uint32_t dtype, const void* table, size_t rows, size_t dim,
+                      size_t table_stride, uint32_t id_type, const void* ids, size_t n,
+                      float scale, void* out, size_t out_stride, cudaStream_t st);
+
 // ---- selection / merge -------------------------------------------------------------------------
 void merge_topk(size_t parts, size_t nq, size_t k, const float* d, const uint64_t* keys,
                 const uint64_t* labels, float* od, uint64_t* ok, uint64_t* ol, cudaStream_t st);
