@@ -78,7 +78,7 @@ void launch_lookup(const void* table, size_t rows, size_t dim, size_t table_stri
 // Stable least-significant-digit radix sort of (id, position) pairs; ids that take no gradient
 // (negative or past the table) become `rows` and end up last. Each pass: per-tile digit counts,
 // a prefix over tiles per digit, and a scatter that ranks a tile's entries in input order.
-constexpr int kSortThreads = 256, kSortItems = 8;
+constexpr int kSortThreads = 256, kSortItems = 4;
 constexpr int kSortTile = kSortThreads * kSortItems;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxDigitBits = 11;
@@ -217,24 +217,108 @@ __global__ void __launch_bounds__(kSortThreads)
   }
 }
 
+// The same sort of up to kBlockSortItems * 1024 entries by one block in one launch: the passes'
+// keys and positions stay in shared memory and the threads' registers.
+constexpr int kBlockSortThreads = 1024, kBlockDigitBits = 8;
+constexpr int kBlockSortWarps = kBlockSortThreads / 32;
+
+template <class Id, int kItems>
+__global__ void __launch_bounds__(kBlockSortThreads)
+    block_sort_kernel(const void* __restrict__ ids, uint32_t n, uint32_t rows, int key_bits,
+                      uint32_t* __restrict__ keys, uint32_t* __restrict__ pos) {
+  constexpr int kBins = 1 << kBlockDigitBits;
+  extern __shared__ uint32_t smem[];
+  uint32_t* skey = smem;                                   // kItems * threads
+  uint16_t* spos = reinterpret_cast<uint16_t*>(skey + kItems * kBlockSortThreads);
+  uint16_t* wcount = spos + kItems * kBlockSortThreads;    // kBlockSortWarps x kBins
+  __shared__ uint32_t total[kBins], wsum[kBins / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t first = warp * 32 * kItems + lane;
+  uint16_t* wc = wcount + warp * kBins;
+  uint32_t key[kItems], p[kItems], rank[kItems];
+#pragma unroll
+  for (int j = 0; j < kItems; ++j) {
+    p[j] = first + j * 32;
+    // Entries past the end carry the largest key and stay last (the sort is stable).
+    key[j] = p[j] < n ? clip_id(load_id<Id>(ids, p[j]), rows) : 0xffffffffu;
+  }
+  for (int shift = 0; shift < key_bits; shift += kBlockDigitBits) {
+    for (int b = lane; b < kBins / 2; b += 32) reinterpret_cast<uint32_t*>(wc)[b] = 0;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) {
+      const uint32_t digit = (key[j] >> shift) & (kBins - 1);
+      const uint32_t same = __match_any_sync(dev::kFull, digit);
+      const uint32_t before = __popc(same & ((1u << lane) - 1));
+      rank[j] = wc[digit] + before;
+      __syncwarp();
+      if (before == 0) wc[digit] = static_cast<uint16_t>(wc[digit] + __popc(same));
+      __syncwarp();
+    }
+    __syncthreads();
+    // Prefix over warps per digit (one thread a digit), then over digits.
+    if (threadIdx.x < kBins) {
+      uint32_t acc = 0;
+#pragma unroll
+      for (int w = 0; w < kBlockSortWarps; ++w) {
+        const uint32_t c = wcount[w * kBins + threadIdx.x];
+        wcount[w * kBins + threadIdx.x] = static_cast<uint16_t>(acc);
+        acc += c;
+      }
+      uint32_t s = acc;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t o = __shfl_up_sync(dev::kFull, s, d);
+        if (lane >= d) s += o;
+      }
+      if (lane == 31) wsum[warp] = s;
+      total[threadIdx.x] = s - acc;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) {
+      const uint32_t digit = (key[j] >> shift) & (kBins - 1);
+      uint32_t o = total[digit] + wc[digit] + rank[j];
+      for (uint32_t w = 0; w < digit >> 5; ++w) o += wsum[w];
+      skey[o] = key[j];
+      spos[o] = static_cast<uint16_t>(p[j]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) {
+      key[j] = skey[first + j * 32];
+      p[j] = spos[first + j * 32];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kItems; ++j) {
+    if (first + j * 32 >= n) continue;
+    keys[first + j * 32] = key[j];
+    pos[first + j * 32] = p[j];
+  }
+}
+
 // ---- gradient: segmented sums ---------------------------------------------------------------------
 // The sorted entries and the table's rows are one sequence: each row's entries, then its row end.
-// Entry e stands at place key[e] + e of it. Equal runs of that sequence go to the units (warps),
-// so a token that fills a tenth of the batch is shared out and empty rows cost what they write.
-// A row that begins in one unit and ends in another is joined afterwards from the units' partial
-// sums, in order: tail[u] is what unit u summed of a row it did not end, head[u] what it summed
-// of the row it ended that began before it.
+// Entry e stands at place key[e] + e of it. Equal runs of that sequence go to the blocks and, within
+// a block, to its warps, so a token that fills a tenth of the batch is shared out and empty rows
+// cost what they write. What a warp summed of a row that it did not end is its tail, what it
+// summed of a row that it ended but that began before it is its head; rows that span warps are
+// joined in order, in the block where they end in it, else by join_rows_kernel from the blocks'
+// tails and heads.
+constexpr int kSumWarps = 8, kSumThreads = 32 * kSumWarps;
+constexpr int kSumBatch = 8;  // rows in flight per lane
+constexpr uint32_t kNoRow = 0xffffffffu;
 
-// Number of entries among the first d places of the sequence: the first e with key[e] + e >= d,
-// found by a warp in 32-way steps.
-__device__ __forceinline__ uint32_t entries_before(const uint32_t* __restrict__ keys, uint32_t n,
-                                                   uint64_t d, int lane) {
-  uint32_t lo = 0, hi = n;  // the answer is in [lo, hi]
+// Number of entries among the first d places of the sequence: the first e in [lo, hi] with
+// key[e] + e >= d, found by a warp in 32-way steps. keys[i] belongs to entry i + base.
+__device__ __forceinline__ uint32_t entries_before(const uint32_t* keys, uint32_t base,
+                                                   uint32_t lo, uint32_t hi, uint64_t d,
+                                                   int lane) {
   while (lo < hi) {
-    const uint32_t len = hi - lo;
-    const uint32_t step = (len + 31) / 32;
+    const uint32_t step = (hi - lo + 31) / 32;
     const uint32_t e = lo + lane * step;
-    const bool in = e < hi && static_cast<uint64_t>(keys[e]) + e < d;
+    const bool in = e < hi && static_cast<uint64_t>(keys[e - base]) + e < d;
     const uint32_t m = __ballot_sync(dev::kFull, in);
     if (m == 0) return lo;
     const uint32_t last = lo + (31 - __clz(m)) * step;  // the last probe that is before d
@@ -244,154 +328,223 @@ __device__ __forceinline__ uint32_t entries_before(const uint32_t* __restrict__ 
   return lo;
 }
 
-constexpr int kSumThreads = 256;
-constexpr int kSumBatch = 8;  // rows in flight per lane
-
 template <class T, int kV>
 __global__ void __launch_bounds__(kSumThreads)
     segment_sum_kernel(const T* __restrict__ up, int64_t up_stride,
                        const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
-                       uint32_t n, uint32_t rows, uint32_t dim, uint32_t run, uint32_t units,
-                       float scale, T* __restrict__ grad, int64_t grad_stride,
-                       float* __restrict__ head, float* __restrict__ tail) {
-  const int lane = threadIdx.x & 31;
-  const uint32_t unit = (blockIdx.x * kSumThreads + threadIdx.x) >> 5;
-  if (unit >= units) return;
-  const uint32_t c = (blockIdx.y * 32 + lane) * kV;
+                       uint32_t n, uint32_t rows, uint32_t dim, uint32_t run, float scale,
+                       T* __restrict__ grad, int64_t grad_stride, float* __restrict__ head,
+                       float* __restrict__ tail, uint32_t* __restrict__ head_row) {
+  extern __shared__ __align__(16) unsigned char sum_smem[];
+  constexpr int kCols = 32 * kV;
+  float* s_head = reinterpret_cast<float*>(sum_smem);             // kSumWarps x kCols
+  float* s_tail = s_head + kSumWarps * kCols;                   // kSumWarps x kCols
+  uint32_t* s_key = reinterpret_cast<uint32_t*>(s_tail + kSumWarps * kCols);  // run * kSumWarps
+  uint32_t* s_pos = s_key + run * kSumWarps;
+  __shared__ uint32_t s_e[2], s_tail_row[kSumWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t col0 = blockIdx.y * kCols;
+  const uint32_t c = col0 + lane * kV;
   const bool on = c < dim;
   const uint64_t total = static_cast<uint64_t>(rows) + n;
-  const uint64_t d0 = static_cast<uint64_t>(unit) * run;
-  const uint64_t d1 = d0 + run < total ? d0 + run : total;
-  const uint32_t e0 = entries_before(keys, n, d0, lane);
-  const uint32_t e1 = entries_before(keys, n, d1, lane);
+  const uint64_t b0 = static_cast<uint64_t>(blockIdx.x) * run * kSumWarps;
+  const uint64_t b1 = min(total, b0 + run * kSumWarps);
+  if (warp < 2) {
+    const uint32_t e = entries_before(keys, 0, 0, n, warp == 0 ? b0 : b1, lane);
+    if (lane == 0) s_e[warp] = e;
+  }
+  __syncthreads();
+  const uint32_t eb0 = s_e[0], eb1 = s_e[1];
+  for (uint32_t e = eb0 + threadIdx.x; e < eb1; e += kSumThreads) {
+    s_key[e - eb0] = keys[e];
+    s_pos[e - eb0] = pos[e];
+  }
+  const uint32_t before_key = eb0 > 0 ? keys[eb0 - 1] : kNoRow;  // the entry ahead of the block's
+  __syncthreads();
+  const uint64_t d0 = min(b1, b0 + static_cast<uint64_t>(warp) * run);
+  const uint64_t d1 = min(b1, d0 + run);
+  const uint32_t e0 = entries_before(s_key, eb0, eb0, eb1, d0, lane);
+  const uint32_t e1 = entries_before(s_key, eb0, eb0, eb1, d1, lane);
   uint32_t r = static_cast<uint32_t>(d0 - e0);
-  const uint32_t r1 = static_cast<uint32_t>(d1 - e1);
-  bool began_before = e0 > 0 && keys[e0 - 1] == r;  // row r has entries in an earlier unit
+  const uint32_t r0 = r, r1 = static_cast<uint32_t>(d1 - e1);
+  const bool began_before = d0 < d1 && (e0 > eb0 ? s_key[e0 - 1 - eb0] : before_key) == r;
+  bool is_head = began_before;
   float acc[kV];
 #pragma unroll
   for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
-  bool open = false;
+  T* out = grad + static_cast<int64_t>(r) * grad_stride + c;
   auto finish_row = [&]() {
-    if (on) {
-      if (began_before) {
+    if (is_head) {
 #pragma unroll
-        for (int j = 0; j < kV; ++j) head[static_cast<size_t>(unit) * dim + c + j] = acc[j];
-      } else {
-        Pack<T, kV> y;
+      for (int j = 0; j < kV; ++j) s_head[warp * kCols + lane * kV + j] = acc[j];
+    } else if (on) {
+      Pack<T, kV> y;
 #pragma unroll
-        for (int j = 0; j < kV; ++j) y.v[j] = dev::from_f32<T>(acc[j] * scale);
-        dev::store_pack<T, kV>(grad + static_cast<int64_t>(r) * grad_stride + c, y);
-      }
+      for (int j = 0; j < kV; ++j) y.v[j] = dev::from_f32<T>(acc[j] * scale);
+      dev::store_pack<T, kV>(out, y);
     }
 #pragma unroll
     for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
-    began_before = false;
-    open = false;
+    is_head = false;
     ++r;
+    out += grad_stride;
   };
-  for (uint32_t e = e0; e < e1; e += 32) {
-    const uint32_t mine = e + lane;
-    const uint32_t my_key = mine < e1 ? keys[mine] : rows;
-    const uint32_t my_pos = mine < e1 ? pos[mine] : 0u;
-    const int count = static_cast<int>(min(32u, e1 - e));
-    for (int b = 0; b < count; b += kSumBatch) {
-      Pack<T, kV> x[kSumBatch];
+  for (uint32_t e = e0; e < e1; e += kSumBatch) {
+    const int count = static_cast<int>(min(static_cast<uint32_t>(kSumBatch), e1 - e));
+    Pack<T, kV> x[kSumBatch];
 #pragma unroll
-      for (int j = 0; j < kSumBatch; ++j) {
-        const uint32_t p = __shfl_sync(dev::kFull, my_pos, (b + j) & 31);
-        if (on && b + j < count) x[j] = dev::load_pack<T, kV>(up + static_cast<int64_t>(p) * up_stride + c);
-      }
+    for (int j = 0; j < kSumBatch; ++j)
+      if (on && j < count)
+        x[j] = dev::load_pack<T, kV>(up + static_cast<int64_t>(s_pos[e + j - eb0]) * up_stride + c);
 #pragma unroll
-      for (int j = 0; j < kSumBatch; ++j) {
-        if (b + j >= count) break;
-        const uint32_t k = __shfl_sync(dev::kFull, my_key, b + j);
-        while (r < k) finish_row();
-        if (on) {
+    for (int j = 0; j < kSumBatch; ++j) {
+      if (j >= count) break;
+      const uint32_t k = s_key[e + j - eb0];
+      while (r < k) finish_row();
+      if (on) {
 #pragma unroll
-          for (int v = 0; v < kV; ++v) acc[v] += dev::to_f32<T>(x[j].v[v]);
-        }
-        open = true;
+        for (int v = 0; v < kV; ++v) acc[v] += dev::to_f32<T>(x[j].v[v]);
       }
     }
   }
   while (r < r1) finish_row();
-  if (open && on) {
+  // Entries of row r1, which ends in a later warp.
+  const bool has_tail = e1 > e0 && s_key[e1 - 1 - eb0] == r1 && r1 < rows;
+  if (has_tail) {
 #pragma unroll
-    for (int j = 0; j < kV; ++j) tail[static_cast<size_t>(unit) * dim + c + j] = acc[j];
+    for (int j = 0; j < kV; ++j) s_tail[warp * kCols + lane * kV + j] = acc[j];
+  }
+  if (lane == 0) s_tail_row[warp] = has_tail ? r1 : kNoRow;
+  __syncthreads();
+  // A row that began in an earlier warp and ended in this one: that run of tails, then the head.
+  if (began_before && r0 < r1) {
+    int v = warp;
+    while (v > 0 && s_tail_row[v - 1] == r0) --v;
+    const bool beyond = v == 0 && before_key == r0;  // it began in an earlier block
+#pragma unroll 1
+    for (int j = lane; j < kCols; j += 32) {
+      if (col0 + j >= dim) break;
+      float s = 0.0f;
+      for (int u = v; u < warp; ++u) s += s_tail[u * kCols + j];
+      s += s_head[warp * kCols + j];
+      if (beyond)
+        head[static_cast<size_t>(blockIdx.x) * dim + col0 + j] = s;
+      else
+        grad[static_cast<int64_t>(r0) * grad_stride + col0 + j] = dev::from_f32<T>(s * scale);
+    }
+    if (beyond && lane == 0 && blockIdx.y == 0) head_row[blockIdx.x] = r0;
+  }
+  if (warp == 0) {
+    // Whether some warp of this block ends the row that was open before it.
+    const uint32_t end_row = static_cast<uint32_t>(b1 - eb1);
+    const uint32_t first_row = static_cast<uint32_t>(b0 - eb0);
+    const bool ends_open = before_key == first_row && first_row < end_row && first_row < rows;
+    if (!ends_open && lane == 0 && blockIdx.y == 0) head_row[blockIdx.x] = kNoRow;
+    // The row left open at the end of the block.
+    const uint32_t open_row = s_tail_row[kSumWarps - 1];
+    if (open_row != kNoRow) {
+      int v = kSumWarps - 1;
+      while (v > 0 && s_tail_row[v - 1] == open_row) --v;
+#pragma unroll 1
+      for (int j = lane; j < kCols; j += 32) {
+        if (col0 + j >= dim) break;
+        float s = 0.0f;
+        for (int u = v; u < kSumWarps; ++u) s += s_tail[u * kCols + j];
+        tail[static_cast<size_t>(blockIdx.x) * dim + col0 + j] = s;
+      }
+    }
   }
 }
 
-// Unit u's first row, when it began in an earlier unit and ends in u: the tails of the units from
-// the one it began in up to u - 1, in order, and head[u]. One warp per unit and 32 columns.
+// Block b's first row, where it began in an earlier block and ends in b: the tails of the blocks
+// from the one it began in up to b - 1, in order, and b's head.
 template <class T>
 __global__ void __launch_bounds__(kSumThreads)
-    join_rows_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t rows, uint32_t dim,
-                     uint32_t run, uint32_t units, float scale, T* __restrict__ grad,
-                     int64_t grad_stride, const float* __restrict__ head,
-                     const float* __restrict__ tail) {
-  const int lane = threadIdx.x & 31;
-  const uint32_t unit = (blockIdx.x * kSumThreads + threadIdx.x) >> 5;
-  if (unit == 0 || unit >= units) return;
-  const uint64_t total = static_cast<uint64_t>(rows) + n;
-  const uint64_t d0 = static_cast<uint64_t>(unit) * run;
-  const uint64_t d1 = d0 + run < total ? d0 + run : total;
-  const uint32_t e0 = entries_before(keys, n, d0, lane);
-  const uint32_t r = static_cast<uint32_t>(d0 - e0);
-  if (e0 == 0 || r >= rows || keys[e0 - 1] != r) return;
-  // The row ends here iff its row end, after its last entry, is one of this unit's places.
-  const uint32_t e1 = entries_before(keys, n, d1, lane);
-  if (static_cast<uint32_t>(d1 - e1) <= r) return;
-  uint32_t first = 0, hi = e0 - 1;  // the row's first entry: keys[first] == r
+    join_rows_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t dim, uint32_t run,
+                     float scale, T* __restrict__ grad, int64_t grad_stride,
+                     const float* __restrict__ head, const float* __restrict__ tail,
+                     const uint32_t* __restrict__ head_row) {
+  const uint32_t r = head_row[blockIdx.x];
+  if (r == kNoRow) return;
+  uint32_t first = 0, hi = n;  // the row's first entry
   while (first < hi) {
     const uint32_t mid = (first + hi) / 2;
     if (keys[mid] < r) first = mid + 1; else hi = mid;
   }
-  const uint32_t u0 = static_cast<uint32_t>((static_cast<uint64_t>(r) + first) / run);
-  for (uint32_t c = blockIdx.y * 32 + lane; c < dim; c += gridDim.y * 32) {
+  const uint32_t began =
+      static_cast<uint32_t>((static_cast<uint64_t>(r) + first) / (run * kSumWarps));
+  for (uint32_t c = blockIdx.y * kSumThreads + threadIdx.x; c < dim; c += gridDim.y * kSumThreads) {
     float s = 0.0f;
-    for (uint32_t u = u0; u < unit; ++u) s += tail[static_cast<size_t>(u) * dim + c];
-    s += head[static_cast<size_t>(unit) * dim + c];
+#pragma unroll 8
+    for (uint32_t u = began; u < blockIdx.x; ++u) s += tail[static_cast<size_t>(u) * dim + c];
+    s += head[static_cast<size_t>(blockIdx.x) * dim + c];
     grad[static_cast<int64_t>(r) * grad_stride + c] = dev::from_f32<T>(s * scale);
   }
 }
 
 struct GradPlan {
-  int passes, bits;         // radix passes and digit width
+  bool one_block;           // sorted by one block
+  int key_bits, passes, bits;  // width of a key, radix passes and digit width
   uint32_t tiles;           // sort tiles
-  uint32_t run, units;      // places per unit, units
-  size_t off_keys[2], off_pos[2], off_counts, off_totals, off_head, off_tail, bytes;
+  uint32_t run, blocks;     // places per warp, blocks
+  size_t off_keys[2], off_pos[2], off_counts, off_totals, off_head, off_tail, off_row, bytes;
 };
 
 GradPlan grad_plan(size_t n, size_t rows, size_t dim) {
   GradPlan p{};
-  int bits = 1;
-  while ((size_t{1} << bits) <= rows) ++bits;  // keys 0 .. rows
-  p.passes = static_cast<int>(ceil_div(bits, kMaxDigitBits));
-  p.bits = static_cast<int>(ceil_div(bits, p.passes));
+  p.key_bits = 1;
+  while ((size_t{1} << p.key_bits) <= rows) ++p.key_bits;  // keys 0 .. rows
+  p.one_block = n <= 8 * kBlockSortThreads;
+  p.passes = p.one_block ? 1 : static_cast<int>(ceil_div(p.key_bits, kMaxDigitBits));
+  p.bits = static_cast<int>(ceil_div(p.key_bits, p.passes));
   p.tiles = static_cast<uint32_t>(ceil_div(n, kSortTile));
-  p.run = static_cast<uint32_t>(std::max<size_t>(32, ceil_div(n + rows, 148 * 64)));
-  p.units = static_cast<uint32_t>(ceil_div(n + rows, p.run));
+  p.run = n + rows <= 148 * 8 * 32 * kSumWarps ? 32 : 64;
+  p.blocks = static_cast<uint32_t>(ceil_div(n + rows, p.run * kSumWarps));
   size_t o = 0;
   auto take = [&](size_t bytes) {
     const size_t at = o;
     o += (bytes + 255) / 256 * 256;
     return at;
   };
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < (p.one_block ? 1 : 2); ++i) {
     p.off_keys[i] = take(n * 4);
     p.off_pos[i] = take(n * 4);
   }
-  p.off_counts = take((size_t{1} << p.bits) * p.tiles * 4);
-  p.off_totals = take((size_t{1} << p.bits) * 4);
-  p.off_head = take(p.units * dim * 4);
-  p.off_tail = take(p.units * dim * 4);
+  if (!p.one_block) {
+    p.off_counts = take((size_t{1} << p.bits) * p.tiles * 4);
+    p.off_totals = take((size_t{1} << p.bits) * 4);
+  }
+  p.off_head = take(p.blocks * dim * 4);
+  p.off_tail = take(p.blocks * dim * 4);
+  p.off_row = take(p.blocks * 4);
   p.bytes = o;
   return p;
+}
+
+template <class Id, int kItems>
+void launch_block_sort(const GradPlan& p, const void* ids, uint32_t n, uint32_t rows,
+                       unsigned char* ws, cudaStream_t st) {
+  constexpr size_t smem =
+      kItems * kBlockSortThreads * 6 + kBlockSortWarps * (size_t{2} << kBlockDigitBits);
+  QV_CUDA(cudaFuncSetAttribute(block_sort_kernel<Id, kItems>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(smem)));
+  block_sort_kernel<Id, kItems><<<1, kBlockSortThreads, smem, st>>>(
+      ids, n, rows, p.key_bits, reinterpret_cast<uint32_t*>(ws + p.off_keys[0]),
+      reinterpret_cast<uint32_t*>(ws + p.off_pos[0]));
+  check_launch("block_sort_kernel");
 }
 
 template <class Id>
 int sort_ids(const GradPlan& p, const void* ids, uint32_t n, uint32_t rows, unsigned char* ws,
              cudaStream_t st) {
+  if (p.one_block) {
+    if (n <= kBlockSortThreads)
+      launch_block_sort<Id, 1>(p, ids, n, rows, ws, st);
+    else
+      launch_block_sort<Id, 8>(p, ids, n, rows, ws, st);
+    return 0;
+  }
   uint32_t* counts = reinterpret_cast<uint32_t*>(ws + p.off_counts);
   uint32_t* totals = reinterpret_cast<uint32_t*>(ws + p.off_totals);
   const int bins = 1 << p.bits;
@@ -431,17 +584,18 @@ void launch_sums(const GradPlan& p, int which, const void* up, size_t up_stride,
   const uint32_t* pos = reinterpret_cast<uint32_t*>(ws + p.off_pos[which]);
   float* head = reinterpret_cast<float*>(ws + p.off_head);
   float* tail = reinterpret_cast<float*>(ws + p.off_tail);
-  const unsigned blocks = static_cast<unsigned>(ceil_div(p.units, kSumThreads / 32));
+  uint32_t* head_row = reinterpret_cast<uint32_t*>(ws + p.off_row);
+  const size_t smem = 2 * kSumWarps * 32 * kV * sizeof(float) + 2 * p.run * kSumWarps * 4;
   segment_sum_kernel<T, kV>
-      <<<dim3(blocks, static_cast<unsigned>(ceil_div(dim, 32 * kV))), kSumThreads, 0, st>>>(
+      <<<dim3(p.blocks, static_cast<unsigned>(ceil_div(dim, 32 * kV))), kSumThreads, smem, st>>>(
           static_cast<const T*>(up), static_cast<int64_t>(up_stride), keys, pos, n, rows, dim,
-          p.run, p.units, scale, static_cast<T*>(grad), static_cast<int64_t>(grad_stride), head,
-          tail);
+          p.run, scale, static_cast<T*>(grad), static_cast<int64_t>(grad_stride), head, tail,
+          head_row);
   check_launch("segment_sum_kernel");
-  join_rows_kernel<T>
-      <<<dim3(blocks, static_cast<unsigned>(std::min<size_t>(ceil_div(dim, 32), 65535))),
-         kSumThreads, 0, st>>>(keys, n, rows, dim, p.run, p.units, scale, static_cast<T*>(grad),
-                               static_cast<int64_t>(grad_stride), head, tail);
+  join_rows_kernel<T><<<dim3(p.blocks, static_cast<unsigned>(ceil_div(dim, kSumThreads))),
+                        kSumThreads, 0, st>>>(keys, n, dim, p.run, scale, static_cast<T*>(grad),
+                                              static_cast<int64_t>(grad_stride), head, tail,
+                                              head_row);
   check_launch("join_rows_kernel");
 }
 

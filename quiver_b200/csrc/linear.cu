@@ -34,51 +34,101 @@ __device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
   p[2] = __float2bfloat16_rn(r - __bfloat162float(p[1]));
 }
 
-__device__ __forceinline__ void put_operand(float x, float, __nv_bfloat16* dst, size_t plane,
-                                            size_t at) {
-  __nv_bfloat16 p[3];
-  split3(x, p);
-  dst[at] = p[0];
-  dst[plane + at] = p[1];
-  dst[2 * plane + at] = p[2];
-}
-template <class T>
-__device__ __forceinline__ void put_operand(float x, T, T* dst, size_t, size_t at) {
-  dst[at] = dev::from_f32<T>(x);
-}
-// The element type the tensor core multiplies for values of type T.
+// The element type the tensor core multiplies for values of type T, and its planes.
 template <class T>
 struct Operand {
   using type = T;
+  static constexpr int kPlanes = 1;
 };
 template <>
 struct Operand<float> {
   using type = __nv_bfloat16;
+  static constexpr int kPlanes = 3;
 };
 
-template <class T>
-__global__ void __launch_bounds__(256)
-    pack_kernel(const T* __restrict__ src, size_t rows, uint32_t cols, int64_t stride,
-                typename Operand<T>::type* __restrict__ dst, uint32_t ld) {
-  const size_t plane = rows * ld;
-  for (size_t r = blockIdx.x; r < rows; r += gridDim.x)
-    for (uint32_t c = threadIdx.x + blockIdx.y * 256; c < cols; c += 256 * gridDim.y)
-      put_operand(dev::to_f32<T>(src[static_cast<int64_t>(r) * stride + c]), T{}, dst, plane,
-                  r * ld + c);
+// Writes kV consecutive values as an operand at dst[at], planes `plane` elements apart.
+template <class T, int kV>
+__device__ __forceinline__ void put_operand(const float (&x)[kV],
+                                            typename Operand<T>::type* __restrict__ dst,
+                                            int64_t plane, int64_t at) {
+  if constexpr (sizeof(T) == 4) {
+    Pack<__nv_bfloat16, kV> y[3];
+#pragma unroll
+    for (int j = 0; j < kV; ++j) {
+      __nv_bfloat16 p[3];
+      split3(x[j], p);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) y[i].v[j] = p[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) dev::store_pack<__nv_bfloat16, kV>(dst + i * plane + at, y[i]);
+  } else {
+    Pack<T, kV> y;
+#pragma unroll
+    for (int j = 0; j < kV; ++j) y.v[j] = dev::from_f32<T>(x[j]);
+    dev::store_pack<T, kV>(dst + at, y);
+  }
+}
+
+// One matrix to pack: rows x cols values, written with rows of ld (a multiple of 8) elements.
+struct PackJob {
+  const void* src;
+  void* dst;
+  int64_t rows, cols, stride, ld;
+};
+
+// Up to two matrices in one launch (blockIdx.y). Bound by memory: every thread moves kV values of
+// kPackRows rows at a time.
+constexpr int kPackRows = 4;
+template <class T, int kV>
+__global__ void __launch_bounds__(256) pack_kernel(const PackJob j0, const PackJob j1) {
+  const PackJob& j = blockIdx.y == 0 ? j0 : j1;
+  using O = typename Operand<T>::type;
+  const T* src = static_cast<const T*>(j.src);
+  O* dst = static_cast<O*>(j.dst);
+  const uint32_t per_row = static_cast<uint32_t>((j.cols + kV - 1) / kV);
+  const int64_t plane = j.rows * j.ld;
+  const int64_t groups = (j.rows + kPackRows - 1) / kPackRows;
+  const int64_t total = groups * per_row;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const int64_t r0 = i / per_row * kPackRows;
+    const int64_t c = (i - i / per_row * per_row) * kV;
+    Pack<T, kV> x[kPackRows];
+#pragma unroll
+    for (int u = 0; u < kPackRows; ++u)
+      if (r0 + u < j.rows) x[u] = dev::load_pack<T, kV>(src + (r0 + u) * j.stride + c);
+#pragma unroll
+    for (int u = 0; u < kPackRows; ++u) {
+      if (r0 + u >= j.rows) break;
+      float f[kV];
+#pragma unroll
+      for (int v = 0; v < kV; ++v) f[v] = dev::to_f32<T>(x[u].v[v]);
+      put_operand<T, kV>(f, dst, plane, (r0 + u) * j.ld + c);
+    }
+  }
 }
 
 // ---- the product kernel -----------------------------------------------------------------------------
+// Warp-specialized and persistent: one thread feeds 128-byte-swizzled tiles of A and B through a
+// ring of shared-memory stages with TMA, one thread issues the MMAs into one of two accumulators
+// in tensor memory, and eight warps finish the other accumulator's elements meanwhile.
+//
+// Large products run in CTA pairs (tcgen05 cta_group::2): 256 x 256 tiles, each CTA loading its
+// 128 rows of A and half of B. A CTA by itself would have to load 384 rows of operands for
+// 128 x 256 results, 96 bytes per SM and cycle at full MMA rate; the pair loads 64.
 
-constexpr int kBM = 128, kBK = 64;
+constexpr int kBM = 128, kBK = 64;  // rows of A per CTA, k per stage
 constexpr int kEpilogueWarps = 8;
 constexpr int kProductThreads = 128 + 32 * kEpilogueWarps;  // producer, MMA, 2 idle, epilogue
 
-template <int kBN>
+template <int kBN, bool kPair>
 struct Tile {
+  static constexpr int kM = kPair ? 2 * kBM : kBM;           // rows of a tile
+  static constexpr int kBRows = kPair ? kBN / 2 : kBN;       // rows of B loaded by one CTA
   static constexpr int kABytes = kBM * kBK * 2;
-  static constexpr int kBBytes = kBN * kBK * 2;
+  static constexpr int kBBytes = kBRows * kBK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = kBN == 256 ? 4 : (kBN == 128 ? 6 : 8);
+  static constexpr int kStages = kStageBytes >= 32768 ? 6 : 8;
   static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + 1024 + 256;
 };
 
@@ -99,13 +149,22 @@ struct ProductArgs {
   uint64_t drain_ns;
 };
 
+// TMA loads; in a pair the bytes are counted on the leader's barrier (a shared::cluster address).
+template <bool kPair>
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y,
                                             int z, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
-      "%3, %4}], [%5];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
-      : "memory");
+  if constexpr (kPair)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
+        "{%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
 }
 // 128-byte swizzled operand tiles. Along k: 64-element rows, 8-row groups 1024 bytes apart.
 // Across k: [64 k][64 m-or-n] blocks of 8 KB (the leading offset), 8-k groups 1024 bytes apart.
@@ -114,14 +173,23 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t across)
          (static_cast<uint64_t>(across ? 8192 >> 4 : 1) << 16) | (64ull << 32) | (1ull << 46) |
          (2ull << 61);
 }
+template <bool kPair>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                         uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
+  if constexpr (kPair)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
@@ -138,23 +206,28 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "memory");
 }
 
-template <class T, int kBN>
+template <class T, int kBN, bool kPair>
 __global__ void __launch_bounds__(kProductThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a,
                    const __grid_constant__ CUtensorMap map_b, const ProductArgs a) {
-  using S = Tile<kBN>;
+  using S = Tile<kBN, kPair>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* tiles = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + S::kStages * S::kStageBytes);
-  // full[stage], empty[stage], acc_full[2], acc_empty[2], drain
+  // full[stage], empty[stage], acc_full[2], acc_empty[2], drain. In a pair the leader's full and
+  // acc_empty barriers stand for both CTAs; empty and acc_full are signalled in each.
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   __shared__ int s_consumed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = kPair ? tc::cluster_ctarank() : 0;
+  const bool leader = rank == 0;
   auto bar = [&](int i) { return tc::smem_u32(bars + i); };
+  auto lbar = [&](int i) { return kPair ? tc::mapa_shared(bar(i), 0) : bar(i); };
   constexpr int FULL = 0, EMPTY = S::kStages, ACC_FULL = 2 * S::kStages, ACC_EMPTY = ACC_FULL + 2,
                 DRAIN = ACC_EMPTY + 2;
+  static_assert((DRAIN + 1) * 8 <= 256, "the barriers fit behind the stages");
   if (threadIdx.x == 0) {
     s_abort = 0;
     s_consumed = 0;
@@ -164,28 +237,42 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       tc::mbar_init(bar(ACC_FULL + b), 1);
-      tc::mbar_init(bar(ACC_EMPTY + b), kEpilogueWarps);
+      tc::mbar_init(bar(ACC_EMPTY + b), (kPair ? 2 : 1) * kEpilogueWarps);
     }
     tc::mbar_init(bar(DRAIN), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     tc::smem_u32(&s_tmem)),
-                 "r"(2 * kBN));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if constexpr (kPair) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       tc::smem_u32(&s_tmem)),
+                   "r"(2 * kBN));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       tc::smem_u32(&s_tmem)),
+                   "r"(2 * kBN));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
   }
   tc::tc_fence_before();
   __syncthreads();
+  if constexpr (kPair) tc::cluster_sync();  // both CTAs' barriers exist before either uses them
   tc::tc_fence_after();
   const uint32_t tmem = s_tmem;
   volatile int* abort_flag = &s_abort;
-  int err_sink = 0;  // mbar_wait's error word: an abort shows in the output (NaN)
+  // Bounded wait; false on timeout or abort, after which the CTA's remaining results are NaN.
   auto wait = [&](uint32_t b, uint32_t parity) {
-    if (tc::mbar_test(b, parity)) return true;
+    auto test = [&] {
+      return kPair ? tc::mbar_test_cluster(b, parity) : tc::mbar_test(b, parity);
+    };
+    auto sleep_test = [&] {
+      return kPair ? tc::mbar_sleep_test_cluster(b, parity) : tc::mbar_sleep_test(b, parity);
+    };
+    if (test()) return true;
     const long long t0 = clock64();
     for (;;) {
-      if (tc::mbar_sleep_test(b, parity)) return true;
+      if (sleep_test()) return true;
       if (*abort_flag) return false;
       if (clock64() - t0 > a.wait_cycles) {
         *abort_flag = 1;
@@ -193,8 +280,9 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       }
     }
   };
-  (void)err_sink;
   const int units = a.tiles_m * a.tiles_n * a.splits;
+  const int worker = kPair ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
+  const int workers = kPair ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
   // Unit u: split u / (tiles), tile row / column of the rest, columns fastest (a wave's CTAs share
   // rows of A and all of B in L2).
   auto coords = [&](int u, int& split, int& tm, int& tn) {
@@ -211,53 +299,76 @@ __global__ void __launch_bounds__(kProductThreads, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      int issued = 0;
+      int issued = 0, s = 0;
+      uint32_t phase = 1;
       bool ok = true;
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      for (int u = worker; u < units && ok; u += workers) {
         int split, tm, tn, b0, b1;
         coords(u, split, tm, tn);
         block_range(split, b0, b1);
+        const int row_a = tm * S::kM + static_cast<int>(rank) * kBM;
+        const int row_b = tn * kBN + static_cast<int>(rank) * S::kBRows;
         for (int p = 0; p < a.pairs && ok; ++p) {
           const int pa = a.pairs == 1 ? 0 : kPairA[p], pb = a.pairs == 1 ? 0 : kPairB[p];
           for (int kb = b0; kb < b1; ++kb) {
-            const int s = issued % S::kStages;
-            if (!wait(bar(EMPTY + s), ((issued / S::kStages) & 1) ^ 1)) {
+            if (!wait(bar(EMPTY + s), phase)) {
               ok = false;
               break;
             }
-            tc::mbar_expect_tx(bar(FULL + s), S::kStageBytes);
+            if (leader) tc::mbar_expect_tx(bar(FULL + s), (kPair ? 2 : 1) * S::kStageBytes);
+            const uint32_t full = lbar(FULL + s);
             const uint32_t da = tc::smem_u32(tiles + s * S::kStageBytes);
             const uint32_t db = da + S::kABytes;
             if (a.a_mn) {
+#pragma unroll
               for (int c = 0; c < kBM / 64; ++c)
-                tma_load_3d(da + c * 8192, &map_a, tm * kBM + c * 64, kb * kBK, pa, bar(FULL + s));
+                tma_load_3d<kPair>(da + c * 8192, &map_a, row_a + c * 64, kb * kBK, pa, full);
             } else {
-              tma_load_3d(da, &map_a, kb * kBK, tm * kBM, pa, bar(FULL + s));
+              tma_load_3d<kPair>(da, &map_a, kb * kBK, row_a, pa, full);
             }
             if (a.b_mn) {
-              for (int c = 0; c < kBN / 64; ++c)
-                tma_load_3d(db + c * 8192, &map_b, tn * kBN + c * 64, kb * kBK, pb, bar(FULL + s));
+#pragma unroll
+              for (int c = 0; c < S::kBRows / 64; ++c)
+                tma_load_3d<kPair>(db + c * 8192, &map_b, row_b + c * 64, kb * kBK, pb, full);
             } else {
-              tma_load_3d(db, &map_b, kb * kBK, tn * kBN, pb, bar(FULL + s));
+              tma_load_3d<kPair>(db, &map_b, kb * kBK, row_b, pb, full);
             }
             ++issued;
+            if (++s == S::kStages) {
+              s = 0;
+              phase ^= 1;
+            }
           }
         }
       }
-      if (*abort_flag) {  // wait (bounded) for the copies that the MMA warp did not consume
+      if (*abort_flag) {
+        // Copies in flight must land before the CTA leaves. A pair's are counted on the leader's
+        // barriers, which the peer cannot poll: it waits out the bound, far longer than any copy.
         const uint64_t t0 = tc::gtimer();
-        for (int f = s_consumed; f < issued; ++f)
-          while (!tc::mbar_test(bar(FULL + f % S::kStages), (f / S::kStages) & 1) &&
-                 tc::gtimer() - t0 < a.drain_ns) {
+        if constexpr (kPair) {
+          while (tc::gtimer() - t0 < a.drain_ns) {
           }
+        } else {
+          for (int f = s_consumed; f < issued; ++f)
+            while (!tc::mbar_test(bar(FULL + f % S::kStages), (f / S::kStages) & 1) &&
+                   tc::gtimer() - t0 < a.drain_ns) {
+            }
+        }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int taken = 0, t = 0;
+    if (lane == 0 && leader) {  // in a pair the leader issues for both CTAs
+      int taken = 0, t = 0, s = 0;
+      uint32_t phase = 0;
       bool ok = true;
       const uint32_t a_step = a.a_mn ? 2048 >> 4 : 32 >> 4, b_step = a.b_mn ? 2048 >> 4 : 32 >> 4;
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++t) {
+      auto commit = [&](int i) {  // signals barrier i (of both CTAs) once the MMAs so far are done
+        if constexpr (kPair)
+          tc::umma_commit_pair_mc(bar(i), 0x3);
+        else
+          tc::umma_commit(bar(i));
+      };
+      for (int u = worker; u < units && ok; u += workers, ++t) {
         int split, tm, tn, b0, b1;
         coords(u, split, tm, tn);
         block_range(split, b0, b1);
@@ -267,8 +378,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         const uint32_t d = tmem + slot * kBN;
         const int blocks = (b1 - b0) * a.pairs;
         for (int i = 0; i < blocks; ++i) {
-          const int s = taken % S::kStages;
-          if (!wait(bar(FULL + s), (taken / S::kStages) & 1)) {
+          if (!wait(bar(FULL + s), phase)) {
             ok = false;
             break;
           }
@@ -279,14 +389,21 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           const uint64_t bd = operand_desc(da + S::kABytes, a.b_mn);
 #pragma unroll
           for (int q = 0; q < kBK / 16; ++q)
-            mma_f16(d, ad + q * a_step, bd + q * b_step, a.idesc, (i | q) != 0);
-          tc::umma_commit(bar(EMPTY + s));
+            mma_f16<kPair>(d, ad + q * a_step, bd + q * b_step, a.idesc, (i | q) != 0);
+          commit(EMPTY + s);
+          if (++s == S::kStages) {
+            s = 0;
+            phase ^= 1;
+          }
         }
         if (!ok) break;
-        tc::umma_commit(bar(ACC_FULL + slot));
+        commit(ACC_FULL + slot);
       }
       if (*abort_flag) {  // wait (bounded) for the MMAs in flight before their memory goes
-        tc::umma_commit(bar(DRAIN));
+        if constexpr (kPair)
+          tc::umma_commit_pair_mc(bar(DRAIN), 0x1);
+        else
+          tc::umma_commit(bar(DRAIN));
         const uint64_t t0 = tc::gtimer();
         while (!tc::mbar_test(bar(DRAIN), 0) && tc::gtimer() - t0 < a.drain_ns) {
         }
@@ -294,16 +411,17 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     }
   } else if (warp >= 4) {
     const int quarter = warp & 3;            // TMEM lanes this warp may read
-    const int half = (warp - 4) >> 2;        // which columns of each 64 it takes
+    const int half = (warp - 4) >> 2;        // which 32 columns of each 64 it takes
     int t = 0;
-    for (int u = blockIdx.x; u < units; u += gridDim.x, ++t) {
+    for (int u = worker; u < units; u += workers, ++t) {
       int split, tm, tn;
       coords(u, split, tm, tn);
       const int slot = t & 1;
       const bool ok = wait(bar(ACC_FULL + slot), (t >> 1) & 1);
       __syncwarp();
       tc::tc_fence_after();
-      const int64_t row = static_cast<int64_t>(tm) * kBM + quarter * 32 + lane;
+      const int64_t row =
+          static_cast<int64_t>(tm) * S::kM + rank * kBM + quarter * 32 + lane;
 #pragma unroll 1
       for (int c = half * 32; c < kBN; c += 64) {
         const int64_t col = static_cast<int64_t>(tn) * kBN + c;
@@ -335,15 +453,26 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       }
       tc::tc_fence_before();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(bar(ACC_EMPTY + slot));
+      if (lane == 0) {
+        if constexpr (kPair)
+          tc::mbar_arrive_cluster(lbar(ACC_EMPTY + slot));
+        else
+          tc::mbar_arrive(bar(ACC_EMPTY + slot));
+      }
     }
   }
   tc::tc_fence_before();
   __syncthreads();
+  // A CTA of a pair stays until the other is done with its barriers, tiles and accumulators.
+  if constexpr (kPair) tc::cluster_sync();
   if (warp == 1) {
     tc::tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                 "r"(2 * kBN));
+    if constexpr (kPair)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                   "r"(2 * kBN));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                   "r"(2 * kBN));
   }
 }
 
@@ -410,34 +539,86 @@ __global__ void __launch_bounds__(128)
 // ---- dz and the bias gradient ----------------------------------------------------------------------
 
 // dz = dy * act'(z), rounded to the operand type (float32: three planes), and float32 column sums
-// of the unrounded dz over this block's rows. Threads walk down columns; blocks are row ranges.
-template <class T, bool kStore>
-__global__ void __launch_bounds__(256)
+// of the unrounded dz over this block's rows. A block takes 32 * kV columns and a range of rows:
+// warp w walks rows w, w + 8, .. of it, and the warps' sums are added in order at the end, so the
+// sums have a fixed order. Bound by memory: dy and z read, dz written.
+constexpr int kDzWarps = 8, kDzRows = 4;  // rows in flight per warp
+
+template <class T, int kV, bool kStore, int kAct>
+__global__ void __launch_bounds__(32 * kDzWarps)
     dz_kernel(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ z,
-              int64_t z_stride, int act, int64_t m, int64_t n, int64_t rows_per_block,
+              int64_t z_stride, int64_t m, int64_t n, int64_t rows_per_block,
               typename Operand<T>::type* __restrict__ dz, int64_t ld, float* __restrict__ sums) {
-  const int64_t col = blockIdx.y * 256ll + threadIdx.x;
-  if (col >= n) return;
-  const int64_t r0 = blockIdx.x * rows_per_block, r1 = min(m, r0 + rows_per_block);
-  float s = 0.0f;
-  for (int64_t r = r0; r < r1; ++r) {
-    float g = dev::to_f32<T>(dy[r * dy_stride + col]);
-    // rounded before the sum in both variants, so that dbias does not depend on which runs
-    if (act != QV_ACT_NONE) g = __fmul_rn(g, act_grad<T>(act, dev::to_f32<T>(z[r * z_stride + col])));
-    s += g;
-    if (kStore) put_operand(g, T{}, dz, static_cast<size_t>(m * ld), static_cast<size_t>(r * ld + col));
+  __shared__ float part[kDzWarps][32 * kV];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t col = (blockIdx.y * 32ll + lane) * kV;
+  const int64_t r1 = min(m, (blockIdx.x + 1) * rows_per_block);
+  float s[kV];
+#pragma unroll
+  for (int j = 0; j < kV; ++j) s[j] = 0.0f;
+  if (col < n) {
+    for (int64_t r = blockIdx.x * rows_per_block + warp; r < r1; r += kDzWarps * kDzRows) {
+      Pack<T, kV> g[kDzRows], x[kDzRows];
+#pragma unroll
+      for (int u = 0; u < kDzRows; ++u) {
+        const int64_t row = r + u * kDzWarps;
+        if (row >= r1) break;
+        g[u] = dev::load_pack<T, kV>(dy + row * dy_stride + col);
+        if (kAct != QV_ACT_NONE) x[u] = dev::load_pack<T, kV>(z + row * z_stride + col);
+      }
+#pragma unroll
+      for (int u = 0; u < kDzRows; ++u) {
+        const int64_t row = r + u * kDzWarps;
+        if (row >= r1) break;
+        float d[kV];
+#pragma unroll
+        for (int j = 0; j < kV; ++j) {
+          d[j] = dev::to_f32<T>(g[u].v[j]);
+          // rounded before the sum in every variant, so that dbias does not depend on which runs
+          if (kAct != QV_ACT_NONE)
+            d[j] = __fmul_rn(d[j], act_grad<T>(kAct, dev::to_f32<T>(x[u].v[j])));
+          s[j] += d[j];
+        }
+        if (kStore) put_operand<T, kV>(d, dz, m * ld, row * ld + col);
+      }
+    }
   }
-  if (sums != nullptr) sums[blockIdx.x * n + col] = s;
+  if (sums == nullptr) return;
+#pragma unroll
+  for (int j = 0; j < kV; ++j) part[warp][lane * kV + j] = s[j];
+  __syncthreads();
+  for (int c = threadIdx.x; c < 32 * kV; c += 32 * kDzWarps) {
+    const int64_t out = blockIdx.y * 32ll * kV + c;
+    if (out >= n) continue;
+    float t = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kDzWarps; ++w) t += part[w][c];
+    sums[blockIdx.x * n + out] = t;
+  }
 }
 
+// Adds the row ranges' sums: 32 columns a block, each warp a run of ranges, then the warps in order.
 template <class T>
 __global__ void __launch_bounds__(256)
-    join_sums_kernel(const float* __restrict__ sums, int64_t blocks, int64_t n, T* __restrict__ db) {
-  const int64_t col = blockIdx.x * 256ll + threadIdx.x;
-  if (col >= n) return;
+    join_sums_kernel(const float* __restrict__ sums, int blocks, int64_t n, T* __restrict__ db) {
+  __shared__ float part[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t col = blockIdx.x * 32ll + lane;
+  const int per = (blocks + 7) / 8;
+  const int b1 = min(blocks, (warp + 1) * per);
   float s = 0.0f;
-  for (int64_t b = 0; b < blocks; ++b) s += sums[b * n + col];
-  db[col] = dev::from_f32<T>(s);
+  if (col < n) {
+#pragma unroll 8
+    for (int b = warp * per; b < b1; ++b) s += sums[b * n + col];
+  }
+  part[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && col < n) {
+    float t = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) t += part[w][lane];
+    db[col] = dev::from_f32<T>(t);
+  }
 }
 
 // ---- host side ----------------------------------------------------------------------------------------
@@ -490,29 +671,35 @@ CUtensorMap operand_map(const Stored& s, uint32_t box_outer) {
 
 struct ProductPlan {
   int bn = 128, splits = 1, blocks_per_split = 1, k_blocks = 1;
+  bool pair = false;
   size_t partial_bytes = 0;
 };
 
-// Tile width and split of k with the least estimated time. In cycles: a 64-wide block of k takes
-// the larger of the MMAs and the copies into shared memory, a tile's results about 12 cycles a
-// column, and the splits are written, read and joined in a launch of their own.
+// Tile and split of k with the least estimated time. In cycles: a 64-wide block of k takes the
+// larger of the MMAs and the copies into shared memory, a tile's results about 10 cycles a column
+// (hidden behind the next tile's blocks when there is one), and the splits are written, read and
+// joined in a launch of their own.
 ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int pairs, int sms) {
   ProductPlan best;
   double best_t = 1e300;
   const int64_t kb = std::max<int64_t>(1, static_cast<int64_t>(ceil_div(k, kBK)));
   for (int bn : {64, 128, 256}) {
-    const double tiles = static_cast<double>(ceil_div(m, kBM)) * ceil_div(n, bn);
-    const double per_block = bn == 256 ? 560 : (bn == 128 ? 330 : 230);
+    const bool pair = bn == 256;
+    const double tiles = static_cast<double>(ceil_div(m, pair ? 2 * kBM : kBM)) * ceil_div(n, bn);
+    const int workers = pair ? sms / 2 : sms;
+    const double per_block = bn == 256 ? 540 : (bn == 128 ? 400 : 280);
     for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-      if (s > 1 && (s > kb || tiles * s > 2.0 * sms)) break;
+      if (s > 1 && (s > kb || tiles * s > 2.0 * workers)) break;
       const int64_t per = static_cast<int64_t>(ceil_div(kb, s));
       const int64_t used = static_cast<int64_t>(ceil_div(kb, per));
-      const double waves = std::ceil(tiles * used / sms);
-      double t = waves * per * pairs * per_block + 12.0 * bn + 1500;
+      const double waves = std::ceil(tiles * used / workers);
+      const double block_t = static_cast<double>(per) * pairs * per_block;
+      double t = waves * std::max(block_t, 10.0 * bn) + 10.0 * bn + 1500;
       if (used > 1) t += 4000 + 8.0 * m * n * used / 3000.0;
       if (t < best_t) {
         best_t = t;
         best.bn = bn;
+        best.pair = pair;
         best.splits = static_cast<int>(used);
         best.blocks_per_split = static_cast<int>(per);
         best.k_blocks = static_cast<int>(kb);
@@ -524,22 +711,37 @@ ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int pairs, int sms) {
   return best;
 }
 
-template <class T, int kBN>
+template <class T, int kBN, bool kPair>
 void launch_product(const ProductArgs& a, const Stored& A, const Stored& B, int sms,
                     cudaStream_t st) {
+  using S = Tile<kBN, kPair>;
   const CUtensorMap ma = operand_map(A, a.a_mn ? kBK : kBM);
-  const CUtensorMap mb = operand_map(B, a.b_mn ? kBK : kBN);
+  const CUtensorMap mb = operand_map(B, a.b_mn ? kBK : S::kBRows);
   static std::once_flag once[16];
   int device = 0;
   QV_CUDA(cudaGetDevice(&device));
   std::call_once(once[device & 15], [&] {
-    QV_CUDA(cudaFuncSetAttribute(product_kernel<T, kBN>,
+    QV_CUDA(cudaFuncSetAttribute(product_kernel<T, kBN, kPair>,
                                  cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 static_cast<int>(Tile<kBN>::kSmem)));
+                                 static_cast<int>(S::kSmem)));
   });
   const int units = a.tiles_m * a.tiles_n * a.splits;
-  product_kernel<T, kBN>
-      <<<std::min(units, sms), kProductThreads, Tile<kBN>::kSmem, st>>>(ma, mb, a);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(kPair ? 2 * std::min(units, sms / 2)
+                                                 : std::min(units, sms)));
+  cfg.blockDim = dim3(kProductThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  if (kPair) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  QV_CUDA(cudaLaunchKernelEx(&cfg, product_kernel<T, kBN, kPair>, ma, mb, a));
   check_launch("product_kernel");
 }
 
@@ -554,26 +756,26 @@ void product(const Stored& A, bool a_mn, const Stored& B, bool b_mn, int64_t m, 
   a.k = k;
   a.pairs = std::is_same_v<T, float> ? 6 : 1;
   a.k_blocks = plan.k_blocks;
-  a.tiles_m = static_cast<int>(ceil_div(m, kBM));
+  a.tiles_m = static_cast<int>(ceil_div(m, plan.pair ? 2 * kBM : kBM));
   a.tiles_n = static_cast<int>(ceil_div(n, plan.bn));
   a.splits = plan.splits;
   a.blocks_per_split = plan.blocks_per_split;
   const uint32_t fmt = A.bf16 ? 1 : 0;
   a.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(a_mn) << 15) |
             (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(plan.bn >> 3) << 17) |
-            (static_cast<uint32_t>(kBM >> 4) << 24);
+            (static_cast<uint32_t>((plan.pair ? 2 * kBM : kBM) >> 4) << 24);
   a.a_mn = a_mn;
   a.b_mn = b_mn;
   a.ep = ep;
   a.partial = static_cast<float*>(partial);
   a.wait_cycles = tc::wait_limit_cycles();
   a.drain_ns = tc::drain_limit_ns();
-  if (plan.bn == 256)
-    launch_product<T, 256>(a, A, B, sms, st);
+  if (plan.pair)
+    launch_product<T, 256, true>(a, A, B, sms, st);
   else if (plan.bn == 128)
-    launch_product<T, 128>(a, A, B, sms, st);
+    launch_product<T, 128, false>(a, A, B, sms, st);
   else
-    launch_product<T, 64>(a, A, B, sms, st);
+    launch_product<T, 64, false>(a, A, B, sms, st);
   if (plan.splits > 1) {
     const size_t items = static_cast<size_t>(m) * ceil_div(n, 16);
     join_splits_kernel<T>
@@ -593,41 +795,59 @@ size_t packed_bytes(uint32_t dtype, size_t rows, size_t cols) {
   return (rows * packed_ld(cols) * 2 * (dtype == QV_DTYPE_F32 ? 3 : 1) + 255) / 256 * 256;
 }
 
+// The operands of one call that have to be packed first, collected and packed in one launch.
 template <class T>
-Stored pack_rows(const void* src, size_t rows, size_t cols, size_t stride, void* dst,
-                 cudaStream_t st) {
-  Stored s;
-  s.p = dst;
-  s.inner = static_cast<int64_t>(cols);
-  s.outer = static_cast<int64_t>(rows);
-  s.ld = static_cast<int64_t>(packed_ld(cols));
-  s.planes = std::is_same_v<T, float> ? 3 : 1;
-  s.bf16 = !std::is_same_v<T, __half>;
-  pack_kernel<T><<<dim3(static_cast<unsigned>(std::min<size_t>(rows, 148 * 32)),
-                        static_cast<unsigned>(std::min<size_t>(ceil_div(cols, 256), 64))),
-                   256, 0, st>>>(static_cast<const T*>(src), rows, static_cast<uint32_t>(cols),
-                                 static_cast<int64_t>(stride),
-                                 static_cast<typename Operand<T>::type*>(dst),
-                                 static_cast<uint32_t>(s.ld));
-  check_launch("pack_kernel");
-  return s;
-}
-template <class T>
-Stored stored_rows(uint32_t dtype, const void* src, size_t rows, size_t cols, size_t stride,
-                   unsigned char*& ws, cudaStream_t st) {
-  if (in_place(dtype, src, rows, stride)) {
+class Packer {
+ public:
+  Packer(uint32_t dtype, unsigned char* ws) : dtype_(dtype), ws_(ws) {}
+  Stored rows(const void* src, size_t rows, size_t cols, size_t stride) {
     Stored s;
-    s.p = src;
     s.inner = static_cast<int64_t>(cols);
     s.outer = static_cast<int64_t>(rows);
-    s.ld = static_cast<int64_t>(stride);
-    s.bf16 = dtype == QV_DTYPE_BF16;
+    s.bf16 = !std::is_same_v<T, __half>;
+    if (in_place(dtype_, src, rows, stride)) {
+      s.p = src;
+      s.ld = static_cast<int64_t>(stride);
+      return s;
+    }
+    s.p = ws_;
+    s.ld = static_cast<int64_t>(packed_ld(cols));
+    s.planes = Operand<T>::kPlanes;
+    jobs_[count_++] = PackJob{src, ws_, s.outer, s.inner, static_cast<int64_t>(stride), s.ld};
+    const size_t e = sizeof(T);
+    align_ = std::min(align_, common_align({reinterpret_cast<uintptr_t>(src),
+                                            rows > 1 ? stride * e : 0, cols * e}));
+    ws_ += packed_bytes(dtype_, rows, cols);
     return s;
   }
-  void* dst = ws;
-  ws += packed_bytes(dtype, rows, cols);
-  return pack_rows<T>(src, rows, cols, stride, dst, st);
-}
+  // Packs what was collected; returns the workspace behind it.
+  unsigned char* run(cudaStream_t st) {
+    if (count_ == 0) return ws_;
+    if (align_ >= 16)
+      launch<16 / sizeof(T)>(st);
+    else if (align_ == 8)
+      launch<8 / sizeof(T)>(st);
+    else
+      launch<1>(st);
+    count_ = 0;
+    return ws_;
+  }
+
+ private:
+  template <int kV>
+  void launch(cudaStream_t st) {
+    size_t most = 0;
+    for (int i = 0; i < count_; ++i)
+      most = std::max(most, ceil_div(jobs_[i].rows, kPackRows) * ceil_div(jobs_[i].cols, kV));
+    const unsigned blocks = static_cast<unsigned>(std::min<size_t>(ceil_div(most, 256), 148 * 8));
+    pack_kernel<T, kV><<<dim3(blocks, count_), 256, 0, st>>>(jobs_[0], jobs_[count_ - 1]);
+    check_launch("pack_kernel");
+  }
+  uint32_t dtype_;
+  unsigned char* ws_;
+  PackJob jobs_[2];
+  int count_ = 0, align_ = 16;
+};
 
 constexpr size_t kMaxFewRows = 8;
 constexpr size_t kMaxDim = 65536;
@@ -757,10 +977,10 @@ void linear_forward(const qv_linear& l, void* workspace, size_t workspace_bytes,
         launch_few<T, 8>(l, ep, st);
       return;
     }
-    unsigned char* ws = static_cast<unsigned char*>(workspace);
-    const Stored x = stored_rows<T>(l.dtype, l.x, l.m, l.k, l.x_stride, ws, st);
-    const Stored w = stored_rows<T>(l.dtype, l.weight, l.n, l.k, l.weight_stride, ws, st);
-    product<T>(x, false, w, false, l.m, l.n, l.k, ep, p.product, ws, sms, st);
+    Packer<T> pack(l.dtype, static_cast<unsigned char*>(workspace));
+    const Stored x = pack.rows(l.x, l.m, l.k, l.x_stride);
+    const Stored w = pack.rows(l.weight, l.n, l.k, l.weight_stride);
+    product<T>(x, false, w, false, l.m, l.n, l.k, ep, p.product, pack.run(st), sms, st);
   });
 }
 
@@ -788,7 +1008,11 @@ void check_linear_grad(const qv_linear_grad& g) {
   if (g.dweight != nullptr) check_matrix("x", g.dtype, g.x, g.m, g.k, g.x_stride);
 }
 
+template <class T>
+constexpr int kWideDz = 16 / static_cast<int>(sizeof(T));
+
 struct GradLayout {
+  bool wide_dz = false;       // 16-byte pieces of the gradient and the preactivations
   bool store_dz = false;      // dz is not the caller's gradient itself
   size_t row_blocks = 0;      // row ranges of the column sums
   int64_t rows_per_block = 0;
@@ -802,8 +1026,14 @@ GradLayout grad_layout(const qv_linear_grad& g, int sms) {
   const bool products = g.dx != nullptr || g.dweight != nullptr;
   L.store_dz = products && (g.activation != QV_ACT_NONE ||
                             !in_place(g.dtype, g.grad, g.m, g.grad_stride));
-  const size_t col_blocks = ceil_div(g.n, 256);
-  L.row_blocks = std::min<size_t>(ceil_div(g.m, 8), std::max<size_t>(1, sms * 8 / col_blocks));
+  const size_t e = dtype_size(g.dtype);
+  L.wide_dz = common_align({reinterpret_cast<uintptr_t>(g.grad),
+                            reinterpret_cast<uintptr_t>(g.preact), g.m > 1 ? g.grad_stride * e : 0,
+                            g.m > 1 ? g.preact_stride * e : 0, g.n * e}) == 16;
+  // About eight blocks an SM, each with at least one round of its warps.
+  const size_t col_blocks = ceil_div(g.n, 32 * (L.wide_dz ? 16 / e : 1));
+  L.row_blocks = std::min<size_t>(ceil_div(g.m, kDzWarps * kDzRows),
+                                  std::max<size_t>(1, sms * 8 / col_blocks));
   L.rows_per_block = static_cast<int64_t>(ceil_div(g.m, L.row_blocks));
   L.row_blocks = ceil_div(g.m, L.rows_per_block);
   size_t o = 0;
@@ -862,20 +1092,35 @@ void linear_grad(const qv_linear_grad& g, void* workspace, size_t workspace_byte
     dz.outer = m;
     dz.bf16 = g.dtype != QV_DTYPE_F16;
     if (L.store_dz || sums != nullptr) {
-      const dim3 grid(static_cast<unsigned>(L.row_blocks),
-                      static_cast<unsigned>(ceil_div(g.n, 256)));
       O* store = reinterpret_cast<O*>(ws + L.off_dz);
       const int64_t ld = static_cast<int64_t>(packed_ld(g.n));
-      if (L.store_dz)
-        dz_kernel<T, true><<<grid, 256, 0, st>>>(
-            static_cast<const T*>(g.grad), g.grad_stride, static_cast<const T*>(g.preact),
-            g.preact_stride, static_cast<int>(g.activation), m, n, L.rows_per_block, store, ld,
-            sums);
+      auto go = [&](auto v, auto act) {
+        constexpr int kV = decltype(v)::value;
+        constexpr int kAct = decltype(act)::value;
+        const dim3 grid(static_cast<unsigned>(L.row_blocks),
+                        static_cast<unsigned>(ceil_div(g.n, 32 * kV)));
+        if (L.store_dz)
+          dz_kernel<T, kV, true, kAct><<<grid, 32 * kDzWarps, 0, st>>>(
+              static_cast<const T*>(g.grad), g.grad_stride, static_cast<const T*>(g.preact),
+              g.preact_stride, m, n, L.rows_per_block, store, ld, sums);
+        else
+          dz_kernel<T, kV, false, kAct><<<grid, 32 * kDzWarps, 0, st>>>(
+              static_cast<const T*>(g.grad), g.grad_stride, static_cast<const T*>(g.preact),
+              g.preact_stride, m, n, L.rows_per_block, store, ld, sums);
+      };
+      auto by_act = [&](auto v) {
+        switch (g.activation) {
+          case QV_ACT_RELU: go(v, std::integral_constant<int, QV_ACT_RELU>{}); break;
+          case QV_ACT_GELU: go(v, std::integral_constant<int, QV_ACT_GELU>{}); break;
+          case QV_ACT_GELU_TANH: go(v, std::integral_constant<int, QV_ACT_GELU_TANH>{}); break;
+          case QV_ACT_SILU: go(v, std::integral_constant<int, QV_ACT_SILU>{}); break;
+          default: go(v, std::integral_constant<int, QV_ACT_NONE>{}); break;
+        }
+      };
+      if (L.wide_dz)
+        by_act(std::integral_constant<int, kWideDz<T>>{});
       else
-        dz_kernel<T, false><<<grid, 256, 0, st>>>(
-            static_cast<const T*>(g.grad), g.grad_stride, static_cast<const T*>(g.preact),
-            g.preact_stride, static_cast<int>(g.activation), m, n, L.rows_per_block, store, ld,
-            sums);
+        by_act(std::integral_constant<int, 1>{});
       check_launch("dz_kernel");
     }
     if (L.store_dz) {
@@ -887,29 +1132,29 @@ void linear_grad(const qv_linear_grad& g, void* workspace, size_t workspace_byte
       dz.ld = static_cast<int64_t>(g.grad_stride);
     }
     if (sums != nullptr) {
-      join_sums_kernel<T><<<static_cast<unsigned>(ceil_div(g.n, 256)), 256, 0, st>>>(
-          sums, static_cast<int64_t>(L.row_blocks), n, static_cast<T*>(g.dbias));
+      join_sums_kernel<T><<<static_cast<unsigned>(ceil_div(g.n, 32)), 256, 0, st>>>(
+          sums, static_cast<int>(L.row_blocks), n, static_cast<T*>(g.dbias));
       check_launch("join_sums_kernel");
     }
-    unsigned char* packed = ws + L.off_packed;
-    if (g.dx != nullptr) {
-      const Stored w = stored_rows<T>(g.dtype, g.weight, g.n, g.k, g.weight_stride, packed, st);
+    Packer<T> pack(g.dtype, ws + L.off_packed);
+    Stored w, x;
+    if (g.dx != nullptr) w = pack.rows(g.weight, g.n, g.k, g.weight_stride);
+    if (g.dweight != nullptr) x = pack.rows(g.x, g.m, g.k, g.x_stride);
+    pack.run(st);
+    auto result = [&](void* p, size_t stride) {
       Epilogue ep{};
-      ep.out = g.dx;
-      ep.out_stride = static_cast<int64_t>(g.dx_stride);
+      ep.out = p;
+      ep.out_stride = static_cast<int64_t>(stride);
       ep.out_f32 = g.dtype == QV_DTYPE_F32;
       ep.set_aligns(e);
-      product<T>(dz, false, w, true, m, k, n, ep, L.dx, ws + L.off_partial, sms, st);
-    }
-    if (g.dweight != nullptr) {
-      const Stored x = stored_rows<T>(g.dtype, g.x, g.m, g.k, g.x_stride, packed, st);
-      Epilogue ep{};
-      ep.out = g.dweight;
-      ep.out_stride = static_cast<int64_t>(g.dweight_stride);
-      ep.out_f32 = g.dtype == QV_DTYPE_F32;
-      ep.set_aligns(e);
-      product<T>(dz, true, x, true, n, k, m, ep, L.dw, ws + L.off_partial, sms, st);
-    }
+      return ep;
+    };
+    if (g.dx != nullptr)
+      product<T>(dz, false, w, true, m, k, n, result(g.dx, g.dx_stride), L.dx,
+                 ws + L.off_partial, sms, st);
+    if (g.dweight != nullptr)
+      product<T>(dz, true, x, true, n, k, m, result(g.dweight, g.dweight_stride), L.dw,
+                 ws + L.off_partial, sms, st);
   });
 }
 

@@ -80,6 +80,23 @@ __device__ __forceinline__ float activate(int act, float z) {
     default: return z;
   }
 }
+// activate over 16 values: the choice of activation is made once, outside the unrolled loops.
+template <class T>
+__device__ __forceinline__ void activate16(int act, float (&v)[16]) {
+#define QV_ACT_CASE(name)                                             \
+  case name: {                                                        \
+    _Pragma("unroll") for (int j = 0; j < 16; ++j) v[j] = activate<T>(name, v[j]); \
+    break;                                                            \
+  }
+  switch (act) {
+    QV_ACT_CASE(QV_ACT_RELU)
+    QV_ACT_CASE(QV_ACT_GELU)
+    QV_ACT_CASE(QV_ACT_GELU_TANH)
+    QV_ACT_CASE(QV_ACT_SILU)
+    default: break;
+  }
+#undef QV_ACT_CASE
+}
 // act'(z); 0 for ReLU at 0.
 template <class T>
 __device__ __forceinline__ float act_grad(int act, float z) {
@@ -193,10 +210,7 @@ __device__ __forceinline__ void finish16(const Epilogue& e, int64_t row, int64_t
   }
   if (e.preact != nullptr)
     put16<T>(static_cast<T*>(e.preact) + row * e.preact_stride + col, v, left, e.preact_align);
-  if (e.act != QV_ACT_NONE) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = activate<T>(e.act, v[j]);
-  }
+  activate16<T>(e.act, v);
   if (e.residual != nullptr) {
     float r[16];
     get16<T>(static_cast<const T*>(e.residual) + row * e.residual_stride + col, r, left,
