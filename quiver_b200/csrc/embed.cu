@@ -18,46 +18,73 @@ __device__ __forceinline__ int64_t load_id(const void* ids, size_t i) {
 }
 
 // ---- lookup ------------------------------------------------------------------------------------
-// The output as one run of n * nv pieces of kV elements: every thread takes kUnroll pieces, so
-// short rows leave no lanes idle and each thread has several loads in flight.
-constexpr int kLookupThreads = 256, kLookupUnroll = 4;
+// kG lanes share a row and move kV elements at a time, four pieces in flight per lane: of one row
+// where the row has more than kG pieces, else of four rows. Written past the L2's older lines
+// (streaming stores), so that the results do not push out table rows other ids will read.
+constexpr int kLookupThreads = 256;
 
-template <class T, class Id, int kV>
+template <class T, int kV>
+__device__ __forceinline__ Pack<T, kV> scaled(const Pack<T, kV>& x, float scale) {
+  Pack<T, kV> y;
+#pragma unroll
+  for (int j = 0; j < kV; ++j) y.v[j] = dev::from_f32<T>(dev::to_f32<T>(x.v[j]) * scale);
+  return y;
+}
+template <class T, int kV>
+__device__ __forceinline__ Pack<T, kV> filled(float f) {
+  Pack<T, kV> y;
+#pragma unroll
+  for (int j = 0; j < kV; ++j) y.v[j] = dev::from_f32<T>(f);
+  return y;
+}
+
+template <class T, class Id, int kV, int kG, bool kLong>
 __global__ void __launch_bounds__(kLookupThreads)
     lookup_kernel(const T* __restrict__ table, int64_t rows, int64_t table_stride,
-                  const void* __restrict__ ids, size_t n, uint32_t nv, float scale,
+                  const Id* __restrict__ ids, int64_t n, int nv, float scale,
                   T* __restrict__ out, int64_t out_stride) {
-  constexpr uint32_t kTile = kLookupThreads * kLookupUnroll;
-  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * kTile;
-  const uint64_t i0 = first / nv;
-  const uint32_t v0 = static_cast<uint32_t>(first - i0 * nv);
-  Pack<T, kV> x[kLookupUnroll];
-  uint64_t row[kLookupUnroll];
-  uint32_t col[kLookupUnroll];
-  int state[kLookupUnroll];  // 0: past the end, 1: a row, 2: zeros (id < 0), 3: NaN (id >= rows)
+  constexpr int kRows = kLong ? 1 : 4;
+  constexpr int kGroups = kLookupThreads / kG;
+  const int lane = threadIdx.x % kG;
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / kG) * kRows;
+  if (first >= n) return;
+  const T* src[kRows];
+  float fill[kRows];
 #pragma unroll
-  for (int u = 0; u < kLookupUnroll; ++u) {
-    const uint32_t p = v0 + u * kLookupThreads + threadIdx.x;
-    const uint32_t q = p / nv;
-    row[u] = i0 + q;
-    col[u] = (p - q * nv) * kV;
-    state[u] = 0;
-    if (row[u] >= n) continue;
-    const int64_t id = load_id<Id>(ids, row[u]);
-    state[u] = id < 0 ? 2 : id >= rows ? 3 : 1;
-    if (state[u] == 1) x[u] = dev::load_pack<T, kV>(table + id * table_stride + col[u]);
+  for (int u = 0; u < kRows; ++u) {
+    const int64_t id = first + u < n ? static_cast<int64_t>(ids[first + u]) : -1;
+    src[u] = id >= 0 && id < rows ? table + id * table_stride : nullptr;
+    fill[u] = id < 0 ? 0.0f : __int_as_float(0x7fc00000);
   }
-#pragma unroll
-  for (int u = 0; u < kLookupUnroll; ++u) {
-    if (state[u] == 0) continue;
-    Pack<T, kV> y;
-#pragma unroll
-    for (int j = 0; j < kV; ++j) {
-      const float f = state[u] == 1 ? dev::to_f32<T>(x[u].v[j]) * scale
-                                    : (state[u] == 2 ? 0.0f : __int_as_float(0x7fc00000));
-      y.v[j] = dev::from_f32<T>(f);
+  T* dst = out + first * out_stride;
+  if constexpr (kLong) {
+    if (src[0] == nullptr) {
+      for (int v = lane; v < nv; v += kG) dev::stream_pack<T, kV>(dst + v * kV, filled<T, kV>(fill[0]));
+      return;
     }
-    dev::store_pack<T, kV>(out + static_cast<int64_t>(row[u]) * out_stride + col[u], y);
+    for (int v = lane; v < nv; v += 4 * kG) {
+      Pack<T, kV> x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (v + u * kG < nv) x[u] = dev::load_pack<T, kV>(src[0] + (v + u * kG) * kV);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (v + u * kG < nv)
+          dev::stream_pack<T, kV>(dst + (v + u * kG) * kV, scaled<T, kV>(x[u], scale));
+    }
+  } else {
+    if (lane >= nv) return;
+    Pack<T, kV> x[kRows];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u)
+      if (src[u] != nullptr) x[u] = dev::load_pack<T, kV>(src[u] + lane * kV);
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      if (first + u >= n) break;
+      dev::stream_pack<T, kV>(dst + u * out_stride + lane * kV,
+                              src[u] != nullptr ? scaled<T, kV>(x[u], scale)
+                                                : filled<T, kV>(fill[u]));
+    }
   }
 }
 
@@ -65,12 +92,28 @@ template <class T, class Id, int kV>
 void launch_lookup(const void* table, size_t rows, size_t dim, size_t table_stride,
                    const void* ids, size_t n, float scale, void* out, size_t out_stride,
                    cudaStream_t st) {
-  const uint32_t nv = static_cast<uint32_t>(dim / kV);
-  const size_t blocks = ceil_div(n * nv, kLookupThreads * kLookupUnroll);
-  lookup_kernel<T, Id, kV><<<static_cast<unsigned>(blocks), kLookupThreads, 0, st>>>(
-      static_cast<const T*>(table), static_cast<int64_t>(rows),
-      static_cast<int64_t>(table_stride), ids, n, nv, scale, static_cast<T*>(out),
-      static_cast<int64_t>(out_stride));
+  const int nv = static_cast<int>(dim / kV);
+  auto go = [&](auto g, auto is_long) {
+    constexpr int kG = decltype(g)::value;
+    constexpr bool kLong = decltype(is_long)::value;
+    const size_t per_block = kLookupThreads / kG * (kLong ? 1 : 4);
+    lookup_kernel<T, Id, kV, kG, kLong>
+        <<<static_cast<unsigned>(ceil_div(n, per_block)), kLookupThreads, 0, st>>>(
+            static_cast<const T*>(table), static_cast<int64_t>(rows),
+            static_cast<int64_t>(table_stride), static_cast<const Id*>(ids),
+            static_cast<int64_t>(n), nv, scale, static_cast<T*>(out),
+            static_cast<int64_t>(out_stride));
+  };
+  if (nv <= 4)
+    go(std::integral_constant<int, 4>{}, std::false_type{});
+  else if (nv <= 8)
+    go(std::integral_constant<int, 8>{}, std::false_type{});
+  else if (nv <= 16)
+    go(std::integral_constant<int, 16>{}, std::false_type{});
+  else if (nv <= 32)
+    go(std::integral_constant<int, 32>{}, std::false_type{});
+  else
+    go(std::integral_constant<int, 32>{}, std::true_type{});
   check_launch("lookup_kernel");
 }
 
@@ -329,7 +372,7 @@ __device__ __forceinline__ uint32_t entries_before(const uint32_t* keys, uint32_
 }
 
 template <class T, int kV>
-__global__ void __launch_bounds__(kSumThreads)
+__global__ void __launch_bounds__(kSumThreads, 4)
     segment_sum_kernel(const T* __restrict__ up, int64_t up_stride,
                        const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
                        uint32_t n, uint32_t rows, uint32_t dim, uint32_t run, float scale,
@@ -381,7 +424,7 @@ __global__ void __launch_bounds__(kSumThreads)
       Pack<T, kV> y;
 #pragma unroll
       for (int j = 0; j < kV; ++j) y.v[j] = dev::from_f32<T>(acc[j] * scale);
-      dev::store_pack<T, kV>(out, y);
+      dev::stream_pack<T, kV>(out, y);
     }
 #pragma unroll
     for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
@@ -649,7 +692,7 @@ void embedding_lookup(uint32_t dtype, const void* table, size_t rows, size_t dim
   check_dtype(dtype);
   check_ids(id_type, ids, n);
   QV_REQUIRE(dim >= 1 && dim <= kMaxEmbedDim, "dimension must be between 1 and 65536");
-  QV_REQUIRE(n < (size_t{1} << 40) / dim, "n * dim is too large");
+  QV_REQUIRE(n < (size_t{1} << 31), "more than 2^31 - 1 ids");
   check_rows("table", dtype, table, rows, dim, table_stride);
   check_rows("out", dtype, out, n, dim, out_stride);
   if (n == 0) return;

@@ -67,5 +67,19 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, kV>& x) {
   *reinterpret_cast<Pack<T, kV>*>(p) = x;
 }
 
+// The same store, marked to leave the L2 first.
+template <class T, int kV>
+__device__ __forceinline__ void stream_pack(T* p, const Pack<T, kV>& x) {
+  constexpr int kBytes = static_cast<int>(sizeof(Pack<T, kV>));
+  if constexpr (kBytes == 16)
+    __stcs(reinterpret_cast<uint4*>(p), reinterpret_cast<const uint4&>(x));
+  else if constexpr (kBytes == 8)
+    __stcs(reinterpret_cast<uint2*>(p), reinterpret_cast<const uint2&>(x));
+  else if constexpr (kBytes == 4)
+    __stcs(reinterpret_cast<unsigned int*>(p), reinterpret_cast<const unsigned int&>(x));
+  else
+    __stcs(reinterpret_cast<unsigned short*>(p), reinterpret_cast<const unsigned short&>(x));
+}
+
 }  // namespace dev
 }  // namespace qv

@@ -111,14 +111,14 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackJob j0, const PackJ
 // ---- the product kernel -----------------------------------------------------------------------------
 // Warp-specialized and persistent: one thread feeds 128-byte-swizzled tiles of A and B through a
 // ring of shared-memory stages with TMA, one thread issues the MMAs into one of two accumulators
-// in tensor memory, and eight warps finish the other accumulator's elements meanwhile.
+// in tensor memory, and sixteen warps finish the other accumulator's elements meanwhile.
 //
 // Large products run in CTA pairs (tcgen05 cta_group::2): 256 x 256 tiles, each CTA loading its
 // 128 rows of A and half of B. A CTA by itself would have to load 384 rows of operands for
 // 128 x 256 results, 96 bytes per SM and cycle at full MMA rate; the pair loads 64.
 
 constexpr int kBM = 128, kBK = 64;  // rows of A per CTA, k per stage
-constexpr int kEpilogueWarps = 8;
+constexpr int kEpilogueWarps = 16;
 constexpr int kProductThreads = 128 + 32 * kEpilogueWarps;  // producer, MMA, 2 idle, epilogue
 
 template <int kBN, bool kPair>
@@ -191,17 +191,15 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
         "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+// 16 columns of this warp's 32 TMEM lanes.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
-      "%30, %31}, [%32];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15}, [%16];\n\t"
       "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]),
+        "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]),
+        "=f"(r[14]), "=f"(r[15])
       : "r"(taddr)
       : "memory");
 }
@@ -411,7 +409,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     }
   } else if (warp >= 4) {
     const int quarter = warp & 3;            // TMEM lanes this warp may read
-    const int half = (warp - 4) >> 2;        // which 32 columns of each 64 it takes
+    const int group = (warp - 4) >> 2;       // which 16 columns of each 64 it takes
+    static_assert(kEpilogueWarps == 16, "four groups of 16 columns, four lane quarters");
     int t = 0;
     for (int u = worker; u < units; u += workers, ++t) {
       int split, tm, tn;
@@ -423,31 +422,23 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       const int64_t row =
           static_cast<int64_t>(tm) * S::kM + rank * kBM + quarter * 32 + lane;
 #pragma unroll 1
-      for (int c = half * 32; c < kBN; c += 64) {
+      for (int c = group * 16; c < kBN; c += 64) {
         const int64_t col = static_cast<int64_t>(tn) * kBN + c;
         if (col >= a.n) break;
-        uint32_t r[32];
+        float v[16];
         if (ok) {
-          tmem_ld32(tmem + slot * kBN + c + (static_cast<uint32_t>(quarter * 32) << 16), r);
+          tmem_ld16(tmem + slot * kBN + c + (static_cast<uint32_t>(quarter * 32) << 16), v);
         } else {  // the pipeline gave up: the tile is written as NaN
 #pragma unroll
-          for (int j = 0; j < 32; ++j) r[j] = 0x7fc00000u;
+          for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(0x7fc00000u);
         }
         if (row < a.m) {
-          float v[16];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[h * 16 + j]);
-            const int left = static_cast<int>(min(static_cast<int64_t>(16), a.n - col - h * 16));
-            if (left <= 0) break;
-            if (a.splits > 1) {
-              float* p = a.partial + (static_cast<int64_t>(split) * a.m + row) * a.n + col + h * 16;
-              put16<float>(p, v, left, (a.n & 3) == 0 ? 16 : 4);
-            } else {
-              finish16<T>(a.ep, row, col + h * 16, v, left);
-            }
-          }
+          const int left = static_cast<int>(min(static_cast<int64_t>(16), a.n - col));
+          if (a.splits > 1)
+            put16<float>(a.partial + (static_cast<int64_t>(split) * a.m + row) * a.n + col, v,
+                         left, (a.n & 3) == 0 ? 16 : 4);
+          else
+            finish16<T>(a.ep, row, col, v, left);
         }
         __syncwarp();
       }
@@ -476,26 +467,18 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   }
 }
 
-// Joins the splits of k in their order and finishes the elements.
+// Joins the splits of k in their order and finishes the elements, one a thread.
 template <class T>
 __global__ void __launch_bounds__(256)
     join_splits_kernel(const float* __restrict__ partial, int splits, int64_t m, int64_t n,
-                       Epilogue ep) {
-  const int64_t per_row = (n + 15) / 16;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < m * per_row; i += gridDim.x * 256ll) {
-    const int64_t row = i / per_row, col = (i - row * per_row) * 16;
-    const int left = static_cast<int>(min(static_cast<int64_t>(16), n - col));
-    float v[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = 0.0f;
-    for (int s = 0; s < splits; ++s) {
-      const float* p = partial + (static_cast<int64_t>(s) * m + row) * n + col;
-      float x[16];
-      get16<float>(p, x, left, (n & 3) == 0 ? 16 : 4);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] += x[j];
-    }
-    finish16<T>(ep, row, col, v, left);
+                       const Epilogue ep) {
+  const int64_t size = m * n;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < size; i += gridDim.x * 256ll) {
+    float s = 0.0f;
+#pragma unroll 8
+    for (int k = 0; k < splits; ++k) s += partial[k * size + i];
+    const int64_t row = i / n;
+    finish1<T>(ep, row, i - row * n, s);
   }
 }
 
@@ -574,11 +557,21 @@ __global__ void __launch_bounds__(32 * kDzWarps)
 #pragma unroll
         for (int j = 0; j < kV; ++j) {
           d[j] = dev::to_f32<T>(g[u].v[j]);
-          // rounded before the sum in every variant, so that dbias does not depend on which runs
-          if (kAct != QV_ACT_NONE)
-            d[j] = __fmul_rn(d[j], act_grad<T>(kAct, dev::to_f32<T>(x[u].v[j])));
-          s[j] += d[j];
         }
+        if constexpr (kAct != QV_ACT_NONE) {
+#pragma unroll
+          for (int j = 0; j < kV; j += 2) {
+            const bool two = j + 1 < kV;
+            const float2 f = act_grad2<sizeof(T) == 2>(
+                kAct, make_float2(dev::to_f32<T>(x[u].v[j]),
+                                  dev::to_f32<T>(x[u].v[two ? j + 1 : j])));
+            // rounded before the sum in every variant, so that dbias does not depend on which runs
+            d[j] = __fmul_rn(d[j], f.x);
+            if (two) d[two ? j + 1 : j] = __fmul_rn(d[two ? j + 1 : j], f.y);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kV; ++j) s[j] += d[j];
         if (kStore) put_operand<T, kV>(d, dz, m * ld, row * ld + col);
       }
     }
@@ -777,7 +770,7 @@ void product(const Stored& A, bool a_mn, const Stored& B, bool b_mn, int64_t m, 
   else
     launch_product<T, 64, false>(a, A, B, sms, st);
   if (plan.splits > 1) {
-    const size_t items = static_cast<size_t>(m) * ceil_div(n, 16);
+    const size_t items = static_cast<size_t>(m) * n;
     join_splits_kernel<T>
         <<<static_cast<unsigned>(std::min<size_t>(ceil_div(items, 256), 148 * 16)), 256, 0, st>>>(
             a.partial, plan.splits, m, n, ep);

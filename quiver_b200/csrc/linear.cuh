@@ -36,87 +36,179 @@ struct Epilogue {
 
 #ifdef __CUDACC__
 
-// exp(-x^2/2) and the upper tail Phi(-|x|) of the normal distribution, for GELU and its derivative.
-// 16-bit results: Abramowitz & Stegun 7.1.26 (absolute error of erfc at most 1.5e-7, far below a
-// 16-bit half step); float32 results: the math library's normcdff.
-template <class T>
-__device__ __forceinline__ float normal_cdf(float x, float& gauss) {
-  if constexpr (sizeof(T) == 4) {
-    gauss = expf(-0.5f * x * x);
-    return normcdff(x);
-  } else {
-    const float z = fabsf(x) * 0.70710678f;
-    const float t = __fdividef(1.0f, fmaf(0.3275911f, z, 1.0f));
-    gauss = __expf(-z * z);
-    float p = fmaf(1.061405429f, t, -1.453152027f);
-    p = fmaf(p, t, 1.421413741f);
-    p = fmaf(p, t, -0.284496736f);
-    p = fmaf(p, t, 0.254829592f);
-    const float q = 0.5f * p * t * gauss;
-    return x >= 0.0f ? 1.0f - q : q;
-  }
+// Two float32 operations per instruction (sm_100a), and the hardware's reciprocal and power of two.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)),
+        "l"(reinterpret_cast<unsigned long long&>(b)),
+        "l"(reinterpret_cast<unsigned long long&>(c)));
+  return d;
 }
-template <class T>
-__device__ __forceinline__ float logistic(float x) {
-  if constexpr (sizeof(T) == 4)
-    return 1.0f / (1.0f + expf(-x));
-  else
-    return __fdividef(1.0f, 1.0f + __expf(-x));
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)),
+        "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
 }
-constexpr float kTanhScale = 1.5957691216f;  // 2 sqrt(2 / pi)
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)),
+        "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float2 rcp2(float2 x) {
+  return make_float2(rcp_approx(x.x), rcp_approx(x.y));
+}
+__device__ __forceinline__ float2 exp2_approx(float2 x) {
+  float2 y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(x.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(x.y));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 
-// act(z), for results of type T.
-template <class T>
-__device__ __forceinline__ float activate(int act, float z) {
+// |x| (at most 20, beyond which nothing of the tail is left), exp(-x^2/2) and the normal
+// distribution's tail Phi(-|x|) for 16-bit results: Abramowitz & Stegun 7.1.26, whose error of
+// erfc is at most 1.5e-7, far below a 16-bit half step.
+struct NormalTail {
+  float2 a, gauss, q;
+};
+__device__ __forceinline__ NormalTail normal_tail(float2 x) {
+  NormalTail n;
+  n.a = make_float2(fminf(fabsf(x.x), 20.0f), fminf(fabsf(x.y), 20.0f));
+  const float2 t = rcp2(fma2(n.a, both(0.3275911f * 0.70710678f), both(1.0f)));
+  n.gauss = exp2_approx(mul2(mul2(n.a, n.a), both(-0.72134752f)));  // -log2(e) / 2
+  float2 p = fma2(both(0.5f * 1.061405429f), t, both(0.5f * -1.453152027f));
+  p = fma2(p, t, both(0.5f * 1.421413741f));
+  p = fma2(p, t, both(0.5f * -0.284496736f));
+  p = fma2(p, t, both(0.5f * 0.254829592f));
+  n.q = mul2(mul2(p, t), n.gauss);
+  return n;
+}
+constexpr float kLog2e = 1.44269504f;
+constexpr float kTanhScale = 1.5957691216f;  // 2 sqrt(2 / pi)
+// 1 / (1 + exp(-x)) for 16-bit results.
+__device__ __forceinline__ float2 logistic2(float2 x) {
+  return rcp2(add2(both(1.0f), exp2_approx(mul2(x, both(-kLog2e)))));
+}
+// 2 u of GELU's tanh form, 0.5 (1 + tanh u) = logistic(2u): 2 sqrt(2/pi) (x + 0.044715 x^3).
+__device__ __forceinline__ float2 tanh_arg2(float2 x) {
+  return mul2(x, fma2(mul2(x, x), both(0.044715f * kTanhScale), both(kTanhScale)));
+}
+__device__ __forceinline__ float tanh_arg(float x) {
+  return kTanhScale * fmaf(0.044715f * x * x, x, x);
+}
+__device__ __forceinline__ float logistic(float x) { return 1.0f / (1.0f + expf(-x)); }
+
+// act(z) of two values: for 16-bit results (kFast) the formulas above, for float32 the math library.
+template <bool kFast>
+__device__ __forceinline__ float2 activate2(int act, float2 z) {
   switch (act) {
-    case QV_ACT_RELU: return z < 0.0f ? 0.0f : z;  // NaN stays NaN
-    case QV_ACT_GELU: {
-      float g;
-      return z * normal_cdf<T>(z, g);
-    }
-    // 0.5 (1 + tanh u) = logistic(2u)
-    case QV_ACT_GELU_TANH: return z * logistic<T>(kTanhScale * fmaf(0.044715f * z * z, z, z));
-    case QV_ACT_SILU: return z * logistic<T>(z);
+    case QV_ACT_RELU: return make_float2(max_nan(z.x, 0.0f), max_nan(z.y, 0.0f));
+    case QV_ACT_GELU:
+      if constexpr (kFast) {  // x Phi(x) = max(x, 0) - |x| Phi(-|x|)
+        const NormalTail n = normal_tail(z);
+        return fma2(make_float2(-n.a.x, -n.a.y), n.q,
+                    make_float2(max_nan(z.x, 0.0f), max_nan(z.y, 0.0f)));
+      } else {
+        return make_float2(z.x * normcdff(z.x), z.y * normcdff(z.y));
+      }
+    case QV_ACT_GELU_TANH:
+      if constexpr (kFast)
+        return mul2(z, logistic2(tanh_arg2(z)));
+      else
+        return make_float2(z.x * logistic(tanh_arg(z.x)), z.y * logistic(tanh_arg(z.y)));
+    case QV_ACT_SILU:
+      if constexpr (kFast)
+        return mul2(z, logistic2(z));
+      else
+        return make_float2(z.x * logistic(z.x), z.y * logistic(z.y));
     default: return z;
   }
 }
-// activate over 16 values: the choice of activation is made once, outside the unrolled loops.
-template <class T>
+
+// activate2 over 16 values: the choice of activation is made once, outside the unrolled loops.
+template <bool kFast>
 __device__ __forceinline__ void activate16(int act, float (&v)[16]) {
-#define QV_ACT_CASE(name)                                             \
-  case name: {                                                        \
-    _Pragma("unroll") for (int j = 0; j < 16; ++j) v[j] = activate<T>(name, v[j]); \
-    break;                                                            \
-  }
+  auto all = [&](auto a) {
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+      const float2 y = activate2<kFast>(decltype(a)::value, make_float2(v[j], v[j + 1]));
+      v[j] = y.x;
+      v[j + 1] = y.y;
+    }
+  };
   switch (act) {
-    QV_ACT_CASE(QV_ACT_RELU)
-    QV_ACT_CASE(QV_ACT_GELU)
-    QV_ACT_CASE(QV_ACT_GELU_TANH)
-    QV_ACT_CASE(QV_ACT_SILU)
+    case QV_ACT_RELU: all(std::integral_constant<int, QV_ACT_RELU>{}); break;
+    case QV_ACT_GELU: all(std::integral_constant<int, QV_ACT_GELU>{}); break;
+    case QV_ACT_GELU_TANH: all(std::integral_constant<int, QV_ACT_GELU_TANH>{}); break;
+    case QV_ACT_SILU: all(std::integral_constant<int, QV_ACT_SILU>{}); break;
     default: break;
   }
-#undef QV_ACT_CASE
 }
-// act'(z); 0 for ReLU at 0.
-template <class T>
-__device__ __forceinline__ float act_grad(int act, float z) {
-  switch (act) {
-    case QV_ACT_RELU: return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
-    case QV_ACT_GELU: {
-      float g;
-      const float c = normal_cdf<T>(z, g);
-      return fmaf(z * 0.39894228f, g, c);
+
+// act'(z) of two values; 0 for ReLU at 0.
+template <bool kFast>
+__device__ __forceinline__ float2 act_grad2(int act, float2 z) {
+  if constexpr (kFast) {
+    switch (act) {
+      case QV_ACT_GELU: {  // Phi(x) + x phi(x)
+        const NormalTail n = normal_tail(z);
+        const float2 cdf = make_float2(z.x >= 0.0f ? 1.0f - n.q.x : n.q.x,
+                                       z.y >= 0.0f ? 1.0f - n.q.y : n.q.y);
+        // x within its clamp, so that infinite x does not meet a zero phi
+        const float2 x = make_float2(copysignf(n.a.x, z.x), copysignf(n.a.y, z.y));
+        return fma2(mul2(x, both(0.39894228f)), n.gauss, cdf);
+      }
+      case QV_ACT_GELU_TANH: {  // q + x q (1 - q) (2u)'
+        const float2 q = logistic2(tanh_arg2(z));
+        const float2 du = fma2(mul2(z, z), both(3.0f * 0.044715f * kTanhScale), both(kTanhScale));
+        const float2 r = add2(both(1.0f), make_float2(-q.x, -q.y));
+        return fma2(mul2(mul2(z, q), r), du, q);
+      }
+      case QV_ACT_SILU: {  // q + x q (1 - q)
+        const float2 q = logistic2(z);
+        return fma2(mul2(z, q), add2(both(1.0f), make_float2(-q.x, -q.y)), q);
+      }
+      default: break;
     }
-    case QV_ACT_GELU_TANH: {
-      const float q = logistic<T>(kTanhScale * fmaf(0.044715f * z * z, z, z));
-      return fmaf(z * q * (1.0f - q), kTanhScale * fmaf(0.134145f * z, z, 1.0f), q);
-    }
-    case QV_ACT_SILU: {
-      const float q = logistic<T>(z);
-      return fmaf(z * q, 1.0f - q, q);
-    }
-    default: return 1.0f;
+  } else {
+    auto one = [&](float x) {
+      switch (act) {
+        case QV_ACT_GELU: return fmaf(x * 0.39894228f, expf(-0.5f * x * x), normcdff(x));
+        case QV_ACT_GELU_TANH: {
+          const float q = logistic(tanh_arg(x));
+          return fmaf(x * q * (1.0f - q), kTanhScale * fmaf(0.134145f * x, x, 1.0f), q);
+        }
+        case QV_ACT_SILU: {
+          const float q = logistic(x);
+          return fmaf(x * q, 1.0f - q, q);
+        }
+        default: return 1.0f;
+      }
+    };
+    if (act != QV_ACT_RELU) return make_float2(one(z.x), one(z.y));
   }
+  if (act == QV_ACT_RELU)
+    return make_float2(z.x > 0.0f ? 1.0f : (z.x <= 0.0f ? 0.0f : z.x),
+                       z.y > 0.0f ? 1.0f : (z.y <= 0.0f ? 0.0f : z.y));
+  return both(1.0f);
 }
 
 // 32-byte accesses, which make a thread's piece of a row whole 32-byte sectors.
@@ -210,7 +302,7 @@ __device__ __forceinline__ void finish16(const Epilogue& e, int64_t row, int64_t
   }
   if (e.preact != nullptr)
     put16<T>(static_cast<T*>(e.preact) + row * e.preact_stride + col, v, left, e.preact_align);
-  activate16<T>(e.act, v);
+  activate16<sizeof(T) == 2>(e.act, v);
   if (e.residual != nullptr) {
     float r[16];
     get16<T>(static_cast<const T*>(e.residual) + row * e.residual_stride + col, r, left,
@@ -229,7 +321,7 @@ __device__ __forceinline__ void finish1(const Epilogue& e, int64_t row, int64_t 
   if (e.bias != nullptr) s += dev::to_f32<T>(static_cast<const T*>(e.bias)[col]);
   if (e.preact != nullptr)
     static_cast<T*>(e.preact)[row * e.preact_stride + col] = dev::from_f32<T>(s);
-  float y = activate<T>(e.act, s);
+  float y = activate2<sizeof(T) == 2>(e.act, both(s)).x;
   if (e.residual != nullptr)
     y += dev::to_f32<T>(static_cast<const T*>(e.residual)[row * e.residual_stride + col]);
   if (e.out_f32)
