@@ -117,6 +117,54 @@ void launch_lookup(const void* table, size_t rows, size_t dim, size_t table_stri
   check_launch("lookup_kernel");
 }
 
+// ---- gradient: zeros ---------------------------------------------------------------------------
+// Most rows of a large table get no gradient, and their zeros are most of the bytes. They are
+// written while the ids are sorted: sorting is a chain of short launches that leaves the memory
+// idle, so each of its launches carries extra blocks that clear a share of the result. Rows that do
+// get a gradient are written once more afterwards.
+struct Clear {
+  unsigned char* p;
+  int64_t rows, row_bytes, stride;  // bytes
+  int align;                        // of every row
+  uint32_t parts;                   // launches that share the work
+};
+
+template <class V>
+__device__ __forceinline__ void clear_rows(const Clear& c, int64_t r0, int64_t r1, int64_t block,
+                                           int64_t blocks) {
+  const int64_t per_row = c.row_bytes / static_cast<int64_t>(sizeof(V));
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int64_t r = r0 + block * warps + warp; r < r1; r += blocks * warps) {
+    V* row = reinterpret_cast<V*>(c.p + r * c.stride);
+    for (int64_t i = lane; i < per_row; i += 32) row[i] = V{};
+  }
+}
+
+// Share `part` of the clearing, by block `block` of `blocks`.
+__device__ __forceinline__ void clear_part(const Clear& c, uint32_t part, uint32_t block,
+                                           uint32_t blocks) {
+  if (c.stride == c.row_bytes && c.align == 16) {
+    const int64_t units = c.rows * (c.row_bytes / 16);
+    const int64_t u1 = units * (part + 1) / c.parts;
+    const int64_t step = static_cast<int64_t>(blocks) * blockDim.x;
+    uint4* p = reinterpret_cast<uint4*>(c.p);
+    int64_t i = units * part / c.parts + static_cast<int64_t>(block) * blockDim.x + threadIdx.x;
+    for (; i + 3 * step < u1; i += 4 * step) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) __stcs(p + i + k * step, uint4{});
+    }
+    for (; i < u1; i += step) __stcs(p + i, uint4{});
+    return;
+  }
+  const int64_t r0 = c.rows * part / c.parts, r1 = c.rows * (part + 1) / c.parts;
+  switch (c.align) {
+    case 16: clear_rows<uint4>(c, r0, r1, block, blocks); break;
+    case 8: clear_rows<uint2>(c, r0, r1, block, blocks); break;
+    case 4: clear_rows<uint32_t>(c, r0, r1, block, blocks); break;
+    default: clear_rows<uint16_t>(c, r0, r1, block, blocks); break;
+  }
+}
+
 // ---- gradient: sorting ids -----------------------------------------------------------------------
 // Stable least-significant-digit radix sort of (id, position) pairs; ids that take no gradient
 // (negative or past the table) become `rows` and end up last. Each pass: per-tile digit counts,
@@ -139,7 +187,12 @@ __device__ __forceinline__ uint32_t sort_key(const void* src, size_t i, uint32_t
 template <class Id, bool kFirst>
 __global__ void __launch_bounds__(kSortThreads)
     digit_count_kernel(const void* __restrict__ src, uint32_t n, uint32_t rows, int shift,
-                       int bits, uint32_t tiles, uint32_t* __restrict__ counts) {
+                       int bits, uint32_t tiles, uint32_t* __restrict__ counts, const Clear clear,
+                       uint32_t part) {
+  if (blockIdx.x >= tiles) {
+    clear_part(clear, part, blockIdx.x - tiles, gridDim.x - tiles);
+    return;
+  }
   extern __shared__ uint32_t hist[];
   const int bins = 1 << bits;
   for (int b = threadIdx.x; b < bins; b += kSortThreads) hist[b] = 0;
@@ -156,8 +209,14 @@ __global__ void __launch_bounds__(kSortThreads)
 
 // One warp per digit: its tiles' counts become the entries of that digit in earlier tiles;
 // totals[digit] their sum.
-__global__ void digit_scan_kernel(uint32_t* __restrict__ counts, int bins, uint32_t tiles,
-                                  uint32_t* __restrict__ totals) {
+__global__ void __launch_bounds__(kSortThreads)
+    digit_scan_kernel(uint32_t* __restrict__ counts, int bins, uint32_t tiles,
+                      uint32_t* __restrict__ totals, uint32_t blocks, const Clear clear,
+                      uint32_t part) {
+  if (blockIdx.x >= blocks) {
+    clear_part(clear, part, blockIdx.x - blocks, gridDim.x - blocks);
+    return;
+  }
   const int b = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
   if (b >= bins) return;
   uint32_t* c = counts + static_cast<size_t>(b) * tiles;
@@ -183,13 +242,28 @@ __global__ void __launch_bounds__(kSortThreads)
                          uint32_t n, uint32_t rows, int shift, int bits, uint32_t tiles,
                          const uint32_t* __restrict__ counts,
                          const uint32_t* __restrict__ totals, uint32_t* __restrict__ keys,
-                         uint32_t* __restrict__ pos) {
+                         uint32_t* __restrict__ pos, const Clear clear, uint32_t part) {
+  if (blockIdx.x >= tiles) {
+    clear_part(clear, part, blockIdx.x - tiles, gridDim.x - tiles);
+    return;
+  }
   extern __shared__ uint32_t smem[];
   const int bins = 1 << bits;
   uint32_t* base = smem;                                             // bins: first slot of a digit
   uint16_t* wcount = reinterpret_cast<uint16_t*>(smem + bins);       // kSortWarps x bins
   __shared__ uint32_t wsum[kSortWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // Each warp ranks its own run of 32 * kSortItems entries in order.
+  uint32_t key[kSortItems], p[kSortItems];
+  uint32_t rank[kSortItems];
+  uint16_t* wc = wcount + warp * bins;
+  const uint32_t first = blockIdx.x * kSortTile + warp * (32 * kSortItems);
+#pragma unroll
+  for (int j = 0; j < kSortItems; ++j) {
+    const uint32_t i = first + j * 32 + lane;
+    key[j] = i < n ? sort_key<Id, kFirst>(src, i, rows) : 0u;
+    p[j] = kFirst ? i : (i < n ? src_pos[i] : 0u);
+  }
   for (int b = threadIdx.x; b < kSortWarps * bins; b += kSortThreads) wcount[b] = 0;
   // Exclusive prefix of the digits' totals: each thread sums a run of digits.
   const int per = (bins + kSortThreads - 1) / kSortThreads;
@@ -215,18 +289,6 @@ __global__ void __launch_bounds__(kSortThreads)
       run += totals[b];
     }
   }
-  // Each warp ranks its own run of 32 * kSortItems entries in order.
-  uint32_t key[kSortItems], p[kSortItems];
-  uint32_t rank[kSortItems];
-  uint16_t* wc = wcount + warp * bins;
-  const uint32_t first = blockIdx.x * kSortTile + warp * (32 * kSortItems);
-#pragma unroll
-  for (int j = 0; j < kSortItems; ++j) {
-    const uint32_t i = first + j * 32 + lane;
-    key[j] = i < n ? sort_key<Id, kFirst>(src, i, rows) : 0u;
-    p[j] = kFirst ? i : (i < n ? src_pos[i] : 0u);
-  }
-  __syncthreads();
 #pragma unroll
   for (int j = 0; j < kSortItems; ++j) {
     const uint32_t i = first + j * 32 + lane;
@@ -242,6 +304,7 @@ __global__ void __launch_bounds__(kSortThreads)
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += kSortThreads) {
     uint32_t acc = 0;
+#pragma unroll
     for (int w = 0; w < kSortWarps; ++w) {
       const uint32_t c = wcount[w * bins + b];
       wcount[w * bins + b] = static_cast<uint16_t>(acc);
@@ -260,15 +323,21 @@ __global__ void __launch_bounds__(kSortThreads)
   }
 }
 
-// The same sort of up to kBlockSortItems * 1024 entries by one block in one launch: the passes'
-// keys and positions stay in shared memory and the threads' registers.
+// The same sort of up to 8 * 1024 entries by one block in one launch: between passes the entries
+// stay in shared memory. (A cluster of eight blocks doing this for 131,072 entries, exchanging them
+// through each other's shared memory, took 88 us; the launches above take about 20.)
 constexpr int kBlockSortThreads = 1024, kBlockDigitBits = 8;
 constexpr int kBlockSortWarps = kBlockSortThreads / 32;
+constexpr int kBlockSortMost = 8 * kBlockSortThreads;
 
 template <class Id, int kItems>
 __global__ void __launch_bounds__(kBlockSortThreads)
     block_sort_kernel(const void* __restrict__ ids, uint32_t n, uint32_t rows, int key_bits,
-                      uint32_t* __restrict__ keys, uint32_t* __restrict__ pos) {
+                      uint32_t* __restrict__ keys, uint32_t* __restrict__ pos, const Clear clear) {
+  if (blockIdx.x > 0) {
+    clear_part(clear, 0, blockIdx.x - 1, gridDim.x - 1);
+    return;
+  }
   constexpr int kBins = 1 << kBlockDigitBits;
   extern __shared__ uint32_t smem[];
   uint32_t* skey = smem;                                   // kItems * threads
@@ -342,157 +411,127 @@ __global__ void __launch_bounds__(kBlockSortThreads)
 }
 
 // ---- gradient: segmented sums ---------------------------------------------------------------------
-// The sorted entries and the table's rows are one sequence: each row's entries, then its row end.
-// Entry e stands at place key[e] + e of it. Equal runs of that sequence go to the blocks and, within
-// a block, to its warps, so a token that fills a tenth of the batch is shared out and empty rows
-// cost what they write. What a warp summed of a row that it did not end is its tail, what it
-// summed of a row that it ended but that began before it is its head; rows that span warps are
-// joined in order, in the block where they end in it, else by join_rows_kernel from the blocks'
-// tails and heads.
+// Equal runs of the sorted entries go to the warps, so a token that fills a tenth of the batch is
+// shared out. What a warp summed of a row that it did not end is its tail, what it summed of a row
+// that it ended but that began before it is its head; rows that span warps are joined in order, in
+// the block where they end in it, else by join_rows_kernel from the blocks' tails and heads.
+// Bound by memory: upstream rows are read once, the rows they sum to written once.
 constexpr int kSumWarps = 8, kSumThreads = 32 * kSumWarps;
 constexpr int kSumBatch = 8;  // rows in flight per lane
+constexpr int kMaxRun = 32;   // entries per warp
 constexpr uint32_t kNoRow = 0xffffffffu;
 
-// Number of entries among the first d places of the sequence: the first e in [lo, hi] with
-// key[e] + e >= d, found by a warp in 32-way steps. keys[i] belongs to entry i + base.
-__device__ __forceinline__ uint32_t entries_before(const uint32_t* keys, uint32_t base,
-                                                   uint32_t lo, uint32_t hi, uint64_t d,
-                                                   int lane) {
-  while (lo < hi) {
-    const uint32_t step = (hi - lo + 31) / 32;
-    const uint32_t e = lo + lane * step;
-    const bool in = e < hi && static_cast<uint64_t>(keys[e - base]) + e < d;
-    const uint32_t m = __ballot_sync(dev::kFull, in);
-    if (m == 0) return lo;
-    const uint32_t last = lo + (31 - __clz(m)) * step;  // the last probe that is before d
-    lo = last + 1;
-    hi = min(hi, last + step);
-  }
-  return lo;
-}
-
 template <class T, int kV>
-__global__ void __launch_bounds__(kSumThreads, 4)
+__global__ void __launch_bounds__(kSumThreads)
     segment_sum_kernel(const T* __restrict__ up, int64_t up_stride,
                        const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
                        uint32_t n, uint32_t rows, uint32_t dim, uint32_t run, float scale,
                        T* __restrict__ grad, int64_t grad_stride, float* __restrict__ head,
                        float* __restrict__ tail, uint32_t* __restrict__ head_row) {
-  extern __shared__ __align__(16) unsigned char sum_smem[];
-  constexpr int kCols = 32 * kV;
-  float* s_head = reinterpret_cast<float*>(sum_smem);             // kSumWarps x kCols
-  float* s_tail = s_head + kSumWarps * kCols;                   // kSumWarps x kCols
-  uint32_t* s_key = reinterpret_cast<uint32_t*>(s_tail + kSumWarps * kCols);  // run * kSumWarps
-  uint32_t* s_pos = s_key + run * kSumWarps;
-  __shared__ uint32_t s_e[2], s_tail_row[kSumWarps];
+  constexpr uint32_t kCols = 32 * kV;
+  __shared__ __align__(16) float s_head[kSumWarps][kCols];
+  __shared__ __align__(16) float s_tail[kSumWarps][kCols];
+  // Keys of the block's entries with the one before and the one after; kNoRow outside.
+  __shared__ uint32_t s_keys[kSumWarps * kMaxRun + 2], s_pos[kSumWarps * kMaxRun];
+  __shared__ uint32_t s_tail_row[kSumWarps];
+  const uint32_t* s_key = s_keys + 1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t b0 = blockIdx.x * run * kSumWarps;
+  const uint32_t count = min(n - b0, run * kSumWarps);
+  for (uint32_t i = threadIdx.x; i < count + 2; i += kSumThreads) {
+    const uint32_t e = b0 + i - 1;  // wraps to 2^32 - 1 ahead of the first entry
+    s_keys[i] = e < n ? keys[e] : kNoRow;
+    if (i < count) s_pos[i] = pos[b0 + i];
+  }
+  __syncthreads();
   const uint32_t col0 = blockIdx.y * kCols;
-  const uint32_t c = col0 + lane * kV;
-  const bool on = c < dim;
-  const uint64_t total = static_cast<uint64_t>(rows) + n;
-  const uint64_t b0 = static_cast<uint64_t>(blockIdx.x) * run * kSumWarps;
-  const uint64_t b1 = min(total, b0 + run * kSumWarps);
-  if (warp < 2) {
-    const uint32_t e = entries_before(keys, 0, 0, n, warp == 0 ? b0 : b1, lane);
-    if (lane == 0) s_e[warp] = e;
-  }
-  __syncthreads();
-  const uint32_t eb0 = s_e[0], eb1 = s_e[1];
-  for (uint32_t e = eb0 + threadIdx.x; e < eb1; e += kSumThreads) {
-    s_key[e - eb0] = keys[e];
-    s_pos[e - eb0] = pos[e];
-  }
-  const uint32_t before_key = eb0 > 0 ? keys[eb0 - 1] : kNoRow;  // the entry ahead of the block's
-  __syncthreads();
-  const uint64_t d0 = min(b1, b0 + static_cast<uint64_t>(warp) * run);
-  const uint64_t d1 = min(b1, d0 + run);
-  const uint32_t e0 = entries_before(s_key, eb0, eb0, eb1, d0, lane);
-  const uint32_t e1 = entries_before(s_key, eb0, eb0, eb1, d1, lane);
-  uint32_t r = static_cast<uint32_t>(d0 - e0);
-  const uint32_t r0 = r, r1 = static_cast<uint32_t>(d1 - e1);
-  const bool began_before = d0 < d1 && (e0 > eb0 ? s_key[e0 - 1 - eb0] : before_key) == r;
-  bool is_head = began_before;
+  const bool on = col0 + lane * kV < dim;
+  const uint32_t c = on ? col0 + lane * kV : col0;  // lanes past the last column read the first
+  const T* src = up + c;
+  const uint32_t e0 = min(count, warp * run), e1 = min(count, e0 + run);
+  const int before = static_cast<int>(e0) - 1;
+  const uint32_t r0 = e0 < e1 ? s_key[e0] : kNoRow;
+  const uint32_t before_key = s_key[-1];
+  const bool began_before = e0 < e1 && r0 < rows && s_key[before] == r0;
+  // The last row of this warp's entries, when it goes on in a later warp.
+  const uint32_t last = e0 < e1 ? s_key[e1 - 1] : kNoRow;
+  const bool has_tail = e0 < e1 && last < rows && s_key[e1] == last;
+  if (lane == 0) s_tail_row[warp] = has_tail ? last : kNoRow;
+  const bool ends_first = began_before && !(has_tail && last == r0);
   float acc[kV];
 #pragma unroll
   for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
-  T* out = grad + static_cast<int64_t>(r) * grad_stride + c;
+  bool is_head = began_before;
+  uint32_t r = r0;
   auto finish_row = [&]() {
     if (is_head) {
 #pragma unroll
-      for (int j = 0; j < kV; ++j) s_head[warp * kCols + lane * kV + j] = acc[j];
-    } else if (on) {
+      for (int j = 0; j < kV; ++j) s_head[warp][lane * kV + j] = acc[j];
+    } else if (on && r < rows) {
       Pack<T, kV> y;
 #pragma unroll
       for (int j = 0; j < kV; ++j) y.v[j] = dev::from_f32<T>(acc[j] * scale);
-      dev::stream_pack<T, kV>(out, y);
+      dev::stream_pack<T, kV>(grad + static_cast<int64_t>(r) * grad_stride + c, y);
     }
 #pragma unroll
     for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
     is_head = false;
-    ++r;
-    out += grad_stride;
   };
   for (uint32_t e = e0; e < e1; e += kSumBatch) {
-    const int count = static_cast<int>(min(static_cast<uint32_t>(kSumBatch), e1 - e));
+    if (s_key[e] >= rows) break;  // ids that take no gradient, all at the end
     Pack<T, kV> x[kSumBatch];
 #pragma unroll
-    for (int j = 0; j < kSumBatch; ++j)
-      if (on && j < count)
-        x[j] = dev::load_pack<T, kV>(up + static_cast<int64_t>(s_pos[e + j - eb0]) * up_stride + c);
+    for (int j = 0; j < kSumBatch; ++j)  // past the run its last row again: loads without a branch
+      x[j] = dev::load_pack<T, kV>(src + s_pos[min(e + j, e1 - 1)] * up_stride);
 #pragma unroll
     for (int j = 0; j < kSumBatch; ++j) {
-      if (j >= count) break;
-      const uint32_t k = s_key[e + j - eb0];
-      while (r < k) finish_row();
-      if (on) {
-#pragma unroll
-        for (int v = 0; v < kV; ++v) acc[v] += dev::to_f32<T>(x[j].v[v]);
+      if (e + j >= e1) break;
+      const uint32_t k = s_key[e + j];
+      if (k != r) {
+        finish_row();
+        r = k;
       }
+#pragma unroll
+      for (int v = 0; v < kV; ++v) acc[v] += dev::to_f32<T>(x[j].v[v]);
     }
   }
-  while (r < r1) finish_row();
-  // Entries of row r1, which ends in a later warp.
-  const bool has_tail = e1 > e0 && s_key[e1 - 1 - eb0] == r1 && r1 < rows;
   if (has_tail) {
 #pragma unroll
-    for (int j = 0; j < kV; ++j) s_tail[warp * kCols + lane * kV + j] = acc[j];
+    for (int j = 0; j < kV; ++j) s_tail[warp][lane * kV + j] = acc[j];
+  } else if (e0 < e1) {
+    finish_row();
   }
-  if (lane == 0) s_tail_row[warp] = has_tail ? r1 : kNoRow;
   __syncthreads();
   // A row that began in an earlier warp and ended in this one: that run of tails, then the head.
-  if (began_before && r0 < r1) {
+  if (ends_first) {
     int v = warp;
     while (v > 0 && s_tail_row[v - 1] == r0) --v;
     const bool beyond = v == 0 && before_key == r0;  // it began in an earlier block
 #pragma unroll 1
-    for (int j = lane; j < kCols; j += 32) {
-      if (col0 + j >= dim) break;
+    for (uint32_t j = lane; j < kCols && col0 + j < dim; j += 32) {
       float s = 0.0f;
-      for (int u = v; u < warp; ++u) s += s_tail[u * kCols + j];
-      s += s_head[warp * kCols + j];
+      for (int u = v; u < warp; ++u) s += s_tail[u][j];
+      s += s_head[warp][j];
       if (beyond)
         head[static_cast<size_t>(blockIdx.x) * dim + col0 + j] = s;
       else
         grad[static_cast<int64_t>(r0) * grad_stride + col0 + j] = dev::from_f32<T>(s * scale);
     }
-    if (beyond && lane == 0 && blockIdx.y == 0) head_row[blockIdx.x] = r0;
   }
   if (warp == 0) {
-    // Whether some warp of this block ends the row that was open before it.
-    const uint32_t end_row = static_cast<uint32_t>(b1 - eb1);
-    const uint32_t first_row = static_cast<uint32_t>(b0 - eb0);
-    const bool ends_open = before_key == first_row && first_row < end_row && first_row < rows;
-    if (!ends_open && lane == 0 && blockIdx.y == 0) head_row[blockIdx.x] = kNoRow;
+    // The row that came open into this block, if it ends in it.
+    const bool ends = before_key < rows && s_key[0] == before_key && s_key[count] != before_key;
+    if (lane == 0 && blockIdx.y == 0) head_row[blockIdx.x] = ends ? before_key : kNoRow;
     // The row left open at the end of the block.
-    const uint32_t open_row = s_tail_row[kSumWarps - 1];
+    const int lw = static_cast<int>((count - 1) / run);  // the last warp with entries
+    const uint32_t open_row = s_tail_row[lw];
     if (open_row != kNoRow) {
-      int v = kSumWarps - 1;
+      int v = lw;
       while (v > 0 && s_tail_row[v - 1] == open_row) --v;
 #pragma unroll 1
-      for (int j = lane; j < kCols; j += 32) {
-        if (col0 + j >= dim) break;
+      for (uint32_t j = lane; j < kCols && col0 + j < dim; j += 32) {
         float s = 0.0f;
-        for (int u = v; u < kSumWarps; ++u) s += s_tail[u * kCols + j];
+        for (int u = v; u <= lw; ++u) s += s_tail[u][j];
         tail[static_cast<size_t>(blockIdx.x) * dim + col0 + j] = s;
       }
     }
@@ -503,33 +542,37 @@ __global__ void __launch_bounds__(kSumThreads, 4)
 // from the one it began in up to b - 1, in order, and b's head.
 template <class T>
 __global__ void __launch_bounds__(kSumThreads)
-    join_rows_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t dim, uint32_t run,
-                     float scale, T* __restrict__ grad, int64_t grad_stride,
+    join_rows_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t dim,
+                     uint32_t per_block, float scale, T* __restrict__ grad, int64_t grad_stride,
                      const float* __restrict__ head, const float* __restrict__ tail,
                      const uint32_t* __restrict__ head_row) {
   const uint32_t r = head_row[blockIdx.x];
   if (r == kNoRow) return;
-  uint32_t first = 0, hi = n;  // the row's first entry
+  uint32_t first = 0, hi = n;  // the row's first entry, found in 32-way steps by every warp
   while (first < hi) {
-    const uint32_t mid = (first + hi) / 2;
-    if (keys[mid] < r) first = mid + 1; else hi = mid;
+    const uint32_t step = (hi - first + 31) / 32;
+    const uint32_t e = first + (threadIdx.x & 31) * step;
+    const uint32_t m = __ballot_sync(dev::kFull, e < hi && keys[e] < r);
+    if (m == 0) break;
+    const uint32_t at = first + (31 - __clz(m)) * step;  // the last probe below r
+    first = at + 1;
+    hi = min(hi, at + step);
   }
-  const uint32_t began =
-      static_cast<uint32_t>((static_cast<uint64_t>(r) + first) / (run * kSumWarps));
   for (uint32_t c = blockIdx.y * kSumThreads + threadIdx.x; c < dim; c += gridDim.y * kSumThreads) {
     float s = 0.0f;
 #pragma unroll 8
-    for (uint32_t u = began; u < blockIdx.x; ++u) s += tail[static_cast<size_t>(u) * dim + c];
+    for (uint32_t u = first / per_block; u < blockIdx.x; ++u)
+      s += tail[static_cast<size_t>(u) * dim + c];
     s += head[static_cast<size_t>(blockIdx.x) * dim + c];
     grad[static_cast<int64_t>(r) * grad_stride + c] = dev::from_f32<T>(s * scale);
   }
 }
 
 struct GradPlan {
-  bool one_block;           // sorted by one block
+  bool one_block;              // sorted by one block
   int key_bits, passes, bits;  // width of a key, radix passes and digit width
-  uint32_t tiles;           // sort tiles
-  uint32_t run, blocks;     // places per warp, blocks
+  uint32_t tiles;              // sort tiles
+  uint32_t run, blocks;        // entries per warp, blocks of the sums
   size_t off_keys[2], off_pos[2], off_counts, off_totals, off_head, off_tail, off_row, bytes;
 };
 
@@ -537,12 +580,13 @@ GradPlan grad_plan(size_t n, size_t rows, size_t dim) {
   GradPlan p{};
   p.key_bits = 1;
   while ((size_t{1} << p.key_bits) <= rows) ++p.key_bits;  // keys 0 .. rows
-  p.one_block = n <= 8 * kBlockSortThreads;
+  p.one_block = n <= kBlockSortMost;
   p.passes = p.one_block ? 1 : static_cast<int>(ceil_div(p.key_bits, kMaxDigitBits));
   p.bits = static_cast<int>(ceil_div(p.key_bits, p.passes));
   p.tiles = static_cast<uint32_t>(ceil_div(n, kSortTile));
-  p.run = n + rows <= 148 * 8 * 32 * kSumWarps ? 32 : 64;
-  p.blocks = static_cast<uint32_t>(ceil_div(n + rows, p.run * kSumWarps));
+  // Short runs while they are what fills the GPU, long ones once there are warps enough.
+  p.run = n <= 148 * 64 * 8 ? 8 : kMaxRun;
+  p.blocks = static_cast<uint32_t>(ceil_div(n, p.run * kSumWarps));
   size_t o = 0;
   auto take = [&](size_t bytes) {
     const size_t at = o;
@@ -564,34 +608,50 @@ GradPlan grad_plan(size_t n, size_t rows, size_t dim) {
   return p;
 }
 
+// Extra blocks of `threads` threads that clear a share of the result: up to 32 KB each.
+uint32_t clear_blocks(const Clear& c, int threads) {
+  const size_t bytes = static_cast<size_t>(c.rows) * c.row_bytes / c.parts;
+  return static_cast<uint32_t>(std::max<size_t>(
+      1, std::min<size_t>(ceil_div(bytes, 32768), 148 * 2048 / threads)));
+}
+
 template <class Id, int kItems>
 void launch_block_sort(const GradPlan& p, const void* ids, uint32_t n, uint32_t rows,
-                       unsigned char* ws, cudaStream_t st) {
+                       const Clear& clear, unsigned char* ws, cudaStream_t st) {
   constexpr size_t smem =
       kItems * kBlockSortThreads * 6 + kBlockSortWarps * (size_t{2} << kBlockDigitBits);
   QV_CUDA(cudaFuncSetAttribute(block_sort_kernel<Id, kItems>,
                                cudaFuncAttributeMaxDynamicSharedMemorySize,
                                static_cast<int>(smem)));
-  block_sort_kernel<Id, kItems><<<1, kBlockSortThreads, smem, st>>>(
-      ids, n, rows, p.key_bits, reinterpret_cast<uint32_t*>(ws + p.off_keys[0]),
-      reinterpret_cast<uint32_t*>(ws + p.off_pos[0]));
+  block_sort_kernel<Id, kItems>
+      <<<1 + clear_blocks(clear, kBlockSortThreads), kBlockSortThreads, smem, st>>>(
+          ids, n, rows, p.key_bits, reinterpret_cast<uint32_t*>(ws + p.off_keys[0]),
+          reinterpret_cast<uint32_t*>(ws + p.off_pos[0]), clear);
   check_launch("block_sort_kernel");
 }
 
+// Sorts the ids and clears the result; returns which key / position buffers hold the order.
 template <class Id>
-int sort_ids(const GradPlan& p, const void* ids, uint32_t n, uint32_t rows, unsigned char* ws,
-             cudaStream_t st) {
+int sort_ids(const GradPlan& p, const void* ids, uint32_t n, uint32_t rows, Clear clear,
+             unsigned char* ws, cudaStream_t st) {
   if (p.one_block) {
+    clear.parts = 1;
     if (n <= kBlockSortThreads)
-      launch_block_sort<Id, 1>(p, ids, n, rows, ws, st);
+      launch_block_sort<Id, 1>(p, ids, n, rows, clear, ws, st);
+    else if (n <= 4 * kBlockSortThreads)
+      launch_block_sort<Id, 4>(p, ids, n, rows, clear, ws, st);
     else
-      launch_block_sort<Id, 8>(p, ids, n, rows, ws, st);
+      launch_block_sort<Id, 8>(p, ids, n, rows, clear, ws, st);
     return 0;
   }
+  clear.parts = static_cast<uint32_t>(3 * p.passes);
+  const uint32_t extra = clear_blocks(clear, kSortThreads);
   uint32_t* counts = reinterpret_cast<uint32_t*>(ws + p.off_counts);
   uint32_t* totals = reinterpret_cast<uint32_t*>(ws + p.off_totals);
   const int bins = 1 << p.bits;
+  const uint32_t scan_blocks = static_cast<uint32_t>(ceil_div(bins, kSortWarps));
   const size_t smem = bins * 4 + static_cast<size_t>(kSortWarps) * bins * 2;
+  uint32_t part = 0;
   for (int k = 0; k < p.passes; ++k) {
     uint32_t* ok = reinterpret_cast<uint32_t*>(ws + p.off_keys[k & 1]);
     uint32_t* op = reinterpret_cast<uint32_t*>(ws + p.off_pos[k & 1]);
@@ -599,21 +659,21 @@ int sort_ids(const GradPlan& p, const void* ids, uint32_t n, uint32_t rows, unsi
     const uint32_t* ip = reinterpret_cast<uint32_t*>(ws + p.off_pos[(k & 1) ^ 1]);
     const int shift = k * p.bits;
     if (k == 0)
-      digit_count_kernel<Id, true><<<p.tiles, kSortThreads, bins * 4, st>>>(
-          ids, n, rows, shift, p.bits, p.tiles, counts);
+      digit_count_kernel<Id, true><<<p.tiles + extra, kSortThreads, bins * 4, st>>>(
+          ids, n, rows, shift, p.bits, p.tiles, counts, clear, part++);
     else
-      digit_count_kernel<Id, false><<<p.tiles, kSortThreads, bins * 4, st>>>(
-          ik, n, rows, shift, p.bits, p.tiles, counts);
+      digit_count_kernel<Id, false><<<p.tiles + extra, kSortThreads, bins * 4, st>>>(
+          ik, n, rows, shift, p.bits, p.tiles, counts, clear, part++);
     check_launch("digit_count_kernel");
-    digit_scan_kernel<<<static_cast<unsigned>(ceil_div(bins, 8)), 256, 0, st>>>(counts, bins,
-                                                                               p.tiles, totals);
+    digit_scan_kernel<<<scan_blocks + extra, kSortThreads, 0, st>>>(
+        counts, bins, p.tiles, totals, scan_blocks, clear, part++);
     check_launch("digit_scan_kernel");
     if (k == 0)
-      digit_scatter_kernel<Id, true><<<p.tiles, kSortThreads, smem, st>>>(
-          ids, nullptr, n, rows, shift, p.bits, p.tiles, counts, totals, ok, op);
+      digit_scatter_kernel<Id, true><<<p.tiles + extra, kSortThreads, smem, st>>>(
+          ids, nullptr, n, rows, shift, p.bits, p.tiles, counts, totals, ok, op, clear, part++);
     else
-      digit_scatter_kernel<Id, false><<<p.tiles, kSortThreads, smem, st>>>(
-          ik, ip, n, rows, shift, p.bits, p.tiles, counts, totals, ok, op);
+      digit_scatter_kernel<Id, false><<<p.tiles + extra, kSortThreads, smem, st>>>(
+          ik, ip, n, rows, shift, p.bits, p.tiles, counts, totals, ok, op, clear, part++);
     check_launch("digit_scatter_kernel");
   }
   return (p.passes - 1) & 1;
@@ -628,15 +688,16 @@ void launch_sums(const GradPlan& p, int which, const void* up, size_t up_stride,
   float* head = reinterpret_cast<float*>(ws + p.off_head);
   float* tail = reinterpret_cast<float*>(ws + p.off_tail);
   uint32_t* head_row = reinterpret_cast<uint32_t*>(ws + p.off_row);
-  const size_t smem = 2 * kSumWarps * 32 * kV * sizeof(float) + 2 * p.run * kSumWarps * 4;
   segment_sum_kernel<T, kV>
-      <<<dim3(p.blocks, static_cast<unsigned>(ceil_div(dim, 32 * kV))), kSumThreads, smem, st>>>(
+      <<<dim3(p.blocks, static_cast<unsigned>(ceil_div(dim, 32 * kV))), kSumThreads, 0, st>>>(
           static_cast<const T*>(up), static_cast<int64_t>(up_stride), keys, pos, n, rows, dim,
           p.run, scale, static_cast<T*>(grad), static_cast<int64_t>(grad_stride), head, tail,
           head_row);
   check_launch("segment_sum_kernel");
+  if (p.blocks == 1) return;
   join_rows_kernel<T><<<dim3(p.blocks, static_cast<unsigned>(ceil_div(dim, kSumThreads))),
-                        kSumThreads, 0, st>>>(keys, n, dim, p.run, scale, static_cast<T*>(grad),
+                        kSumThreads, 0, st>>>(keys, n, dim, p.run * kSumWarps, scale,
+                                              static_cast<T*>(grad),
                                               static_cast<int64_t>(grad_stride), head, tail,
                                               head_row);
   check_launch("join_rows_kernel");
@@ -749,11 +810,18 @@ void embedding_grad(uint32_t dtype, const void* up, size_t up_stride, uint32_t i
   QV_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   const uint32_t n32 = static_cast<uint32_t>(n), rows32 = static_cast<uint32_t>(rows);
-  const int which = id_type == QV_ID_I32 ? sort_ids<int32_t>(p, ids, n32, rows32, ws, st)
-                                         : sort_ids<int64_t>(p, ids, n32, rows32, ws, st);
   const int align =
       common_align({reinterpret_cast<uintptr_t>(up), reinterpret_cast<uintptr_t>(grad),
-                    up_stride * e, grad_stride * e, dim * e});
+                    n > 1 ? up_stride * e : 0, rows > 1 ? grad_stride * e : 0, dim * e});
+  Clear clear{};
+  clear.p = static_cast<unsigned char*>(grad);
+  clear.rows = static_cast<int64_t>(rows);
+  clear.row_bytes = static_cast<int64_t>(dim * e);
+  clear.stride = static_cast<int64_t>(rows > 1 ? grad_stride * e : dim * e);
+  clear.align = common_align({reinterpret_cast<uintptr_t>(grad),
+                              static_cast<uint64_t>(clear.stride), dim * e});
+  const int which = id_type == QV_ID_I32 ? sort_ids<int32_t>(p, ids, n32, rows32, clear, ws, st)
+                                         : sort_ids<int64_t>(p, ids, n32, rows32, clear, ws, st);
   by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     by_pack(sizeof(T), align, [&](auto v) {

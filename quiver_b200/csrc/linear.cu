@@ -544,8 +544,8 @@ __global__ void __launch_bounds__(32 * kDzWarps)
       Pack<T, kV> g[kDzRows], x[kDzRows];
 #pragma unroll
       for (int u = 0; u < kDzRows; ++u) {
-        const int64_t row = r + u * kDzWarps;
-        if (row >= r1) break;
+        // Past the range the last row again: loads without a branch, so that all are in flight.
+        const int64_t row = min(r + u * kDzWarps, r1 - 1);
         g[u] = dev::load_pack<T, kV>(dy + row * dy_stride + col);
         if (kAct != QV_ACT_NONE) x[u] = dev::load_pack<T, kV>(z + row * z_stride + col);
       }
