@@ -161,7 +161,7 @@ def _load():
 
 
 def lib():
-    return _load()
+    return _lib if _lib is not None else _load()
 
 
 class QuiverError(ValueError):

@@ -218,6 +218,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   __shared__ int s_consumed;
+  // Each epilogue warp's columns of the bias, two tiles' worth.
+  __shared__ __align__(16) float s_bias[kEpilogueWarps][2][kBN / 4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = kPair ? tc::cluster_ctarank() : 0;
   const bool leader = rank == 0;
@@ -416,6 +418,13 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       int split, tm, tn;
       coords(u, split, tm, tn);
       const int slot = t & 1;
+      float* bias = s_bias[warp - 4][slot];
+      if (a.ep.bias != nullptr) {  // loaded ahead of the wait
+        for (int j = lane; j < kBN / 4; j += 32) {
+          const int64_t col = static_cast<int64_t>(tn) * kBN + (j >> 4) * 64 + group * 16 + (j & 15);
+          bias[j] = col < a.n ? dev::to_f32<T>(static_cast<const T*>(a.ep.bias)[col]) : 0.0f;
+        }
+      }
       const bool ok = wait(bar(ACC_FULL + slot), (t >> 1) & 1);
       __syncwarp();
       tc::tc_fence_after();
@@ -438,7 +447,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             put16<float>(a.partial + (static_cast<int64_t>(split) * a.m + row) * a.n + col, v,
                          left, (a.n & 3) == 0 ? 16 : 4);
           else
-            finish16<T>(a.ep, row, col, v, left);
+            finish16<T>(a.ep, row, col, v, left, bias + (c >> 6) * 16);
         }
         __syncwarp();
       }
@@ -734,7 +743,7 @@ void launch_product(const ProductArgs& a, const Stored& A, const Stored& B, int 
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }
-  QV_CUDA(cudaLaunchKernelEx(&cfg, product_kernel<T, kBN, kPair>, ma, mb, a));
+  cudaLaunchKernelEx(&cfg, product_kernel<T, kBN, kPair>, ma, mb, a);
   check_launch("product_kernel");
 }
 

@@ -19,7 +19,7 @@ struct Epilogue {
   void* preact;
   int64_t preact_stride;
   // Bytes that 16-column pieces of each array are aligned to (up to 32).
-  int out_align, residual_align, preact_align, bias_align;
+  int out_align, residual_align, preact_align;
 
   static int align32(const void* p, int64_t stride_bytes) {
     const uint64_t bits = 32 | reinterpret_cast<uintptr_t>(p) | static_cast<uint64_t>(stride_bytes);
@@ -30,7 +30,6 @@ struct Epilogue {
     out_align = align32(out, out_stride * (out_f32 ? 4 : e));
     residual_align = align32(residual, residual_stride * e);
     preact_align = align32(preact, preact_stride * e);
-    bias_align = align32(bias, 0);
   }
 };
 
@@ -290,15 +289,22 @@ __device__ __forceinline__ void get16(const T* p, float (&v)[16], int left, int 
   for (int j = 0; j < 16; ++j) v[j] = j < left ? dev::to_f32<T>(u.t[j]) : 0.0f;
 }
 
-// Finishes 16 elements (row, col .. col + left - 1) of a product with inputs of type T.
+// Finishes 16 elements (row, col .. col + left - 1) of a product with inputs of type T; bias: their
+// 16 bias values as float32 in shared memory (16-byte aligned).
 template <class T>
 __device__ __forceinline__ void finish16(const Epilogue& e, int64_t row, int64_t col,
-                                         float (&v)[16], int left) {
+                                         float (&v)[16], int left, const float* bias) {
   if (e.bias != nullptr) {
-    float b[16];
-    get16<T>(static_cast<const T*>(e.bias) + col, b, left, e.bias_align);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] += b[j];
+    for (int j = 0; j < 16; j += 4) {
+      const float4 b = *reinterpret_cast<const float4*>(bias + j);
+      const float2 lo = add2(make_float2(v[j], v[j + 1]), make_float2(b.x, b.y));
+      const float2 hi = add2(make_float2(v[j + 2], v[j + 3]), make_float2(b.z, b.w));
+      v[j] = lo.x;
+      v[j + 1] = lo.y;
+      v[j + 2] = hi.x;
+      v[j + 3] = hi.y;
+    }
   }
   if (e.preact != nullptr)
     put16<T>(static_cast<T*>(e.preact) + row * e.preact_stride + col, v, left, e.preact_align);

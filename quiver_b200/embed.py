@@ -38,70 +38,67 @@ _ID_TYPES = {torch.int32: 0, torch.int64: 1}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 
-def _dtype_code(t: torch.Tensor, what: str) -> int:
-    try:
-        return _DTYPES[t.dtype]
-    except KeyError:
-        raise ValueError(f"{what}: expected float32, float16 or bfloat16, got {t.dtype}") from None
+# The handle of PyTorch's current stream, as torch.cuda.current_stream(i).cuda_stream, without
+# building a Stream object: that costs as much host time as a kernel launch.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _bad(what: str, expected: str, got) -> ValueError:
+    return ValueError(f"{what}: expected {expected}, got {got}")
+
+
+def _dtype_code(t, what: str) -> int:
+    """The element type's code of a CUDA tensor; refuses anything else."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{what}: expected a CUDA tensor")
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise _bad(what, "float32, float16 or bfloat16", t.dtype)
+    return code
 
 
 def _activation_code(activation: str) -> int:
-    try:
-        return ACTIVATIONS[activation]
-    except KeyError:
+    code = ACTIVATIONS.get(activation)
+    if code is None:
         raise ValueError(f"unknown activation '{activation}' (expected one of "
-                         f"{', '.join(ACTIVATIONS)})") from None
-
-
-def _cuda(t, what: str) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise ValueError(f"{what}: expected a CUDA tensor")
-    return t
+                         f"{', '.join(ACTIVATIONS)})")
+    return code
 
 
 def _like(t, ref: torch.Tensor, what: str, shape) -> torch.Tensor:
-    _cuda(t, what)
-    if t.dtype != ref.dtype:
-        raise ValueError(f"{what}: expected {ref.dtype}, got {t.dtype}")
-    if t.device != ref.device:
-        raise ValueError(f"{what}: expected a tensor on {ref.device}, got {t.device}")
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not isinstance(t, torch.Tensor) or t.dtype != ref.dtype or t.device != ref.device or \
+            t.shape != shape:
+        if not isinstance(t, torch.Tensor):
+            raise _bad(what, "a CUDA tensor", type(t).__name__)
+        raise _bad(what, f"{ref.dtype} {tuple(shape)} on {ref.device}",
+                   f"{t.dtype} {tuple(t.shape)} on {t.device}")
     return t
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """A 2-D tensor whose rows are contiguous and do not overlap, copied only when t's are not."""
-    if (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1):
+    rows, cols = t.shape
+    s0, s1 = t.stride()
+    if (s1 == 1 or cols == 1) and (s0 >= cols or rows <= 1):
         return t
     return t.contiguous()
 
 
-def _ids(ids: torch.Tensor, device) -> Tuple[torch.Tensor, int]:
-    _cuda(ids, "ids")
-    if ids.dtype not in _ID_TYPES:
-        raise ValueError(f"ids: expected int32 or int64, got {ids.dtype}")
+def _ids(ids, device) -> Tuple[torch.Tensor, int]:
+    if not isinstance(ids, torch.Tensor) or not ids.is_cuda:
+        raise ValueError("ids: expected a CUDA tensor")
+    code = _ID_TYPES.get(ids.dtype)
+    if code is None:
+        raise _bad("ids", "int32 or int64", ids.dtype)
     if ids.device != device:
-        raise ValueError(f"ids: expected a tensor on {device}, got {ids.device}")
-    return ids.contiguous(), _ID_TYPES[ids.dtype]
-
-
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def _workspace(nbytes: int, device):
-    if nbytes == 0:
-        return None, 0
-    return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
+        raise _bad("ids", f"a tensor on {device}", ids.device)
+    return ids.contiguous(), code
 
 
 def _check_out(out, shape, dtype, device):
-    """A caller's result tensor: rows contiguous, or a new tensor when None."""
-    if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    _cuda(out, "out")
-    if out.dtype != dtype or out.device != device or tuple(out.shape) != tuple(shape):
+    """A caller's result tensor."""
+    if not isinstance(out, torch.Tensor) or out.dtype != dtype or out.device != device or \
+            tuple(out.shape) != tuple(shape):
         raise ValueError(f"out: expected {dtype} {tuple(shape)} on {device}")
     if out.requires_grad:
         raise ValueError("out: must not require a gradient")
@@ -114,16 +111,22 @@ def _check_out(out, shape, dtype, device):
 
 
 def _lookup(table, ids, scale, out):
-    if table.dim() != 2:
-        raise ValueError(f"table: expected [rows, dim], got shape {tuple(table.shape)}")
     code = _dtype_code(table, "table")
-    i, id_code = _ids(ids, table.device)
+    if table.dim() != 2:
+        raise _bad("table", "[rows, dim]", f"shape {tuple(table.shape)}")
+    device = table.device
+    i, id_code = _ids(ids, device)
     t = _rows(table)
     rows, dim = t.shape
-    out = _check_out(out, tuple(ids.shape) + (dim,), table.dtype, table.device)
-    check(lib().qv_embedding_lookup_device(table.device.index, code, t.data_ptr(), rows, dim,
+    shape = (*ids.shape, dim)
+    if out is None:
+        out = table.new_empty(shape)
+    else:
+        _check_out(out, shape, table.dtype, device)
+    index = device.index
+    check(lib().qv_embedding_lookup_device(index, code, t.data_ptr(), rows, dim,
                                            max(t.stride(0), dim), id_code, i.data_ptr(), i.numel(),
-                                           scale, out.data_ptr(), dim, _stream(table.device)))
+                                           scale, out.data_ptr(), dim, _raw_stream(index)))
     return out
 
 
@@ -146,8 +149,7 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0,
     """``scale * table[ids]`` for a table [rows, dim] and int32 / int64 ids of any shape: returns
     ``[*ids.shape, dim]``. A negative id (an unfilled search result slot) gives zeros, an id of
     ``rows`` or more a row of NaN. Differentiable in the table (unless ``out`` is given)."""
-    _cuda(table, "table")
-    if out is None and torch.is_grad_enabled() and table.requires_grad:
+    if out is None and torch.is_grad_enabled() and getattr(table, "requires_grad", False):
         return _Lookup.apply(table, ids, float(scale))
     return _lookup(table, ids, float(scale), out)
 
@@ -158,27 +160,29 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, rows: int, scale: floa
     ``scale * sum of grad[i] over ids[i] == r`` in row r, zeros where no id points. ``grad`` is
     ``[*ids.shape, dim]``; ids outside ``[0, rows)`` take no gradient. Sums are float32 in the order
     of the ids, so equal calls give equal bits."""
-    _cuda(grad, "grad")
     code = _dtype_code(grad, "grad")
-    i, id_code = _ids(ids, grad.device)
-    if grad.dim() < 1 or tuple(grad.shape[:-1]) != tuple(ids.shape):
-        raise ValueError(f"grad: expected shape {tuple(ids.shape)} + (dim,), got "
-                         f"{tuple(grad.shape)}")
+    device = grad.device
+    i, id_code = _ids(ids, device)
+    if grad.dim() < 1 or grad.shape[:-1] != ids.shape:
+        raise _bad("grad", f"shape {tuple(ids.shape)} + (dim,)", tuple(grad.shape))
     rows = int(rows)
     if rows < 0:
         raise ValueError("rows must not be negative")
     dim = grad.shape[-1]
-    g = _rows(grad.reshape(-1, dim) if grad.dim() != 2 else grad)
-    out = _check_out(out, (rows, dim), grad.dtype, grad.device)
     n = i.numel()
+    g = _rows(grad if grad.dim() == 2 else grad.reshape(n, dim))
     size = C.c_size_t()
-    check(lib().qv_embedding_grad_workspace(n, rows, dim, C.byref(size)))
-    ws, nbytes = _workspace(size.value, grad.device)
-    check(lib().qv_embedding_grad_device(grad.device.index, code, g.data_ptr(),
-                                         max(g.stride(0), dim), id_code, i.data_ptr(), n, rows,
-                                         dim, float(scale), out.data_ptr(), dim,
-                                         ws.data_ptr() if ws is not None else None, nbytes,
-                                         _stream(grad.device)))
+    call = lib()
+    check(call.qv_embedding_grad_workspace(n, rows, dim, C.byref(size)))
+    if out is None:
+        out = grad.new_empty((rows, dim))
+    else:
+        _check_out(out, (rows, dim), grad.dtype, device)
+    ws = torch.empty(size.value, dtype=torch.uint8, device=device)
+    index = device.index
+    check(call.qv_embedding_grad_device(index, code, g.data_ptr(), max(g.stride(0), dim), id_code,
+                                        i.data_ptr(), n, rows, dim, float(scale), out.data_ptr(),
+                                        dim, ws.data_ptr(), size.value, _raw_stream(index)))
     return out
 
 
@@ -187,46 +191,53 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, rows: int, scale: floa
 
 def _linear(x, weight, bias, residual, activation, out_dtype, want_preact, out=None):
     """The checked call: (out, preact or None), both shaped [*x.shape[:-1], n]."""
-    _cuda(x, "x")
     code = _dtype_code(x, "x")
     act = _activation_code(activation)
-    _cuda(weight, "weight")
+    _dtype_code(weight, "weight")
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"expected x [..., k] and weight [n, k], got {tuple(x.shape)} and "
                          f"{tuple(weight.shape)}")
     n, k = weight.shape
-    shape = tuple(x.shape[:-1]) + (n,)
     _like(weight, x, "weight", (n, k))
-    if bias is not None:
-        bias = _like(bias, x, "bias", (n,)).contiguous()
-    if out_dtype is None:
-        out_dtype = x.dtype
-    if out_dtype not in (x.dtype, torch.float32):
-        raise ValueError(f"out_dtype: expected {x.dtype} or torch.float32, got {out_dtype}")
-    out = _check_out(out, shape, out_dtype, x.device)
-    x2 = _rows(x.reshape(-1, k) if x.dim() != 2 else x)
-    w = _rows(weight)
+    device = x.device
+    x2 = _rows(x if x.dim() == 2 else x.reshape(x.numel() // k if k else 0, k))
     m = x2.shape[0]
-    a = _native.qv_linear(code, _DTYPES[out_dtype], act, m, n, k, x2.data_ptr(),
-                          max(x2.stride(0), k), w.data_ptr(), max(w.stride(0), k),
-                          bias.data_ptr() if bias is not None else None)
+    shape = (*x.shape[:-1], n)
+    w = _rows(weight)
+    bias_ptr = residual_ptr = preact = None
+    residual_stride = 0
+    if bias is not None:
+        bias = _like(bias, x, "bias", (n,)).contiguous()  # held until the call is enqueued
+        bias_ptr = bias.data_ptr()
     if residual is not None:
         r = _like(residual, x, "residual", shape)
-        r = r.reshape(-1, n) if r.dim() != 2 else r
-        if not (r.shape[0] > 1 and r.stride(0) == 0 and (r.stride(1) == 1 or n == 1)):
+        r = r if r.dim() == 2 else r.reshape(m, n)
+        if not (r.stride(0) == 0 and (r.stride(1) == 1 or n == 1)):
             r = _rows(r)
-        a.residual, a.residual_stride = r.data_ptr(), r.stride(0) if m > 1 else n
-    preact = None
+        residual_ptr, residual_stride = r.data_ptr(), r.stride(0) if m > 1 else n
+    if out_dtype is None:
+        out_dtype = x.dtype
+    elif out_dtype != x.dtype and out_dtype != torch.float32:
+        raise _bad("out_dtype", f"{x.dtype} or torch.float32", out_dtype)
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype, device=device)
+    else:
+        _check_out(out, shape, out_dtype, device)
     if want_preact:
-        preact = torch.empty(shape, dtype=x.dtype, device=x.device)
-        a.preact, a.preact_stride = preact.data_ptr(), n
-    a.out, a.out_stride = out.data_ptr(), n
+        preact = x.new_empty(shape)
+    a = _native.qv_linear(code, _DTYPES[out_dtype], act, m, n, k, x2.data_ptr(),
+                          max(x2.stride(0), k), w.data_ptr(), max(w.stride(0), k), bias_ptr,
+                          residual_ptr, residual_stride, out.data_ptr(), n,
+                          preact.data_ptr() if want_preact else None, n)
     size = C.c_size_t()
-    device = x.device.index
-    check(lib().qv_linear_workspace(device, C.byref(a), C.byref(size)))
-    ws, nbytes = _workspace(size.value, x.device)
-    check(lib().qv_linear_device(device, C.byref(a), ws.data_ptr() if ws is not None else None,
-                                 nbytes, _stream(x.device)))
+    index = device.index
+    call, ref = lib(), C.byref(a)
+    check(call.qv_linear_workspace(index, ref, C.byref(size)))
+    if size.value:
+        ws = torch.empty(size.value, dtype=torch.uint8, device=device)
+        check(call.qv_linear_device(index, ref, ws.data_ptr(), size.value, _raw_stream(index)))
+    else:
+        check(call.qv_linear_device(index, ref, None, 0, _raw_stream(index)))
     return out, preact
 
 
@@ -244,7 +255,7 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, grad):
         x, weight, preact = ctx.saved_tensors
         need = ctx.needs_input_grad
-        g = grad.to(x.dtype)  # of a float32 result
+        g = grad if grad.dtype == x.dtype else grad.to(x.dtype)  # of a float32 result
         dx, dw, db = (None, None, None)
         if need[0] or need[1] or need[2]:
             dx, dw, db = linear_grad(g, x, weight, preact, ctx.activation, need=need[:3])
@@ -260,7 +271,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     :data:`ACTIVATIONS`; ``out_dtype`` may be torch.float32 to leave the result unrounded.
     Differentiable in all four tensors (unless ``out`` is given)."""
     if out is None and torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+            [isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, bias, residual)]):
         return _Linear.apply(x, weight, bias, residual, activation, out_dtype)
     return _linear(x, weight, bias, residual, activation, out_dtype, False, out)[0]
 
@@ -279,46 +290,42 @@ def linear_grad(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
     """The gradients (dx, dweight, dbias) of :func:`linear` for ``grad`` = d loss / d result, in x's
     type; those not asked for in ``need`` are None. ``preact`` (from :func:`linear_preact`) may be
     None without an activation. The residual's gradient is ``grad`` itself."""
-    _cuda(x, "x")
     code = _dtype_code(x, "x")
     act = _activation_code(activation)
-    _cuda(weight, "weight")
+    _dtype_code(weight, "weight")
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"expected x [..., k] and weight [n, k], got {tuple(x.shape)} and "
                          f"{tuple(weight.shape)}")
     n, k = weight.shape
     _like(weight, x, "weight", (n, k))
-    shape = tuple(x.shape[:-1]) + (n,)
-    _like(grad, x, "grad", shape)
-    g = _rows(grad.reshape(-1, n) if grad.dim() != 2 else grad)
-    x2 = _rows(x.reshape(-1, k) if x.dim() != 2 else x)
-    w = _rows(weight)
+    x2 = _rows(x if x.dim() == 2 else x.reshape(x.numel() // k if k else 0, k))
     m = x2.shape[0]
-    a = _native.qv_linear_grad(code, act, m, n, k, g.data_ptr(), max(g.stride(0), n),
-                               x2.data_ptr(), max(x2.stride(0), k), w.data_ptr(),
-                               max(w.stride(0), k))
+    shape = (*x.shape[:-1], n)
+    _like(grad, x, "grad", shape)
+    g = _rows(grad if grad.dim() == 2 else grad.reshape(m, n))
+    w = _rows(weight)
+    preact_ptr, preact_stride = None, 0
     if act != 0:
         if preact is None:
             raise ValueError("preact: needed for the gradient of an activation")
         p = _like(preact, x, "preact", shape)
-        p = _rows(p.reshape(-1, n) if p.dim() != 2 else p)
-        a.preact, a.preact_stride = p.data_ptr(), max(p.stride(0), n)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
-    dw = torch.empty((n, k), dtype=x.dtype, device=x.device) if need[1] else None
-    db = torch.empty((n,), dtype=x.dtype, device=x.device) if need[2] else None
-    if dx is not None:
-        a.dx, a.dx_stride = dx.data_ptr(), k
-    if dw is not None:
-        a.dweight, a.dweight_stride = dw.data_ptr(), k
-    if db is not None:
-        a.dbias = db.data_ptr()
+        p = _rows(p if p.dim() == 2 else p.reshape(m, n))
+        preact_ptr, preact_stride = p.data_ptr(), max(p.stride(0), n)
+    dx = x.new_empty(x.shape) if need[0] else None
+    dw = x.new_empty((n, k)) if need[1] else None
+    db = x.new_empty((n,)) if need[2] else None
+    a = _native.qv_linear_grad(code, act, m, n, k, g.data_ptr(), max(g.stride(0), n),
+                               x2.data_ptr(), max(x2.stride(0), k), w.data_ptr(),
+                               max(w.stride(0), k), preact_ptr, preact_stride,
+                               dx.data_ptr() if need[0] else None, k,
+                               dw.data_ptr() if need[1] else None, k,
+                               db.data_ptr() if need[2] else None)
     size = C.c_size_t()
-    device = x.device.index
-    check(lib().qv_linear_grad_workspace(device, C.byref(a), C.byref(size)))
-    ws, nbytes = _workspace(size.value, x.device)
-    check(lib().qv_linear_grad_device(device, C.byref(a),
-                                      ws.data_ptr() if ws is not None else None, nbytes,
-                                      _stream(x.device)))
+    index = x.device.index
+    call, ref = lib(), C.byref(a)
+    check(call.qv_linear_grad_workspace(index, ref, C.byref(size)))
+    ws = torch.empty(size.value, dtype=torch.uint8, device=x.device)
+    check(call.qv_linear_grad_device(index, ref, ws.data_ptr(), size.value, _raw_stream(index)))
     return dx, dw, db
 
 
@@ -329,7 +336,6 @@ class Adapter:
 
     def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
                  activation: str = "none", residual: bool = False):
-        _cuda(weight, "weight")
         _dtype_code(weight, "weight")
         _activation_code(activation)
         if weight.dim() != 2:

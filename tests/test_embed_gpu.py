@@ -169,11 +169,12 @@ def test_grad_distributions(embed, n, kind):
 
 def test_grad_wide_table(embed):
     """More rows than one radix pass tells apart, and than 2^22."""
-    for rows in (2048, 2049, 4_200_000):
-        g = gen(rows)
-        ids = torch.randint(0, rows, (9000,), generator=g, device="cuda")
-        ids[::3] = ids[0]
-        check_grad(embed, normal(g, 9000, 4), ids, rows)
+    for rows in (2047, 2048, 2049, 3_000_000, 4_200_000):
+        for n in (9000, 300):
+            g = gen(rows)
+            ids = torch.randint(0, rows, (n,), generator=g, device="cuda")
+            ids[::3] = ids[0]
+            check_grad(embed, normal(g, n, 4), ids, rows)
 
 
 def test_grad_strides_and_empty(embed):
