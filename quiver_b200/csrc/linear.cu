@@ -145,8 +145,16 @@ struct ProductArgs {
   uint32_t a_mn, b_mn;    // operand stored across k (MN-major)
   Epilogue ep;
   float* partial;         // splits > 1: [split][m][n] float32 sums, joined afterwards
+};
+// Up to two products of one launch (a layer's dx and dW), their tiles one list of work units.
+struct ProductGroup {
+  ProductArgs p[2];
+  int units[2];
   long long wait_cycles;
   uint64_t drain_ns;
+};
+struct ProductMaps {
+  CUtensorMap a[2], b[2];
 };
 
 // TMA loads; in a pair the bytes are counted on the leader's barrier (a shared::cluster address).
@@ -206,8 +214,8 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&r)[16]) {
 
 template <class T, int kBN, bool kPair>
 __global__ void __launch_bounds__(kProductThreads, 1)
-    product_kernel(const __grid_constant__ CUtensorMap map_a,
-                   const __grid_constant__ CUtensorMap map_b, const ProductArgs a) {
+    product_kernel(const __grid_constant__ ProductMaps maps,
+                   const __grid_constant__ ProductGroup g) {
   using S = Tile<kBN, kPair>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* tiles = reinterpret_cast<unsigned char*>(
@@ -274,27 +282,33 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     for (;;) {
       if (sleep_test()) return true;
       if (*abort_flag) return false;
-      if (clock64() - t0 > a.wait_cycles) {
+      if (clock64() - t0 > g.wait_cycles) {
         *abort_flag = 1;
         return false;
       }
     }
   };
-  const int units = a.tiles_m * a.tiles_n * a.splits;
+  const int units = g.units[0] + g.units[1];
   const int worker = kPair ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
   const int workers = kPair ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
-  // Unit u: split u / (tiles), tile row / column of the rest, columns fastest (a wave's CTAs share
-  // rows of A and all of B in L2).
-  auto coords = [&](int u, int& split, int& tm, int& tn) {
-    const int per = a.tiles_m * a.tiles_n;
-    split = u / per;
-    const int t = u - split * per;
-    tm = t / a.tiles_n;
-    tn = t - tm * a.tiles_n;
+  // Unit u: product q, split, then tile row / column, columns fastest (a wave's CTAs share rows of
+  // A and all of B in L2), and the split's blocks of k.
+  struct Unit {
+    int q, split, tm, tn, b0, b1;
   };
-  auto block_range = [&](int split, int& b0, int& b1) {
-    b0 = split * a.blocks_per_split;
-    b1 = min(a.k_blocks, b0 + a.blocks_per_split);
+  auto unit = [&](int u) {
+    Unit w;
+    w.q = u >= g.units[0];
+    u -= w.q ? g.units[0] : 0;
+    const ProductArgs& a = g.p[w.q];
+    const int per = a.tiles_m * a.tiles_n;
+    w.split = u / per;
+    const int t = u - w.split * per;
+    w.tm = t / a.tiles_n;
+    w.tn = t - w.tm * a.tiles_n;
+    w.b0 = w.split * a.blocks_per_split;
+    w.b1 = min(a.k_blocks, w.b0 + a.blocks_per_split);
+    return w;
   };
 
   if (warp == 0) {
@@ -303,14 +317,16 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       uint32_t phase = 1;
       bool ok = true;
       for (int u = worker; u < units && ok; u += workers) {
-        int split, tm, tn, b0, b1;
-        coords(u, split, tm, tn);
-        block_range(split, b0, b1);
-        const int row_a = tm * S::kM + static_cast<int>(rank) * kBM;
-        const int row_b = tn * kBN + static_cast<int>(rank) * S::kBRows;
+        const Unit w = unit(u);
+        const ProductArgs& a = g.p[w.q];
+        const CUtensorMap* map_a = &maps.a[w.q];
+        const CUtensorMap* map_b = &maps.b[w.q];
+        const bool a_mn = a.a_mn, b_mn = a.b_mn;
+        const int row_a = w.tm * S::kM + static_cast<int>(rank) * kBM;
+        const int row_b = w.tn * kBN + static_cast<int>(rank) * S::kBRows;
         for (int p = 0; p < a.pairs && ok; ++p) {
           const int pa = a.pairs == 1 ? 0 : kPairA[p], pb = a.pairs == 1 ? 0 : kPairB[p];
-          for (int kb = b0; kb < b1; ++kb) {
+          for (int kb = w.b0; kb < w.b1; ++kb) {
             if (!wait(bar(EMPTY + s), phase)) {
               ok = false;
               break;
@@ -319,19 +335,19 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             const uint32_t full = lbar(FULL + s);
             const uint32_t da = tc::smem_u32(tiles + s * S::kStageBytes);
             const uint32_t db = da + S::kABytes;
-            if (a.a_mn) {
+            if (a_mn) {
 #pragma unroll
               for (int c = 0; c < kBM / 64; ++c)
-                tma_load_3d<kPair>(da + c * 8192, &map_a, row_a + c * 64, kb * kBK, pa, full);
+                tma_load_3d<kPair>(da + c * 8192, map_a, row_a + c * 64, kb * kBK, pa, full);
             } else {
-              tma_load_3d<kPair>(da, &map_a, kb * kBK, row_a, pa, full);
+              tma_load_3d<kPair>(da, map_a, kb * kBK, row_a, pa, full);
             }
-            if (a.b_mn) {
+            if (b_mn) {
 #pragma unroll
               for (int c = 0; c < S::kBRows / 64; ++c)
-                tma_load_3d<kPair>(db + c * 8192, &map_b, row_b + c * 64, kb * kBK, pb, full);
+                tma_load_3d<kPair>(db + c * 8192, map_b, row_b + c * 64, kb * kBK, pb, full);
             } else {
-              tma_load_3d<kPair>(db, &map_b, kb * kBK, row_b, pb, full);
+              tma_load_3d<kPair>(db, map_b, kb * kBK, row_b, pb, full);
             }
             ++issued;
             if (++s == S::kStages) {
@@ -346,12 +362,12 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         // barriers, which the peer cannot poll: it waits out the bound, far longer than any copy.
         const uint64_t t0 = tc::gtimer();
         if constexpr (kPair) {
-          while (tc::gtimer() - t0 < a.drain_ns) {
+          while (tc::gtimer() - t0 < g.drain_ns) {
           }
         } else {
           for (int f = s_consumed; f < issued; ++f)
             while (!tc::mbar_test(bar(FULL + f % S::kStages), (f / S::kStages) & 1) &&
-                   tc::gtimer() - t0 < a.drain_ns) {
+                   tc::gtimer() - t0 < g.drain_ns) {
             }
         }
       }
@@ -361,7 +377,6 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       int taken = 0, t = 0, s = 0;
       uint32_t phase = 0;
       bool ok = true;
-      const uint32_t a_step = a.a_mn ? 2048 >> 4 : 32 >> 4, b_step = a.b_mn ? 2048 >> 4 : 32 >> 4;
       auto commit = [&](int i) {  // signals barrier i (of both CTAs) once the MMAs so far are done
         if constexpr (kPair)
           tc::umma_commit_pair_mc(bar(i), 0x3);
@@ -369,14 +384,15 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           tc::umma_commit(bar(i));
       };
       for (int u = worker; u < units && ok; u += workers, ++t) {
-        int split, tm, tn, b0, b1;
-        coords(u, split, tm, tn);
-        block_range(split, b0, b1);
+        const Unit w = unit(u);
+        const ProductArgs& a = g.p[w.q];
+        const uint32_t a_mn = a.a_mn, b_mn = a.b_mn, idesc = a.idesc;
+        const uint32_t a_step = a_mn ? 2048 >> 4 : 32 >> 4, b_step = b_mn ? 2048 >> 4 : 32 >> 4;
         const int slot = t & 1;
         if (!wait(bar(ACC_EMPTY + slot), ((t >> 1) & 1) ^ 1)) break;
         tc::tc_fence_after();
         const uint32_t d = tmem + slot * kBN;
-        const int blocks = (b1 - b0) * a.pairs;
+        const int blocks = (w.b1 - w.b0) * a.pairs;
         for (int i = 0; i < blocks; ++i) {
           if (!wait(bar(FULL + s), phase)) {
             ok = false;
@@ -385,11 +401,11 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           s_consumed = ++taken;
           tc::tc_fence_after();
           const uint32_t da = tc::smem_u32(tiles + s * S::kStageBytes);
-          const uint64_t ad = operand_desc(da, a.a_mn);
-          const uint64_t bd = operand_desc(da + S::kABytes, a.b_mn);
+          const uint64_t ad = operand_desc(da, a_mn);
+          const uint64_t bd = operand_desc(da + S::kABytes, b_mn);
 #pragma unroll
           for (int q = 0; q < kBK / 16; ++q)
-            mma_f16<kPair>(d, ad + q * a_step, bd + q * b_step, a.idesc, (i | q) != 0);
+            mma_f16<kPair>(d, ad + q * a_step, bd + q * b_step, idesc, (i | q) != 0);
           commit(EMPTY + s);
           if (++s == S::kStages) {
             s = 0;
@@ -405,7 +421,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         else
           tc::umma_commit(bar(DRAIN));
         const uint64_t t0 = tc::gtimer();
-        while (!tc::mbar_test(bar(DRAIN), 0) && tc::gtimer() - t0 < a.drain_ns) {
+        while (!tc::mbar_test(bar(DRAIN), 0) && tc::gtimer() - t0 < g.drain_ns) {
         }
       }
     }
@@ -415,8 +431,9 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     static_assert(kEpilogueWarps == 16, "four groups of 16 columns, four lane quarters");
     int t = 0;
     for (int u = worker; u < units; u += workers, ++t) {
-      int split, tm, tn;
-      coords(u, split, tm, tn);
+      const Unit w = unit(u);
+      const ProductArgs& a = g.p[w.q];
+      const int tm = w.tm, tn = w.tn;
       const int slot = t & 1;
       float* bias = s_bias[warp - 4][slot];
       if (a.ep.bias != nullptr) {  // loaded ahead of the wait
@@ -444,7 +461,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         if (row < a.m) {
           const int left = static_cast<int>(min(static_cast<int64_t>(16), a.n - col));
           if (a.splits > 1)
-            put16<float>(a.partial + (static_cast<int64_t>(split) * a.m + row) * a.n + col, v,
+            put16<float>(a.partial + (static_cast<int64_t>(w.split) * a.m + row) * a.n + col, v,
                          left, (a.n & 3) == 0 ? 16 : 4);
           else
             finish16<T>(a.ep, row, col, v, left, bias + (c >> 6) * 16);
@@ -476,18 +493,63 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   }
 }
 
-// Joins the splits of k in their order and finishes the elements, one a thread.
+// What is left after a launch of products, by block row: the splits of each one's k joined in their
+// order and their elements finished, one a thread, and the bias gradient from its row ranges' sums.
+struct SplitJob {
+  const float* partial;
+  int splits;  // 0: nothing to join
+  int64_t m, n;
+  Epilogue ep;
+};
+struct SumsJob {
+  const float* sums;  // nullptr: none
+  int blocks;
+  int64_t n;
+  void* db;
+};
+struct JoinJobs {
+  SplitJob split[2];
+  SumsJob sums;
+};
 template <class T>
-__global__ void __launch_bounds__(256)
-    join_splits_kernel(const float* __restrict__ partial, int splits, int64_t m, int64_t n,
-                       const Epilogue ep) {
-  const int64_t size = m * n;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < size; i += gridDim.x * 256ll) {
-    float s = 0.0f;
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinJobs jobs) {
+  if (blockIdx.y < 2) {
+    const SplitJob& j = jobs.split[blockIdx.y];
+    if (j.splits == 0) return;
+    const int64_t size = j.m * j.n, n = j.n;
+    const int splits = j.splits;
+    const float* partial = j.partial;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < size; i += gridDim.x * 256ll) {
+      float s = 0.0f;
 #pragma unroll 8
-    for (int k = 0; k < splits; ++k) s += partial[k * size + i];
-    const int64_t row = i / n;
-    finish1<T>(ep, row, i - row * n, s);
+      for (int k = 0; k < splits; ++k) s += partial[k * size + i];
+      const int64_t row = i / n;
+      finish1<T>(j.ep, row, i - row * n, s);
+    }
+    return;
+  }
+  // 32 columns at a time: each warp a run of row ranges, then the warps in order.
+  const SumsJob& j = jobs.sums;
+  __shared__ float part[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per = (j.blocks + 7) / 8;
+  const int b1 = min(j.blocks, (warp + 1) * per);
+  for (int64_t c0 = blockIdx.x * 32ll; c0 < j.n; c0 += gridDim.x * 32ll) {
+    const int64_t col = c0 + lane;
+    float s = 0.0f;
+    if (col < j.n) {
+#pragma unroll 8
+      for (int b = warp * per; b < b1; ++b) s += j.sums[b * j.n + col];
+    }
+    part[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && col < j.n) {
+      float t = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) t += part[w][lane];
+      static_cast<T*>(j.db)[col] = dev::from_f32<T>(t);
+    }
+    __syncthreads();
   }
 }
 
@@ -599,30 +661,6 @@ __global__ void __launch_bounds__(32 * kDzWarps)
   }
 }
 
-// Adds the row ranges' sums: 32 columns a block, each warp a run of ranges, then the warps in order.
-template <class T>
-__global__ void __launch_bounds__(256)
-    join_sums_kernel(const float* __restrict__ sums, int blocks, int64_t n, T* __restrict__ db) {
-  __shared__ float part[8][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t col = blockIdx.x * 32ll + lane;
-  const int per = (blocks + 7) / 8;
-  const int b1 = min(blocks, (warp + 1) * per);
-  float s = 0.0f;
-  if (col < n) {
-#pragma unroll 8
-    for (int b = warp * per; b < b1; ++b) s += sums[b * n + col];
-  }
-  part[warp][lane] = s;
-  __syncthreads();
-  if (warp == 0 && col < n) {
-    float t = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) t += part[w][lane];
-    db[col] = dev::from_f32<T>(t);
-  }
-}
-
 // ---- host side ----------------------------------------------------------------------------------------
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -671,54 +709,85 @@ CUtensorMap operand_map(const Stored& s, uint32_t box_outer) {
   return m;
 }
 
+// One product of a launch: D[m][n] = sum_k A B, finished by `ep`. a_mn / b_mn: the operand is
+// stored with m (n) inner.
+struct Product {
+  int64_t m, n, k;
+  bool a_mn, b_mn;
+  Stored a, b;
+  Epilogue ep;
+};
 struct ProductPlan {
-  int bn = 128, splits = 1, blocks_per_split = 1, k_blocks = 1;
+  int bn = 128;
   bool pair = false;
-  size_t partial_bytes = 0;
+  int splits[2] = {1, 1}, blocks_per_split[2] = {1, 1}, k_blocks[2] = {1, 1};
+  size_t partial_bytes[2] = {0, 0};
 };
 
-// Tile and split of k with the least estimated time. In cycles: a 64-wide block of k takes the
+// Tiles and splits of k with the least estimated time. In cycles: a 64-wide block of k takes the
 // larger of the MMAs and the copies into shared memory, a tile's results about 10 cycles a column
 // (hidden behind the next tile's blocks when there is one), and the splits are written, read and
-// joined in a launch of their own.
-ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int pairs, int sms) {
+// joined in a launch of their own. Splits of a product are chosen with the tile width alone.
+ProductPlan plan_products(const Product* p, int count, int pairs, int sms) {
   ProductPlan best;
   double best_t = 1e300;
-  const int64_t kb = std::max<int64_t>(1, static_cast<int64_t>(ceil_div(k, kBK)));
   for (int bn : {64, 128, 256}) {
-    const bool pair = bn == 256;
-    const double tiles = static_cast<double>(ceil_div(m, pair ? 2 * kBM : kBM)) * ceil_div(n, bn);
-    const int workers = pair ? sms / 2 : sms;
+    ProductPlan plan;
+    plan.bn = bn;
+    plan.pair = bn == 256;
+    const int workers = plan.pair ? sms / 2 : sms;
     const double per_block = bn == 256 ? 540 : (bn == 128 ? 400 : 280);
-    for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-      if (s > 1 && (s > kb || tiles * s > 2.0 * workers)) break;
-      const int64_t per = static_cast<int64_t>(ceil_div(kb, s));
-      const int64_t used = static_cast<int64_t>(ceil_div(kb, per));
-      const double waves = std::ceil(tiles * used / workers);
-      const double block_t = static_cast<double>(per) * pairs * per_block;
-      double t = waves * std::max(block_t, 10.0 * bn) + 10.0 * bn + 1500;
-      if (used > 1) t += 4000 + 8.0 * m * n * used / 3000.0;
-      if (t < best_t) {
-        best_t = t;
-        best.bn = bn;
-        best.pair = pair;
-        best.splits = static_cast<int>(used);
-        best.blocks_per_split = static_cast<int>(per);
-        best.k_blocks = static_cast<int>(kb);
+    double work = 0, longest = 0, joins = 0, waves_t = 0;
+    for (int q = 0; q < count; ++q) {
+      const int64_t m = p[q].m, n = p[q].n;
+      const int64_t kb = std::max<int64_t>(1, static_cast<int64_t>(ceil_div(p[q].k, kBK)));
+      const double tiles =
+          static_cast<double>(ceil_div(m, plan.pair ? 2 * kBM : kBM)) * ceil_div(n, bn);
+      double best_q = 1e300, unit_q = 0, units_q = 0, join_q = 0;
+      for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+        if (s > 1 && (s > kb || tiles * s > 2.0 * workers)) break;
+        const int64_t per = static_cast<int64_t>(ceil_div(kb, s));
+        const int64_t used = static_cast<int64_t>(ceil_div(kb, per));
+        const double unit = std::max(static_cast<double>(per) * pairs * per_block, 10.0 * bn);
+        const double join = used > 1 ? 4000 + 8.0 * m * n * used / 3000.0 : 0.0;
+        const double t = std::ceil(tiles * used / workers) * unit + join;
+        if (t < best_q) {
+          best_q = t;
+          unit_q = unit;
+          units_q = tiles * used;
+          join_q = join;
+          plan.splits[q] = static_cast<int>(used);
+          plan.blocks_per_split[q] = static_cast<int>(per);
+          plan.k_blocks[q] = static_cast<int>(kb);
+        }
       }
+      work += unit_q * units_q / workers;
+      longest = std::max(longest, unit_q);
+      joins = std::max(joins, join_q);
+      waves_t = std::ceil(units_q / workers) * unit_q;
+      plan.partial_bytes[q] =
+          plan.splits[q] > 1 ? (static_cast<size_t>(plan.splits[q]) * m * n * 4 + 255) / 256 * 256
+                             : 0;
+    }
+    const double t =
+        (count == 1 ? waves_t : std::max(longest, work + 0.5 * longest)) + joins + 10.0 * bn;
+    if (t < best_t) {
+      best_t = t;
+      best = plan;
     }
   }
-  best.partial_bytes =
-      best.splits > 1 ? static_cast<size_t>(best.splits) * m * n * sizeof(float) : 0;
   return best;
 }
 
 template <class T, int kBN, bool kPair>
-void launch_product(const ProductArgs& a, const Stored& A, const Stored& B, int sms,
-                    cudaStream_t st) {
+void launch_products(const Product* p, int count, const ProductGroup& g, int sms,
+                     cudaStream_t st) {
   using S = Tile<kBN, kPair>;
-  const CUtensorMap ma = operand_map(A, a.a_mn ? kBK : kBM);
-  const CUtensorMap mb = operand_map(B, a.b_mn ? kBK : S::kBRows);
+  ProductMaps maps;
+  for (int q = 0; q < count; ++q) {
+    maps.a[q] = operand_map(p[q].a, p[q].a_mn ? kBK : kBM);
+    maps.b[q] = operand_map(p[q].b, p[q].b_mn ? kBK : S::kBRows);
+  }
   static std::once_flag once[16];
   int device = 0;
   QV_CUDA(cudaGetDevice(&device));
@@ -727,7 +796,7 @@ void launch_product(const ProductArgs& a, const Stored& A, const Stored& B, int 
                                  cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  static_cast<int>(S::kSmem)));
   });
-  const int units = a.tiles_m * a.tiles_n * a.splits;
+  const int units = g.units[0] + g.units[1];
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(kPair ? 2 * std::min(units, sms / 2)
                                                  : std::min(units, sms)));
@@ -743,47 +812,62 @@ void launch_product(const ProductArgs& a, const Stored& A, const Stored& B, int 
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }
-  cudaLaunchKernelEx(&cfg, product_kernel<T, kBN, kPair>, ma, mb, a);
+  cudaLaunchKernelEx(&cfg, product_kernel<T, kBN, kPair>, maps, g);  // reported by check_launch
   check_launch("product_kernel");
 }
 
-// D[m][n] = sum_k A B, finished by `ep`. a_mn / b_mn: the operand is stored with m (n) inner.
+// Runs the products and what joins them (with the bias gradient's sums). partial: the plan's
+// partial bytes, product by product.
 template <class T>
-void product(const Stored& A, bool a_mn, const Stored& B, bool b_mn, int64_t m, int64_t n,
-             int64_t k, const Epilogue& ep, const ProductPlan& plan, void* partial, int sms,
-             cudaStream_t st) {
-  ProductArgs a{};
-  a.m = m;
-  a.n = n;
-  a.k = k;
-  a.pairs = std::is_same_v<T, float> ? 6 : 1;
-  a.k_blocks = plan.k_blocks;
-  a.tiles_m = static_cast<int>(ceil_div(m, plan.pair ? 2 * kBM : kBM));
-  a.tiles_n = static_cast<int>(ceil_div(n, plan.bn));
-  a.splits = plan.splits;
-  a.blocks_per_split = plan.blocks_per_split;
-  const uint32_t fmt = A.bf16 ? 1 : 0;
-  a.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(a_mn) << 15) |
-            (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(plan.bn >> 3) << 17) |
-            (static_cast<uint32_t>((plan.pair ? 2 * kBM : kBM) >> 4) << 24);
-  a.a_mn = a_mn;
-  a.b_mn = b_mn;
-  a.ep = ep;
-  a.partial = static_cast<float*>(partial);
-  a.wait_cycles = tc::wait_limit_cycles();
-  a.drain_ns = tc::drain_limit_ns();
-  if (plan.pair)
-    launch_product<T, 256, true>(a, A, B, sms, st);
-  else if (plan.bn == 128)
-    launch_product<T, 128, false>(a, A, B, sms, st);
-  else
-    launch_product<T, 64, false>(a, A, B, sms, st);
-  if (plan.splits > 1) {
-    const size_t items = static_cast<size_t>(m) * n;
-    join_splits_kernel<T>
-        <<<static_cast<unsigned>(std::min<size_t>(ceil_div(items, 256), 148 * 16)), 256, 0, st>>>(
-            a.partial, plan.splits, m, n, ep);
-    check_launch("join_splits_kernel");
+void run_products(const Product* p, int count, const ProductPlan& plan, unsigned char* partial,
+                  const SumsJob& sums, int sms, cudaStream_t st) {
+  ProductGroup g{};
+  JoinJobs jobs{};
+  jobs.sums = sums;
+  size_t items = 0;
+  for (int q = 0; q < count; ++q) {
+    ProductArgs& a = g.p[q];
+    a.m = p[q].m;
+    a.n = p[q].n;
+    a.k = p[q].k;
+    a.pairs = std::is_same_v<T, float> ? 6 : 1;
+    a.k_blocks = plan.k_blocks[q];
+    a.tiles_m = static_cast<int>(ceil_div(a.m, plan.pair ? 2 * kBM : kBM));
+    a.tiles_n = static_cast<int>(ceil_div(a.n, plan.bn));
+    a.splits = plan.splits[q];
+    a.blocks_per_split = plan.blocks_per_split[q];
+    const uint32_t fmt = p[q].a.bf16 ? 1 : 0;
+    a.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(p[q].a_mn) << 15) |
+              (static_cast<uint32_t>(p[q].b_mn) << 16) |
+              (static_cast<uint32_t>(plan.bn >> 3) << 17) |
+              (static_cast<uint32_t>((plan.pair ? 2 * kBM : kBM) >> 4) << 24);
+    a.a_mn = p[q].a_mn;
+    a.b_mn = p[q].b_mn;
+    a.ep = p[q].ep;
+    a.partial = reinterpret_cast<float*>(partial);
+    partial += plan.partial_bytes[q];
+    g.units[q] = a.tiles_m * a.tiles_n * a.splits;
+    if (a.splits > 1) {
+      jobs.split[q] = SplitJob{a.partial, a.splits, a.m, a.n, a.ep};
+      items = std::max(items, static_cast<size_t>(a.m) * a.n);
+    }
+  }
+  g.wait_cycles = tc::wait_limit_cycles();
+  g.drain_ns = tc::drain_limit_ns();
+  if (count > 0) {
+    if (plan.pair)
+      launch_products<T, 256, true>(p, count, g, sms, st);
+    else if (plan.bn == 128)
+      launch_products<T, 128, false>(p, count, g, sms, st);
+    else
+      launch_products<T, 64, false>(p, count, g, sms, st);
+  }
+  if (sums.sums != nullptr) items = std::max(items, static_cast<size_t>(sums.n) * 8);
+  if (items > 0) {
+    join_kernel<T><<<dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(items, 256), 148 * 8)),
+                          sums.sums != nullptr ? 3 : 2),
+                     256, 0, st>>>(jobs);
+    check_launch("join_kernel");
   }
 }
 
@@ -919,11 +1003,15 @@ LinearPlan linear_plan(const qv_linear& l, int sms) {
   LinearPlan p;
   p.few = l.m <= kMaxFewRows;
   if (p.few || l.m == 0) return p;
-  p.product = plan_product(l.m, l.n, l.k, l.dtype == QV_DTYPE_F32 ? 6 : 1, sms);
+  Product d{};
+  d.m = static_cast<int64_t>(l.m);
+  d.n = static_cast<int64_t>(l.n);
+  d.k = static_cast<int64_t>(l.k);
+  p.product = plan_products(&d, 1, l.dtype == QV_DTYPE_F32 ? 6 : 1, sms);
   if (!in_place(l.dtype, l.x, l.m, l.x_stride)) p.bytes += packed_bytes(l.dtype, l.m, l.k);
   if (!in_place(l.dtype, l.weight, l.n, l.weight_stride))
     p.bytes += packed_bytes(l.dtype, l.n, l.k);
-  p.bytes += p.product.partial_bytes;
+  p.bytes += p.product.partial_bytes[0];
   return p;
 }
 
@@ -980,9 +1068,14 @@ void linear_forward(const qv_linear& l, void* workspace, size_t workspace_bytes,
       return;
     }
     Packer<T> pack(l.dtype, static_cast<unsigned char*>(workspace));
-    const Stored x = pack.rows(l.x, l.m, l.k, l.x_stride);
-    const Stored w = pack.rows(l.weight, l.n, l.k, l.weight_stride);
-    product<T>(x, false, w, false, l.m, l.n, l.k, ep, p.product, pack.run(st), sms, st);
+    Product d{};
+    d.m = static_cast<int64_t>(l.m);
+    d.n = static_cast<int64_t>(l.n);
+    d.k = static_cast<int64_t>(l.k);
+    d.a = pack.rows(l.x, l.m, l.k, l.x_stride);
+    d.b = pack.rows(l.weight, l.n, l.k, l.weight_stride);
+    d.ep = ep;
+    run_products<T>(&d, 1, p.product, pack.run(st), SumsJob{}, sms, st);
   });
 }
 
@@ -1018,7 +1111,9 @@ struct GradLayout {
   bool store_dz = false;      // dz is not the caller's gradient itself
   size_t row_blocks = 0;      // row ranges of the column sums
   int64_t rows_per_block = 0;
-  ProductPlan dx, dw;
+  Product products[2];        // dx and dweight, those that are asked for
+  int count = 0;
+  ProductPlan plan;
   size_t off_dz = 0, off_sums = 0, off_packed = 0, off_partial = 0, bytes = 0;
 };
 GradLayout grad_layout(const qv_linear_grad& g, int sms) {
@@ -1047,15 +1142,27 @@ GradLayout grad_layout(const qv_linear_grad& g, int sms) {
   L.off_dz = take(L.store_dz ? packed_bytes(g.dtype, g.m, g.n) : 0);
   L.off_sums = take(g.dbias != nullptr ? L.row_blocks * g.n * sizeof(float) : 0);
   L.off_packed = o;
-  if (g.dx != nullptr) {
-    L.dx = plan_product(g.m, g.k, g.n, pairs, sms);
-    if (!in_place(g.dtype, g.weight, g.n, g.weight_stride)) take(packed_bytes(g.dtype, g.n, g.k));
-  }
+  // dweight first: its units are the longest where there are many rows.
   if (g.dweight != nullptr) {
-    L.dw = plan_product(g.n, g.k, g.m, pairs, sms);
+    Product& d = L.products[L.count++];
+    d = Product{};
+    d.m = static_cast<int64_t>(g.n);
+    d.n = static_cast<int64_t>(g.k);
+    d.k = static_cast<int64_t>(g.m);
+    d.a_mn = d.b_mn = true;
     if (!in_place(g.dtype, g.x, g.m, g.x_stride)) take(packed_bytes(g.dtype, g.m, g.k));
   }
-  L.off_partial = take(std::max(L.dx.partial_bytes, L.dw.partial_bytes));
+  if (g.dx != nullptr) {
+    Product& d = L.products[L.count++];
+    d = Product{};
+    d.m = static_cast<int64_t>(g.m);
+    d.n = static_cast<int64_t>(g.k);
+    d.k = static_cast<int64_t>(g.n);
+    d.b_mn = true;
+    if (!in_place(g.dtype, g.weight, g.n, g.weight_stride)) take(packed_bytes(g.dtype, g.n, g.k));
+  }
+  if (L.count > 0) L.plan = plan_products(L.products, L.count, pairs, sms);
+  L.off_partial = take(L.plan.partial_bytes[0] + L.plan.partial_bytes[1]);
   L.bytes = o;
   return L;
 }
@@ -1078,7 +1185,7 @@ void linear_grad(const qv_linear_grad& g, void* workspace, size_t workspace_byte
     if (g.dbias != nullptr) QV_CUDA(cudaMemsetAsync(g.dbias, 0, g.n * e, st));
     return;
   }
-  const GradLayout L = grad_layout(g, sms);
+  GradLayout L = grad_layout(g, sms);
   QV_REQUIRE(L.bytes == 0 || (workspace != nullptr && workspace_bytes >= L.bytes),
              "workspace too small: qv_linear_grad_workspace tells the size");
   QV_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0 || L.bytes == 0,
@@ -1087,7 +1194,7 @@ void linear_grad(const qv_linear_grad& g, void* workspace, size_t workspace_byte
   by_type(g.dtype, [&](auto t) {
     using T = decltype(t);
     using O = typename Operand<T>::type;
-    const int64_t m = g.m, n = g.n, k = g.k;
+    const int64_t m = g.m, n = g.n;
     float* sums = g.dbias != nullptr ? reinterpret_cast<float*>(ws + L.off_sums) : nullptr;
     Stored dz;
     dz.inner = n;
@@ -1133,16 +1240,7 @@ void linear_grad(const qv_linear_grad& g, void* workspace, size_t workspace_byte
       dz.p = g.grad;
       dz.ld = static_cast<int64_t>(g.grad_stride);
     }
-    if (sums != nullptr) {
-      join_sums_kernel<T><<<static_cast<unsigned>(ceil_div(g.n, 32)), 256, 0, st>>>(
-          sums, static_cast<int>(L.row_blocks), n, static_cast<T*>(g.dbias));
-      check_launch("join_sums_kernel");
-    }
     Packer<T> pack(g.dtype, ws + L.off_packed);
-    Stored w, x;
-    if (g.dx != nullptr) w = pack.rows(g.weight, g.n, g.k, g.weight_stride);
-    if (g.dweight != nullptr) x = pack.rows(g.x, g.m, g.k, g.x_stride);
-    pack.run(st);
     auto result = [&](void* p, size_t stride) {
       Epilogue ep{};
       ep.out = p;
@@ -1151,12 +1249,23 @@ void linear_grad(const qv_linear_grad& g, void* workspace, size_t workspace_byte
       ep.set_aligns(e);
       return ep;
     };
-    if (g.dx != nullptr)
-      product<T>(dz, false, w, true, m, k, n, result(g.dx, g.dx_stride), L.dx,
-                 ws + L.off_partial, sms, st);
-    if (g.dweight != nullptr)
-      product<T>(dz, true, x, true, n, k, m, result(g.dweight, g.dweight_stride), L.dw,
-                 ws + L.off_partial, sms, st);
+    int q = 0;
+    if (g.dweight != nullptr) {
+      Product& d = L.products[q++];
+      d.a = dz;
+      d.b = pack.rows(g.x, g.m, g.k, g.x_stride);
+      d.ep = result(g.dweight, g.dweight_stride);
+    }
+    if (g.dx != nullptr) {
+      Product& d = L.products[q++];
+      d.a = dz;
+      d.b = pack.rows(g.weight, g.n, g.k, g.weight_stride);
+      d.ep = result(g.dx, g.dx_stride);
+    }
+    pack.run(st);
+    SumsJob sj{};
+    if (sums != nullptr) sj = SumsJob{sums, static_cast<int>(L.row_blocks), n, g.dbias};
+    run_products<T>(L.products, L.count, L.plan, ws + L.off_partial, sj, sms, st);
   });
 }
 
