@@ -120,6 +120,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackJob j0, const PackJ
 constexpr int kBM = 128, kBK = 64;  // rows of A per CTA, k per stage
 constexpr int kEpilogueWarps = 16;
 constexpr int kProductThreads = 128 + 32 * kEpilogueWarps;  // producer, MMA, 2 idle, epilogue
+constexpr int kPieceBytes = 4096;  // an epilogue warp's piece of the result: 32 rows x 128 bytes
 
 template <int kBN, bool kPair>
 struct Tile {
@@ -128,8 +129,9 @@ struct Tile {
   static constexpr int kABytes = kBM * kBK * 2;
   static constexpr int kBBytes = kBRows * kBK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = kStageBytes >= 32768 ? 6 : 8;
-  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + 1024 + 256;
+  static constexpr int kStages = kStageBytes >= 32768 ? 4 : 5;  // 6 measured no faster
+  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes +
+                                  kEpilogueWarps * kPieceBytes + 1024 + 512;
 };
 
 // Plane pairs of a float32 product, smallest terms first.
@@ -154,7 +156,7 @@ struct ProductGroup {
   uint64_t drain_ns;
 };
 struct ProductMaps {
-  CUtensorMap a[2], b[2];
+  CUtensorMap a[2], b[2], out[2], residual[2];
 };
 
 // TMA loads; in a pair the bytes are counted on the leader's barrier (a shared::cluster address).
@@ -173,6 +175,16 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         "{%2, %3, %4}], [%5];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
+}
+// One lane of a converged warp, the same each time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(p));
+  return p != 0;
 }
 // 128-byte swizzled operand tiles. Along k: 64-element rows, 8-row groups 1024 bytes apart.
 // Across k: [64 k][64 m-or-n] blocks of 8 KB (the leading offset), 8-k groups 1024 bytes apart.
@@ -199,6 +211,13 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
         "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(src)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
 // 16 columns of this warp's 32 TMEM lanes.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&r)[16]) {
   asm volatile(
@@ -220,12 +239,12 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* tiles = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + S::kStages * S::kStageBytes);
-  // full[stage], empty[stage], acc_full[2], acc_empty[2], drain. In a pair the leader's full and
+  unsigned char* pieces = tiles + S::kStages * S::kStageBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(pieces + kEpilogueWarps * kPieceBytes);
+  // full[stage], empty[stage], acc_full[2], acc_empty[2], drain, residual[epilogue warp]. In a pair the leader's full and
   // acc_empty barriers stand for both CTAs; empty and acc_full are signalled in each.
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
-  __shared__ int s_consumed;
   // Each epilogue warp's columns of the bias, two tiles' worth.
   __shared__ __align__(16) float s_bias[kEpilogueWarps][2][kBN / 4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -234,11 +253,10 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   auto bar = [&](int i) { return tc::smem_u32(bars + i); };
   auto lbar = [&](int i) { return kPair ? tc::mapa_shared(bar(i), 0) : bar(i); };
   constexpr int FULL = 0, EMPTY = S::kStages, ACC_FULL = 2 * S::kStages, ACC_EMPTY = ACC_FULL + 2,
-                DRAIN = ACC_EMPTY + 2;
-  static_assert((DRAIN + 1) * 8 <= 256, "the barriers fit behind the stages");
+                DRAIN = ACC_EMPTY + 2, RESIDUAL = DRAIN + 1;
+  static_assert((RESIDUAL + kEpilogueWarps) * 8 <= 512, "the barriers fit behind the pieces");
   if (threadIdx.x == 0) {
     s_abort = 0;
-    s_consumed = 0;
     for (int s = 0; s < S::kStages; ++s) {
       tc::mbar_init(bar(FULL + s), 1);
       tc::mbar_init(bar(EMPTY + s), 1);
@@ -248,6 +266,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       tc::mbar_init(bar(ACC_EMPTY + b), (kPair ? 2 : 1) * kEpilogueWarps);
     }
     tc::mbar_init(bar(DRAIN), 1);
+    for (int w = 0; w < kEpilogueWarps; ++w) tc::mbar_init(bar(RESIDUAL + w), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -311,160 +330,259 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     return w;
   };
 
+  // The producer and MMA loops run warp-uniformly and elect a lane for the copies and MMAs alone:
+  // their addresses and descriptors then stay in uniform registers, which those instructions take.
+  // With a single lane in the whole loop, operands moved there one by one, a block of k took
+  // 620 cycles to issue where its MMAs take 512.
+  const uint32_t tiles_at = tc::smem_u32(tiles), full_at = lbar(FULL), empty_at = bar(EMPTY);
   if (warp == 0) {
-    if (lane == 0) {
-      int issued = 0, s = 0;
-      uint32_t phase = 1;
-      bool ok = true;
-      for (int u = worker; u < units && ok; u += workers) {
-        const Unit w = unit(u);
-        const ProductArgs& a = g.p[w.q];
-        const CUtensorMap* map_a = &maps.a[w.q];
-        const CUtensorMap* map_b = &maps.b[w.q];
-        const bool a_mn = a.a_mn, b_mn = a.b_mn;
-        const int row_a = w.tm * S::kM + static_cast<int>(rank) * kBM;
-        const int row_b = w.tn * kBN + static_cast<int>(rank) * S::kBRows;
-        for (int p = 0; p < a.pairs && ok; ++p) {
-          const int pa = a.pairs == 1 ? 0 : kPairA[p], pb = a.pairs == 1 ? 0 : kPairB[p];
-          for (int kb = w.b0; kb < w.b1; ++kb) {
-            if (!wait(bar(EMPTY + s), phase)) {
-              ok = false;
-              break;
-            }
-            if (leader) tc::mbar_expect_tx(bar(FULL + s), (kPair ? 2 : 1) * S::kStageBytes);
-            const uint32_t full = lbar(FULL + s);
-            const uint32_t da = tc::smem_u32(tiles + s * S::kStageBytes);
-            const uint32_t db = da + S::kABytes;
-            if (a_mn) {
+    int s = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    auto produce = [&](auto a_mn, auto b_mn, const Unit& w, int q) {
+      const ProductArgs& a = g.p[q];
+      const CUtensorMap* map_a = &maps.a[q];
+      const CUtensorMap* map_b = &maps.b[q];
+      const int row_a = w.tm * S::kM + static_cast<int>(rank) * kBM;
+      const int row_b = w.tn * kBN + static_cast<int>(rank) * S::kBRows;
+      for (int p = 0; p < a.pairs && ok; ++p) {
+        const int pa = a.pairs == 1 ? 0 : kPairA[p], pb = a.pairs == 1 ? 0 : kPairB[p];
+        for (int k0 = w.b0 * kBK; k0 < w.b1 * kBK; k0 += kBK) {
+          if (!wait(empty_at + s * 8, phase)) {
+            ok = false;
+            break;
+          }
+          if (elect_one()) {
+            const uint32_t full = full_at + s * 8;
+            const uint32_t da = tiles_at + s * S::kStageBytes, db = da + S::kABytes;
+            if (leader) tc::mbar_expect_tx(bar(FULL) + s * 8, (kPair ? 2 : 1) * S::kStageBytes);
+            if constexpr (decltype(a_mn)::value) {
 #pragma unroll
               for (int c = 0; c < kBM / 64; ++c)
-                tma_load_3d<kPair>(da + c * 8192, map_a, row_a + c * 64, kb * kBK, pa, full);
+                tma_load_3d<kPair>(da + c * 8192, map_a, row_a + c * 64, k0, pa, full);
             } else {
-              tma_load_3d<kPair>(da, map_a, kb * kBK, row_a, pa, full);
+              tma_load_3d<kPair>(da, map_a, k0, row_a, pa, full);
             }
-            if (b_mn) {
+            if constexpr (decltype(b_mn)::value) {
 #pragma unroll
               for (int c = 0; c < S::kBRows / 64; ++c)
-                tma_load_3d<kPair>(db + c * 8192, map_b, row_b + c * 64, kb * kBK, pb, full);
+                tma_load_3d<kPair>(db + c * 8192, map_b, row_b + c * 64, k0, pb, full);
             } else {
-              tma_load_3d<kPair>(db, map_b, kb * kBK, row_b, pb, full);
-            }
-            ++issued;
-            if (++s == S::kStages) {
-              s = 0;
-              phase ^= 1;
+              tma_load_3d<kPair>(db, map_b, k0, row_b, pb, full);
             }
           }
+          s = s + 1 == S::kStages ? 0 : s + 1;
+          phase ^= s == 0;
         }
       }
-      if (*abort_flag) {
-        // Copies in flight must land before the CTA leaves. A pair's are counted on the leader's
-        // barriers, which the peer cannot poll: it waits out the bound, far longer than any copy.
-        const uint64_t t0 = tc::gtimer();
-        if constexpr (kPair) {
-          while (tc::gtimer() - t0 < g.drain_ns) {
-          }
-        } else {
-          for (int f = s_consumed; f < issued; ++f)
-            while (!tc::mbar_test(bar(FULL + f % S::kStages), (f / S::kStages) & 1) &&
-                   tc::gtimer() - t0 < g.drain_ns) {
-            }
-        }
+    };
+    for (int u = worker; u < units && ok; u += workers) {
+      const Unit w = unit(u);
+      const int q = w.q;
+      // The three forms of a layer's products: x W^T, dz W, dz^T x.
+      if (g.p[q].a_mn)
+        produce(std::true_type{}, std::true_type{}, w, q);
+      else if (g.p[q].b_mn)
+        produce(std::false_type{}, std::true_type{}, w, q);
+      else
+        produce(std::false_type{}, std::false_type{}, w, q);
+    }
+    if (*abort_flag) {
+      // Copies in flight must land before the CTA leaves. They may be counted on barriers that
+      // this CTA cannot poll (a pair's leader's): wait out the bound, far longer than any copy.
+      const uint64_t t0 = tc::gtimer();
+      while (tc::gtimer() - t0 < g.drain_ns) {
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && leader) {  // in a pair the leader issues for both CTAs
-      int taken = 0, t = 0, s = 0;
+    if (leader) {  // in a pair the leader issues for both CTAs
+      int t = 0, s = 0;
       uint32_t phase = 0;
       bool ok = true;
-      auto commit = [&](int i) {  // signals barrier i (of both CTAs) once the MMAs so far are done
+      auto commit = [&](uint32_t at) {  // signals a barrier (of both CTAs) after the MMAs so far
         if constexpr (kPair)
-          tc::umma_commit_pair_mc(bar(i), 0x3);
+          tc::umma_commit_pair_mc(at, 0x3);
         else
-          tc::umma_commit(bar(i));
+          tc::umma_commit(at);
       };
       for (int u = worker; u < units && ok; u += workers, ++t) {
         const Unit w = unit(u);
         const ProductArgs& a = g.p[w.q];
-        const uint32_t a_mn = a.a_mn, b_mn = a.b_mn, idesc = a.idesc;
-        const uint32_t a_step = a_mn ? 2048 >> 4 : 32 >> 4, b_step = b_mn ? 2048 >> 4 : 32 >> 4;
+        const uint32_t idesc = a.idesc;
+        const uint32_t a_step = a.a_mn ? 2048 >> 4 : 32 >> 4, b_step = a.b_mn ? 2048 >> 4 : 32 >> 4;
+        const uint64_t ad0 = operand_desc(tiles_at, a.a_mn);
+        const uint64_t bd0 = operand_desc(tiles_at + S::kABytes, a.b_mn);
         const int slot = t & 1;
         if (!wait(bar(ACC_EMPTY + slot), ((t >> 1) & 1) ^ 1)) break;
         tc::tc_fence_after();
         const uint32_t d = tmem + slot * kBN;
         const int blocks = (w.b1 - w.b0) * a.pairs;
         for (int i = 0; i < blocks; ++i) {
-          if (!wait(bar(FULL + s), phase)) {
+          if (!wait(bar(FULL) + s * 8, phase)) {
             ok = false;
             break;
           }
-          s_consumed = ++taken;
           tc::tc_fence_after();
-          const uint32_t da = tc::smem_u32(tiles + s * S::kStageBytes);
-          const uint64_t ad = operand_desc(da, a_mn);
-          const uint64_t bd = operand_desc(da + S::kABytes, b_mn);
+          if (elect_one()) {
+            const uint64_t ad = ad0 + static_cast<uint32_t>(s * (S::kStageBytes >> 4));
+            const uint64_t bd = bd0 + static_cast<uint32_t>(s * (S::kStageBytes >> 4));
 #pragma unroll
-          for (int q = 0; q < kBK / 16; ++q)
-            mma_f16<kPair>(d, ad + q * a_step, bd + q * b_step, idesc, (i | q) != 0);
-          commit(EMPTY + s);
-          if (++s == S::kStages) {
-            s = 0;
-            phase ^= 1;
+            for (int q = 0; q < kBK / 16; ++q)
+              mma_f16<kPair>(d, ad + q * a_step, bd + q * b_step, idesc, (i | q) != 0);
+            commit(empty_at + s * 8);
+            if (i == blocks - 1) commit(bar(ACC_FULL + slot));
           }
+          __syncwarp();
+          s = s + 1 == S::kStages ? 0 : s + 1;
+          phase ^= s == 0;
         }
-        if (!ok) break;
-        commit(ACC_FULL + slot);
       }
       if (*abort_flag) {  // wait (bounded) for the MMAs in flight before their memory goes
-        if constexpr (kPair)
-          tc::umma_commit_pair_mc(bar(DRAIN), 0x1);
-        else
-          tc::umma_commit(bar(DRAIN));
+        if (elect_one()) {
+          if constexpr (kPair)
+            tc::umma_commit_pair_mc(bar(DRAIN), 0x1);
+          else
+            tc::umma_commit(bar(DRAIN));
+        }
+        __syncwarp();
         const uint64_t t0 = tc::gtimer();
         while (!tc::mbar_test(bar(DRAIN), 0) && tc::gtimer() - t0 < g.drain_ns) {
         }
       }
     }
   } else if (warp >= 4) {
+    // Each warp finishes a quarter of the tile's rows and of its columns: a row per lane, 16
+    // columns at a time. Results (and residuals) that TMA can address go through a piece of 32
+    // rows x up to 128 bytes in shared memory, in the tensor map's swizzle, so that memory sees
+    // whole lines and the residual is on its way while the tile is still being multiplied; the
+    // others are stored from registers.
     const int quarter = warp & 3;            // TMEM lanes this warp may read
-    const int group = (warp - 4) >> 2;       // which 16 columns of each 64 it takes
-    static_assert(kEpilogueWarps == 16, "four groups of 16 columns, four lane quarters");
+    const int group = (warp - 4) >> 2;       // which quarter of the columns it takes
+    constexpr int kCols = kBN / 4;
+    unsigned char* piece = pieces + (warp - 4) * kPieceBytes;
+    const uint32_t res_bar = bar(RESIDUAL + warp - 4);
+    uint32_t res_phase = 0;
     int t = 0;
     for (int u = worker; u < units; u += workers, ++t) {
       const Unit w = unit(u);
       const ProductArgs& a = g.p[w.q];
-      const int tm = w.tm, tn = w.tn;
       const int slot = t & 1;
+      const int64_t col0 = static_cast<int64_t>(w.tn) * kBN + group * kCols;
+      const int64_t row0 = static_cast<int64_t>(w.tm) * S::kM + rank * kBM + quarter * 32;
+      const int64_t row = row0 + lane;
       float* bias = s_bias[warp - 4][slot];
       if (a.ep.bias != nullptr) {  // loaded ahead of the wait
-        for (int j = lane; j < kBN / 4; j += 32) {
-          const int64_t col = static_cast<int64_t>(tn) * kBN + (j >> 4) * 64 + group * 16 + (j & 15);
-          bias[j] = col < a.n ? dev::to_f32<T>(static_cast<const T*>(a.ep.bias)[col]) : 0.0f;
-        }
+        for (int j = lane; j < kCols; j += 32)
+          bias[j] = col0 + j < a.n
+                        ? dev::to_f32<T>(static_cast<const T*>(a.ep.bias)[col0 + j]) : 0.0f;
       }
-      const bool ok = wait(bar(ACC_FULL + slot), (t >> 1) & 1);
-      __syncwarp();
-      tc::tc_fence_after();
-      const int64_t row =
-          static_cast<int64_t>(tm) * S::kM + rank * kBM + quarter * 32 + lane;
+      const bool in_tiles = a.splits == 1 && a.ep.out_tiles;
+      const bool res_tiles = a.splits == 1 && a.ep.residual_tiles;
+      // The piece's columns: 128 bytes of the result at most.
+      const int elem = a.ep.out_f32 ? 4 : 2;
+      const int per_piece = min(kCols, 128 / elem);
+      const int row_bytes = per_piece * elem;
+      const uint32_t swizzle = row_bytes == 128 ? 7 : (row_bytes == 64 ? 3 : 1);
+      bool ok = false;
 #pragma unroll 1
-      for (int c = group * 16; c < kBN; c += 64) {
-        const int64_t col = static_cast<int64_t>(tn) * kBN + c;
-        if (col >= a.n) break;
-        float v[16];
-        if (ok) {
-          tmem_ld16(tmem + slot * kBN + c + (static_cast<uint32_t>(quarter * 32) << 16), v);
-        } else {  // the pipeline gave up: the tile is written as NaN
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(0x7fc00000u);
+      for (int c = 0; c < kCols; c += per_piece) {
+        const int64_t col = col0 + c;
+        const bool any = col < a.n && row0 < a.m;
+        if (in_tiles && any) {
+          if (lane == 0) {
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the piece is free
+            if (res_tiles) {
+              tc::mbar_expect_tx(res_bar, 32 * row_bytes);
+              tc::tma_load_2d(tc::smem_u32(piece), &maps.residual[w.q], static_cast<int>(col),
+                              static_cast<int>(row0), res_bar);
+            }
+          }
+          __syncwarp();
         }
-        if (row < a.m) {
-          const int left = static_cast<int>(min(static_cast<int64_t>(16), a.n - col));
-          if (a.splits > 1)
-            put16<float>(a.partial + (static_cast<int64_t>(w.split) * a.m + row) * a.n + col, v,
-                         left, (a.n & 3) == 0 ? 16 : 4);
-          else
-            finish16<T>(a.ep, row, col, v, left, bias + (c >> 6) * 16);
+        if (c == 0) {
+          ok = wait(bar(ACC_FULL + slot), (t >> 1) & 1);
+          __syncwarp();
+          tc::tc_fence_after();
+        }
+        if (!any) continue;
+        if (res_tiles) {
+          if (!wait(res_bar, res_phase)) {
+            // Given up: the copy in flight must land before the piece goes.
+            const uint64_t t0 = tc::gtimer();
+            while (!tc::mbar_test(res_bar, res_phase) && tc::gtimer() - t0 < g.drain_ns) {
+            }
+            ok = false;
+          }
+          res_phase ^= 1;
+          __syncwarp();
+        }
+#pragma unroll 1
+        for (int i = 0; i < per_piece; i += 16) {
+          float v[16];
+          tmem_ld16(tmem + slot * kBN + group * kCols + c + i +
+                        (static_cast<uint32_t>(quarter * 32) << 16), v);
+          if (!ok) {  // the pipeline gave up: the tile is written as NaN
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(0x7fc00000u);
+          }
+          // Columns left, none for a row past the last.
+          const int left =
+              row < a.m ? static_cast<int>(min(static_cast<int64_t>(16), a.n - col - i)) : 0;
+          if (a.splits > 1) {
+            if (left > 0)
+              put16<float>(a.partial + (static_cast<int64_t>(w.split) * a.m + row) * a.n + col + i,
+                           v, left, (a.n & 3) == 0 ? 16 : 4);
+            continue;
+          }
+          finish16_act<T>(a.ep, row, col + i, v, left, bias + c + i);
+          if (!in_tiles) {
+            if (left > 0) finish16_store<T>(a.ep, row, col + i, v, left);
+            continue;
+          }
+          if (!res_tiles && a.ep.residual != nullptr && left > 0) {
+            float r[16];
+            get16<T>(static_cast<const T*>(a.ep.residual) + row * a.ep.residual_stride + col + i,
+                     r, left, a.ep.residual_align);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] += r[j];
+          }
+          auto chunk = [&](int k) {  // 16 bytes of this lane's row of the piece
+            const uint32_t off = lane * row_bytes + i * elem + k * 16;
+            return piece + (off ^ (((off >> 7) & swizzle) << 4));
+          };
+          if (elem == 4) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float4* p = reinterpret_cast<float4*>(chunk(k));
+              float4 y = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+              if (res_tiles) {
+                const float4 r = *p;
+                y = make_float4(y.x + r.x, y.y + r.y, y.z + r.z, y.w + r.w);
+              }
+              *p = y;
+            }
+          } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              Pack<T, 8>* p = reinterpret_cast<Pack<T, 8>*>(chunk(k));
+              if (res_tiles) {
+                const Pack<T, 8> r = *p;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[8 * k + j] += dev::to_f32<T>(r.v[j]);
+              }
+              Pack<T, 8> y;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) y.v[j] = dev::from_f32<T>(v[8 * k + j]);
+              *p = y;
+            }
+          }
+        }
+        if (in_tiles) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0)
+            tma_store_2d(&maps.out[w.q], static_cast<int>(col), static_cast<int>(row0),
+                         tc::smem_u32(piece));
         }
         __syncwarp();
       }
@@ -477,6 +595,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           tc::mbar_arrive(bar(ACC_EMPTY + slot));
       }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -717,6 +836,32 @@ struct Product {
   Stored a, b;
   Epilogue ep;
 };
+// A result or residual of the epilogue's pieces: 32 rows x 128 bytes at most.
+CUtensorMap piece_map(const void* p, int64_t rows, int64_t cols, int64_t stride, uint32_t dtype,
+                      int tile_cols) {
+  CUtensorMap m;
+  const int64_t elem = dtype == QV_DTYPE_F32 ? 4 : 2;
+  const int64_t per_piece = std::min<int64_t>(tile_cols, 128 / elem);
+  const int64_t ld = rows > 1 ? stride : (cols + 7) / 8 * 8;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld * elem)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(per_piece), 32};
+  const cuuint32_t estr[2] = {1, 1};
+  const int64_t bytes = per_piece * elem;
+  const CUresult r = encode_fn()(
+      &m,
+      dtype == QV_DTYPE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+      : dtype == QV_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                              : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+      2, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+      : bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                    : CU_TENSOR_MAP_SWIZZLE_32B,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) fail(QV_ERR_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string(r));
+  return m;
+}
+
 struct ProductPlan {
   int bn = 128;
   bool pair = false;
@@ -787,6 +932,16 @@ void launch_products(const Product* p, int count, const ProductGroup& g, int sms
   for (int q = 0; q < count; ++q) {
     maps.a[q] = operand_map(p[q].a, p[q].a_mn ? kBK : kBM);
     maps.b[q] = operand_map(p[q].b, p[q].b_mn ? kBK : S::kBRows);
+    const Epilogue& ep = p[q].ep;
+    const uint32_t type = std::is_same_v<T, float>    ? QV_DTYPE_F32
+                          : std::is_same_v<T, __half> ? QV_DTYPE_F16
+                                                      : QV_DTYPE_BF16;
+    if (g.p[q].splits == 1 && ep.out_tiles)
+      maps.out[q] = piece_map(ep.out, p[q].m, p[q].n, ep.out_stride,
+                              ep.out_f32 ? QV_DTYPE_F32 : type, kBN / 4);
+    if (g.p[q].splits == 1 && ep.residual_tiles)
+      maps.residual[q] =
+          piece_map(ep.residual, p[q].m, p[q].n, ep.residual_stride, type, kBN / 4);
   }
   static std::once_flag once[16];
   int device = 0;

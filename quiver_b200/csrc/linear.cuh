@@ -20,6 +20,8 @@ struct Epilogue {
   int64_t preact_stride;
   // Bytes that 16-column pieces of each array are aligned to (up to 32).
   int out_align, residual_align, preact_align;
+  // The result (and the residual) can be stored (loaded) as whole tiles by TMA.
+  bool out_tiles, residual_tiles;
 
   static int align32(const void* p, int64_t stride_bytes) {
     const uint64_t bits = 32 | reinterpret_cast<uintptr_t>(p) | static_cast<uint64_t>(stride_bytes);
@@ -30,6 +32,9 @@ struct Epilogue {
     out_align = align32(out, out_stride * (out_f32 ? 4 : e));
     residual_align = align32(residual, residual_stride * e);
     preact_align = align32(preact, preact_stride * e);
+    out_tiles = out_align >= 16;
+    residual_tiles = out_tiles && residual != nullptr && residual_align >= 16 &&
+                     residual_stride != 0 && (out_f32 ? 4 : e) == e;
   }
 };
 
@@ -289,11 +294,11 @@ __device__ __forceinline__ void get16(const T* p, float (&v)[16], int left, int 
   for (int j = 0; j < 16; ++j) v[j] = j < left ? dev::to_f32<T>(u.t[j]) : 0.0f;
 }
 
-// Finishes 16 elements (row, col .. col + left - 1) of a product with inputs of type T; bias: their
-// 16 bias values as float32 in shared memory (16-byte aligned).
+// Finishes 16 elements (row, col .. col + left - 1) of a product with inputs of type T up to the
+// residual; bias: their 16 bias values as float32 in shared memory (16-byte aligned).
 template <class T>
-__device__ __forceinline__ void finish16(const Epilogue& e, int64_t row, int64_t col,
-                                         float (&v)[16], int left, const float* bias) {
+__device__ __forceinline__ void finish16_act(const Epilogue& e, int64_t row, int64_t col,
+                                             float (&v)[16], int left, const float* bias) {
   if (e.bias != nullptr) {
 #pragma unroll
     for (int j = 0; j < 16; j += 4) {
@@ -306,9 +311,14 @@ __device__ __forceinline__ void finish16(const Epilogue& e, int64_t row, int64_t
       v[j + 3] = hi.y;
     }
   }
-  if (e.preact != nullptr)
+  if (e.preact != nullptr && left > 0)
     put16<T>(static_cast<T*>(e.preact) + row * e.preact_stride + col, v, left, e.preact_align);
   activate16<sizeof(T) == 2>(e.act, v);
+}
+// The rest, with plain loads and stores.
+template <class T>
+__device__ __forceinline__ void finish16_store(const Epilogue& e, int64_t row, int64_t col,
+                                               float (&v)[16], int left) {
   if (e.residual != nullptr) {
     float r[16];
     get16<T>(static_cast<const T*>(e.residual) + row * e.residual_stride + col, r, left,
