@@ -231,6 +231,62 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&r)[16]) {
       : "memory");
 }
 
+// One epilogue warp's piece of a tile: 32 rows (one a lane) x kCols columns of 16-bit results, out of
+// tensor memory into shared memory in the tensor map's swizzle. residual: the piece holds it.
+// preact: this lane's row, or nullptr.
+template <class T, int kCols, int kAct>
+__device__ __forceinline__ void finish_piece(uint32_t taddr, const float* bias, T* preact,
+                                             bool preact_wide, bool residual,
+                                             unsigned char* piece, int lane) {
+  constexpr uint32_t kRow = kCols * 2;
+  constexpr uint32_t kSwizzle = kRow == 128 ? 7 : (kRow == 64 ? 3 : 1);
+  const uint32_t row = tc::smem_u32(piece) + lane * kRow;
+  const uint32_t swizzle = ((lane * kRow >> 7) & kSwizzle) << 4;
+#pragma unroll
+  for (int i = 0; i < kCols; i += 16) {
+    float v[16];
+    tmem_ld16(taddr + i, v);
+    if (bias != nullptr) {
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(bias + i + j);
+        const float2 lo = add2(make_float2(v[j], v[j + 1]), make_float2(b.x, b.y));
+        const float2 hi = add2(make_float2(v[j + 2], v[j + 3]), make_float2(b.z, b.w));
+        v[j] = lo.x;
+        v[j + 1] = lo.y;
+        v[j + 2] = hi.x;
+        v[j + 3] = hi.y;
+      }
+    }
+    if (preact != nullptr) put16<T>(preact + i, v, 16, preact_wide ? 32 : 16);
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+      const float2 y = activate2<true>(kAct, make_float2(v[j], v[j + 1]));
+      v[j] = y.x;
+      v[j + 1] = y.y;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t at = row + ((i * 2 + k * 16) ^ swizzle);
+      if (residual) {
+        Pack<T, 8> r;
+        uint4& q = reinterpret_cast<uint4&>(r);
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+                     : "r"(at));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[8 * k + j] += dev::to_f32<T>(r.v[j]);
+      }
+      Pack<T, 8> y;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y.v[j] = dev::from_f32<T>(v[8 * k + j]);
+      const uint4& q = reinterpret_cast<const uint4&>(y);
+      asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(q.x), "r"(q.y),
+                   "r"(q.z), "r"(q.w));
+    }
+  }
+}
+
 template <class T, int kBN, bool kPair>
 __global__ void __launch_bounds__(kProductThreads, 1)
     product_kernel(const __grid_constant__ ProductMaps maps,
@@ -462,6 +518,18 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     unsigned char* piece = pieces + (warp - 4) * kPieceBytes;
     const uint32_t res_bar = bar(RESIDUAL + warp - 4);
     uint32_t res_phase = 0;
+    // Waits for the piece's residual; given up, its copy must still land before the piece goes.
+    auto wait_residual = [&](uint32_t b, uint32_t& phase, bool ok) {
+      if (!wait(b, phase)) {
+        const uint64_t t0 = tc::gtimer();
+        while (!tc::mbar_test(b, phase) && tc::gtimer() - t0 < g.drain_ns) {
+        }
+        ok = false;
+      }
+      phase ^= 1;
+      __syncwarp();
+      return ok;
+    };
     int t = 0;
     for (int u = worker; u < units; u += workers, ++t) {
       const Unit w = unit(u);
@@ -505,16 +573,46 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           tc::tc_fence_after();
         }
         if (!any) continue;
-        if (res_tiles) {
-          if (!wait(res_bar, res_phase)) {
-            // Given up: the copy in flight must land before the piece goes.
-            const uint64_t t0 = tc::gtimer();
-            while (!tc::mbar_test(res_bar, res_phase) && tc::gtimer() - t0 < g.drain_ns) {
+        // 16-bit results in tiles: the parameters in registers and the activation chosen once per
+        // piece. (Reading them per 16 columns made a 128 x 256 tile's epilogue take 10,500 cycles,
+        // more than the MMAs of k = 1024.)
+        if constexpr (sizeof(T) == 2) {
+          if (ok && in_tiles && elem == 2 && (a.ep.residual == nullptr || res_tiles) &&
+              (a.ep.preact == nullptr || (col0 + kCols <= a.n && a.ep.preact_align >= 16))) {
+            if (res_tiles) ok = wait_residual(res_bar, res_phase, ok);
+            if (ok) {
+              const uint32_t taddr = tmem + slot * kBN + group * kCols +
+                                     (static_cast<uint32_t>(quarter * 32) << 16);
+              T* preact = a.ep.preact != nullptr && row < a.m
+                              ? static_cast<T*>(a.ep.preact) + row * a.ep.preact_stride + col0
+                              : nullptr;
+              const bool wide = a.ep.preact_align >= 32;
+              auto finish = [&](auto act) {
+                finish_piece<T, kCols, decltype(act)::value>(
+                    taddr, a.ep.bias != nullptr ? bias : nullptr, preact, wide, res_tiles, piece,
+                    lane);
+              };
+              switch (a.ep.act) {
+                case QV_ACT_RELU: finish(std::integral_constant<int, QV_ACT_RELU>{}); break;
+                case QV_ACT_GELU: finish(std::integral_constant<int, QV_ACT_GELU>{}); break;
+                case QV_ACT_GELU_TANH:
+                  finish(std::integral_constant<int, QV_ACT_GELU_TANH>{});
+                  break;
+                case QV_ACT_SILU: finish(std::integral_constant<int, QV_ACT_SILU>{}); break;
+                default: finish(std::integral_constant<int, QV_ACT_NONE>{}); break;
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+              if (lane == 0)
+                tma_store_2d(&maps.out[w.q], static_cast<int>(col), static_cast<int>(row0),
+                             tc::smem_u32(piece));
+              continue;
             }
-            ok = false;
+          } else if (res_tiles) {
+            ok = wait_residual(res_bar, res_phase, ok);
           }
-          res_phase ^= 1;
-          __syncwarp();
+        } else if (res_tiles) {
+          ok = wait_residual(res_bar, res_phase, ok);
         }
 #pragma unroll 1
         for (int i = 0; i < per_piece; i += 16) {
