@@ -3,10 +3,16 @@
 //
 // The three products run in one tensor-core kernel, product_kernel: D[m][n] = sum_k A[m][k] B[n][k]
 // with either operand stored along k or across it, so that no operand is transposed in memory.
-// 16-bit operands are multiplied as they are. A float32 operand is split into three bfloat16
-// planes whose sum it is (8 + 8 + 8 bits of mantissa), and the product is the sum of the six
-// plane products that reach float32's last bit. Batches of a few rows (single queries) take a
-// kernel that reads the weights once with plain loads.
+// 16-bit operands are multiplied as they are. Float32 operands are split into 16-bit planes whose
+// sum they are, and the product is the sum of the plane products that reach float32's last bit:
+// * x W^T: every row is scaled by a power of two that brings its largest element below 2^15, then
+//   split into two float16 (11 + 11 bits and the sign of the remainder: off by at most 2^-24 of the
+//   element, or 2^-39 of the row's largest where that is more), three products; the scales come off
+//   each result exactly. The sums run along the rows, so a row's scale is a result's.
+// * dz W and dz^T x, whose sums run across the rows: three bfloat16 planes (8 + 8 + 8 bits, no
+//   scales needed), six products.
+// Batches of a few rows (single queries) take a kernel that reads the weights once with plain
+// loads.
 #include <algorithm>
 #include <mutex>
 
@@ -75,7 +81,49 @@ struct PackJob {
   const void* src;
   void* dst;
   int64_t rows, cols, stride, ld;
+  int* exponents;  // scaled rows: each row's scale was 2^-exponent
 };
+
+// float32 rows scaled and split into two float16 planes; one warp per row, which reads it twice
+// (the second time out of the L1).
+template <int kV>
+__global__ void __launch_bounds__(256) split_rows_kernel(const PackJob j0, const PackJob j1) {
+  const PackJob& j = blockIdx.y == 0 ? j0 : j1;
+  const int lane = threadIdx.x & 31;
+  const int64_t plane = j.rows * j.ld;
+  const int64_t warps = gridDim.x * 8ll;
+  for (int64_t r = blockIdx.x * 8ll + (threadIdx.x >> 5); r < j.rows; r += warps) {
+    const float* src = static_cast<const float*>(j.src) + r * j.stride;
+    __half* dst = static_cast<__half*>(j.dst) + r * j.ld;
+    uint32_t top = 0;  // bits of the largest magnitude (which order like the magnitudes)
+#pragma unroll 8
+    for (int64_t c = lane * kV; c < j.cols; c += 32 * kV) {
+      const Pack<float, kV> x = dev::load_pack<float, kV>(src + c);
+#pragma unroll
+      for (int v = 0; v < kV; ++v) top = max(top, __float_as_uint(x.v[v]) & 0x7fffffffu);
+    }
+    top = __reduce_max_sync(dev::kFull, top);
+    // A row of zeros, or one that holds infinity or NaN, stays as it is.
+    const int shift =
+        top == 0 || top >= 0x7f800000u ? 0 : min(14 + 127 - static_cast<int>(top >> 23), 126);
+    const float scale = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
+    if (lane == 0) j.exponents[r] = -shift;
+#pragma unroll 4
+    for (int64_t c = lane * kV; c < j.cols; c += 32 * kV) {
+      const Pack<float, kV> x = dev::load_pack<float, kV>(src + c);
+      Pack<__half, kV> hi, lo;
+#pragma unroll
+      for (int v = 0; v < kV; ++v) {
+        const float y = x.v[v] * scale;
+        hi.v[v] = __float2half_rn(y);
+        lo.v[v] = __hisinf(hi.v[v]) ? __float2half_rn(0.0f)
+                                    : __float2half_rn(y - __half2float(hi.v[v]));
+      }
+      dev::store_pack<__half, kV>(dst + c, hi);
+      dev::store_pack<__half, kV>(dst + plane + c, lo);
+    }
+  }
+}
 
 // Up to two matrices in one launch (blockIdx.y). Bound by memory: every thread moves kV values of
 // kPackRows rows at a time.
@@ -134,13 +182,22 @@ struct Tile {
                                   kEpilogueWarps * kPieceBytes + 1024 + 512;
 };
 
-// Plane pairs of a float32 product, smallest terms first.
-__constant__ int8_t kPairA[6] = {2, 0, 1, 1, 0, 0};
-__constant__ int8_t kPairB[6] = {0, 2, 1, 0, 1, 0};
+// Plane pairs of a product, smallest terms first: of three planes, of two, of one.
+__constant__ int8_t kPairA[10] = {2, 0, 1, 1, 0, 0, 1, 0, 0, 0};
+__constant__ int8_t kPairB[10] = {0, 2, 1, 0, 1, 0, 0, 1, 0, 0};
+__device__ __forceinline__ int first_pair(int pairs) { return pairs == 6 ? 0 : (pairs == 3 ? 6 : 9); }
+// v * 2^e for -252 <= e <= 252: in two steps, neither of which overflows or underflows before the
+// result does.
+__device__ __forceinline__ float times_pow2(float v, int e) {
+  const int h = e >> 1;
+  return v * __int_as_float((127 + h) << 23) * __int_as_float((127 + e - h) << 23);
+}
 
 struct ProductArgs {
   int64_t m, n, k;
-  int pairs;              // plane pairs: 1, or 6 for float32
+  int pairs;              // plane pairs: 1, or 3 or 6 for float32
+  const int* exp_a;       // scaled rows of A and B: their exponents, or nullptr
+  const int* exp_b;
   int k_blocks;           // 64-wide blocks of k
   int tiles_m, tiles_n, splits, blocks_per_split;
   uint32_t idesc;
@@ -303,6 +360,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   __shared__ int s_abort;
   // Each epilogue warp's columns of the bias, two tiles' worth.
   __shared__ __align__(16) float s_bias[kEpilogueWarps][2][kBN / 4];
+  __shared__ int s_exp[kEpilogueWarps][2][sizeof(T) == 4 ? kBN / 4 : 1];  // and of exp_b
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = kPair ? tc::cluster_ctarank() : 0;
   const bool leader = rank == 0;
@@ -402,7 +460,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       const int row_a = w.tm * S::kM + static_cast<int>(rank) * kBM;
       const int row_b = w.tn * kBN + static_cast<int>(rank) * S::kBRows;
       for (int p = 0; p < a.pairs && ok; ++p) {
-        const int pa = a.pairs == 1 ? 0 : kPairA[p], pb = a.pairs == 1 ? 0 : kPairB[p];
+        const int pa = kPairA[first_pair(a.pairs) + p], pb = kPairB[first_pair(a.pairs) + p];
         for (int k0 = w.b0 * kBK; k0 < w.b1 * kBK; k0 += kBK) {
           if (!wait(empty_at + s * 8, phase)) {
             ok = false;
@@ -544,6 +602,14 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           bias[j] = col0 + j < a.n
                         ? dev::to_f32<T>(static_cast<const T*>(a.ep.bias)[col0 + j]) : 0.0f;
       }
+      int* exp_b = s_exp[warp - 4][slot];
+      int exp_a = 0;
+      if constexpr (sizeof(T) == 4) {
+        if (a.exp_a != nullptr) {
+          exp_a = row < a.m ? a.exp_a[row] : 0;
+          for (int j = lane; j < kCols; j += 32) exp_b[j] = col0 + j < a.n ? a.exp_b[col0 + j] : 0;
+        }
+      }
       const bool in_tiles = a.splits == 1 && a.ep.out_tiles;
       const bool res_tiles = a.splits == 1 && a.ep.residual_tiles;
       // The piece's columns: 128 bytes of the result at most.
@@ -622,6 +688,12 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           if (!ok) {  // the pipeline gave up: the tile is written as NaN
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(0x7fc00000u);
+          }
+          if constexpr (sizeof(T) == 4) {
+            if (a.exp_a != nullptr) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[j] = times_pow2(v[j], exp_a + exp_b[c + i + j]);
+            }
           }
           // Columns left, none for a row past the last.
           const int left =
@@ -901,6 +973,7 @@ EncodeFn encode_fn() {
 
 // A stored operand: `outer` rows of `inner` elements, ld apart, `planes` copies plane_stride apart.
 struct Stored {
+  const int* exponents = nullptr;  // of scaled rows
   const void* p = nullptr;
   int64_t inner = 0, outer = 0, ld = 0;
   int planes = 1;
@@ -1083,7 +1156,9 @@ void run_products(const Product* p, int count, const ProductPlan& plan, unsigned
     a.m = p[q].m;
     a.n = p[q].n;
     a.k = p[q].k;
-    a.pairs = std::is_same_v<T, float> ? 6 : 1;
+    a.pairs = p[q].a.planes == 3 ? 6 : (p[q].a.planes == 2 ? 3 : 1);
+    a.exp_a = p[q].a.exponents;
+    a.exp_b = p[q].b.exponents;
     a.k_blocks = plan.k_blocks[q];
     a.tiles_m = static_cast<int>(ceil_div(a.m, plan.pair ? 2 * kBM : kBM));
     a.tiles_n = static_cast<int>(ceil_div(a.n, plan.bn));
@@ -1130,6 +1205,10 @@ bool in_place(uint32_t dtype, const void* p, size_t rows, size_t stride) {
          (rows <= 1 || (stride * 2) % 16 == 0);
 }
 size_t packed_ld(size_t cols) { return (cols + 7) / 8 * 8; }
+// A scaled float32 operand: two float16 planes and the rows' exponents.
+size_t scaled_bytes(size_t rows, size_t cols) {
+  return (rows * packed_ld(cols) * 4 + 255) / 256 * 256 + (rows * 4 + 255) / 256 * 256;
+}
 size_t packed_bytes(uint32_t dtype, size_t rows, size_t cols) {
   return (rows * packed_ld(cols) * 2 * (dtype == QV_DTYPE_F32 ? 3 : 1) + 255) / 256 * 256;
 }
@@ -1138,7 +1217,9 @@ size_t packed_bytes(uint32_t dtype, size_t rows, size_t cols) {
 template <class T>
 class Packer {
  public:
-  Packer(uint32_t dtype, unsigned char* ws) : dtype_(dtype), ws_(ws) {}
+  // scaled: float32 rows as two float16 planes, for products whose sums run along the rows.
+  Packer(uint32_t dtype, bool scaled, unsigned char* ws)
+      : dtype_(dtype), scaled_(scaled && sizeof(T) == 4), ws_(ws) {}
   Stored rows(const void* src, size_t rows, size_t cols, size_t stride) {
     Stored s;
     s.inner = static_cast<int64_t>(cols);
@@ -1151,12 +1232,19 @@ class Packer {
     }
     s.p = ws_;
     s.ld = static_cast<int64_t>(packed_ld(cols));
-    s.planes = Operand<T>::kPlanes;
-    jobs_[count_++] = PackJob{src, ws_, s.outer, s.inner, static_cast<int64_t>(stride), s.ld};
+    s.planes = scaled_ ? 2 : Operand<T>::kPlanes;
+    s.bf16 = s.bf16 && !scaled_;
+    int* exponents = nullptr;
+    if (scaled_)
+      exponents = reinterpret_cast<int*>(ws_ + scaled_bytes(rows, cols) -
+                                         (rows * 4 + 255) / 256 * 256);
+    s.exponents = exponents;
+    jobs_[count_++] =
+        PackJob{src, ws_, s.outer, s.inner, static_cast<int64_t>(stride), s.ld, exponents};
     const size_t e = sizeof(T);
     align_ = std::min(align_, common_align({reinterpret_cast<uintptr_t>(src),
                                             rows > 1 ? stride * e : 0, cols * e}));
-    ws_ += packed_bytes(dtype_, rows, cols);
+    ws_ += scaled_ ? scaled_bytes(rows, cols) : packed_bytes(dtype_, rows, cols);
     return s;
   }
   // Packs what was collected; returns the workspace behind it.
@@ -1175,6 +1263,16 @@ class Packer {
  private:
   template <int kV>
   void launch(cudaStream_t st) {
+    if constexpr (sizeof(T) == 4) {
+      if (scaled_) {
+        const size_t rows = static_cast<size_t>(std::max(jobs_[0].rows, jobs_[count_ - 1].rows));
+        split_rows_kernel<kV>
+            <<<dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(rows, 8), 148 * 8)), count_),
+               256, 0, st>>>(jobs_[0], jobs_[count_ - 1]);
+        check_launch("split_rows_kernel");
+        return;
+      }
+    }
     size_t most = 0;
     for (int i = 0; i < count_; ++i)
       most = std::max(most, ceil_div(jobs_[i].rows, kPackRows) * ceil_div(jobs_[i].cols, kV));
@@ -1183,6 +1281,7 @@ class Packer {
     check_launch("pack_kernel");
   }
   uint32_t dtype_;
+  bool scaled_;
   unsigned char* ws_;
   PackJob jobs_[2];
   int count_ = 0, align_ = 16;
@@ -1260,10 +1359,12 @@ LinearPlan linear_plan(const qv_linear& l, int sms) {
   d.m = static_cast<int64_t>(l.m);
   d.n = static_cast<int64_t>(l.n);
   d.k = static_cast<int64_t>(l.k);
-  p.product = plan_products(&d, 1, l.dtype == QV_DTYPE_F32 ? 6 : 1, sms);
-  if (!in_place(l.dtype, l.x, l.m, l.x_stride)) p.bytes += packed_bytes(l.dtype, l.m, l.k);
-  if (!in_place(l.dtype, l.weight, l.n, l.weight_stride))
-    p.bytes += packed_bytes(l.dtype, l.n, l.k);
+  p.product = plan_products(&d, 1, l.dtype == QV_DTYPE_F32 ? 3 : 1, sms);
+  auto packed = [&](const void* src, size_t rows, size_t stride) -> size_t {
+    if (in_place(l.dtype, src, rows, stride)) return 0;
+    return l.dtype == QV_DTYPE_F32 ? scaled_bytes(rows, l.k) : packed_bytes(l.dtype, rows, l.k);
+  };
+  p.bytes += packed(l.x, l.m, l.x_stride) + packed(l.weight, l.n, l.weight_stride);
   p.bytes += p.product.partial_bytes[0];
   return p;
 }
@@ -1320,7 +1421,7 @@ void linear_forward(const qv_linear& l, void* workspace, size_t workspace_bytes,
         launch_few<T, 8>(l, ep, st);
       return;
     }
-    Packer<T> pack(l.dtype, static_cast<unsigned char*>(workspace));
+    Packer<T> pack(l.dtype, true, static_cast<unsigned char*>(workspace));
     Product d{};
     d.m = static_cast<int64_t>(l.m);
     d.n = static_cast<int64_t>(l.n);
@@ -1493,7 +1594,7 @@ void linear_grad(const qv_linear_grad& g, void* workspace, size_t workspace_byte
       dz.p = g.grad;
       dz.ld = static_cast<int64_t>(g.grad_stride);
     }
-    Packer<T> pack(g.dtype, ws + L.off_packed);
+    Packer<T> pack(g.dtype, false, ws + L.off_packed);
     auto result = [&](void* p, size_t stride) {
       Epilogue ep{};
       ep.out = p;

@@ -325,6 +325,27 @@ def test_linear_shapes_and_strides(embed):
         assert torch.equal(out, embed.linear(x[0], w))
 
 
+def test_linear_float32_ranges(embed):
+    """Rows of very different magnitudes, up to float32's ends: each row keeps float32's accuracy
+    relative to its own largest element."""
+    g = gen(23)
+    m, k, n = 200, 80, 72
+    for xs, ws in ((120, -110), (-120, 100), (0, -126), (-126, 126), (60, 60)):
+        x = normal(g, m, k) * 2.0 ** torch.linspace(xs - 6, xs, m, device="cuda")[:, None]
+        w = normal(g, n, k) * 2.0 ** torch.linspace(ws - 4, ws - 2, n, device="cuda")[:, None]
+        x[5], w[7] = 0, 0
+        want = x.double() @ w.double().t()
+        bound = (x.double().abs() @ w.double().abs().t()) * (k + 8) * 2 * U \
+            + x.double().abs().amax(1, keepdim=True) * w.double().abs().sum(1) * 2.0 ** -38 \
+            + x.double().abs().sum(1, keepdim=True) * w.double().abs().amax(1) * 2.0 ** -38 \
+            + TINY[torch.float32]
+        got = embed.linear(x, w)
+        top = torch.finfo(torch.float32).max
+        inside = (want.abs() + bound) < top
+        assert_within(got[inside], want[inside], bound[inside])
+        assert (got[want.abs() > top * 1.01].isinf()).all()
+
+
 def test_linear_special_values(embed):
     """A row holding NaN or infinity leaves the other rows alone; magnitudes at the types' ends."""
     for t in TYPES.values():
