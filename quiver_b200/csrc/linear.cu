@@ -161,13 +161,20 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackJob j0, const PackJ
 // ring of shared-memory stages with TMA, one thread issues the MMAs into one of two accumulators
 // in tensor memory, and sixteen warps finish the other accumulator's elements meanwhile.
 //
+// The tensor core's float32 sums are cut, not rounded, after each 16 terms: over k terms of one
+// sign the result falls short by about k / 32 * 1.7e-7 of itself (2.6e-5 measured at k = 4096), and
+// sums of random signs lose a fifth of that. So no sum stays there for more than `chunk` blocks of
+// 64 terms: the epilogue warps then add it to one in their registers, rounding, while the next
+// chunk's MMAs fill the other accumulator. Float32 products take chunks of 2 blocks (7e-7), 16-bit
+// ones 128 (5e-5, a fortieth of bfloat16's half step and a tenth of float16's).
+//
 // Large products run in CTA pairs (tcgen05 cta_group::2): 256 x 256 tiles, each CTA loading its
 // 128 rows of A and half of B. A CTA by itself would have to load 384 rows of operands for
 // 128 x 256 results, 96 bytes per SM and cycle at full MMA rate; the pair loads 64.
 
 constexpr int kBM = 128, kBK = 64;  // rows of A per CTA, k per stage
 constexpr int kEpilogueWarps = 16;
-constexpr int kProductThreads = 128 + 32 * kEpilogueWarps;  // producer, MMA, 2 idle, epilogue
+constexpr int kProductThreads = 64 + 32 * kEpilogueWarps;  // producer, MMA, epilogue
 constexpr int kPieceBytes = 4096;  // an epilogue warp's piece of the result: 32 rows x 128 bytes
 
 template <int kBN, bool kPair>
@@ -200,6 +207,7 @@ struct ProductArgs {
   const int* exp_b;
   int k_blocks;           // 64-wide blocks of k
   int tiles_m, tiles_n, splits, blocks_per_split;
+  int chunk;              // blocks of k whose sum stays in tensor memory
   uint32_t idesc;
   uint32_t a_mn, b_mn;    // operand stored across k (MN-major)
   Epilogue ep;
@@ -288,21 +296,38 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&r)[16]) {
       : "memory");
 }
 
-// One epilogue warp's piece of a tile: 32 rows (one a lane) x kCols columns of 16-bit results, out of
-// tensor memory into shared memory in the tensor map's swizzle. residual: the piece holds it.
-// preact: this lane's row, or nullptr.
-template <class T, int kCols, int kAct>
-__device__ __forceinline__ void finish_piece(uint32_t taddr, const float* bias, T* preact,
-                                             bool preact_wide, bool residual,
-                                             unsigned char* piece, int lane) {
-  constexpr uint32_t kRow = kCols * 2;
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16};" ::"r"(taddr),
+      "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]),
+      "f"(r[8]), "f"(r[9]), "f"(r[10]), "f"(r[11]), "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15])
+      : "memory");
+}
+
+// One epilogue warp's piece of a tile: 32 rows (one a lane) x kCols columns of results of type Out,
+// out of tensor memory into shared memory in the tensor map's swizzle. exp_b: the columns'
+// exponents (exp_a: this lane's row's) where operands were scaled, or nullptr. residual: the piece
+// holds it, in type Out. preact: this lane's row, or nullptr.
+template <class T, class Out, int kCols, int kAct>
+__device__ __forceinline__ void finish_piece(uint32_t taddr, const float* bias, const int* exp_b,
+                                             int exp_a, T* preact, bool preact_wide,
+                                             bool residual, unsigned char* piece, int lane) {
+  constexpr uint32_t kRow = kCols * sizeof(Out);
   constexpr uint32_t kSwizzle = kRow == 128 ? 7 : (kRow == 64 ? 3 : 1);
+  constexpr int kPer = 16 / static_cast<int>(sizeof(Out));  // elements of 16 bytes
   const uint32_t row = tc::smem_u32(piece) + lane * kRow;
   const uint32_t swizzle = ((lane * kRow >> 7) & kSwizzle) << 4;
-#pragma unroll
+#pragma unroll(sizeof(T) == 2 ? kCols / 16 : 1)
   for (int i = 0; i < kCols; i += 16) {
     float v[16];
     tmem_ld16(taddr + i, v);
+    if constexpr (sizeof(T) == 4) {
+      if (exp_b != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = times_pow2(v[j], exp_a + exp_b[i + j]);
+      }
+    }
     if (bias != nullptr) {
 #pragma unroll
       for (int j = 0; j < 16; j += 4) {
@@ -318,25 +343,25 @@ __device__ __forceinline__ void finish_piece(uint32_t taddr, const float* bias, 
     if (preact != nullptr) put16<T>(preact + i, v, 16, preact_wide ? 32 : 16);
 #pragma unroll
     for (int j = 0; j < 16; j += 2) {
-      const float2 y = activate2<true>(kAct, make_float2(v[j], v[j + 1]));
+      const float2 y = activate2<sizeof(T) == 2>(kAct, make_float2(v[j], v[j + 1]));
       v[j] = y.x;
       v[j + 1] = y.y;
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const uint32_t at = row + ((i * 2 + k * 16) ^ swizzle);
+    for (int k = 0; k < 16 / kPer; ++k) {
+      const uint32_t at = row + ((i * static_cast<uint32_t>(sizeof(Out)) + k * 16) ^ swizzle);
       if (residual) {
-        Pack<T, 8> r;
+        Pack<Out, kPer> r;
         uint4& q = reinterpret_cast<uint4&>(r);
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
                      : "r"(at));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[8 * k + j] += dev::to_f32<T>(r.v[j]);
+        for (int j = 0; j < kPer; ++j) v[kPer * k + j] += dev::to_f32<Out>(r.v[j]);
       }
-      Pack<T, 8> y;
+      Pack<Out, kPer> y;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y.v[j] = dev::from_f32<T>(v[8 * k + j]);
+      for (int j = 0; j < kPer; ++j) y.v[j] = dev::from_f32<Out>(v[kPer * k + j]);
       const uint4& q = reinterpret_cast<const uint4&>(y);
       asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(q.x), "r"(q.y),
                    "r"(q.z), "r"(q.w));
@@ -344,7 +369,7 @@ __device__ __forceinline__ void finish_piece(uint32_t taddr, const float* bias, 
   }
 }
 
-template <class T, int kBN, bool kPair>
+template <class T, int kBN, bool kPair, bool kChunked>
 __global__ void __launch_bounds__(kProductThreads, 1)
     product_kernel(const __grid_constant__ ProductMaps maps,
                    const __grid_constant__ ProductGroup g) {
@@ -459,9 +484,10 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       const CUtensorMap* map_b = &maps.b[q];
       const int row_a = w.tm * S::kM + static_cast<int>(rank) * kBM;
       const int row_b = w.tn * kBN + static_cast<int>(rank) * S::kBRows;
-      for (int p = 0; p < a.pairs && ok; ++p) {
-        const int pa = kPairA[first_pair(a.pairs) + p], pb = kPairB[first_pair(a.pairs) + p];
-        for (int k0 = w.b0 * kBK; k0 < w.b1 * kBK; k0 += kBK) {
+      for (int pass = 0, c0 = w.b0; c0 < w.b1 && ok;) {  // pairs of planes within chunks of k
+        const int pa = kPairA[first_pair(a.pairs) + pass], pb = kPairB[first_pair(a.pairs) + pass];
+        const int c1 = min(w.b1, c0 + a.chunk);
+        for (int k0 = c0 * kBK; k0 < c1 * kBK; k0 += kBK) {
           if (!wait(empty_at + s * 8, phase)) {
             ok = false;
             break;
@@ -488,6 +514,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           s = s + 1 == S::kStages ? 0 : s + 1;
           phase ^= s == 0;
         }
+        pass = pass + 1 == a.pairs ? 0 : pass + 1;
+        c0 = pass == 0 ? c1 : c0;
       }
     };
     for (int u = worker; u < units && ok; u += workers) {
@@ -519,36 +547,42 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         else
           tc::umma_commit(at);
       };
-      for (int u = worker; u < units && ok; u += workers, ++t) {
+      for (int u = worker; u < units && ok; u += workers) {
         const Unit w = unit(u);
         const ProductArgs& a = g.p[w.q];
         const uint32_t idesc = a.idesc;
         const uint32_t a_step = a.a_mn ? 2048 >> 4 : 32 >> 4, b_step = a.b_mn ? 2048 >> 4 : 32 >> 4;
         const uint64_t ad0 = operand_desc(tiles_at, a.a_mn);
         const uint64_t bd0 = operand_desc(tiles_at + S::kABytes, a.b_mn);
-        const int slot = t & 1;
-        if (!wait(bar(ACC_EMPTY + slot), ((t >> 1) & 1) ^ 1)) break;
-        tc::tc_fence_after();
-        const uint32_t d = tmem + slot * kBN;
-        const int blocks = (w.b1 - w.b0) * a.pairs;
-        for (int i = 0; i < blocks; ++i) {
-          if (!wait(bar(FULL) + s * 8, phase)) {
+        const int pairs = a.pairs, chunk = a.chunk;
+        for (int c0 = w.b0; c0 < w.b1 && ok; c0 += chunk, ++t) {
+          const int slot = t & 1;
+          if (!wait(bar(ACC_EMPTY + slot), ((t >> 1) & 1) ^ 1)) {
             ok = false;
             break;
           }
           tc::tc_fence_after();
-          if (elect_one()) {
-            const uint64_t ad = ad0 + static_cast<uint32_t>(s * (S::kStageBytes >> 4));
-            const uint64_t bd = bd0 + static_cast<uint32_t>(s * (S::kStageBytes >> 4));
+          const uint32_t d = tmem + slot * kBN;
+          const int blocks = min(chunk, w.b1 - c0) * pairs;
+          for (int i = 0; i < blocks; ++i) {
+            if (!wait(bar(FULL) + s * 8, phase)) {
+              ok = false;
+              break;
+            }
+            tc::tc_fence_after();
+            if (elect_one()) {
+              const uint64_t ad = ad0 + static_cast<uint32_t>(s * (S::kStageBytes >> 4));
+              const uint64_t bd = bd0 + static_cast<uint32_t>(s * (S::kStageBytes >> 4));
 #pragma unroll
-            for (int q = 0; q < kBK / 16; ++q)
-              mma_f16<kPair>(d, ad + q * a_step, bd + q * b_step, idesc, (i | q) != 0);
-            commit(empty_at + s * 8);
-            if (i == blocks - 1) commit(bar(ACC_FULL + slot));
+              for (int q = 0; q < kBK / 16; ++q)
+                mma_f16<kPair>(d, ad + q * a_step, bd + q * b_step, idesc, (i | q) != 0);
+              commit(empty_at + s * 8);
+              if (i == blocks - 1) commit(bar(ACC_FULL + slot));
+            }
+            __syncwarp();
+            s = s + 1 == S::kStages ? 0 : s + 1;
+            phase ^= s == 0;
           }
-          __syncwarp();
-          s = s + 1 == S::kStages ? 0 : s + 1;
-          phase ^= s == 0;
         }
       }
       if (*abort_flag) {  // wait (bounded) for the MMAs in flight before their memory goes
@@ -564,17 +598,18 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         }
       }
     }
-  } else if (warp >= 4) {
+  } else {
     // Each warp finishes a quarter of the tile's rows and of its columns: a row per lane, 16
     // columns at a time. Results (and residuals) that TMA can address go through a piece of 32
     // rows x up to 128 bytes in shared memory, in the tensor map's swizzle, so that memory sees
     // whole lines and the residual is on its way while the tile is still being multiplied; the
     // others are stored from registers.
     const int quarter = warp & 3;            // TMEM lanes this warp may read
-    const int group = (warp - 4) >> 2;       // which quarter of the columns it takes
+    const int ew = warp - 2;
+    const int group = ew >> 2;               // which quarter of the columns it takes
     constexpr int kCols = kBN / 4;
-    unsigned char* piece = pieces + (warp - 4) * kPieceBytes;
-    const uint32_t res_bar = bar(RESIDUAL + warp - 4);
+    unsigned char* piece = pieces + ew * kPieceBytes;
+    const uint32_t res_bar = bar(RESIDUAL + ew);
     uint32_t res_phase = 0;
     // Waits for the piece's residual; given up, its copy must still land before the piece goes.
     auto wait_residual = [&](uint32_t b, uint32_t& phase, bool ok) {
@@ -588,21 +623,31 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       __syncwarp();
       return ok;
     };
-    int t = 0;
-    for (int u = worker; u < units; u += workers, ++t) {
+    auto release = [&](int slot) {  // the accumulator may be overwritten
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (kPair)
+          tc::mbar_arrive_cluster(lbar(ACC_EMPTY + slot));
+        else
+          tc::mbar_arrive(bar(ACC_EMPTY + slot));
+      }
+    };
+    int t = 0, parity = 0;  // chunks read so far; of units
+    for (int u = worker; u < units; u += workers, parity ^= 1) {
       const Unit w = unit(u);
       const ProductArgs& a = g.p[w.q];
-      const int slot = t & 1;
+      int slot = 0;  // accumulator of the unit's last chunk, where its sums end up
       const int64_t col0 = static_cast<int64_t>(w.tn) * kBN + group * kCols;
       const int64_t row0 = static_cast<int64_t>(w.tm) * S::kM + rank * kBM + quarter * 32;
       const int64_t row = row0 + lane;
-      float* bias = s_bias[warp - 4][slot];
+      float* bias = s_bias[ew][parity];
       if (a.ep.bias != nullptr) {  // loaded ahead of the wait
         for (int j = lane; j < kCols; j += 32)
           bias[j] = col0 + j < a.n
                         ? dev::to_f32<T>(static_cast<const T*>(a.ep.bias)[col0 + j]) : 0.0f;
       }
-      int* exp_b = s_exp[warp - 4][slot];
+      int* exp_b = s_exp[ew][parity];
       int exp_a = 0;
       if constexpr (sizeof(T) == 4) {
         if (a.exp_a != nullptr) {
@@ -634,51 +679,82 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           __syncwarp();
         }
         if (c == 0) {
-          ok = wait(bar(ACC_FULL + slot), (t >> 1) & 1);
+          ok = wait(bar(ACC_FULL + (t & 1)), (t >> 1) & 1);
           __syncwarp();
           tc::tc_fence_after();
+          slot = t & 1;
+          ++t;
+          if (kChunked && w.b1 - w.b0 > a.chunk) {  // chunks before the last, added up in registers
+            const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+            float sum[kCols];
+#pragma unroll
+            for (int i = 0; i < kCols; i += 16)
+              tmem_ld16(tmem + slot * kBN + group * kCols + i + lanes, *reinterpret_cast<float(*)[16]>(sum + i));
+            for (int c0 = w.b0 + a.chunk; c0 < w.b1; c0 += a.chunk, ++t) {
+              release(slot);
+              slot = t & 1;
+              ok = wait(bar(ACC_FULL + slot), (t >> 1) & 1) && ok;
+              __syncwarp();
+              tc::tc_fence_after();
+#pragma unroll
+              for (int i = 0; i < kCols; i += 16) {
+                float v[16];
+                tmem_ld16(tmem + slot * kBN + group * kCols + i + lanes, v);
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) {
+                  const float2 y = add2(make_float2(sum[i + j], sum[i + j + 1]),
+                                        make_float2(v[j], v[j + 1]));
+                  sum[i + j] = y.x;
+                  sum[i + j + 1] = y.y;
+                }
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < kCols; i += 16)
+              tmem_st16(tmem + slot * kBN + group * kCols + i + lanes, *reinterpret_cast<float(*)[16]>(sum + i));
+            tc::tmem_wait_st();
+          }
         }
         if (!any) continue;
-        // 16-bit results in tiles: the parameters in registers and the activation chosen once per
-        // piece. (Reading them per 16 columns made a 128 x 256 tile's epilogue take 10,500 cycles,
-        // more than the MMAs of k = 1024.)
-        if constexpr (sizeof(T) == 2) {
-          if (ok && in_tiles && elem == 2 && (a.ep.residual == nullptr || res_tiles) &&
-              (a.ep.preact == nullptr || (col0 + kCols <= a.n && a.ep.preact_align >= 16))) {
-            if (res_tiles) ok = wait_residual(res_bar, res_phase, ok);
-            if (ok) {
-              const uint32_t taddr = tmem + slot * kBN + group * kCols +
-                                     (static_cast<uint32_t>(quarter * 32) << 16);
-              T* preact = a.ep.preact != nullptr && row < a.m
-                              ? static_cast<T*>(a.ep.preact) + row * a.ep.preact_stride + col0
-                              : nullptr;
-              const bool wide = a.ep.preact_align >= 32;
-              auto finish = [&](auto act) {
-                finish_piece<T, kCols, decltype(act)::value>(
-                    taddr, a.ep.bias != nullptr ? bias : nullptr, preact, wide, res_tiles, piece,
-                    lane);
-              };
-              switch (a.ep.act) {
-                case QV_ACT_RELU: finish(std::integral_constant<int, QV_ACT_RELU>{}); break;
-                case QV_ACT_GELU: finish(std::integral_constant<int, QV_ACT_GELU>{}); break;
-                case QV_ACT_GELU_TANH:
-                  finish(std::integral_constant<int, QV_ACT_GELU_TANH>{});
-                  break;
-                case QV_ACT_SILU: finish(std::integral_constant<int, QV_ACT_SILU>{}); break;
-                default: finish(std::integral_constant<int, QV_ACT_NONE>{}); break;
+        // Results in tiles: the parameters in registers and the activation chosen once per piece.
+        // (Reading them per 16 columns made a 128 x 256 tile's epilogue take 10,500 cycles, more
+        // than the MMAs of k = 1024.)
+        if (res_tiles) ok = wait_residual(res_bar, res_phase, ok);
+        if (ok && in_tiles && (a.ep.residual == nullptr || res_tiles) &&
+            (a.ep.preact == nullptr || (col + per_piece <= a.n && a.ep.preact_align >= 16))) {
+          const uint32_t taddr = tmem + slot * kBN + group * kCols + c +
+                                 (static_cast<uint32_t>(quarter * 32) << 16);
+          T* preact = a.ep.preact != nullptr && row < a.m
+                          ? static_cast<T*>(a.ep.preact) + row * a.ep.preact_stride + col
+                          : nullptr;
+          const float* b = a.ep.bias != nullptr ? bias + c : nullptr;
+          const int* e = sizeof(T) == 4 && a.exp_a != nullptr ? exp_b + c : nullptr;
+          const bool wide = a.ep.preact_align >= 32;
+          auto finish = [&](auto act) {
+            constexpr int kAct = decltype(act)::value;
+            if constexpr (sizeof(T) == 2) {
+              if (!a.ep.out_f32) {
+                finish_piece<T, T, kCols, kAct>(taddr, b, e, exp_a, preact, wide, res_tiles, piece,
+                                                lane);
+                return;
               }
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              __syncwarp();
-              if (lane == 0)
-                tma_store_2d(&maps.out[w.q], static_cast<int>(col), static_cast<int>(row0),
-                             tc::smem_u32(piece));
-              continue;
             }
-          } else if (res_tiles) {
-            ok = wait_residual(res_bar, res_phase, ok);
+            finish_piece<T, float, (kCols < 32 ? kCols : 32), kAct>(
+                taddr, b, e, exp_a, preact, wide, res_tiles, piece, lane);
+          };
+          switch (a.ep.act) {
+            case QV_ACT_RELU: finish(std::integral_constant<int, QV_ACT_RELU>{}); break;
+            case QV_ACT_GELU: finish(std::integral_constant<int, QV_ACT_GELU>{}); break;
+            case QV_ACT_GELU_TANH: finish(std::integral_constant<int, QV_ACT_GELU_TANH>{}); break;
+            case QV_ACT_SILU: finish(std::integral_constant<int, QV_ACT_SILU>{}); break;
+            default: finish(std::integral_constant<int, QV_ACT_NONE>{}); break;
           }
-        } else if (res_tiles) {
-          ok = wait_residual(res_bar, res_phase, ok);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0)
+            tma_store_2d(&maps.out[w.q], static_cast<int>(col), static_cast<int>(row0),
+                         tc::smem_u32(piece));
+          continue;
         }
 #pragma unroll 1
         for (int i = 0; i < per_piece; i += 16) {
@@ -756,14 +832,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         }
         __syncwarp();
       }
-      tc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (kPair)
-          tc::mbar_arrive_cluster(lbar(ACC_EMPTY + slot));
-        else
-          tc::mbar_arrive(bar(ACC_EMPTY + slot));
-      }
+      release(slot);
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
@@ -1095,7 +1164,7 @@ ProductPlan plan_products(const Product* p, int count, int pairs, int sms) {
   return best;
 }
 
-template <class T, int kBN, bool kPair>
+template <class T, int kBN, bool kPair, bool kChunked>
 void launch_products(const Product* p, int count, const ProductGroup& g, int sms,
                      cudaStream_t st) {
   using S = Tile<kBN, kPair>;
@@ -1118,7 +1187,7 @@ void launch_products(const Product* p, int count, const ProductGroup& g, int sms
   int device = 0;
   QV_CUDA(cudaGetDevice(&device));
   std::call_once(once[device & 15], [&] {
-    QV_CUDA(cudaFuncSetAttribute(product_kernel<T, kBN, kPair>,
+    QV_CUDA(cudaFuncSetAttribute(product_kernel<T, kBN, kPair, kChunked>,
                                  cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  static_cast<int>(S::kSmem)));
   });
@@ -1138,7 +1207,7 @@ void launch_products(const Product* p, int count, const ProductGroup& g, int sms
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }
-  cudaLaunchKernelEx(&cfg, product_kernel<T, kBN, kPair>, maps, g);  // reported by check_launch
+  cudaLaunchKernelEx(&cfg, product_kernel<T, kBN, kPair, kChunked>, maps, g);  // reported by check_launch
   check_launch("product_kernel");
 }
 
@@ -1164,6 +1233,7 @@ void run_products(const Product* p, int count, const ProductPlan& plan, unsigned
     a.tiles_n = static_cast<int>(ceil_div(a.n, plan.bn));
     a.splits = plan.splits[q];
     a.blocks_per_split = plan.blocks_per_split[q];
+    a.chunk = a.pairs > 1 ? 2 : 128;
     const uint32_t fmt = p[q].a.bf16 ? 1 : 0;
     a.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(p[q].a_mn) << 15) |
               (static_cast<uint32_t>(p[q].b_mn) << 16) |
@@ -1183,12 +1253,25 @@ void run_products(const Product* p, int count, const ProductPlan& plan, unsigned
   g.wait_cycles = tc::wait_limit_cycles();
   g.drain_ns = tc::drain_limit_ns();
   if (count > 0) {
-    if (plan.pair)
-      launch_products<T, 256, true>(p, count, g, sms, st);
-    else if (plan.bn == 128)
-      launch_products<T, 128, false>(p, count, g, sms, st);
+    auto launch = [&](auto chunked) {
+      constexpr bool kChunked = decltype(chunked)::value;
+      if (plan.pair)
+        launch_products<T, 256, true, kChunked>(p, count, g, sms, st);
+      else if (plan.bn == 128)
+        launch_products<T, 128, false, kChunked>(p, count, g, sms, st);
+      else
+        launch_products<T, 64, false, kChunked>(p, count, g, sms, st);
+    };
+    // Sums of one chunk (16-bit operands with k up to 8192) leave the adding out of the kernel,
+    // whose registers cost 4 % there.
+    bool chunked = std::is_same_v<T, float>;
+    for (int q = 0; q < count; ++q) chunked |= plan.blocks_per_split[q] > g.p[q].chunk;
+    if constexpr (std::is_same_v<T, float>)
+      launch(std::true_type{});
+    else if (chunked)
+      launch(std::true_type{});
     else
-      launch_products<T, 64, false>(p, count, g, sms, st);
+      launch(std::false_type{});
   }
   if (sums.sums != nullptr) items = std::max(items, static_cast<size_t>(sums.n) * 8);
   if (items > 0) {
