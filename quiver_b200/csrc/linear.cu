@@ -88,6 +88,7 @@ struct PackJob {
 // (the second time out of the L1).
 template <int kV>
 __global__ void __launch_bounds__(256) split_rows_kernel(const PackJob j0, const PackJob j1) {
+  dev::allow_next();
   const PackJob& j = blockIdx.y == 0 ? j0 : j1;
   const int lane = threadIdx.x & 31;
   const int64_t plane = j.rows * j.ld;
@@ -123,6 +124,7 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const PackJob j0, const
       dev::store_pack<__half, kV>(dst + plane + c, lo);
     }
   }
+  dev::wait_previous();
 }
 
 // Up to two matrices in one launch (blockIdx.y). Bound by memory: every thread moves kV values of
@@ -130,6 +132,7 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const PackJob j0, const
 constexpr int kPackRows = 4;
 template <class T, int kV>
 __global__ void __launch_bounds__(256) pack_kernel(const PackJob j0, const PackJob j1) {
+  dev::allow_next();
   const PackJob& j = blockIdx.y == 0 ? j0 : j1;
   using O = typename Operand<T>::type;
   const T* src = static_cast<const T*>(j.src);
@@ -154,6 +157,8 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackJob j0, const PackJ
       put_operand<T, kV>(f, dst, plane, (r0 + u) * j.ld + c);
     }
   }
+  // Chained after the dz kernel, whose results are not used here: its end is this kernel's.
+  dev::wait_previous();
 }
 
 // ---- the product kernel -----------------------------------------------------------------------------
@@ -240,6 +245,9 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         "{%2, %3, %4}], [%5];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 // One lane of a converged warp, the same each time.
 __device__ __forceinline__ bool elect_one() {
@@ -391,9 +399,40 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   const bool leader = rank == 0;
   auto bar = [&](int i) { return tc::smem_u32(bars + i); };
   auto lbar = [&](int i) { return kPair ? tc::mapa_shared(bar(i), 0) : bar(i); };
+  dev::allow_next();
   constexpr int FULL = 0, EMPTY = S::kStages, ACC_FULL = 2 * S::kStages, ACC_EMPTY = ACC_FULL + 2,
                 DRAIN = ACC_EMPTY + 2, RESIDUAL = DRAIN + 1;
   static_assert((RESIDUAL + kEpilogueWarps) * 8 <= 512, "the barriers fit behind the pieces");
+  const int units = g.units[0] + g.units[1];
+  const int worker = kPair ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
+  const int workers = kPair ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
+  // Unit u: product q, split, then tile row / column, columns fastest (a wave's CTAs share rows of
+  // A and all of B in L2), and the split's blocks of k.
+  struct Unit {
+    int q, split, tm, tn, b0, b1;
+  };
+  auto unit = [&](int u) {
+    Unit w;
+    w.q = u >= g.units[0];
+    u -= w.q ? g.units[0] : 0;
+    const ProductArgs& a = g.p[w.q];
+    const int per = a.tiles_m * a.tiles_n;
+    w.split = u / per;
+    const int t = u - w.split * per;
+    w.tm = t / a.tiles_n;
+    w.tn = t - w.tm * a.tiles_n;
+    w.b0 = w.split * a.blocks_per_split;
+    w.b1 = min(a.k_blocks, w.b0 + a.blocks_per_split);
+    return w;
+  };
+
+  // Ahead of the set-up's barrier: the first unit's parameters and tensor maps are on their way
+  // while tensor memory is allocated.
+  const Unit first = unit(worker < units ? worker : 0);
+  if (warp == 0 && elect_one()) {
+    prefetch_map(&maps.a[first.q]);
+    prefetch_map(&maps.b[first.q]);
+  }
   if (threadIdx.x == 0) {
     s_abort = 0;
     for (int s = 0; s < S::kStages; ++s) {
@@ -425,6 +464,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   __syncthreads();
   if constexpr (kPair) tc::cluster_sync();  // both CTAs' barriers exist before either uses them
   tc::tc_fence_after();
+  dev::wait_previous();  // what packed the operands
   const uint32_t tmem = s_tmem;
   volatile int* abort_flag = &s_abort;
   // Bounded wait; false on timeout or abort, after which the CTA's remaining results are NaN.
@@ -446,29 +486,6 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       }
     }
   };
-  const int units = g.units[0] + g.units[1];
-  const int worker = kPair ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
-  const int workers = kPair ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
-  // Unit u: product q, split, then tile row / column, columns fastest (a wave's CTAs share rows of
-  // A and all of B in L2), and the split's blocks of k.
-  struct Unit {
-    int q, split, tm, tn, b0, b1;
-  };
-  auto unit = [&](int u) {
-    Unit w;
-    w.q = u >= g.units[0];
-    u -= w.q ? g.units[0] : 0;
-    const ProductArgs& a = g.p[w.q];
-    const int per = a.tiles_m * a.tiles_n;
-    w.split = u / per;
-    const int t = u - w.split * per;
-    w.tm = t / a.tiles_n;
-    w.tn = t - w.tm * a.tiles_n;
-    w.b0 = w.split * a.blocks_per_split;
-    w.b1 = min(a.k_blocks, w.b0 + a.blocks_per_split);
-    return w;
-  };
-
   // The producer and MMA loops run warp-uniformly and elect a lane for the copies and MMAs alone:
   // their addresses and descriptors then stay in uniform registers, which those instructions take.
   // With a single lane in the whole loop, operands moved there one by one, a block of k took
@@ -519,7 +536,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       }
     };
     for (int u = worker; u < units && ok; u += workers) {
-      const Unit w = unit(u);
+      const Unit w = u == worker ? first : unit(u);
       const int q = w.q;
       // The three forms of a layer's products: x W^T, dz W, dz^T x.
       if (g.p[q].a_mn)
@@ -548,7 +565,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           tc::umma_commit(at);
       };
       for (int u = worker; u < units && ok; u += workers) {
-        const Unit w = unit(u);
+        const Unit w = u == worker ? first : unit(u);
         const ProductArgs& a = g.p[w.q];
         const uint32_t idesc = a.idesc;
         const uint32_t a_step = a.a_mn ? 2048 >> 4 : 32 >> 4, b_step = a.b_mn ? 2048 >> 4 : 32 >> 4;
@@ -635,7 +652,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     };
     int t = 0, parity = 0;  // chunks read so far; of units
     for (int u = worker; u < units; u += workers, parity ^= 1) {
-      const Unit w = unit(u);
+      const Unit w = u == worker ? first : unit(u);
       const ProductArgs& a = g.p[w.q];
       int slot = 0;  // accumulator of the unit's last chunk, where its sums end up
       const int64_t col0 = static_cast<int64_t>(w.tn) * kBN + group * kCols;
@@ -834,7 +851,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       }
       release(slot);
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    // The pieces stay until the last stores have read them.
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -871,6 +889,7 @@ struct JoinJobs {
 };
 template <class T>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinJobs jobs) {
+  dev::wait_previous();
   if (blockIdx.y < 2) {
     const SplitJob& j = jobs.split[blockIdx.y];
     if (j.splits == 0) return;
@@ -930,12 +949,11 @@ __global__ void __launch_bounds__(128)
     const Pack<T, kV> a = dev::load_pack<T, kV>(wr + c);
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      if (r < m) {
-        const Pack<T, kV> b = dev::load_pack<T, kV>(x + r * x_stride + c);
+      // Rows past the last read it again: loads without a branch, so that all are in flight.
+      const Pack<T, kV> b = dev::load_pack<T, kV>(x + min(r, m - 1) * x_stride + c);
 #pragma unroll
-        for (int j = 0; j < kV; ++j)
-          acc[r] = fmaf(dev::to_f32<T>(a.v[j]), dev::to_f32<T>(b.v[j]), acc[r]);
-      }
+      for (int j = 0; j < kV; ++j)
+        acc[r] = fmaf(dev::to_f32<T>(a.v[j]), dev::to_f32<T>(b.v[j]), acc[r]);
     }
   }
 #pragma unroll
@@ -961,6 +979,7 @@ __global__ void __launch_bounds__(32 * kDzWarps)
     dz_kernel(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ z,
               int64_t z_stride, int64_t m, int64_t n, int64_t rows_per_block,
               typename Operand<T>::type* __restrict__ dz, int64_t ld, float* __restrict__ sums) {
+  dev::allow_next();
   __shared__ float part[kDzWarps][32 * kV];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t col = (blockIdx.y * 32ll + lane) * kV;
@@ -1165,7 +1184,7 @@ ProductPlan plan_products(const Product* p, int count, int pairs, int sms) {
 }
 
 template <class T, int kBN, bool kPair, bool kChunked>
-void launch_products(const Product* p, int count, const ProductGroup& g, int sms,
+void launch_products(const Product* p, int count, const ProductGroup& g, bool chained, int sms,
                      cudaStream_t st) {
   using S = Tile<kBN, kPair>;
   ProductMaps maps;
@@ -1198,24 +1217,25 @@ void launch_products(const Product* p, int count, const ProductGroup& g, int sms
   cfg.blockDim = dim3(kProductThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  if (kPair) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-  }
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = chained ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = kPair ? 2 : 1;
   cudaLaunchKernelEx(&cfg, product_kernel<T, kBN, kPair, kChunked>, maps, g);  // reported by check_launch
   check_launch("product_kernel");
 }
 
-// Runs the products and what joins them (with the bias gradient's sums). partial: the plan's
+// Runs the products and what joins them (with the bias gradient's sums); chained: after another
+// launch of the same call. partial: the plan's
 // partial bytes, product by product.
 template <class T>
 void run_products(const Product* p, int count, const ProductPlan& plan, unsigned char* partial,
-                  const SumsJob& sums, int sms, cudaStream_t st) {
+                  const SumsJob& sums, bool chained, int sms, cudaStream_t st) {
   ProductGroup g{};
   JoinJobs jobs{};
   jobs.sums = sums;
@@ -1256,11 +1276,11 @@ void run_products(const Product* p, int count, const ProductPlan& plan, unsigned
     auto launch = [&](auto chunked) {
       constexpr bool kChunked = decltype(chunked)::value;
       if (plan.pair)
-        launch_products<T, 256, true, kChunked>(p, count, g, sms, st);
+        launch_products<T, 256, true, kChunked>(p, count, g, chained, sms, st);
       else if (plan.bn == 128)
-        launch_products<T, 128, false, kChunked>(p, count, g, sms, st);
+        launch_products<T, 128, false, kChunked>(p, count, g, chained, sms, st);
       else
-        launch_products<T, 64, false, kChunked>(p, count, g, sms, st);
+        launch_products<T, 64, false, kChunked>(p, count, g, chained, sms, st);
     };
     // Sums of one chunk (16-bit operands with k up to 8192) leave the adding out of the kernel,
     // whose registers cost 4 % there.
@@ -1275,9 +1295,10 @@ void run_products(const Product* p, int count, const ProductPlan& plan, unsigned
   }
   if (sums.sums != nullptr) items = std::max(items, static_cast<size_t>(sums.n) * 8);
   if (items > 0) {
-    join_kernel<T><<<dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(items, 256), 148 * 8)),
-                          sums.sums != nullptr ? 3 : 2),
-                     256, 0, st>>>(jobs);
+    launch_chained(join_kernel<T>,
+                   dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(items, 256), 148 * 8)),
+                        sums.sums != nullptr ? 3 : 2),
+                   256, 0, st, jobs);
     check_launch("join_kernel");
   }
 }
@@ -1330,22 +1351,24 @@ class Packer {
     ws_ += scaled_ ? scaled_bytes(rows, cols) : packed_bytes(dtype_, rows, cols);
     return s;
   }
-  // Packs what was collected; returns the workspace behind it.
-  unsigned char* run(cudaStream_t st) {
+  int count() const { return count_; }
+  // Packs what was collected (chained: after another launch of the same call); returns the
+  // workspace behind it.
+  unsigned char* run(bool chained, cudaStream_t st) {
     if (count_ == 0) return ws_;
     if (align_ >= 16)
-      launch<16 / sizeof(T)>(st);
+      launch<16 / sizeof(T)>(chained, st);
     else if (align_ == 8)
-      launch<8 / sizeof(T)>(st);
+      launch<8 / sizeof(T)>(chained, st);
     else
-      launch<1>(st);
+      launch<1>(chained, st);
     count_ = 0;
     return ws_;
   }
 
  private:
   template <int kV>
-  void launch(cudaStream_t st) {
+  void launch(bool chained, cudaStream_t st) {
     if constexpr (sizeof(T) == 4) {
       if (scaled_) {
         const size_t rows = static_cast<size_t>(std::max(jobs_[0].rows, jobs_[count_ - 1].rows));
@@ -1360,7 +1383,11 @@ class Packer {
     for (int i = 0; i < count_; ++i)
       most = std::max(most, ceil_div(jobs_[i].rows, kPackRows) * ceil_div(jobs_[i].cols, kV));
     const unsigned blocks = static_cast<unsigned>(std::min<size_t>(ceil_div(most, 256), 148 * 8));
-    pack_kernel<T, kV><<<dim3(blocks, count_), 256, 0, st>>>(jobs_[0], jobs_[count_ - 1]);
+    if (chained)
+      launch_chained(pack_kernel<T, kV>, dim3(blocks, count_), 256, 0, st, jobs_[0],
+                     jobs_[count_ - 1]);
+    else
+      pack_kernel<T, kV><<<dim3(blocks, count_), 256, 0, st>>>(jobs_[0], jobs_[count_ - 1]);
     check_launch("pack_kernel");
   }
   uint32_t dtype_;
@@ -1498,6 +1525,8 @@ void linear_forward(const qv_linear& l, void* workspace, size_t workspace_bytes,
     if (p.few) {
       if (l.m == 1)
         launch_few<T, 1>(l, ep, st);
+      else if (l.m == 2)
+        launch_few<T, 2>(l, ep, st);
       else if (l.m <= 4)
         launch_few<T, 4>(l, ep, st);
       else
@@ -1512,7 +1541,8 @@ void linear_forward(const qv_linear& l, void* workspace, size_t workspace_bytes,
     d.a = pack.rows(l.x, l.m, l.k, l.x_stride);
     d.b = pack.rows(l.weight, l.n, l.k, l.weight_stride);
     d.ep = ep;
-    run_products<T>(&d, 1, p.product, pack.run(st), SumsJob{}, sms, st);
+    const bool packed = pack.count() > 0;
+    run_products<T>(&d, 1, p.product, pack.run(false, st), SumsJob{}, packed, sms, st);
   });
 }
 
@@ -1699,10 +1729,12 @@ void linear_grad(const qv_linear_grad& g, void* workspace, size_t workspace_byte
       d.b = pack.rows(g.weight, g.n, g.k, g.weight_stride);
       d.ep = result(g.dx, g.dx_stride);
     }
-    pack.run(st);
+    const bool first = L.store_dz || sums != nullptr;  // the dz kernel ran
+    const bool chained = first || pack.count() > 0;
+    pack.run(first, st);
     SumsJob sj{};
     if (sums != nullptr) sj = SumsJob{sums, static_cast<int>(L.row_blocks), n, g.dbias};
-    run_products<T>(L.products, L.count, L.plan, ws + L.off_partial, sj, sms, st);
+    run_products<T>(L.products, L.count, L.plan, ws + L.off_partial, sj, chained, sms, st);
   });
 }
 
