@@ -84,8 +84,9 @@ struct PackJob {
   int* exponents;  // scaled rows: each row's scale was 2^-exponent
 };
 
-// float32 rows scaled and split into two float16 planes; one warp per row, which reads it twice
-// (the second time out of the L1).
+// float32 rows scaled and split into two float16 planes; one warp per row, which keeps up to
+// 32 * kSplitHeld pieces of it in registers and reads what is more a second time.
+constexpr int kSplitHeld = 8;
 template <int kV>
 __global__ void __launch_bounds__(256) split_rows_kernel(const PackJob j0, const PackJob j1) {
   dev::allow_next();
@@ -96,22 +97,29 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const PackJob j0, const
   for (int64_t r = blockIdx.x * 8ll + (threadIdx.x >> 5); r < j.rows; r += warps) {
     const float* src = static_cast<const float*>(j.src) + r * j.stride;
     __half* dst = static_cast<__half*>(j.dst) + r * j.ld;
+    Pack<float, kV> held[kSplitHeld];
     uint32_t top = 0;  // bits of the largest magnitude (which order like the magnitudes)
-#pragma unroll 8
-    for (int64_t c = lane * kV; c < j.cols; c += 32 * kV) {
-      const Pack<float, kV> x = dev::load_pack<float, kV>(src + c);
+    auto see = [&](const Pack<float, kV>& x) {
 #pragma unroll
       for (int v = 0; v < kV; ++v) top = max(top, __float_as_uint(x.v[v]) & 0x7fffffffu);
-    }
+    };
+    const int64_t last = j.cols - kV;  // pieces past the row's end read its last: no branches
+#pragma unroll
+    for (int h = 0; h < kSplitHeld; ++h)
+      held[h] = dev::load_pack<float, kV>(src + min(static_cast<int64_t>((h * 32 + lane) * kV), last));
+#pragma unroll
+    for (int h = 0; h < kSplitHeld; ++h) see(held[h]);
+    constexpr int64_t kHeld = kSplitHeld * 32 * kV;
+#pragma unroll 4
+    for (int64_t c = kHeld + lane * kV; c < j.cols; c += 32 * kV)
+      see(dev::load_pack<float, kV>(src + c));
     top = __reduce_max_sync(dev::kFull, top);
     // A row of zeros, or one that holds infinity or NaN, stays as it is.
     const int shift =
         top == 0 || top >= 0x7f800000u ? 0 : min(14 + 127 - static_cast<int>(top >> 23), 126);
     const float scale = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
     if (lane == 0) j.exponents[r] = -shift;
-#pragma unroll 4
-    for (int64_t c = lane * kV; c < j.cols; c += 32 * kV) {
-      const Pack<float, kV> x = dev::load_pack<float, kV>(src + c);
+    auto split = [&](const Pack<float, kV>& x, int64_t c) {
       Pack<__half, kV> hi, lo;
 #pragma unroll
       for (int v = 0; v < kV; ++v) {
@@ -122,7 +130,15 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const PackJob j0, const
       }
       dev::store_pack<__half, kV>(dst + c, hi);
       dev::store_pack<__half, kV>(dst + plane + c, lo);
+    };
+#pragma unroll
+    for (int h = 0; h < kSplitHeld; ++h) {
+      const int64_t c = (h * 32ll + lane) * kV;
+      if (c < j.cols) split(held[h], c);
     }
+#pragma unroll 4
+    for (int64_t c = kHeld + lane * kV; c < j.cols; c += 32 * kV)
+      split(dev::load_pack<float, kV>(src + c), c);
   }
   dev::wait_previous();
 }
@@ -932,38 +948,72 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinJ
 
 // ---- few rows: every weight read once with plain loads -------------------------------------------
 
-// One warp per output column for up to kRows rows of x: lanes stride over k, float32 sums.
-template <class T, int kRows, int kV>
+// One warp per kCols output columns and kRows rows of x: lanes stride over k, float32 sums two terms
+// at a time, and every piece of x is unpacked once for the warp's columns. One row is bound by
+// reading the weights (4096 x 4096 bfloat16: 5.3 us); with eight the arithmetic costs more (18 us
+// with two columns a warp, 20 with one), and narrow layers have too few warps for two columns each
+// (8 rows of 768 x 768: 4.3 us against 5.3).
+template <class T, int kRows, int kCols, int kV>
 __global__ void __launch_bounds__(128)
     few_rows_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ w,
                     int64_t w_stride, int m, int64_t n, int64_t k, Epilogue ep) {
   const int lane = threadIdx.x & 31;
-  const int64_t col = (blockIdx.x * 128ll + threadIdx.x) >> 5;
+  const int64_t col = ((blockIdx.x * 128ll + threadIdx.x) >> 5) * kCols;
   if (col >= n) return;
-  const T* wr = w + col * w_stride;
-  float acc[kRows];
-#pragma unroll
-  for (int r = 0; r < kRows; ++r) acc[r] = 0.0f;
-#pragma unroll 4
-  for (int64_t c = lane * kV; c < k; c += 32 * kV) {
-    const Pack<T, kV> a = dev::load_pack<T, kV>(wr + c);
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      // Rows past the last read it again: loads without a branch, so that all are in flight.
-      const Pack<T, kV> b = dev::load_pack<T, kV>(x + min(r, m - 1) * x_stride + c);
-#pragma unroll
-      for (int j = 0; j < kV; ++j)
-        acc[r] = fmaf(dev::to_f32<T>(a.v[j]), dev::to_f32<T>(b.v[j]), acc[r]);
-    }
-  }
+  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * kRows;
+  x += row0 * x_stride;
+  m -= static_cast<int>(row0);
+  float2 acc[kRows][kCols];
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) acc[r] += __shfl_xor_sync(dev::kFull, acc[r], d);
+    for (int q = 0; q < kCols; ++q) acc[r][q] = both(0.0f);
+  }
+#pragma unroll(kRows* kCols >= 16 ? 1 : 4)
+  for (int64_t c = lane * kV; c < k; c += 32 * kV) {
+    // Columns and rows past the last read it again: loads without a branch, all in flight.
+    Pack<T, kV> a[kCols];
+#pragma unroll
+    for (int q = 0; q < kCols; ++q)
+      a[q] = dev::load_pack<T, kV>(w + min(col + q, n - 1) * w_stride + c);
+    Pack<T, kV> b[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+      b[r] = dev::load_pack<T, kV>(x + min(r, m - 1) * x_stride + c);
+    if constexpr (kV == 1) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+        for (int q = 0; q < kCols; ++q)
+          acc[r][q].x = fmaf(dev::to_f32<T>(a[q].v[0]), dev::to_f32<T>(b[r].v[0]), acc[r][q].x);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kV; j += 2) {
+        float2 wf[kCols];
+#pragma unroll
+        for (int q = 0; q < kCols; ++q)
+          wf[q] = make_float2(dev::to_f32<T>(a[q].v[j]), dev::to_f32<T>(a[q].v[j + (kV > 1)]));
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          const float2 xf =
+              make_float2(dev::to_f32<T>(b[r].v[j]), dev::to_f32<T>(b[r].v[j + (kV > 1)]));
+#pragma unroll
+          for (int q = 0; q < kCols; ++q) acc[r][q] = fma2(wf[q], xf, acc[r][q]);
+        }
+      }
+    }
   }
 #pragma unroll
-  for (int r = 0; r < kRows; ++r)
-    if (r < m && lane == r) finish1<T>(ep, r, col, acc[r]);
+  for (int q = 0; q < kCols; ++q) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      float s = acc[r][q].x + acc[r][q].y;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(dev::kFull, s, d);
+      if (r < m && lane == r && col + q < n) finish1<T>(ep, row0 + r, col + q, s);
+    }
+  }
 }
 
 // ---- dz and the bias gradient ----------------------------------------------------------------------
@@ -1397,7 +1447,17 @@ class Packer {
   int count_ = 0, align_ = 16;
 };
 
-constexpr size_t kMaxFewRows = 8;
+constexpr size_t kWideFew = 2048;  // output columns from which a warp takes two
+// Whether the batch takes the few-rows kernel, by the estimated times in us for W million weights.
+// Measured, 4096 x 4096: 16-bit 4 rows 10.8, 8 rows 18, the tensor cores 12 to 14; float32 8 rows
+// 17, the tensor cores (which split all the weights first) 61. 768 x 768: 8 rows 4.3 and 5.5, the
+// tensor cores 7 and 12.
+bool few_rows(uint32_t dtype, size_t m, size_t n, size_t k) {
+  const double w = static_cast<double>(n) * k * 1e-6;
+  const double groups = static_cast<double>(ceil_div(m, 8));  // each reads the weights again
+  const double few = w * (0.25 + 0.104 * std::min<size_t>(m, 8)) * (1 + 2.2 * (groups - 1));
+  return m <= 256 && few < (dtype == QV_DTYPE_F32 ? 12.0 + 2.9 * w : 7.0 + 0.35 * w);
+}
 constexpr size_t kMaxDim = 65536;
 constexpr size_t kMaxLinearRows = (size_t{1} << 31) - 256;
 
@@ -1463,7 +1523,7 @@ struct LinearPlan {
 };
 LinearPlan linear_plan(const qv_linear& l, int sms) {
   LinearPlan p;
-  p.few = l.m <= kMaxFewRows;
+  p.few = few_rows(l.dtype, l.m, l.n, l.k);
   if (p.few || l.m == 0) return p;
   Product d{};
   d.m = static_cast<int64_t>(l.m);
@@ -1479,17 +1539,18 @@ LinearPlan linear_plan(const qv_linear& l, int sms) {
   return p;
 }
 
-template <class T, int kRows>
+template <class T, int kRows, int kCols>
 void launch_few(const qv_linear& l, const Epilogue& ep, cudaStream_t st) {
   const size_t e = sizeof(T);
   const int align = common_align({reinterpret_cast<uintptr_t>(l.x),
                                   reinterpret_cast<uintptr_t>(l.weight),
                                   l.m > 1 ? l.x_stride * e : 0, l.n > 1 ? l.weight_stride * e : 0,
                                   l.k * e});
-  const unsigned blocks = static_cast<unsigned>(ceil_div(l.n, 4));
+  const dim3 blocks(static_cast<unsigned>(ceil_div(l.n, 4 * kCols)),
+                    static_cast<unsigned>(ceil_div(l.m, kRows)));
   auto go = [&](auto v) {
     constexpr int kV = decltype(v)::value;
-    few_rows_kernel<T, kRows, kV><<<blocks, 128, 0, st>>>(
+    few_rows_kernel<T, kRows, kCols, kV><<<blocks, 128, 0, st>>>(
         static_cast<const T*>(l.x), static_cast<int64_t>(l.x_stride),
         static_cast<const T*>(l.weight), static_cast<int64_t>(l.weight_stride),
         static_cast<int>(l.m), static_cast<int64_t>(l.n), static_cast<int64_t>(l.k), ep);
@@ -1501,6 +1562,18 @@ void launch_few(const qv_linear& l, const Epilogue& ep, cudaStream_t st) {
   else
     go(std::integral_constant<int, 1>{});
   check_launch("few_rows_kernel");
+}
+template <class T>
+void launch_few(const qv_linear& l, const Epilogue& ep, cudaStream_t st) {
+  const bool wide = l.n >= kWideFew;
+  if (l.m == 1)
+    launch_few<T, 1, 1>(l, ep, st);
+  else if (l.m == 2)
+    wide ? launch_few<T, 2, 2>(l, ep, st) : launch_few<T, 2, 1>(l, ep, st);
+  else if (l.m <= 4)
+    wide ? launch_few<T, 4, 2>(l, ep, st) : launch_few<T, 4, 1>(l, ep, st);
+  else
+    wide ? launch_few<T, 8, 2>(l, ep, st) : launch_few<T, 8, 1>(l, ep, st);
 }
 
 }  // namespace
@@ -1523,14 +1596,7 @@ void linear_forward(const qv_linear& l, void* workspace, size_t workspace_bytes,
   by_type(l.dtype, [&](auto t) {
     using T = decltype(t);
     if (p.few) {
-      if (l.m == 1)
-        launch_few<T, 1>(l, ep, st);
-      else if (l.m == 2)
-        launch_few<T, 2>(l, ep, st);
-      else if (l.m <= 4)
-        launch_few<T, 4>(l, ep, st);
-      else
-        launch_few<T, 8>(l, ep, st);
+      launch_few<T>(l, ep, st);
       return;
     }
     Packer<T> pack(l.dtype, true, static_cast<unsigned char*>(workspace));
