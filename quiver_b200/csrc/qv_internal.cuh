@@ -36,6 +36,7 @@ struct Failure {
   do {                                                                                        \
     cudaError_t e_ = (call);                                                                  \
     if (e_ != cudaSuccess) {                                                                  \
+      (void)cudaGetLastError(); /* reported here, not by the next launch's check */           \
       ::qv::fail(e_ == cudaErrorMemoryAllocation ? QV_ERR_OOM : QV_ERR_CUDA,                  \
                  std::string(#call) + ": " + cudaGetErrorString(e_));                         \
     }                                                                                         \

@@ -107,6 +107,24 @@ def _check_out(out, shape, dtype, device):
     return out
 
 
+def _extent(t: torch.Tensor):
+    """First and last-past byte address a tensor reaches."""
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _apart(out: torch.Tensor, **inputs) -> None:
+    """Refuses a caller's result that shares memory with an input."""
+    a, b = _extent(out)
+    for what, t in inputs.items():
+        if t is not None:
+            c, d = _extent(t)
+            if a < d and c < b:
+                raise ValueError(f"out: must not share memory with {what}")
+
+
 # ---- embedding tables -------------------------------------------------------------------------------
 
 
@@ -122,7 +140,7 @@ def _lookup(table, ids, scale, out):
     if out is None:
         out = table.new_empty(shape)
     else:
-        _check_out(out, shape, table.dtype, device)
+        _apart(_check_out(out, shape, table.dtype, device), table=table, ids=ids)
     index = device.index
     check(lib().qv_embedding_lookup_device(index, code, t.data_ptr(), rows, dim,
                                            max(t.stride(0), dim), id_code, i.data_ptr(), i.numel(),
@@ -177,7 +195,7 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, rows: int, scale: floa
     if out is None:
         out = grad.new_empty((rows, dim))
     else:
-        _check_out(out, (rows, dim), grad.dtype, device)
+        _apart(_check_out(out, (rows, dim), grad.dtype, device), grad=grad, ids=ids)
     ws = torch.empty(size.value, dtype=torch.uint8, device=device)
     index = device.index
     check(call.qv_embedding_grad_device(index, code, g.data_ptr(), max(g.stride(0), dim), id_code,
@@ -222,7 +240,8 @@ def _linear(x, weight, bias, residual, activation, out_dtype, want_preact, out=N
     if out is None:
         out = torch.empty(shape, dtype=out_dtype, device=device)
     else:
-        _check_out(out, shape, out_dtype, device)
+        _apart(_check_out(out, shape, out_dtype, device), x=x, weight=weight, bias=bias,
+               residual=residual)
     if want_preact:
         preact = x.new_empty(shape)
     a = _native.qv_linear(code, _DTYPES[out_dtype], act, m, n, k, x2.data_ptr(),
@@ -257,8 +276,8 @@ class _Linear(torch.autograd.Function):
         need = ctx.needs_input_grad
         g = grad if grad.dtype == x.dtype else grad.to(x.dtype)  # of a float32 result
         dx, dw, db = (None, None, None)
-        if need[0] or need[1] or need[2]:
-            dx, dw, db = linear_grad(g, x, weight, preact, ctx.activation, need=need[:3])
+        if need[0] or need[1] or need[2]:  # what the forward pass checked
+            dx, dw, db = _linear_grad(g, x, weight, preact, ACTIVATIONS[ctx.activation], need)
         return dx, dw, db, g if need[3] else None, None, None
 
 
@@ -290,7 +309,7 @@ def linear_grad(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
     """The gradients (dx, dweight, dbias) of :func:`linear` for ``grad`` = d loss / d result, in x's
     type; those not asked for in ``need`` are None. ``preact`` (from :func:`linear_preact`) may be
     None without an activation. The residual's gradient is ``grad`` itself."""
-    code = _dtype_code(x, "x")
+    _dtype_code(x, "x")
     act = _activation_code(activation)
     _dtype_code(weight, "weight")
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
@@ -298,23 +317,30 @@ def linear_grad(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
                          f"{tuple(weight.shape)}")
     n, k = weight.shape
     _like(weight, x, "weight", (n, k))
-    x2 = _rows(x if x.dim() == 2 else x.reshape(x.numel() // k if k else 0, k))
-    m = x2.shape[0]
     shape = (*x.shape[:-1], n)
     _like(grad, x, "grad", shape)
+    if act != 0:
+        if preact is None:
+            raise ValueError("preact: needed for the gradient of an activation")
+        _like(preact, x, "preact", shape)
+    return _linear_grad(grad, x, weight, preact, act, need)
+
+
+def _linear_grad(grad, x, weight, preact, act, need):
+    """:func:`linear_grad` of checked arguments."""
+    n, k = weight.shape
+    x2 = _rows(x if x.dim() == 2 else x.reshape(x.numel() // k if k else 0, k))
+    m = x2.shape[0]
     g = _rows(grad if grad.dim() == 2 else grad.reshape(m, n))
     w = _rows(weight)
     preact_ptr, preact_stride = None, 0
     if act != 0:
-        if preact is None:
-            raise ValueError("preact: needed for the gradient of an activation")
-        p = _like(preact, x, "preact", shape)
-        p = _rows(p if p.dim() == 2 else p.reshape(m, n))
+        p = _rows(preact if preact.dim() == 2 else preact.reshape(m, n))
         preact_ptr, preact_stride = p.data_ptr(), max(p.stride(0), n)
     dx = x.new_empty(x.shape) if need[0] else None
     dw = x.new_empty((n, k)) if need[1] else None
     db = x.new_empty((n,)) if need[2] else None
-    a = _native.qv_linear_grad(code, act, m, n, k, g.data_ptr(), max(g.stride(0), n),
+    a = _native.qv_linear_grad(_DTYPES[x.dtype], act, m, n, k, g.data_ptr(), max(g.stride(0), n),
                                x2.data_ptr(), max(x2.stride(0), k), w.data_ptr(),
                                max(w.stride(0), k), preact_ptr, preact_stride,
                                dx.data_ptr() if need[0] else None, k,

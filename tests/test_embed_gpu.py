@@ -294,7 +294,7 @@ def test_linear_activations(embed, t, act, m):
 
 @pytest.mark.parametrize("t", list(TYPES))
 @pytest.mark.parametrize("m,k,n", [(64, 8192, 128), (40, 4096, 520), (2500, 256, 1100),
-                                   (5000, 1024, 264)])
+                                   (5000, 1024, 264), (6000, 16500, 520), (9000, 20000, 256)])
 def test_linear_splits_and_waves(embed, t, m, k, n):
     """Long sums split over several blocks, and more tiles than the GPU holds at once."""
     x, w, b, r = make(9, m, k, n, TYPES[t])
@@ -653,6 +653,86 @@ def test_rows_behind_the_result_stay(embed):
     assert (out[:5, 24:] == 5).all() and (out[5:] == 5).all()
 
 
+def test_far_offsets(embed):
+    """Tables, results and gradients past 2^31 elements."""
+    rows, dim = 4_300_000, 512
+    table = torch.zeros(rows, dim, dtype=torch.bfloat16, device="cuda")
+    ids = torch.tensor([0, rows - 1, 4_194_304, rows - 1], device="cuda")
+    g = gen(98)
+    mark = normal(g, 3, dim, t=torch.bfloat16)
+    table[ids[:3]] = mark
+    assert torch.equal(embed.embedding_lookup(table, ids), mark[[0, 1, 2, 1]])
+    many = torch.arange(rows, device="cuda").flip(0)
+    got = embed.embedding_lookup(table, many)
+    assert torch.equal(got[[rows - 1, 0, rows - 1 - 4_194_304]], mark)
+    del got
+    up = normal(g, 4, dim, t=torch.bfloat16)
+    grad = embed.embedding_grad(up, ids, rows)
+    assert torch.equal(grad[ids[[0, 2]]], up[[0, 2]])
+    assert torch.equal(grad[rows - 1], (up[1].float() + up[3].float()).bfloat16())
+    assert int((grad != 0).any(1).sum()) == 3
+    del grad
+    # the table as upstream rows: few targets, the same sums
+    target = (many % 3).int()
+    grad = embed.embedding_grad(table, target, 3)
+    want = torch.zeros(3, dim, dtype=torch.float64, device="cuda")
+    want.index_add_(0, target[ids[:3]].long(), mark.double())
+    assert_within(grad, want, want.abs() * half_step(torch.bfloat16) + 2.0 ** -12)
+    del table, grad, many, target
+    # a result past 2^31 elements, and its gradients
+    m, n = 2_200_000, 1024
+    x = normal(g, m, 16, t=torch.bfloat16)
+    w = normal(g, n, 16, t=torch.bfloat16)
+    y = embed.linear(x, w, activation="relu")
+    tail = slice(m - 300, m)
+    assert torch.equal(y[tail], embed.linear(x[tail], w, activation="relu"))
+    dx, dw, _ = embed.linear_grad(y, x, w, need=(True, True, False))
+    want = y[tail].double() @ w.double()
+    mass = y[tail].double().abs() @ w.double().abs()
+    assert_within(dx[tail], want, want.abs() * half_step(torch.bfloat16) + mass * 1032 * 2 * U)
+    part = torch.zeros(n, 16, dtype=torch.float64, device="cuda")
+    for i in range(0, m, 100_000):
+        part += y[i:i + 100_000].double().t() @ x[i:i + 100_000].double()
+    # every partial sum is cut at most once per 16 terms, at 2^-23 of its magnitude
+    mass = torch.zeros_like(part)
+    for i in range(0, m, 100_000):
+        mass += y[i:i + 100_000].double().t() @ x[i:i + 100_000].double().abs()
+    assert_within(dw, part, part.abs() * half_step(torch.bfloat16) + mass * 1024 * 2 * U)
+
+
+@pytest.mark.parametrize("m,k,n,t", [(2000, 512, 512, "bf16"), (8192, 1024, 1024, "bf16"),
+                                     (600, 512, 300, "f32"), (6000, 512, 768, "f32")])
+def test_wait_limit_runs_out(embed, monkeypatch, m, k, n, t):
+    """A pipeline wait that runs out marks its results NaN; the next call is right again. (Single
+    blocks and pairs of them, sums of one chunk and of several.)"""
+    x, w, _, _ = make(99, m, k, n, TYPES[t])
+    want = embed.linear(x, w)
+    r = normal(gen(1), m, n, t=TYPES[t])
+    monkeypatch.setenv("QV_TC_WAIT_LIMIT_US", "1")
+    for res in (None, r):
+        got = embed.linear(x, w, residual=res)
+        ref = want if res is None else embed.linear(x, w, residual=res)
+        torch.cuda.synchronize()
+        ok = got.isnan() | ref.isnan() | (got == ref)
+        assert ok.all()
+    monkeypatch.delenv("QV_TC_WAIT_LIMIT_US")
+    assert torch.equal(embed.linear(x, w), want)
+
+
+def test_bad_device_leaves_no_error(embed):
+    import ctypes as C
+    from quiver_b200 import _native
+    lib = _native.lib()
+    t = torch.ones(4, 8, device="cuda")
+    ids = torch.zeros(2, dtype=torch.long, device="cuda")
+    out = torch.empty(2, 8, device="cuda")
+    with pytest.raises(RuntimeError):
+        _native.check(lib.qv_embedding_lookup_device(97, 0, t.data_ptr(), 4, 8, 8, 1,
+                                                     ids.data_ptr(), 2, 1.0, out.data_ptr(), 8,
+                                                     C.c_void_p(0)))
+    assert torch.equal(embed.embedding_lookup(t, ids), t[:2])
+
+
 def test_refusals(embed):
     x, w, b, r = make(97, 20, 16, 24, torch.float32)
     ids = torch.zeros(3, dtype=torch.long, device="cuda")
@@ -674,6 +754,10 @@ def test_refusals(embed):
               lambda: embed.embedding_grad(x[:3], ids, -1),
               lambda: embed.embedding_grad(x[:3], ids, 2 ** 31),
               lambda: embed.Adapter(w, b, residual=True),
+              lambda: embed.linear(x, x[:16], out=x[:, :].view(20, 16)),
+              lambda: embed.linear(x, w, residual=r, out=r),
+              lambda: embed.embedding_grad(x[:3], ids, 3, out=x[:3]),
+              lambda: embed.embedding_lookup(x, ids, out=x[2:5]),
               lambda: embed.Adapter(w, b[:4])):
         with pytest.raises(E):
             f()
