@@ -152,14 +152,24 @@ __device__ __forceinline__ void clear_rows(const Clear& c, int64_t r0, int64_t r
 // beside ordinary stores instead of 34).
 __device__ __forceinline__ void clear_part(const Clear& c, uint32_t part, uint32_t block,
                                            uint32_t blocks) {
-  if (c.stride == c.row_bytes && c.align == 16) {
+  if (c.stride == c.row_bytes) {
     constexpr int64_t kPiece = 8192;
     __shared__ __align__(128) uint4 zeros[kPiece / 16];
     for (uint32_t i = threadIdx.x; i < kPiece / 16; i += blockDim.x) zeros[i] = uint4{};
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
+    // Whole 16-byte units; what is left at the two ends (2-byte elements) by the first block.
+    const int64_t bytes = c.rows * c.row_bytes;
+    const int64_t lead = min(bytes, static_cast<int64_t>(-reinterpret_cast<intptr_t>(c.p) & 15));
+    const int64_t units = (bytes - lead) / 16;
+    unsigned char* body = c.p + lead;
+    if (part == 0 && block == 0) {
+      for (int64_t i = threadIdx.x * 2; i < lead; i += blockDim.x * 2)
+        *reinterpret_cast<uint16_t*>(c.p + i) = 0;
+      for (int64_t i = units * 16 + threadIdx.x * 2; i < bytes - lead; i += blockDim.x * 2)
+        *reinterpret_cast<uint16_t*>(body + i) = 0;
+    }
     if (threadIdx.x != 0) return;
-    const int64_t units = c.rows * (c.row_bytes / 16);
     const int64_t u0 = units * part / c.parts, u1 = units * (part + 1) / c.parts;
     const int64_t per = (u1 - u0 + blocks - 1) / blocks;
     const int64_t begin = (u0 + per * block) * 16, end = min(u1, u0 + per * (block + 1)) * 16;
@@ -172,7 +182,7 @@ __device__ __forceinline__ void clear_part(const Clear& c, uint32_t part, uint32
         told = true;
       }
       const uint32_t bytes = static_cast<uint32_t>(min(kPiece, end - at));
-      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(c.p + at),
+      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(body + at),
                    "r"(static_cast<uint32_t>(__cvta_generic_to_shared(zeros))), "r"(bytes)
                    : "memory");
       asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 3;" ::: "memory");
@@ -460,18 +470,18 @@ constexpr int kSumBatch = 4;  // rows in flight per lane
 constexpr int kMaxRun = 32;   // entries per warp
 constexpr uint32_t kNoRow = 0xffffffffu;
 
-template <class T, int kV>
+template <class T, int kV, int kC>
 __global__ void __launch_bounds__(kSumThreads, 5)
     segment_sum_kernel(const T* __restrict__ up, int64_t up_stride,
                        const uint32_t* keys, const uint32_t* pos, uint32_t n, uint32_t rows,
-                       uint32_t dim, uint32_t run, uint32_t col_tiles, float scale, T* __restrict__ grad,
-                       int64_t grad_stride, float* head, float* tail, uint32_t* head_row,
+                       uint32_t dim, uint32_t run, uint32_t col_tiles, float scale,
+                       T* __restrict__ grad, int64_t grad_stride, float* head, float* tail, uint32_t* head_row,
                        uint32_t* tail_row) {
   dev::allow_next();
   dev::wait_previous();
   // The column tiles of the same entries are neighbours: they read the same rows at a time.
   const uint32_t block = blockIdx.x / col_tiles, col_tile = blockIdx.x - block * col_tiles;
-  constexpr uint32_t kCols = 32 * kV;
+  constexpr uint32_t kCols = 32 * kV * kC;
   __shared__ __align__(16) float s_head[kSumWarps][kCols];
   __shared__ __align__(16) float s_tail[kSumWarps][kCols];
   // Keys of the block's entries with the one before and the one after; kNoRow outside.
@@ -488,9 +498,15 @@ __global__ void __launch_bounds__(kSumThreads, 5)
   }
   __syncthreads();
   const uint32_t col0 = col_tile * kCols;
-  const bool on = col0 + lane * kV < dim;
-  const uint32_t c = on ? col0 + lane * kV : col0;  // lanes past the last column read the first
-  const T* src = up + c;
+  // This lane's columns: kC pieces of kV. Pieces past the last column read the first.
+  uint32_t c[kC];
+  bool on[kC];
+#pragma unroll
+  for (int q = 0; q < kC; ++q) {
+    c[q] = col0 + (q * 32 + lane) * kV;
+    on[q] = c[q] < dim;
+    if (!on[q]) c[q] = col0;
+  }
   const uint32_t e0 = min(count, warp * run), e1 = min(count, e0 + run);
   const int before = static_cast<int>(e0) - 1;
   const uint32_t r0 = e0 < e1 ? s_key[e0] : kNoRow;
@@ -501,31 +517,49 @@ __global__ void __launch_bounds__(kSumThreads, 5)
   const bool has_tail = e0 < e1 && last < rows && s_key[e1] == last;
   if (lane == 0) s_tail_row[warp] = has_tail ? last : kNoRow;
   const bool ends_first = began_before && !(has_tail && last == r0);
-  float acc[kV];
+  float acc[kC][kV];
+  auto clear_acc = [&]() {
 #pragma unroll
-  for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
+    for (int q = 0; q < kC; ++q) {
+#pragma unroll
+      for (int j = 0; j < kV; ++j) acc[q][j] = 0.0f;
+    }
+  };
+  auto keep = [&](float* to) {
+#pragma unroll
+    for (int q = 0; q < kC; ++q) {
+#pragma unroll
+      for (int j = 0; j < kV; ++j) to[(q * 32 + lane) * kV + j] = acc[q][j];
+    }
+  };
+  clear_acc();
   bool is_head = began_before;
   uint32_t r = r0;
   auto finish_row = [&]() {
     if (is_head) {
+      keep(s_head[warp]);
+    } else if (r < rows) {
 #pragma unroll
-      for (int j = 0; j < kV; ++j) s_head[warp][lane * kV + j] = acc[j];
-    } else if (on && r < rows) {
-      Pack<T, kV> y;
+      for (int q = 0; q < kC; ++q) {
+        if (!on[q]) continue;
+        Pack<T, kV> y;
 #pragma unroll
-      for (int j = 0; j < kV; ++j) y.v[j] = dev::from_f32<T>(acc[j] * scale);
-      dev::stream_pack<T, kV>(grad + static_cast<int64_t>(r) * grad_stride + c, y);
+        for (int j = 0; j < kV; ++j) y.v[j] = dev::from_f32<T>(acc[q][j] * scale);
+        dev::stream_pack<T, kV>(grad + static_cast<int64_t>(r) * grad_stride + c[q], y);
+      }
     }
-#pragma unroll
-    for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
+    clear_acc();
     is_head = false;
   };
   for (uint32_t e = e0; e < e1; e += kSumBatch) {
     if (s_key[e] >= rows) break;  // ids that take no gradient, all at the end
-    Pack<T, kV> x[kSumBatch];
+    Pack<T, kV> x[kSumBatch][kC];
 #pragma unroll
-    for (int j = 0; j < kSumBatch; ++j)  // past the run its last row again: loads without a branch
-      x[j] = dev::load_once<T, kV>(src + s_pos[min(e + j, e1 - 1)] * up_stride);
+    for (int j = 0; j < kSumBatch; ++j) {  // past the run its last row again: no branches
+      const T* src = up + s_pos[min(e + j, e1 - 1)] * up_stride;
+#pragma unroll
+      for (int q = 0; q < kC; ++q) x[j][q] = dev::load_once<T, kV>(src + c[q]);
+    }
 #pragma unroll
     for (int j = 0; j < kSumBatch; ++j) {
       if (e + j >= e1) break;
@@ -535,12 +569,14 @@ __global__ void __launch_bounds__(kSumThreads, 5)
         r = k;
       }
 #pragma unroll
-      for (int v = 0; v < kV; ++v) acc[v] += dev::to_f32<T>(x[j].v[v]);
+      for (int q = 0; q < kC; ++q) {
+#pragma unroll
+        for (int v = 0; v < kV; ++v) acc[q][v] += dev::to_f32<T>(x[j][q].v[v]);
+      }
     }
   }
   if (has_tail) {
-#pragma unroll
-    for (int j = 0; j < kV; ++j) s_tail[warp][lane * kV + j] = acc[j];
+    keep(s_tail[warp]);
   } else if (e0 < e1) {
     finish_row();
   }
@@ -743,9 +779,10 @@ void launch_sums(const GradPlan& p, int which, const void* up, size_t up_stride,
   float* tail = reinterpret_cast<float*>(ws + p.off_tail);
   uint32_t* head_row = reinterpret_cast<uint32_t*>(ws + p.off_row);
   uint32_t* tail_row = reinterpret_cast<uint32_t*>(ws + p.off_open);
-  const size_t col_tiles = ceil_div(dim, 32 * kV);
+  constexpr int kC = kV * sizeof(T) < 8 ? 4 : 1;  // narrow pieces: four a lane
+  const size_t col_tiles = ceil_div(dim, 32 * kV * kC);
   QV_REQUIRE(p.blocks * col_tiles < (size_t{1} << 31), "n * dim is too large");
-  launch_chained(segment_sum_kernel<T, kV>,
+  launch_chained(segment_sum_kernel<T, kV, kC>,
                  static_cast<unsigned>(p.blocks * col_tiles), kSumThreads, 0, st,
                  static_cast<const T*>(up), static_cast<int64_t>(up_stride), keys, pos, n, rows,
                  dim, p.run, static_cast<uint32_t>(col_tiles), scale, static_cast<T*>(grad), static_cast<int64_t>(grad_stride), head,

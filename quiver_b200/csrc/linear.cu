@@ -332,11 +332,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&r)[16]) 
 // One epilogue warp's piece of a tile: 32 rows (one a lane) x kCols columns of results of type Out,
 // out of tensor memory into shared memory in the tensor map's swizzle. exp_b: the columns'
 // exponents (exp_a: this lane's row's) where operands were scaled, or nullptr. residual: the piece
-// holds it, in type Out. preact: this lane's row, or nullptr.
+// holds it, in type Out. preact: this lane's row, or nullptr. !ok: the pipeline gave up, NaN.
 template <class T, class Out, int kCols, int kAct>
-__device__ __forceinline__ void finish_piece(uint32_t taddr, const float* bias, const int* exp_b,
-                                             int exp_a, T* preact, bool preact_wide,
-                                             bool residual, unsigned char* piece, int lane) {
+__device__ __forceinline__ void finish_piece(uint32_t taddr, bool ok, const float* bias,
+                                             const int* exp_b, int exp_a, T* preact,
+                                             bool preact_wide, bool residual,
+                                             unsigned char* piece, int lane) {
   constexpr uint32_t kRow = kCols * sizeof(Out);
   constexpr uint32_t kSwizzle = kRow == 128 ? 7 : (kRow == 64 ? 3 : 1);
   constexpr int kPer = 16 / static_cast<int>(sizeof(Out));  // elements of 16 bytes
@@ -346,6 +347,10 @@ __device__ __forceinline__ void finish_piece(uint32_t taddr, const float* bias, 
   for (int i = 0; i < kCols; i += 16) {
     float v[16];
     tmem_ld16(taddr + i, v);
+    if (!ok) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(0x7fc00000u);
+    }
     if constexpr (sizeof(T) == 4) {
       if (exp_b != nullptr) {
 #pragma unroll
@@ -389,6 +394,58 @@ __device__ __forceinline__ void finish_piece(uint32_t taddr, const float* bias, 
       const uint4& q = reinterpret_cast<const uint4&>(y);
       asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(q.x), "r"(q.y),
                    "r"(q.z), "r"(q.w));
+    }
+  }
+}
+
+// The preactivations of a piece's columns where they can neither be stored whole nor through the
+// piece: each lane its row.
+template <class T>
+__device__ __forceinline__ void store_preact(uint32_t taddr, bool ok, const float* bias,
+                                             const int* exp_b, int exp_a, T* first,
+                                             int64_t stride, int rows, int cols, int lane) {
+  for (int i = 0; i < cols; i += 16) {
+    float v[16];
+    tmem_ld16(taddr + i, v);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      if (sizeof(T) == 4 && exp_b != nullptr) v[j] = times_pow2(v[j], exp_a + exp_b[i + j]);
+      if (bias != nullptr) v[j] += bias[i + j];
+      if (!ok) v[j] = __uint_as_float(0x7fc00000u);
+    }
+    if (lane < rows) put16<T>(first + lane * stride + i, v, min(16, cols - i), 2);
+  }
+}
+
+// Stores a piece of kCols float32 columns to rows of any alignment: lanes along a row, so that a row's
+// columns are written together; residual (at the piece's first element, or nullptr) is added first.
+template <class T, class Out, int kCols>
+__device__ __forceinline__ void store_piece(const unsigned char* piece, Out* out, int64_t stride,
+                                            const T* residual, int64_t residual_stride, int rows,
+                                            int cols, int lane) {
+  constexpr uint32_t kRow = kCols * 4;
+  constexpr uint32_t kSwizzle = kRow == 128 ? 7 : 3;
+  constexpr int kPerStep = 32 / kCols;  // rows at a time
+  constexpr int kBatch = 8;             // steps whose residuals are in flight together
+  const int c = lane % kCols;
+  const bool in = c < cols;
+#pragma unroll 1
+  for (int b = 0; b < 32; b += kBatch * kPerStep) {
+    T res[kBatch];
+    if (residual != nullptr) {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int r = min(b + u * kPerStep + lane / kCols, rows - 1);
+        res[u] = residual[r * residual_stride + min(c, cols - 1)];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int r = b + u * kPerStep + lane / kCols;
+      const uint32_t off = r * kRow + c * 4;
+      float v = *reinterpret_cast<const float*>(piece + (off ^ (((off >> 7) & kSwizzle) << 4)));
+      if (residual != nullptr) v += dev::to_f32<T>(res[u]);
+      if (in && r < rows) out[r * stride + c] = dev::from_f32<Out>(v);
     }
   }
 }
@@ -688,23 +745,23 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           for (int j = lane; j < kCols; j += 32) exp_b[j] = col0 + j < a.n ? a.exp_b[col0 + j] : 0;
         }
       }
-      const bool in_tiles = a.splits == 1 && a.ep.out_tiles;
       const bool res_tiles = a.splits == 1 && a.ep.residual_tiles;
-      // The piece's columns: 128 bytes of the result at most.
-      const int elem = a.ep.out_f32 ? 4 : 2;
-      const int per_piece = min(kCols, 128 / elem);
-      const int row_bytes = per_piece * elem;
-      const uint32_t swizzle = row_bytes == 128 ? 7 : (row_bytes == 64 ? 3 : 1);
+      const bool in_tiles =
+          a.splits == 1 && a.ep.out_tiles && (a.ep.residual == nullptr || res_tiles);
+      // The piece's columns: 128 bytes at most, of the result or, where that is not stored as a
+      // tile, of float32.
+      constexpr int kWide = kCols < 32 ? kCols : 32;
+      const int per_piece = in_tiles && !a.ep.out_f32 ? kCols : kWide;
       bool ok = false;
 #pragma unroll 1
       for (int c = 0; c < kCols; c += per_piece) {
         const int64_t col = col0 + c;
         const bool any = col < a.n && row0 < a.m;
-        if (in_tiles && any) {
+        if (any) {
           if (lane == 0) {
             asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the piece is free
             if (res_tiles) {
-              tc::mbar_expect_tx(res_bar, 32 * row_bytes);
+              tc::mbar_expect_tx(res_bar, 32 * per_piece * (a.ep.out_f32 ? 4 : 2));
               tc::tma_load_2d(tc::smem_u32(piece), &maps.residual[w.q], static_cast<int>(col),
                               static_cast<int>(row0), res_bar);
             }
@@ -749,39 +806,58 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           }
         }
         if (!any) continue;
-        // Results in tiles: the parameters in registers and the activation chosen once per piece.
-        // (Reading them per 16 columns made a 128 x 256 tile's epilogue take 10,500 cycles, more
-        // than the MMAs of k = 1024.)
+        // The parameters in registers and the activation chosen once per piece. (Reading them per
+        // 16 columns made a 128 x 256 tile's epilogue take 10,500 cycles, more than the MMAs of
+        // k = 1024.)
         if (res_tiles) ok = wait_residual(res_bar, res_phase, ok);
-        if (ok && in_tiles && (a.ep.residual == nullptr || res_tiles) &&
-            (a.ep.preact == nullptr || (col + per_piece <= a.n && a.ep.preact_align >= 16))) {
-          const uint32_t taddr = tmem + slot * kBN + group * kCols + c +
-                                 (static_cast<uint32_t>(quarter * 32) << 16);
-          T* preact = a.ep.preact != nullptr && row < a.m
-                          ? static_cast<T*>(a.ep.preact) + row * a.ep.preact_stride + col
-                          : nullptr;
-          const float* b = a.ep.bias != nullptr ? bias + c : nullptr;
-          const int* e = sizeof(T) == 4 && a.exp_a != nullptr ? exp_b + c : nullptr;
-          const bool wide = a.ep.preact_align >= 32;
-          auto finish = [&](auto act) {
-            constexpr int kAct = decltype(act)::value;
-            if constexpr (sizeof(T) == 2) {
-              if (!a.ep.out_f32) {
-                finish_piece<T, T, kCols, kAct>(taddr, b, e, exp_a, preact, wide, res_tiles, piece,
-                                                lane);
-                return;
-              }
-            }
-            finish_piece<T, float, (kCols < 32 ? kCols : 32), kAct>(
-                taddr, b, e, exp_a, preact, wide, res_tiles, piece, lane);
-          };
-          switch (a.ep.act) {
+        const uint32_t taddr = tmem + slot * kBN + group * kCols + c +
+                               (static_cast<uint32_t>(quarter * 32) << 16);
+        const float* b = a.splits == 1 && a.ep.bias != nullptr ? bias + c : nullptr;
+        const int* e = sizeof(T) == 4 && a.exp_a != nullptr ? exp_b + c : nullptr;
+        auto by_act = [&](int act, auto&& finish) {
+          switch (act) {
             case QV_ACT_RELU: finish(std::integral_constant<int, QV_ACT_RELU>{}); break;
             case QV_ACT_GELU: finish(std::integral_constant<int, QV_ACT_GELU>{}); break;
             case QV_ACT_GELU_TANH: finish(std::integral_constant<int, QV_ACT_GELU_TANH>{}); break;
             case QV_ACT_SILU: finish(std::integral_constant<int, QV_ACT_SILU>{}); break;
             default: finish(std::integral_constant<int, QV_ACT_NONE>{}); break;
           }
+        };
+        auto finish_f32 = [&](int act, T* preact, bool wide, bool residual) {
+          by_act(act, [&](auto k) {
+            finish_piece<T, float, kWide, decltype(k)::value>(taddr, ok, b, e, exp_a, preact, wide,
+                                                              residual, piece, lane);
+          });
+          __syncwarp();
+        };
+        const int rows = static_cast<int>(min(static_cast<int64_t>(32), a.m - row0));
+        const int cols = static_cast<int>(min(static_cast<int64_t>(per_piece), a.n - col));
+        // Preactivations: whole aligned pieces straight from the registers, others by a pass of
+        // their own.
+        T* preact = nullptr;
+        bool wide = false;
+        if (a.splits == 1 && a.ep.preact != nullptr) {
+          T* first = static_cast<T*>(a.ep.preact) + row0 * a.ep.preact_stride + col;
+          if (in_tiles && cols == per_piece && a.ep.preact_align >= 16) {
+            preact = row < a.m ? first + lane * a.ep.preact_stride : nullptr;
+            wide = a.ep.preact_align >= 32;
+          } else if (!res_tiles && per_piece == kWide) {
+            finish_f32(QV_ACT_NONE, nullptr, false, false);
+            store_piece<T, T, kWide>(piece, first, a.ep.preact_stride, nullptr, 0, rows, cols, lane);
+            __syncwarp();
+          } else {  // the piece holds the residual, or more columns than float32 has room for
+            store_preact<T>(taddr, ok, b, e, exp_a, first, a.ep.preact_stride, rows, cols, lane);
+          }
+        }
+        if (in_tiles) {
+          if constexpr (sizeof(T) == 2) {
+            if (!a.ep.out_f32)
+              by_act(a.ep.act, [&](auto k) {
+                finish_piece<T, T, kCols, decltype(k)::value>(taddr, ok, b, e, exp_a, preact, wide,
+                                                              res_tiles, piece, lane);
+              });
+          }
+          if (sizeof(T) == 4 || a.ep.out_f32) finish_f32(a.ep.act, preact, wide, res_tiles);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0)
@@ -789,79 +865,26 @@ __global__ void __launch_bounds__(kProductThreads, 1)
                          tc::smem_u32(piece));
           continue;
         }
-#pragma unroll 1
-        for (int i = 0; i < per_piece; i += 16) {
-          float v[16];
-          tmem_ld16(tmem + slot * kBN + group * kCols + c + i +
-                        (static_cast<uint32_t>(quarter * 32) << 16), v);
-          if (!ok) {  // the pipeline gave up: the tile is written as NaN
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(0x7fc00000u);
-          }
-          if constexpr (sizeof(T) == 4) {
-            if (a.exp_a != nullptr) {
-#pragma unroll
-              for (int j = 0; j < 16; ++j) v[j] = times_pow2(v[j], exp_a + exp_b[c + i + j]);
-            }
-          }
-          // Columns left, none for a row past the last.
-          const int left =
-              row < a.m ? static_cast<int>(min(static_cast<int64_t>(16), a.n - col - i)) : 0;
-          if (a.splits > 1) {
-            if (left > 0)
-              put16<float>(a.partial + (static_cast<int64_t>(w.split) * a.m + row) * a.n + col + i,
-                           v, left, (a.n & 3) == 0 ? 16 : 4);
-            continue;
-          }
-          finish16_act<T>(a.ep, row, col + i, v, left, bias + c + i);
-          if (!in_tiles) {
-            if (left > 0) finish16_store<T>(a.ep, row, col + i, v, left);
-            continue;
-          }
-          if (!res_tiles && a.ep.residual != nullptr && left > 0) {
-            float r[16];
-            get16<T>(static_cast<const T*>(a.ep.residual) + row * a.ep.residual_stride + col + i,
-                     r, left, a.ep.residual_align);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] += r[j];
-          }
-          auto chunk = [&](int k) {  // 16 bytes of this lane's row of the piece
-            const uint32_t off = lane * row_bytes + i * elem + k * 16;
-            return piece + (off ^ (((off >> 7) & swizzle) << 4));
-          };
-          if (elem == 4) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              float4* p = reinterpret_cast<float4*>(chunk(k));
-              float4 y = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-              if (res_tiles) {
-                const float4 r = *p;
-                y = make_float4(y.x + r.x, y.y + r.y, y.z + r.z, y.w + r.w);
-              }
-              *p = y;
-            }
-          } else if constexpr (sizeof(T) == 2) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              Pack<T, 8>* p = reinterpret_cast<Pack<T, 8>*>(chunk(k));
-              if (res_tiles) {
-                const Pack<T, 8> r = *p;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[8 * k + j] += dev::to_f32<T>(r.v[j]);
-              }
-              Pack<T, 8> y;
-#pragma unroll
-              for (int j = 0; j < 8; ++j) y.v[j] = dev::from_f32<T>(v[8 * k + j]);
-              *p = y;
-            }
-          }
-        }
-        if (in_tiles) {
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0)
-            tma_store_2d(&maps.out[w.q], static_cast<int>(col), static_cast<int>(row0),
-                         tc::smem_u32(piece));
+        // Rows that TMA cannot address, a residual that it cannot, or a split's sums.
+        finish_f32(a.splits > 1 ? QV_ACT_NONE : a.ep.act, preact, wide, false);
+        if (a.splits > 1) {
+          store_piece<T, float, kWide>(
+              piece, a.partial + (static_cast<int64_t>(w.split) * a.m + row0) * a.n + col, a.n,
+              nullptr, 0, rows, cols, lane);
+        } else {
+          const T* residual = a.ep.residual != nullptr
+                                  ? static_cast<const T*>(a.ep.residual) +
+                                        row0 * a.ep.residual_stride + col
+                                  : nullptr;
+          if (a.ep.out_f32)
+            store_piece<T, float, kWide>(
+                piece, static_cast<float*>(a.ep.out) + row0 * a.ep.out_stride + col,
+                a.ep.out_stride, residual, a.ep.residual_stride, rows, cols, lane);
+          else
+            store_piece<T, T, kWide>(piece,
+                                     static_cast<T*>(a.ep.out) + row0 * a.ep.out_stride + col,
+                                     a.ep.out_stride, residual, a.ep.residual_stride, rows, cols,
+                                     lane);
         }
         __syncwarp();
       }

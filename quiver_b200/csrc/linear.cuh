@@ -147,26 +147,6 @@ __device__ __forceinline__ float2 activate2(int act, float2 z) {
   }
 }
 
-// activate2 over 16 values: the choice of activation is made once, outside the unrolled loops.
-template <bool kFast>
-__device__ __forceinline__ void activate16(int act, float (&v)[16]) {
-  auto all = [&](auto a) {
-#pragma unroll
-    for (int j = 0; j < 16; j += 2) {
-      const float2 y = activate2<kFast>(decltype(a)::value, make_float2(v[j], v[j + 1]));
-      v[j] = y.x;
-      v[j + 1] = y.y;
-    }
-  };
-  switch (act) {
-    case QV_ACT_RELU: all(std::integral_constant<int, QV_ACT_RELU>{}); break;
-    case QV_ACT_GELU: all(std::integral_constant<int, QV_ACT_GELU>{}); break;
-    case QV_ACT_GELU_TANH: all(std::integral_constant<int, QV_ACT_GELU_TANH>{}); break;
-    case QV_ACT_SILU: all(std::integral_constant<int, QV_ACT_SILU>{}); break;
-    default: break;
-  }
-}
-
 // act'(z) of two values; 0 for ReLU at 0.
 template <bool kFast>
 __device__ __forceinline__ float2 act_grad2(int act, float2 z) {
@@ -221,14 +201,6 @@ __device__ __forceinline__ void st_global_32(void* p, const uint32_t (&r)[8]) {
                "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
-__device__ __forceinline__ void ld_global_32(const void* p, uint32_t (&r)[8]) {
-  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
-                 "=r"(r[6]), "=r"(r[7])
-               : "l"(p)
-               : "memory");
-}
-
 // 16 consecutive elements of type T (left < 16: the first `left`), `align` bytes aligned.
 template <class T>
 __device__ __forceinline__ void put16(T* p, const float (&v)[16], int left, int align) {
@@ -261,77 +233,7 @@ __device__ __forceinline__ void put16(T* p, const float (&v)[16], int left, int 
       if (j < left) p[j] = u.t[j];
   }
 }
-template <class T>
-__device__ __forceinline__ void get16(const T* p, float (&v)[16], int left, int align) {
-  union {
-    T t[16];
-    uint32_t w[sizeof(T) * 4];
-    uint4 q[sizeof(T)];
-    uint2 d[sizeof(T) * 2];
-  } u;
-  if (left == 16 && align >= 32) {
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
-      uint32_t r[8];
-      ld_global_32(reinterpret_cast<const char*>(p) + i * 32, r);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) u.w[i * 8 + j] = r[j];
-    }
-  } else if (left == 16 && align == 16) {
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i)
-      u.q[i] = reinterpret_cast<const uint4*>(p)[i];
-  } else if (left == 16 && align == 8) {
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) * 2; ++i)
-      u.d[i] = reinterpret_cast<const uint2*>(p)[i];
-  } else {
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (j < left) u.t[j] = p[j];
-  }
-#pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] = j < left ? dev::to_f32<T>(u.t[j]) : 0.0f;
-}
-
-// Finishes 16 elements (row, col .. col + left - 1) of a product with inputs of type T up to the
-// residual; bias: their 16 bias values as float32 in shared memory (16-byte aligned).
-template <class T>
-__device__ __forceinline__ void finish16_act(const Epilogue& e, int64_t row, int64_t col,
-                                             float (&v)[16], int left, const float* bias) {
-  if (e.bias != nullptr) {
-#pragma unroll
-    for (int j = 0; j < 16; j += 4) {
-      const float4 b = *reinterpret_cast<const float4*>(bias + j);
-      const float2 lo = add2(make_float2(v[j], v[j + 1]), make_float2(b.x, b.y));
-      const float2 hi = add2(make_float2(v[j + 2], v[j + 3]), make_float2(b.z, b.w));
-      v[j] = lo.x;
-      v[j + 1] = lo.y;
-      v[j + 2] = hi.x;
-      v[j + 3] = hi.y;
-    }
-  }
-  if (e.preact != nullptr && left > 0)
-    put16<T>(static_cast<T*>(e.preact) + row * e.preact_stride + col, v, left, e.preact_align);
-  activate16<sizeof(T) == 2>(e.act, v);
-}
-// The rest, with plain loads and stores.
-template <class T>
-__device__ __forceinline__ void finish16_store(const Epilogue& e, int64_t row, int64_t col,
-                                               float (&v)[16], int left) {
-  if (e.residual != nullptr) {
-    float r[16];
-    get16<T>(static_cast<const T*>(e.residual) + row * e.residual_stride + col, r, left,
-             e.residual_align);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] += r[j];
-  }
-  if (e.out_f32)
-    put16<float>(static_cast<float*>(e.out) + row * e.out_stride + col, v, left, e.out_align);
-  else
-    put16<T>(static_cast<T*>(e.out) + row * e.out_stride + col, v, left, e.out_align);
-}
-// The same for one element.
+// Finishes one element of a product with inputs of type T.
 template <class T>
 __device__ __forceinline__ void finish1(const Epilogue& e, int64_t row, int64_t col, float s) {
   if (e.bias != nullptr) s += dev::to_f32<T>(static_cast<const T*>(e.bias)[col]);
