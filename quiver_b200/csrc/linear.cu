@@ -1042,10 +1042,13 @@ __global__ void __launch_bounds__(128)
 // ---- dz and the bias gradient ----------------------------------------------------------------------
 
 // dz = dy * act'(z), rounded to the operand type (float32: three planes), and float32 column sums
-// of the unrounded dz over this block's rows. A block takes 32 * kV columns and a range of rows:
+// of the unrounded dz over this block's rows. A block takes 32 pieces' columns and a range of rows:
 // warp w walks rows w, w + 8, .. of it, and the warps' sums are added in order at the end, so the
 // sums have a fixed order. Bound by memory: dy and z read, dz written.
 constexpr int kDzWarps = 8, kDzRows = 4;  // rows in flight per warp
+constexpr int dz_pieces(size_t piece_bytes) {  // 2-byte pieces: four a lane
+  return piece_bytes == 2 ? 4 : 1;
+}
 
 template <class T, int kV, bool kStore, int kAct>
 __global__ void __launch_bounds__(32 * kDzWarps)
@@ -1053,61 +1056,74 @@ __global__ void __launch_bounds__(32 * kDzWarps)
               int64_t z_stride, int64_t m, int64_t n, int64_t rows_per_block,
               typename Operand<T>::type* __restrict__ dz, int64_t ld, float* __restrict__ sums) {
   dev::allow_next();
-  __shared__ float part[kDzWarps][32 * kV];
+  constexpr int kC = dz_pieces(sizeof(T) * kV);  // pieces of a row per lane
+  constexpr int kCols = 32 * kV * kC;
+  __shared__ float part[kDzWarps][kCols];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t col = (blockIdx.y * 32ll + lane) * kV;
+  const int64_t col0 = static_cast<int64_t>(blockIdx.y) * kCols;
   const int64_t r1 = min(m, (blockIdx.x + 1) * rows_per_block);
-  float s[kV];
+  int64_t col[kC];
+  bool on[kC];
+  float s[kC][kV];
 #pragma unroll
-  for (int j = 0; j < kV; ++j) s[j] = 0.0f;
-  if (col < n) {
-    for (int64_t r = blockIdx.x * rows_per_block + warp; r < r1; r += kDzWarps * kDzRows) {
-      Pack<T, kV> g[kDzRows], x[kDzRows];
+  for (int q = 0; q < kC; ++q) {
+    col[q] = col0 + (q * 32 + lane) * kV;
+    on[q] = col[q] < n;
+    if (!on[q]) col[q] = col0;  // pieces past the last column read the first: no branches
 #pragma unroll
-      for (int u = 0; u < kDzRows; ++u) {
-        // Past the range the last row again: loads without a branch, so that all are in flight.
-        const int64_t row = min(r + u * kDzWarps, r1 - 1);
-        g[u] = dev::load_pack<T, kV>(dy + row * dy_stride + col);
-        if (kAct != QV_ACT_NONE) x[u] = dev::load_pack<T, kV>(z + row * z_stride + col);
+    for (int j = 0; j < kV; ++j) s[q][j] = 0.0f;
+  }
+  for (int64_t r = blockIdx.x * rows_per_block + warp; r < r1; r += kDzWarps * kDzRows) {
+    Pack<T, kV> g[kDzRows][kC], x[kDzRows][kC];
+#pragma unroll
+    for (int u = 0; u < kDzRows; ++u) {
+      const int64_t row = min(r + u * kDzWarps, r1 - 1);  // past the range its last row again
+#pragma unroll
+      for (int q = 0; q < kC; ++q) {
+        g[u][q] = dev::load_pack<T, kV>(dy + row * dy_stride + col[q]);
+        if (kAct != QV_ACT_NONE) x[u][q] = dev::load_pack<T, kV>(z + row * z_stride + col[q]);
       }
+    }
 #pragma unroll
-      for (int u = 0; u < kDzRows; ++u) {
-        const int64_t row = r + u * kDzWarps;
-        if (row >= r1) break;
+    for (int u = 0; u < kDzRows; ++u) {
+      const int64_t row = r + u * kDzWarps;
+      if (row >= r1) break;
+#pragma unroll
+      for (int q = 0; q < kC; ++q) {
         float d[kV];
 #pragma unroll
-        for (int j = 0; j < kV; ++j) {
-          d[j] = dev::to_f32<T>(g[u].v[j]);
-        }
+        for (int j = 0; j < kV; ++j) d[j] = dev::to_f32<T>(g[u][q].v[j]);
         if constexpr (kAct != QV_ACT_NONE) {
 #pragma unroll
           for (int j = 0; j < kV; j += 2) {
             const bool two = j + 1 < kV;
             const float2 f = act_grad2<sizeof(T) == 2>(
-                kAct, make_float2(dev::to_f32<T>(x[u].v[j]),
-                                  dev::to_f32<T>(x[u].v[two ? j + 1 : j])));
+                kAct, make_float2(dev::to_f32<T>(x[u][q].v[j]),
+                                  dev::to_f32<T>(x[u][q].v[two ? j + 1 : j])));
             // rounded before the sum in every variant, so that dbias does not depend on which runs
             d[j] = __fmul_rn(d[j], f.x);
             if (two) d[two ? j + 1 : j] = __fmul_rn(d[two ? j + 1 : j], f.y);
           }
         }
 #pragma unroll
-        for (int j = 0; j < kV; ++j) s[j] += d[j];
-        if (kStore) put_operand<T, kV>(d, dz, m * ld, row * ld + col);
+        for (int j = 0; j < kV; ++j) s[q][j] += d[j];
+        if (kStore && on[q]) put_operand<T, kV>(d, dz, m * ld, row * ld + col[q]);
       }
     }
   }
   if (sums == nullptr) return;
 #pragma unroll
-  for (int j = 0; j < kV; ++j) part[warp][lane * kV + j] = s[j];
+  for (int q = 0; q < kC; ++q) {
+#pragma unroll
+    for (int j = 0; j < kV; ++j) part[warp][(q * 32 + lane) * kV + j] = s[q][j];
+  }
   __syncthreads();
-  for (int c = threadIdx.x; c < 32 * kV; c += 32 * kDzWarps) {
-    const int64_t out = blockIdx.y * 32ll * kV + c;
-    if (out >= n) continue;
+  for (int c = threadIdx.x; c < kCols; c += 32 * kDzWarps) {
+    if (col0 + c >= n) continue;
     float t = 0.0f;
 #pragma unroll
     for (int w = 0; w < kDzWarps; ++w) t += part[w][c];
-    sums[blockIdx.x * n + out] = t;
+    sums[blockIdx.x * n + col0 + c] = t;
   }
 }
 
@@ -1684,7 +1700,7 @@ GradLayout grad_layout(const qv_linear_grad& g, int sms) {
                             reinterpret_cast<uintptr_t>(g.preact), g.m > 1 ? g.grad_stride * e : 0,
                             g.m > 1 ? g.preact_stride * e : 0, g.n * e}) == 16;
   // About eight blocks an SM, each with at least one round of its warps.
-  const size_t col_blocks = ceil_div(g.n, 32 * (L.wide_dz ? 16 / e : 1));
+  const size_t col_blocks = ceil_div(g.n, L.wide_dz ? 32 * 16 / e : 32 * dz_pieces(e));
   L.row_blocks = std::min<size_t>(ceil_div(g.m, kDzWarps * kDzRows),
                                   std::max<size_t>(1, sms * 8 / col_blocks));
   L.rows_per_block = static_cast<int64_t>(ceil_div(g.m, L.row_blocks));
@@ -1763,7 +1779,7 @@ void linear_grad(const qv_linear_grad& g, void* workspace, size_t workspace_byte
         constexpr int kV = decltype(v)::value;
         constexpr int kAct = decltype(act)::value;
         const dim3 grid(static_cast<unsigned>(L.row_blocks),
-                        static_cast<unsigned>(ceil_div(g.n, 32 * kV)));
+                        static_cast<unsigned>(ceil_div(g.n, 32 * kV * dz_pieces(sizeof(T) * kV))));
         if (L.store_dz)
           dz_kernel<T, kV, true, kAct><<<grid, 32 * kDzWarps, 0, st>>>(
               static_cast<const T*>(g.grad), g.grad_stride, static_cast<const T*>(g.preact),
