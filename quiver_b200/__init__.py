@@ -105,6 +105,7 @@ class FlatIndex:
 
     def __init__(self, dim: int, metric: str = "l2", *, device: int = 0, _native_handle=None):
         self._h = C.c_void_p()
+        self._device = int(device)
         if _native_handle is not None:
             self._h = _native_handle
         else:
@@ -140,6 +141,9 @@ class FlatIndex:
         the same checks and results as :meth:`add` (no counterpart in the reference). With an
         ``adapter`` (:class:`quiver_b200.embed.Adapter`) the rows are ``adapter(vectors)``."""
         if adapter is not None:
+            import torch
+            # One stream for the map and the add: the caller's, or PyTorch's current one.
+            stream = stream or torch.cuda.current_stream(self._device).cuda_stream
             vectors = _adapted(adapter, vectors, stream)
         if vectors.dim() != 2 or vectors.shape[1] != self.dim or not vectors.is_contiguous():
             raise ValueError(f"expected a contiguous [n, {self.dim}] tensor")
@@ -161,6 +165,8 @@ class FlatIndex:
         q = queries if adapter is None else _adapted(adapter, queries, None)
         if q.dim() != 2 or q.shape[1] != self.dim or q.dtype != torch.float32 or not q.is_cuda:
             raise ValueError(f"expected a float32 CUDA tensor [nq, {self.dim}]")
+        if q.device.index != self._device:
+            raise ValueError(f"expected a tensor on cuda:{self._device}, got {q.device}")
         if k <= 0:
             raise ValueError("k must be positive")
         q = q.contiguous()
@@ -182,6 +188,8 @@ class FlatIndex:
         codes = {torch.int32: 0, torch.int64: 1}
         if not rows.is_cuda or rows.dtype not in codes:
             raise ValueError("expected an int32 or int64 CUDA tensor of row numbers")
+        if rows.device.index != self._device:
+            raise ValueError(f"expected a tensor on cuda:{self._device}, got {rows.device}")
         r = rows.contiguous()
         dim = self.dim
         out = torch.empty(tuple(rows.shape) + (dim,), dtype=torch.float32, device=rows.device)
@@ -222,7 +230,7 @@ class FlatIndex:
         h = C.c_void_p()
         check(lib().qv_flat_load(int(device), str(path).encode(), int(verify_checksums),
                                  C.byref(h)))
-        return cls(0, _native_handle=h)
+        return cls(0, device=device, _native_handle=h)
 
     def __len__(self) -> int:
         return self._info()[0]

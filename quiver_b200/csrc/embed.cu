@@ -278,7 +278,8 @@ template <class Id, bool kFirst>
 __global__ void __launch_bounds__(kSortThreads)
     digit_scatter_kernel(const void* src, const uint32_t* src_pos, uint32_t n, uint32_t rows,
                          int shift, int bits, uint32_t tiles, const uint32_t* counts,
-                         const uint32_t* totals, uint32_t* keys, uint32_t* pos, const Clear clear, uint32_t part) {
+                         const uint32_t* totals, uint32_t* keys, uint32_t* pos,
+                         const Clear clear, uint32_t part) {
   if (blockIdx.x >= tiles) {
     clear_part(clear, part, blockIdx.x - tiles, gridDim.x - tiles);
     return;

@@ -31,7 +31,8 @@ from torch.autograd.function import once_differentiable
 from . import _native
 from ._native import check, lib
 
-__all__ = ["ACTIVATIONS", "Adapter", "embedding_grad", "embedding_lookup", "linear", "linear_grad"]
+__all__ = ["ACTIVATIONS", "Adapter", "embedding_grad", "embedding_lookup", "linear", "linear_grad",
+           "linear_preact"]
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _ID_TYPES = {torch.int32: 0, torch.int64: 1}
@@ -358,7 +359,8 @@ def _linear_grad(grad, x, weight, preact, act, need):
 class Adapter:
     """One linear map for the vectors of an index: ``activation(v W^T + bias)``, plus v itself with
     ``residual=True`` (W square). ``adapter(v)`` gives float32 vectors, ready for
-    :meth:`FlatIndex.add_device` and the device searches, which also take it as ``adapter=``."""
+    :meth:`FlatIndex.add_device` and the device searches, which also take it as ``adapter=``. The same
+    vector in batches of different sizes may differ in its last bits (sums run in another order)."""
 
     def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
                  activation: str = "none", residual: bool = False):

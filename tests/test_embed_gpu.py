@@ -545,6 +545,45 @@ def test_flat_lookup_and_adapter(gpu, embed):
     assert near.shape == (2, 3, 48) and torch.equal(near[0, 0], ax.lookup_device(label[0, :1])[0] / 2)
 
 
+def test_flat_adapter_on_a_side_stream(gpu, embed, tmp_path):
+    """The map and the add or search that takes it run on one stream, PyTorch's current one."""
+    g = gen(72)
+    w = normal(g, 64, 512, t=torch.bfloat16, scale=512 ** -0.5)
+    adapter = embed.Adapter(w)
+    x = normal(g, 40_000, 512, t=torch.bfloat16)
+    want = adapter(x)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        y = x * 1  # work ahead of the map on the same stream
+        for _ in range(20):
+            y = y * 1
+        ix = gpu.FlatIndex(64, "l2")
+        ix.add_device(y, adapter=adapter)
+        dist, label = ix.search_device(y[:50] * 1, 1, adapter=adapter)
+    side.synchronize()
+    assert torch.equal(torch.from_numpy(ix.rows()[0]).cuda(), want)
+    # The query batch and the row batch may sum in different orders: each element is off by at most
+    # yerr + half a float32 step in both, the squared distance by the squares of twice that (and its
+    # own 64 roundings).
+    ref, yerr, _, _ = linear_ref(x[:50], w, None, None, "none", torch.float32)
+    off = 2 * (yerr + ref.abs() * U)
+    assert (dist[:, 0].double() <= (off * off).sum(1) * (1 + 2.0 ** -16)).all()
+    assert label[:, 0].tolist() == list(range(50))
+    assert torch.equal(ix.lookup_device(label[:, 0]), want[label[:, 0]])
+    path = str(tmp_path / "a.qvr")
+    ix.save(path)
+    again = gpu.FlatIndex.load(path)
+    assert torch.equal(again.lookup_device(label[:, 0].int()), want[label[:, 0]])
+    for bad in (label.cpu(), label.float()):
+        with pytest.raises(ValueError):
+            ix.lookup_device(bad)
+    with pytest.raises(ValueError):
+        ix.search_device(x, 1)
+    with pytest.raises(ValueError):
+        ix.search_device(want[:3], 0)
+
+
 # ---- streams, graphs, threads, refusals -------------------------------------------------------------
 
 
@@ -589,6 +628,42 @@ def test_streams_and_graph(embed):
         for _, _, res in graphs:
             for p, q in zip(res, want[s]):
                 assert torch.equal(p, q)
+
+
+def test_captured_training_step(embed):
+    """A step with autograd, captured after a warm-up on a side stream and replayed on new inputs."""
+    table = normal(gen(1), 500, 64, t=torch.bfloat16).requires_grad_()
+    x0, w, b, _ = make(2, 300, 64, 64, torch.bfloat16, residual=False)
+    w.requires_grad_(), b.requires_grad_()
+    ids = torch.zeros(300, dtype=torch.long, device="cuda")
+    dy = torch.zeros(300, 64, dtype=torch.bfloat16, device="cuda")
+
+    def step():
+        e = embed.embedding_lookup(table, ids, 8.0)
+        y = embed.linear(e, w, b, residual=e, activation="silu")
+        return [y.detach()] + list(torch.autograd.grad(y, (table, w, b), dy))
+
+    def fill(seed):
+        g = gen(seed)
+        ids.copy_(torch.randint(-1, 500, (300,), generator=g, device="cuda"))
+        dy.copy_(normal(g, 300, 64, t=torch.bfloat16))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (5, 6):
+        fill(seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [v.clone() for v in got]
+        for p, q in zip(replayed, step()):
+            assert torch.equal(p, q)
 
 
 def test_threads(embed):
