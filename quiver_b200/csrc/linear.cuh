@@ -87,6 +87,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
   return y;
 }
 
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
 // |x| (at most 20, beyond which nothing of the tail is left), exp(-x^2/2) and the normal
 // distribution's tail Phi(-|x|) for 16-bit results: Abramowitz & Stegun 7.1.26, whose error of
 // erfc is at most 1.5e-7, far below a 16-bit half step.
@@ -95,7 +101,7 @@ struct NormalTail {
 };
 __device__ __forceinline__ NormalTail normal_tail(float2 x) {
   NormalTail n;
-  n.a = make_float2(fminf(fabsf(x.x), 20.0f), fminf(fabsf(x.y), 20.0f));
+  n.a = make_float2(min_nan(fabsf(x.x), 20.0f), min_nan(fabsf(x.y), 20.0f));
   const float2 t = rcp2(fma2(n.a, both(0.3275911f * 0.70710678f), both(1.0f)));
   n.gauss = exp2_approx(mul2(mul2(n.a, n.a), both(-0.72134752f)));  // -log2(e) / 2
   float2 p = fma2(both(0.5f * 1.061405429f), t, both(0.5f * -1.453152027f));
@@ -147,31 +153,31 @@ __device__ __forceinline__ float2 activate2(int act, float2 z) {
   }
 }
 
-// act'(z) of two values; 0 for ReLU at 0.
+// act'(z) of two values; 0 for ReLU at 0. The derivatives are constant to float32's last bit beyond
+// |z| = 100, where infinite z must not meet a zero factor.
 template <bool kFast>
 __device__ __forceinline__ float2 act_grad2(int act, float2 z) {
+  if (act == QV_ACT_RELU)
+    return make_float2(z.x > 0.0f ? 1.0f : (z.x <= 0.0f ? 0.0f : z.x),
+                       z.y > 0.0f ? 1.0f : (z.y <= 0.0f ? 0.0f : z.y));
+  if (act == QV_ACT_NONE) return both(1.0f);
+  if (kFast && act == QV_ACT_GELU) {  // Phi(x) + x phi(x), Phi(x) = 0.5 + sign(x) (0.5 - Phi(-|x|))
+    const NormalTail n = normal_tail(z);
+    const float2 half = add2(both(0.5f), make_float2(-n.q.x, -n.q.y));
+    const float2 cdf =
+        add2(both(0.5f), make_float2(copysignf(half.x, z.x), copysignf(half.y, z.y)));
+    const float2 x = make_float2(copysignf(n.a.x, z.x), copysignf(n.a.y, z.y));
+    return fma2(mul2(x, both(0.39894228f)), n.gauss, cdf);
+  }
+  z = make_float2(max_nan(min_nan(z.x, 100.0f), -100.0f), max_nan(min_nan(z.y, 100.0f), -100.0f));
   if constexpr (kFast) {
-    switch (act) {
-      case QV_ACT_GELU: {  // Phi(x) + x phi(x)
-        const NormalTail n = normal_tail(z);
-        const float2 cdf = make_float2(z.x >= 0.0f ? 1.0f - n.q.x : n.q.x,
-                                       z.y >= 0.0f ? 1.0f - n.q.y : n.q.y);
-        // x within its clamp, so that infinite x does not meet a zero phi
-        const float2 x = make_float2(copysignf(n.a.x, z.x), copysignf(n.a.y, z.y));
-        return fma2(mul2(x, both(0.39894228f)), n.gauss, cdf);
-      }
-      case QV_ACT_GELU_TANH: {  // q + x q (1 - q) (2u)'
-        const float2 q = logistic2(tanh_arg2(z));
-        const float2 du = fma2(mul2(z, z), both(3.0f * 0.044715f * kTanhScale), both(kTanhScale));
-        const float2 r = add2(both(1.0f), make_float2(-q.x, -q.y));
-        return fma2(mul2(mul2(z, q), r), du, q);
-      }
-      case QV_ACT_SILU: {  // q + x q (1 - q)
-        const float2 q = logistic2(z);
-        return fma2(mul2(z, q), add2(both(1.0f), make_float2(-q.x, -q.y)), q);
-      }
-      default: break;
-    }
+    const bool tanh = act == QV_ACT_GELU_TANH;  // q + z q (1 - q) u' with q = logistic(u)
+    const float2 q = logistic2(tanh ? tanh_arg2(z) : z);
+    const float2 r = add2(both(1.0f), make_float2(-q.x, -q.y));
+    float2 zq = mul2(z, q);
+    if (tanh)
+      zq = mul2(zq, fma2(mul2(z, z), both(3.0f * 0.044715f * kTanhScale), both(kTanhScale)));
+    return fma2(zq, r, q);
   } else {
     auto one = [&](float x) {
       switch (act) {
@@ -180,19 +186,14 @@ __device__ __forceinline__ float2 act_grad2(int act, float2 z) {
           const float q = logistic(tanh_arg(x));
           return fmaf(x * q * (1.0f - q), kTanhScale * fmaf(0.134145f * x, x, 1.0f), q);
         }
-        case QV_ACT_SILU: {
+        default: {
           const float q = logistic(x);
           return fmaf(x * q, 1.0f - q, q);
         }
-        default: return 1.0f;
       }
     };
-    if (act != QV_ACT_RELU) return make_float2(one(z.x), one(z.y));
+    return make_float2(one(z.x), one(z.y));
   }
-  if (act == QV_ACT_RELU)
-    return make_float2(z.x > 0.0f ? 1.0f : (z.x <= 0.0f ? 0.0f : z.x),
-                       z.y > 0.0f ? 1.0f : (z.y <= 0.0f ? 0.0f : z.y));
-  return both(1.0f);
 }
 
 // 32-byte accesses, which make a thread's piece of a row whole 32-byte sectors.

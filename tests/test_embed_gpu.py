@@ -362,6 +362,20 @@ def test_linear_special_values(embed):
             keep = torch.ones(m, dtype=torch.bool, device="cuda")
             keep[[1, 3]] = False
             assert torch.equal(got[keep], clean[keep])
+            # gradients: the NaN row's dx is NaN, an infinite z has a finite derivative
+            dy = normal(gen(22), m, 72, t=t)
+            for act in ACTS[1:]:
+                z = normal(gen(23), m, 72, t=t)
+                clean = embed.linear_grad(dy, x, w, z, act, need=(True, False, False))[0]
+                z[1, 3], z[2, 4], z[3, 5] = math.nan, math.inf, -math.inf
+                z[0, 6], z[0, 7] = 6e4, -6e4
+                dx = embed.linear_grad(dy, x, w, z, act, need=(True, False, False))[0]
+                assert dx[1].isnan().all() and dx[[0, 2, 3]].isfinite().all()
+                assert torch.equal(dx[4:], clean[4:])
+                one = torch.zeros(m, 72, device="cuda", dtype=t)
+                one[2, 4] = one[3, 5] = one[0, 6] = one[0, 7] = 1
+                db = embed.linear_grad(one, x, w, z, act, need=(False, False, True))[2]
+                assert db[[4, 6]].tolist() == [1, 1] and db[[5, 7]].abs().max() <= 2.0 ** -100
     big = torch.full((130, 64), torch.finfo(torch.float32).max, device="cuda")
     eye = torch.eye(64, device="cuda")
     assert torch.equal(embed.linear(big, eye), big)
