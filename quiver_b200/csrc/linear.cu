@@ -222,7 +222,7 @@ __device__ __forceinline__ float times_pow2(float v, int e) {
 }
 
 struct ProductArgs {
-  int64_t m, n, k;
+  int64_t m, n;
   int pairs;              // plane pairs: 1, or 3 or 6 for float32
   const int* exp_a;       // scaled rows of A and B: their exponents, or nullptr
   const int* exp_b;
@@ -506,18 +506,12 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     prefetch_map(&maps.a[first.q]);
     prefetch_map(&maps.b[first.q]);
   }
-  if (threadIdx.x == 0) {
-    s_abort = 0;
-    for (int s = 0; s < S::kStages; ++s) {
-      tc::mbar_init(bar(FULL + s), 1);
-      tc::mbar_init(bar(EMPTY + s), 1);
-    }
-    for (int b = 0; b < 2; ++b) {
-      tc::mbar_init(bar(ACC_FULL + b), 1);
-      tc::mbar_init(bar(ACC_EMPTY + b), (kPair ? 2 : 1) * kEpilogueWarps);
-    }
-    tc::mbar_init(bar(DRAIN), 1);
-    for (int w = 0; w < kEpilogueWarps; ++w) tc::mbar_init(bar(RESIDUAL + w), 1);
+  constexpr int kBars = RESIDUAL + kEpilogueWarps;
+  static_assert(kBars <= 32, "one barrier a lane");
+  if (threadIdx.x < kBars) {
+    if (threadIdx.x == 0) s_abort = 0;
+    const bool acc_empty = threadIdx.x == ACC_EMPTY || threadIdx.x == ACC_EMPTY + 1;
+    tc::mbar_init(bar(threadIdx.x), acc_empty ? (kPair ? 2 : 1) * kEpilogueWarps : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -1333,7 +1327,6 @@ void run_products(const Product* p, int count, const ProductPlan& plan, unsigned
     ProductArgs& a = g.p[q];
     a.m = p[q].m;
     a.n = p[q].n;
-    a.k = p[q].k;
     a.pairs = p[q].a.planes == 3 ? 6 : (p[q].a.planes == 2 ? 3 : 1);
     a.exp_a = p[q].a.exponents;
     a.exp_b = p[q].b.exponents;
