@@ -903,7 +903,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
 }
 
 // What is left after a launch of products, by block row: the splits of each one's k joined in their
-// order and their elements finished, one a thread, and the bias gradient from its row ranges' sums.
+// order and their elements finished, kV neighbours a thread, and the bias gradient from its row
+// ranges' sums.
 struct SplitJob {
   const float* partial;
   int splits;  // 0: nothing to join
@@ -920,21 +921,30 @@ struct JoinJobs {
   SplitJob split[2];
   SumsJob sums;
 };
-template <class T>
+template <class T, int kV>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinJobs jobs) {
   dev::wait_previous();
   if (blockIdx.y < 2) {
     const SplitJob& j = jobs.split[blockIdx.y];
     if (j.splits == 0) return;
-    const int64_t size = j.m * j.n, n = j.n;
+    const int64_t size = j.m * j.n;
     const int splits = j.splits;
     const float* partial = j.partial;
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < size; i += gridDim.x * 256ll) {
-      float s = 0.0f;
+    const uint32_t per_row = static_cast<uint32_t>(j.n / kV);
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < size / kV; i += gridDim.x * 256ll) {
+      float s[kV];
+#pragma unroll
+      for (int v = 0; v < kV; ++v) s[v] = 0.0f;
 #pragma unroll 8
-      for (int k = 0; k < splits; ++k) s += partial[k * size + i];
-      const int64_t row = i / n;
-      finish1<T>(j.ep, row, i - row * n, s);
+      for (int k = 0; k < splits; ++k) {
+        const Pack<float, kV> x = dev::load_pack<float, kV>(partial + k * size + i * kV);
+#pragma unroll
+        for (int v = 0; v < kV; ++v) s[v] += x.v[v];
+      }
+      const int64_t row = i >> 32 ? i / per_row : static_cast<uint32_t>(i) / per_row;
+      const int64_t col = (i - row * per_row) * kV;
+#pragma unroll
+      for (int v = 0; v < kV; ++v) finish1<T>(j.ep, row, col + v, s[v]);
     }
     return;
   }
@@ -1377,8 +1387,11 @@ void run_products(const Product* p, int count, const ProductPlan& plan, unsigned
   }
   if (sums.sums != nullptr) items = std::max(items, static_cast<size_t>(sums.n) * 8);
   if (items > 0) {
-    launch_chained(join_kernel<T>,
-                   dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(items, 256), 148 * 8)),
+    bool four = true;
+    for (int q = 0; q < count; ++q) four &= plan.splits[q] == 1 || p[q].n % 4 == 0;
+    const size_t threads = four ? ceil_div(items, 4) : items;
+    launch_chained(four ? join_kernel<T, 4> : join_kernel<T, 1>,
+                   dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(threads, 256), 148 * 8)),
                         sums.sums != nullptr ? 3 : 2),
                    256, 0, st, jobs);
     check_launch("join_kernel");
