@@ -18,11 +18,12 @@ __device__ __forceinline__ int64_t load_id(const void* ids, size_t i) {
 }
 
 // ---- lookup ------------------------------------------------------------------------------------
-// kG lanes share a row and move kV elements at a time, four pieces in flight per lane: of one row
-// where the row has more than kG pieces, else of four rows. Written past the L2's older lines
+// kG lanes share a row and move kV elements at a time, with two to eight pieces in flight per lane
+// where the row has more than kG of them, else a piece of each of four rows. Written past the L2's older lines
 // (streaming stores), so that the results do not push out table rows other ids will read.
-// 131,072 rows of 1024 bfloat16 by a power law of ids: 63 us, 5.3 TB/s of the bytes that have to
-// move; one thread per piece of the result, with a division to find its row, took 104 us.
+// 131,072 rows of 1024 bfloat16 by a power law of ids: 57 us, 5.9 TB/s of the bytes that have to
+// move (64 us with a branch around each load, which then wait for one another; 104 us with one
+// thread per piece of the result and a division to find its row).
 constexpr int kLookupThreads = 256;
 
 template <class T, int kV>
@@ -40,52 +41,55 @@ __device__ __forceinline__ Pack<T, kV> filled(float f) {
   return y;
 }
 
-template <class T, class Id, int kV, int kG, bool kLong>
+template <class T, class Id, int kV, int kG, int kPieces>
 __global__ void __launch_bounds__(kLookupThreads)
     lookup_kernel(const T* __restrict__ table, int64_t rows, int64_t table_stride,
                   const Id* __restrict__ ids, int64_t n, int nv, float scale,
                   T* __restrict__ out, int64_t out_stride) {
+  constexpr bool kLong = kPieces > 0;  // rows of more than kG pieces, kPieces in flight
   constexpr int kRows = kLong ? 1 : 4;
   constexpr int kGroups = kLookupThreads / kG;
   const int lane = threadIdx.x % kG;
   const int64_t first = (static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / kG) * kRows;
   if (first >= n) return;
   const T* src[kRows];
+  bool held[kRows];
   float fill[kRows];
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
     const int64_t id = first + u < n ? static_cast<int64_t>(ids[first + u]) : -1;
-    src[u] = id >= 0 && id < rows ? table + id * table_stride : nullptr;
+    held[u] = id >= 0 && id < rows;
+    src[u] = table + (held[u] ? id : 0) * table_stride;
     fill[u] = id < 0 ? 0.0f : __int_as_float(0x7fc00000);
   }
   T* dst = out + first * out_stride;
   if constexpr (kLong) {
-    if (src[0] == nullptr) {
+    if (!held[0]) {
       for (int v = lane; v < nv; v += kG) dev::stream_pack<T, kV>(dst + v * kV, filled<T, kV>(fill[0]));
       return;
     }
-    for (int v = lane; v < nv; v += 4 * kG) {
-      Pack<T, kV> x[4];
+    for (int v = lane; v < nv; v += kPieces * kG) {
+      Pack<T, kV> x[kPieces];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (v + u * kG < nv) x[u] = dev::load_pack<T, kV>(src[0] + (v + u * kG) * kV);
+      for (int u = 0; u < kPieces; ++u)  // past the row's end its last piece: no branches
+        x[u] = dev::load_pack<T, kV>(src[0] + min(v + u * kG, nv - 1) * kV);
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < kPieces; ++u)
         if (v + u * kG < nv)
           dev::stream_pack<T, kV>(dst + (v + u * kG) * kV, scaled<T, kV>(x[u], scale));
     }
   } else {
     if (lane >= nv) return;
     Pack<T, kV> x[kRows];
+    if (rows > 0) {  // ids without a row read the first: no branches
 #pragma unroll
-    for (int u = 0; u < kRows; ++u)
-      if (src[u] != nullptr) x[u] = dev::load_pack<T, kV>(src[u] + lane * kV);
+      for (int u = 0; u < kRows; ++u) x[u] = dev::load_pack<T, kV>(src[u] + lane * kV);
+    }
 #pragma unroll
     for (int u = 0; u < kRows; ++u) {
       if (first + u >= n) break;
       dev::stream_pack<T, kV>(dst + u * out_stride + lane * kV,
-                              src[u] != nullptr ? scaled<T, kV>(x[u], scale)
-                                                : filled<T, kV>(fill[u]));
+                              held[u] ? scaled<T, kV>(x[u], scale) : filled<T, kV>(fill[u]));
     }
   }
 }
@@ -95,27 +99,32 @@ void launch_lookup(const void* table, size_t rows, size_t dim, size_t table_stri
                    const void* ids, size_t n, float scale, void* out, size_t out_stride,
                    cudaStream_t st) {
   const int nv = static_cast<int>(dim / kV);
-  auto go = [&](auto g, auto is_long) {
+  auto go = [&](auto g, auto pieces) {
     constexpr int kG = decltype(g)::value;
-    constexpr bool kLong = decltype(is_long)::value;
-    const size_t per_block = kLookupThreads / kG * (kLong ? 1 : 4);
-    lookup_kernel<T, Id, kV, kG, kLong>
+    constexpr int kPieces = decltype(pieces)::value;
+    const size_t per_block = kLookupThreads / kG * (kPieces > 0 ? 1 : 4);
+    lookup_kernel<T, Id, kV, kG, kPieces>
         <<<static_cast<unsigned>(ceil_div(n, per_block)), kLookupThreads, 0, st>>>(
             static_cast<const T*>(table), static_cast<int64_t>(rows),
             static_cast<int64_t>(table_stride), static_cast<const Id*>(ids),
             static_cast<int64_t>(n), nv, scale, static_cast<T*>(out),
             static_cast<int64_t>(out_stride));
   };
+  using Short = std::integral_constant<int, 0>;
   if (nv <= 4)
-    go(std::integral_constant<int, 4>{}, std::false_type{});
+    go(std::integral_constant<int, 4>{}, Short{});
   else if (nv <= 8)
-    go(std::integral_constant<int, 8>{}, std::false_type{});
+    go(std::integral_constant<int, 8>{}, Short{});
   else if (nv <= 16)
-    go(std::integral_constant<int, 16>{}, std::false_type{});
+    go(std::integral_constant<int, 16>{}, Short{});
   else if (nv <= 32)
-    go(std::integral_constant<int, 32>{}, std::false_type{});
-  else
-    go(std::integral_constant<int, 32>{}, std::true_type{});
+    go(std::integral_constant<int, 32>{}, Short{});
+  else if (nv <= 64)
+    go(std::integral_constant<int, 32>{}, std::integral_constant<int, 2>{});
+  else if (nv <= 128 || kV * sizeof(T) > 8)
+    go(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{});
+  else  // long rows of narrow pieces
+    go(std::integral_constant<int, 32>{}, std::integral_constant<int, 8>{});
   check_launch("lookup_kernel");
 }
 

@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackJob j0, const PackJ
     Pack<T, kV> x[kPackRows];
 #pragma unroll
     for (int u = 0; u < kPackRows; ++u)
-      if (r0 + u < j.rows) x[u] = dev::load_pack<T, kV>(src + (r0 + u) * j.stride + c);
+      x[u] = dev::load_pack<T, kV>(src + min(r0 + u, j.rows - 1) * j.stride + c);
 #pragma unroll
     for (int u = 0; u < kPackRows; ++u) {
       if (r0 + u >= j.rows) break;
