@@ -332,12 +332,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&r)[16]) 
 // One epilogue warp's piece of a tile: 32 rows (one a lane) x kCols columns of results of type Out,
 // out of tensor memory into shared memory in the tensor map's swizzle. exp_b: the columns'
 // exponents (exp_a: this lane's row's) where operands were scaled, or nullptr. residual: the piece
-// holds it, in type Out. preact: this lane's row, or nullptr. !ok: the pipeline gave up, NaN.
+// holds it, in type Out. preact: this lane's row, or nullptr.
 template <class T, class Out, int kCols, int kAct>
-__device__ __forceinline__ void finish_piece(uint32_t taddr, bool ok, const float* bias,
-                                             const int* exp_b, int exp_a, T* preact,
-                                             bool preact_wide, bool residual,
-                                             unsigned char* piece, int lane) {
+__device__ __forceinline__ void finish_piece(uint32_t taddr, const float* bias, const int* exp_b,
+                                             int exp_a, T* preact, bool preact_wide,
+                                             bool residual, unsigned char* piece, int lane) {
   constexpr uint32_t kRow = kCols * sizeof(Out);
   constexpr uint32_t kSwizzle = kRow == 128 ? 7 : (kRow == 64 ? 3 : 1);
   constexpr int kPer = 16 / static_cast<int>(sizeof(Out));  // elements of 16 bytes
@@ -347,10 +346,6 @@ __device__ __forceinline__ void finish_piece(uint32_t taddr, bool ok, const floa
   for (int i = 0; i < kCols; i += 16) {
     float v[16];
     tmem_ld16(taddr + i, v);
-    if (!ok) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(0x7fc00000u);
-    }
     if constexpr (sizeof(T) == 4) {
       if (exp_b != nullptr) {
 #pragma unroll
@@ -396,6 +391,13 @@ __device__ __forceinline__ void finish_piece(uint32_t taddr, bool ok, const floa
                    "r"(q.z), "r"(q.w));
     }
   }
+}
+
+// NaN over a piece (this lane's row of it), where the pipeline gave up.
+template <class Out, int kCols>
+__device__ __noinline__ void poison_piece(unsigned char* piece, int lane) {
+  Out* row = reinterpret_cast<Out*>(piece) + lane * kCols;
+  for (int c = 0; c < kCols; ++c) row[c] = dev::from_f32<Out>(__uint_as_float(0x7fc00000u));
 }
 
 // The preactivations of a piece's columns where they can neither be stored whole nor through the
@@ -819,9 +821,10 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         };
         auto finish_f32 = [&](int act, T* preact, bool wide, bool residual) {
           by_act(act, [&](auto k) {
-            finish_piece<T, float, kWide, decltype(k)::value>(taddr, ok, b, e, exp_a, preact, wide,
+            finish_piece<T, float, kWide, decltype(k)::value>(taddr, b, e, exp_a, preact, wide,
                                                               residual, piece, lane);
           });
+          if (!ok) poison_piece<float, kWide>(piece, lane);
           __syncwarp();
         };
         const int rows = static_cast<int>(min(static_cast<int64_t>(32), a.m - row0));
@@ -832,7 +835,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         bool wide = false;
         if (a.splits == 1 && a.ep.preact != nullptr) {
           T* first = static_cast<T*>(a.ep.preact) + row0 * a.ep.preact_stride + col;
-          if (in_tiles && cols == per_piece && a.ep.preact_align >= 16) {
+          if (ok && in_tiles && cols == per_piece && a.ep.preact_align >= 16) {
             preact = row < a.m ? first + lane * a.ep.preact_stride : nullptr;
             wide = a.ep.preact_align >= 32;
           } else if (!res_tiles && per_piece == kWide) {
@@ -845,11 +848,13 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         }
         if (in_tiles) {
           if constexpr (sizeof(T) == 2) {
-            if (!a.ep.out_f32)
+            if (!a.ep.out_f32) {
               by_act(a.ep.act, [&](auto k) {
-                finish_piece<T, T, kCols, decltype(k)::value>(taddr, ok, b, e, exp_a, preact, wide,
+                finish_piece<T, T, kCols, decltype(k)::value>(taddr, b, e, exp_a, preact, wide,
                                                               res_tiles, piece, lane);
               });
+              if (!ok) poison_piece<T, kCols>(piece, lane);
+            }
           }
           if (sizeof(T) == 4 || a.ep.out_f32) finish_f32(a.ep.act, preact, wide, res_tiles);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

@@ -161,11 +161,10 @@ __device__ __forceinline__ float2 act_grad2(int act, float2 z) {
     return make_float2(z.x > 0.0f ? 1.0f : (z.x <= 0.0f ? 0.0f : z.x),
                        z.y > 0.0f ? 1.0f : (z.y <= 0.0f ? 0.0f : z.y));
   if (act == QV_ACT_NONE) return both(1.0f);
-  if (kFast && act == QV_ACT_GELU) {  // Phi(x) + x phi(x), Phi(x) = 0.5 + sign(x) (0.5 - Phi(-|x|))
+  if (kFast && act == QV_ACT_GELU) {  // Phi(x) + x phi(x)
     const NormalTail n = normal_tail(z);
-    const float2 half = add2(both(0.5f), make_float2(-n.q.x, -n.q.y));
-    const float2 cdf =
-        add2(both(0.5f), make_float2(copysignf(half.x, z.x), copysignf(half.y, z.y)));
+    const float2 cdf = make_float2(z.x >= 0.0f ? 1.0f - n.q.x : n.q.x,
+                                   z.y >= 0.0f ? 1.0f - n.q.y : n.q.y);
     const float2 x = make_float2(copysignf(n.a.x, z.x), copysignf(n.a.y, z.y));
     return fma2(mul2(x, both(0.39894228f)), n.gauss, cdf);
   }
