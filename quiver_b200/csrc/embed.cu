@@ -769,8 +769,10 @@ int sort_ids(const GradPlan& p, const void* ids, uint32_t n, uint32_t rows, Clea
                    p.tiles, totals, scan_blocks, clear, part++);
     check_launch("digit_scan_kernel");
     auto* scatter = k == 0 ? digit_scatter_kernel<Id, true> : digit_scatter_kernel<Id, false>;
+    // The widest digits' need whatever this call's is: the limit is the kernel's, and another
+    // thread's call may set it between this line and the launch.
     QV_CUDA(cudaFuncSetAttribute(scatter, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 static_cast<int>(smem)));
+                                 (4 + 2 * kSortWarps) << kMaxDigitBits));
     launch_chained(scatter, p.tiles + extra, kSortThreads, smem, st, k == 0 ? ids : ik,
                    k == 0 ? nullptr : ip, n, rows, shift, p.bits, p.tiles, counts, totals, ok, op,
                    clear, part++);
