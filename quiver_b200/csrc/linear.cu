@@ -615,13 +615,6 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       else
         produce(std::false_type{}, std::false_type{}, w, q);
     }
-    if (*abort_flag) {
-      // Copies in flight must land before the CTA leaves. They may be counted on barriers that
-      // this CTA cannot poll (a pair's leader's): wait out the bound, far longer than any copy.
-      const uint64_t t0 = tc::gtimer();
-      while (tc::gtimer() - t0 < g.drain_ns) {
-      }
-    }
   } else if (warp == 1) {
     if (leader) {  // in a pair the leader issues for both CTAs
       int t = 0, s = 0;
@@ -894,6 +887,16 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   }
   tc::tc_fence_before();
   __syncthreads();
+  if (*abort_flag) {
+    // Whoever gave up, copies that the producer issued may still be in flight (it may itself be
+    // done long before), and they must land before the CTA leaves. They may be counted on barriers
+    // that this CTA cannot poll (a pair's leader's): wait out the bound, far longer than any copy.
+    // Without the flag every copy was multiplied, or no result would have come.
+    const uint64_t t0 = tc::gtimer();
+    while (tc::gtimer() - t0 < g.drain_ns) {
+    }
+    __syncthreads();
+  }
   // A CTA of a pair stays until the other is done with its barriers, tiles and accumulators.
   if constexpr (kPair) tc::cluster_sync();
   if (warp == 1) {
