@@ -536,7 +536,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   dev::wait_previous();  // what packed the operands
   const uint32_t tmem = s_tmem;
   volatile int* abort_flag = &s_abort;
-  // Bounded wait; false on timeout or abort, after which the CTA's remaining results are NaN.
+  // Bounded wait of a whole warp; false on timeout or abort, after which the CTA's remaining results
+  // are NaN.
   auto wait = [&](uint32_t b, uint32_t parity) {
     auto test = [&] {
       return kPair ? tc::mbar_test_cluster(b, parity) : tc::mbar_test(b, parity);
@@ -544,12 +545,12 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     auto sleep_test = [&] {
       return kPair ? tc::mbar_sleep_test_cluster(b, parity) : tc::mbar_sleep_test(b, parity);
     };
-    if (test()) return true;
+    // Every exit is the warp's vote: warp-wide instructions follow each wait.
+    if (__all_sync(dev::kFull, test())) return true;
     const long long t0 = clock64();
     for (;;) {
-      if (sleep_test()) return true;
-      if (*abort_flag) return false;
-      if (clock64() - t0 > g.wait_cycles) {
+      if (__all_sync(dev::kFull, sleep_test())) return true;
+      if (__any_sync(dev::kFull, *abort_flag != 0 || clock64() - t0 > g.wait_cycles)) {
         *abort_flag = 1;
         return false;
       }
