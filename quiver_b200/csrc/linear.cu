@@ -692,12 +692,12 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     const uint32_t res_bar = bar(RESIDUAL + ew);
     uint32_t res_phase = 0;
     // Waits for the piece's residual; given up, its copy must still land before the piece goes.
-    auto wait_residual = [&](uint32_t b, uint32_t& phase, bool ok) {
-      if (!wait(b, phase)) {
+    auto wait_residual = [&](uint32_t b, uint32_t& phase) {
+      const bool ok = wait(b, phase);
+      if (!ok) {
         const uint64_t t0 = tc::gtimer();
         while (!tc::mbar_test(b, phase) && tc::gtimer() - t0 < g.drain_ns) {
         }
-        ok = false;
       }
       phase ^= 1;
       __syncwarp();
@@ -713,6 +713,10 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           tc::mbar_arrive(bar(ACC_EMPTY + slot));
       }
     };
+    // Once a wait has failed, this warp neither waits nor arrives any more, and all its remaining
+    // results are NaN: a barrier that nobody advances would satisfy the wait after next with the
+    // phase before, and arrivals out of turn would stand in for the other CTA's.
+    bool alive = true;
     int t = 0, parity = 0;  // chunks read so far; of units
     for (int u = worker; u < units; u += workers, parity ^= 1) {
       const Unit w = u == worker ? first : unit(u);
@@ -742,15 +746,15 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       // tile, of float32.
       constexpr int kWide = kCols < 32 ? kCols : 32;
       const int per_piece = in_tiles && !a.ep.out_f32 ? kCols : kWide;
-      bool ok = false;
 #pragma unroll 1
       for (int c = 0; c < kCols; c += per_piece) {
         const int64_t col = col0 + c;
         const bool any = col < a.n && row0 < a.m;
+        const bool load = any && res_tiles && alive;
         if (any) {
           if (lane == 0) {
             asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the piece is free
-            if (res_tiles) {
+            if (load) {
               tc::mbar_expect_tx(res_bar, 32 * per_piece * (a.ep.out_f32 ? 4 : 2));
               tc::tma_load_2d(tc::smem_u32(piece), &maps.residual[w.q], static_cast<int>(col),
                               static_cast<int>(row0), res_bar);
@@ -758,13 +762,12 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           }
           __syncwarp();
         }
-        if (c == 0) {
-          ok = wait(bar(ACC_FULL + (t & 1)), (t >> 1) & 1);
-          __syncwarp();
+        if (c == 0 && alive) {
+          alive = wait(bar(ACC_FULL + (t & 1)), (t >> 1) & 1);
           tc::tc_fence_after();
           slot = t & 1;
           ++t;
-          if (kChunked && w.b1 - w.b0 > a.chunk) {  // chunks before the last, added up in registers
+          if (kChunked && alive && w.b1 - w.b0 > a.chunk) {  // chunks before the last, added up in registers
             const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
             float sum[kCols];
 #pragma unroll
@@ -773,8 +776,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             for (int c0 = w.b0 + a.chunk; c0 < w.b1; c0 += a.chunk, ++t) {
               release(slot);
               slot = t & 1;
-              ok = wait(bar(ACC_FULL + slot), (t >> 1) & 1) && ok;
-              __syncwarp();
+              alive = wait(bar(ACC_FULL + slot), (t >> 1) & 1);
+              if (!alive) break;
               tc::tc_fence_after();
 #pragma unroll
               for (int i = 0; i < kCols; i += 16) {
@@ -799,7 +802,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         // The parameters in registers and the activation chosen once per piece. (Reading them per
         // 16 columns made a 128 x 256 tile's epilogue take 10,500 cycles, more than the MMAs of
         // k = 1024.)
-        if (res_tiles) ok = wait_residual(res_bar, res_phase, ok);
+        if (load) alive = wait_residual(res_bar, res_phase) && alive;
         const uint32_t taddr = tmem + slot * kBN + group * kCols + c +
                                (static_cast<uint32_t>(quarter * 32) << 16);
         const float* b = a.splits == 1 && a.ep.bias != nullptr ? bias + c : nullptr;
@@ -818,7 +821,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             finish_piece<T, float, kWide, decltype(k)::value>(taddr, b, e, exp_a, preact, wide,
                                                               residual, piece, lane);
           });
-          if (!ok) poison_piece<float, kWide>(piece, lane);
+          if (!alive) poison_piece<float, kWide>(piece, lane);
           __syncwarp();
         };
         const int rows = static_cast<int>(min(static_cast<int64_t>(32), a.m - row0));
@@ -829,7 +832,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         bool wide = false;
         if (a.splits == 1 && a.ep.preact != nullptr) {
           T* first = static_cast<T*>(a.ep.preact) + row0 * a.ep.preact_stride + col;
-          if (ok && in_tiles && cols == per_piece && a.ep.preact_align >= 16) {
+          if (alive && in_tiles && cols == per_piece && a.ep.preact_align >= 16) {
             preact = row < a.m ? first + lane * a.ep.preact_stride : nullptr;
             wide = a.ep.preact_align >= 32;
           } else if (!res_tiles && per_piece == kWide) {
@@ -837,7 +840,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             store_piece<T, T, kWide>(piece, first, a.ep.preact_stride, nullptr, 0, rows, cols, lane);
             __syncwarp();
           } else {  // the piece holds the residual, or more columns than float32 has room for
-            store_preact<T>(taddr, ok, b, e, exp_a, first, a.ep.preact_stride, rows, cols, lane);
+            store_preact<T>(taddr, alive, b, e, exp_a, first, a.ep.preact_stride, rows, cols, lane);
           }
         }
         if (in_tiles) {
@@ -847,7 +850,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
                 finish_piece<T, T, kCols, decltype(k)::value>(taddr, b, e, exp_a, preact, wide,
                                                               res_tiles, piece, lane);
               });
-              if (!ok) poison_piece<T, kCols>(piece, lane);
+              if (!alive) poison_piece<T, kCols>(piece, lane);
             }
           }
           if (sizeof(T) == 4 || a.ep.out_f32) finish_f32(a.ep.act, preact, wide, res_tiles);
@@ -881,7 +884,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         }
         __syncwarp();
       }
-      release(slot);
+      if (alive) release(slot);
     }
     // The pieces stay until the last stores have read them.
     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");

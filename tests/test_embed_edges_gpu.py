@@ -81,3 +81,35 @@ def test_threads_with_tables_of_different_sizes(embed):
     for t in threads:
         t.join()
     assert not bad, bad
+
+
+@pytest.mark.parametrize("m,k,n,t", [(32768, 128, 2048, "bf16"), (32768, 192, 2048, "f16"),
+                                     (32768, 1024, 2048, "bf16"), (16384, 16384, 1024, "bf16"),
+                                     (20000, 200, 640, "f32"), (32768, 512, 1024, "f32")])
+def test_wait_that_runs_out_over_many_units(embed, monkeypatch, m, k, n, t):
+    """Blocks (of 64 and 128 columns, and pairs) with six units and more each: whatever a pipeline
+    that gave up still returns is right, and the rest is NaN."""
+    x = normal(gen(1), m, k, t=TYPES[t])
+    w = normal(gen(2), n, k, t=TYPES[t])
+    b = normal(gen(3), n, t=TYPES[t])
+    r = normal(gen(4), m, n, t=TYPES[t])
+    calls = (lambda: (embed.linear(x, w),), lambda: (embed.linear(x, w, b, residual=r),),
+             lambda: embed.linear_preact(x, w, b, activation="relu"),
+             lambda: embed.linear_preact(x, w, b, residual=r, activation="relu"),
+             lambda: embed.linear_grad(r, x, w, need=(True, True, False))[:2])
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    lost = 0
+    for limit in ("1", "2", "4", "8"):
+        monkeypatch.setenv("QV_TC_WAIT_LIMIT_US", limit)
+        got = [c() for c in calls]
+        torch.cuda.synchronize()
+        monkeypatch.delenv("QV_TC_WAIT_LIMIT_US")
+        for i, (g, v) in enumerate(zip(got, want)):
+            for p, q in zip(g, v):
+                gone = p.isnan()
+                lost += int(gone.sum())
+                assert torch.equal(p[~gone], q[~gone]), (limit, i)
+    assert lost > 0
+    for c, v in zip(calls, want):
+        assert all(torch.equal(p, q) for p, q in zip(c(), v))
