@@ -6,11 +6,14 @@
 // 16-bit operands are multiplied as they are. Float32 operands are split into 16-bit planes whose
 // sum they are, and the product is the sum of the plane products that reach float32's last bit:
 // * x W^T: every row is scaled by a power of two that brings its largest element below 2^15, then
-//   split into two float16 (11 + 11 bits and the sign of the remainder: off by at most 2^-24 of the
-//   element, or 2^-39 of the row's largest where that is more), three products; the scales come off
-//   each result exactly. The sums run along the rows, so a row's scale is a result's.
-// * dz W and dz^T x, whose sums run across the rows: three bfloat16 planes (8 + 8 + 8 bits, no
-//   scales needed), six products.
+//   split into two float16 (11 + 11 bits and the sign of the remainder: off by at most 2^-23 of the
+//   element, or 2^-39 of the row's largest where that is more), three products; the product of the
+//   two low planes, at most 2^-22 of a term, is left out. The scales come off each result exactly.
+//   The sums run along the rows, so a row's scale is a result's. Rows whose elements differ too
+//   widely for that (split_rows_kernel) take the next form, with another scale (lifted).
+// * dz W and dz^T x, whose sums run across the rows: three bfloat16 planes (8 + 8 + 8 bits, the
+//   element itself down to the planes' last bit, 2^-133), six products; what is left out is at most
+//   2^-24 of a term.
 // Batches of a few rows (single queries) take a kernel that reads the weights once with plain
 // loads.
 #include <algorithm>
@@ -86,12 +89,25 @@ struct PackJob {
 
 // float32 rows scaled and split into two float16 planes; one warp per row, which keeps up to
 // 32 * kSplitHeld pieces of it in registers and reads what is more a second time.
-constexpr int kSplitHeld = 8;
+//
+// The planes hold an element to 2^-23 of itself or 2^-39 of the row's largest, X. The second part
+// adds up to 2^-39 (X sum|w| + W sum|x|) <= 2^-38 k X W to a result, which is nothing beside
+// S = sum |x||w| unless the large elements of x meet small ones of w. So the rows tell which share
+// of their elements lies within 2^-6 of their largest, in 256ths: where the least shares p of x and
+// q of w have p + q >= 1 + 1/8, at least k / 8 terms of every result have both factors there,
+// S >= 2^-15 k X W, and the addition is at most 2^-23 S. Otherwise the call's product takes three
+// bfloat16 planes (choose_planes_kernel). Vectors of normally distributed elements have shares of
+// 0.9 and more, half of them zero (ReLU) about 0.45. Rows of zeros and rows that hold infinity or
+// NaN (whose results do not depend on the planes' last bits) tell 256.
+constexpr int kSplitHeld = 8, kSplitBlocks = 148 * 8;
+constexpr uint32_t kShareOne = 256, kSharesNeeded = kShareOne + kShareOne / 8;
 template <int kV>
-__global__ void __launch_bounds__(256) split_rows_kernel(const PackJob j0, const PackJob j1) {
+__global__ void __launch_bounds__(256)
+    split_rows_kernel(const PackJob j0, const PackJob j1, uint32_t* __restrict__ shares) {
   dev::allow_next();
   const PackJob& j = blockIdx.y == 0 ? j0 : j1;
   const int lane = threadIdx.x & 31;
+  uint32_t least = kShareOne;
   const int64_t plane = j.rows * j.ld;
   const int64_t warps = gridDim.x * 8ll;
   for (int64_t r = blockIdx.x * 8ll + (threadIdx.x >> 5); r < j.rows; r += warps) {
@@ -119,11 +135,14 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const PackJob j0, const
         top == 0 || top >= 0x7f800000u ? 0 : min(14 + 127 - static_cast<int>(top >> 23), 126);
     const float scale = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
     if (lane == 0) j.exponents[r] = -shift;
+    const float from = __uint_as_float(top) * scale * 0x1p-6f;
+    uint32_t large = 0;
     auto split = [&](const Pack<float, kV>& x, int64_t c) {
       Pack<__half, kV> hi, lo;
 #pragma unroll
       for (int v = 0; v < kV; ++v) {
         const float y = x.v[v] * scale;
+        large += fabsf(y) >= from;
         hi.v[v] = __float2half_rn(y);
         lo.v[v] = __hisinf(hi.v[v]) ? __float2half_rn(0.0f)
                                     : __float2half_rn(y - __half2float(hi.v[v]));
@@ -139,17 +158,31 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const PackJob j0, const
 #pragma unroll 4
     for (int64_t c = kHeld + lane * kV; c < j.cols; c += 32 * kV)
       split(dev::load_pack<float, kV>(src + c), c);
+    large = __reduce_add_sync(dev::kFull, large);
+    if (top != 0 && top < 0x7f800000u)
+      least = min(least, large * kShareOne / static_cast<uint32_t>(j.cols));
+  }
+  __shared__ uint32_t s_least[8];
+  if (lane == 0) s_least[threadIdx.x >> 5] = least;
+  __syncthreads();
+  if (threadIdx.x < 8) {
+    least = __reduce_min_sync(0xffu, s_least[threadIdx.x]);
+    if (threadIdx.x == 0) shares[blockIdx.y * gridDim.x + blockIdx.x] = least;
   }
   dev::wait_previous();
 }
 
+// A row's exponent as three bfloat16 planes, from its exponent as two float16 planes. The planes end
+// at 2^-133, bfloat16's last bit, so that elements below 2^-110 would lose bits: rows whose largest
+// is below 2^-20 are brought up to that, which keeps every product with another row in range.
+__device__ __forceinline__ int lifted(int exponent) { return min(0, exponent + 34); }
+
 // Up to two matrices in one launch (blockIdx.y). Bound by memory: every thread moves kV values of
 // kPackRows rows at a time.
 constexpr int kPackRows = 4;
-template <class T, int kV>
-__global__ void __launch_bounds__(256) pack_kernel(const PackJob j0, const PackJob j1) {
-  dev::allow_next();
-  const PackJob& j = blockIdx.y == 0 ? j0 : j1;
+// kLift: rows whose scale for the float16 planes was 2^-exponent are lifted by 2^-lifted(exponent).
+template <class T, int kV, bool kLift>
+__device__ __forceinline__ void pack_rows(const PackJob& j) {
   using O = typename Operand<T>::type;
   const T* src = static_cast<const T*>(j.src);
   O* dst = static_cast<O*>(j.dst);
@@ -170,11 +203,51 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackJob j0, const PackJ
       float f[kV];
 #pragma unroll
       for (int v = 0; v < kV; ++v) f[v] = dev::to_f32<T>(x[u].v[v]);
+      if constexpr (kLift) {
+        const float scale = __int_as_float((127 - lifted(j.exponents[r0 + u])) << 23);
+#pragma unroll
+        for (int v = 0; v < kV; ++v) f[v] *= scale;
+      }
       put_operand<T, kV>(f, dst, plane, (r0 + u) * j.ld + c);
     }
   }
+}
+template <class T, int kV>
+__global__ void __launch_bounds__(256) pack_kernel(const PackJob j0, const PackJob j1) {
+  dev::allow_next();
+  pack_rows<T, kV, false>(blockIdx.y == 0 ? j0 : j1);
   // Chained after the dz kernel, whose results are not used here: its end is this kernel's.
   dev::wait_previous();
+}
+
+// Whether the two operands that split_rows_kernel made (in `blocks` blocks each) serve every
+// result; where they do not, three bfloat16 planes of each in their place.
+template <int kV>
+__global__ void __launch_bounds__(256)
+    choose_planes_kernel(const PackJob j0, const PackJob j1, const uint32_t* shares,
+                         uint32_t blocks, int* wide) {
+  dev::allow_next();
+  dev::wait_previous();
+  __shared__ uint32_t s_least[2][8];
+  uint32_t a = kShareOne, b = kShareOne;
+  for (uint32_t i = threadIdx.x; i < blocks; i += 256) {
+    a = min(a, shares[i]);
+    b = min(b, shares[blocks + i]);
+  }
+  a = __reduce_min_sync(dev::kFull, a);
+  b = __reduce_min_sync(dev::kFull, b);
+  if ((threadIdx.x & 31) == 0) {
+    s_least[0][threadIdx.x >> 5] = a;
+    s_least[1][threadIdx.x >> 5] = b;
+  }
+  __syncthreads();
+  for (int w = 0; w < 8; ++w) {
+    a = min(a, s_least[0][w]);
+    b = min(b, s_least[1][w]);
+  }
+  const bool planes = a + b < kSharesNeeded;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *wide = planes;
+  if (planes) pack_rows<float, kV, true>(blockIdx.y == 0 ? j0 : j1);
 }
 
 // ---- the product kernel -----------------------------------------------------------------------------
@@ -238,6 +311,10 @@ struct ProductArgs {
 struct ProductGroup {
   ProductArgs p[2];
   int units[2];
+  // One float32 product whose operands are either scaled or three planes (maps.a[1], maps.b[1]):
+  // the word that says so, and the instruction descriptor of the planes; or nullptr.
+  const int* wide;
+  uint32_t wide_idesc;
   long long wait_cycles;
   uint64_t drain_ns;
 };
@@ -535,6 +612,9 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   tc::tc_fence_after();
   dev::wait_previous();  // what packed the operands
   const uint32_t tmem = s_tmem;
+  bool wide = false;  // a vote, so that what depends on it stays uniform
+  if constexpr (sizeof(T) == 4)
+    wide = g.wide != nullptr && __any_sync(dev::kFull, *static_cast<const volatile int*>(g.wide) != 0);
   volatile int* abort_flag = &s_abort;
   // Bounded wait of a whole warp; false on timeout or abort, after which the CTA's remaining results
   // are NaN.
@@ -567,12 +647,14 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     bool ok = true;
     auto produce = [&](auto a_mn, auto b_mn, const Unit& w, int q) {
       const ProductArgs& a = g.p[q];
-      const CUtensorMap* map_a = &maps.a[q];
-      const CUtensorMap* map_b = &maps.b[q];
+      const int form = wide ? 1 : q;
+      const int pairs = wide ? 6 : a.pairs;
+      const CUtensorMap* map_a = &maps.a[form];
+      const CUtensorMap* map_b = &maps.b[form];
       const int row_a = w.tm * S::kM + static_cast<int>(rank) * kBM;
       const int row_b = w.tn * kBN + static_cast<int>(rank) * S::kBRows;
       for (int pass = 0, c0 = w.b0; c0 < w.b1 && ok;) {  // pairs of planes within chunks of k
-        const int pa = kPairA[first_pair(a.pairs) + pass], pb = kPairB[first_pair(a.pairs) + pass];
+        const int pa = kPairA[first_pair(pairs) + pass], pb = kPairB[first_pair(pairs) + pass];
         const int c1 = min(w.b1, c0 + a.chunk);
         for (int k0 = c0 * kBK; k0 < c1 * kBK; k0 += kBK) {
           if (!wait(empty_at + s * 8, phase)) {
@@ -601,7 +683,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           s = s + 1 == S::kStages ? 0 : s + 1;
           phase ^= s == 0;
         }
-        pass = pass + 1 == a.pairs ? 0 : pass + 1;
+        pass = pass + 1 == pairs ? 0 : pass + 1;
         c0 = pass == 0 ? c1 : c0;
       }
     };
@@ -630,11 +712,11 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       for (int u = worker; u < units && ok; u += workers) {
         const Unit w = u == worker ? first : unit(u);
         const ProductArgs& a = g.p[w.q];
-        const uint32_t idesc = a.idesc;
+        const uint32_t idesc = wide ? g.wide_idesc : a.idesc;
         const uint32_t a_step = a.a_mn ? 2048 >> 4 : 32 >> 4, b_step = a.b_mn ? 2048 >> 4 : 32 >> 4;
         const uint64_t ad0 = operand_desc(tiles_at, a.a_mn);
         const uint64_t bd0 = operand_desc(tiles_at + S::kABytes, a.b_mn);
-        const int pairs = a.pairs, chunk = a.chunk;
+        const int pairs = wide ? 6 : a.pairs, chunk = a.chunk;
         for (int c0 = w.b0; c0 < w.b1 && ok; c0 += chunk, ++t) {
           const int slot = t & 1;
           if (!wait(bar(ACC_EMPTY + slot), ((t >> 1) & 1) ^ 1)) {
@@ -735,8 +817,10 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       int exp_a = 0;
       if constexpr (sizeof(T) == 4) {
         if (a.exp_a != nullptr) {
-          exp_a = row < a.m ? a.exp_a[row] : 0;
-          for (int j = lane; j < kCols; j += 32) exp_b[j] = col0 + j < a.n ? a.exp_b[col0 + j] : 0;
+          auto form = [&](int e) { return wide ? lifted(e) : e; };
+          exp_a = row < a.m ? form(a.exp_a[row]) : 0;
+          for (int j = lane; j < kCols; j += 32)
+            exp_b[j] = col0 + j < a.n ? form(a.exp_b[col0 + j]) : 0;
         }
       }
       const bool res_tiles = a.splits == 1 && a.ep.residual_tiles;
@@ -1199,7 +1283,14 @@ struct Product {
   bool a_mn, b_mn;
   Stored a, b;
   Epilogue ep;
+  const int* wide = nullptr;  // scaled operands that may be three planes instead: which they are
 };
+// Scaled rows where choose_planes_kernel has replaced them.
+Stored as_planes(Stored s) {
+  s.planes = 3;
+  s.bf16 = true;
+  return s;
+}
 // A result or residual of the epilogue's pieces: 32 rows x 128 bytes at most.
 CUtensorMap piece_map(const void* p, int64_t rows, int64_t cols, int64_t stride, uint32_t dtype,
                       int tile_cols) {
@@ -1307,6 +1398,10 @@ void launch_products(const Product* p, int count, const ProductGroup& g, bool ch
       maps.residual[q] =
           piece_map(ep.residual, p[q].m, p[q].n, ep.residual_stride, type, kBN / 4);
   }
+  if (p[0].wide != nullptr) {  // along k, by itself
+    maps.a[1] = operand_map(as_planes(p[0].a), kBM);
+    maps.b[1] = operand_map(as_planes(p[0].b), S::kBRows);
+  }
   static std::once_flag once[16];
   int device = 0;
   QV_CUDA(cudaGetDevice(&device));
@@ -1358,11 +1453,18 @@ void run_products(const Product* p, int count, const ProductPlan& plan, unsigned
     a.splits = plan.splits[q];
     a.blocks_per_split = plan.blocks_per_split[q];
     a.chunk = a.pairs > 1 ? 2 : 128;
-    const uint32_t fmt = p[q].a.bf16 ? 1 : 0;
-    a.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(p[q].a_mn) << 15) |
-              (static_cast<uint32_t>(p[q].b_mn) << 16) |
-              (static_cast<uint32_t>(plan.bn >> 3) << 17) |
-              (static_cast<uint32_t>((plan.pair ? 2 * kBM : kBM) >> 4) << 24);
+    auto idesc = [&](bool bf16) {
+      const uint32_t fmt = bf16 ? 1 : 0;
+      return (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(p[q].a_mn) << 15) |
+             (static_cast<uint32_t>(p[q].b_mn) << 16) |
+             (static_cast<uint32_t>(plan.bn >> 3) << 17) |
+             (static_cast<uint32_t>((plan.pair ? 2 * kBM : kBM) >> 4) << 24);
+    };
+    a.idesc = idesc(p[q].a.bf16);
+    if (p[q].wide != nullptr) {
+      g.wide = p[q].wide;
+      g.wide_idesc = idesc(true);
+    }
     a.a_mn = p[q].a_mn;
     a.b_mn = p[q].b_mn;
     a.ep = p[q].ep;
@@ -1416,13 +1518,15 @@ bool in_place(uint32_t dtype, const void* p, size_t rows, size_t stride) {
          (rows <= 1 || (stride * 2) % 16 == 0);
 }
 size_t packed_ld(size_t cols) { return (cols + 7) / 8 * 8; }
-// A scaled float32 operand: two float16 planes and the rows' exponents.
-size_t scaled_bytes(size_t rows, size_t cols) {
-  return (rows * packed_ld(cols) * 4 + 255) / 256 * 256 + (rows * 4 + 255) / 256 * 256;
-}
 size_t packed_bytes(uint32_t dtype, size_t rows, size_t cols) {
   return (rows * packed_ld(cols) * 2 * (dtype == QV_DTYPE_F32 ? 3 : 1) + 255) / 256 * 256;
 }
+// A scaled float32 operand: two float16 planes, or three bfloat16 ones in their place, and the rows'
+// exponents; behind both operands the rows' shares and the word that says which it is.
+size_t scaled_bytes(size_t rows, size_t cols) {
+  return packed_bytes(QV_DTYPE_F32, rows, cols) + (rows * 4 + 255) / 256 * 256;
+}
+constexpr size_t kSharesBytes = (2 * kSplitBlocks * 4 + 255) / 256 * 256, kChoiceBytes = kSharesBytes + 256;
 
 // The operands of one call that have to be packed first, collected and packed in one launch.
 template <class T>
@@ -1472,17 +1576,28 @@ class Packer {
     count_ = 0;
     return ws_;
   }
+  // Of a scaled call, after run(): which planes its operands are.
+  const int* wide() const { return wide_; }
 
  private:
   template <int kV>
   void launch(bool chained, cudaStream_t st) {
     if constexpr (sizeof(T) == 4) {
       if (scaled_) {
-        const size_t rows = static_cast<size_t>(std::max(jobs_[0].rows, jobs_[count_ - 1].rows));
-        split_rows_kernel<kV>
-            <<<dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(rows, 8), 148 * 8)), count_),
-               256, 0, st>>>(jobs_[0], jobs_[count_ - 1]);
+        // Both operands are float32, so both are here.
+        const size_t rows = static_cast<size_t>(std::max(jobs_[0].rows, jobs_[1].rows));
+        const unsigned blocks =
+            static_cast<unsigned>(std::min<size_t>(ceil_div(rows, 8), kSplitBlocks));
+        uint32_t* shares = reinterpret_cast<uint32_t*>(ws_);
+        int* wide = reinterpret_cast<int*>(ws_ + kSharesBytes);
+        ws_ += kChoiceBytes;
+        wide_ = wide;
+        split_rows_kernel<kV><<<dim3(blocks, 2), 256, 0, st>>>(jobs_[0], jobs_[1], shares);
         check_launch("split_rows_kernel");
+        // Two blocks an SM in all: it rarely packs.
+        launch_chained(choose_planes_kernel<kV>, dim3(std::min(blocks, 148u), 2), 256, 0, st,
+                       jobs_[0], jobs_[1], static_cast<const uint32_t*>(shares), blocks, wide);
+        check_launch("choose_planes_kernel");
         return;
       }
     }
@@ -1502,6 +1617,7 @@ class Packer {
   unsigned char* ws_;
   PackJob jobs_[2];
   int count_ = 0, align_ = 16;
+  const int* wide_ = nullptr;
 };
 
 constexpr size_t kWideFew = 2048;  // output columns from which a warp takes two
@@ -1592,6 +1708,7 @@ LinearPlan linear_plan(const qv_linear& l, int sms) {
     return l.dtype == QV_DTYPE_F32 ? scaled_bytes(rows, l.k) : packed_bytes(l.dtype, rows, l.k);
   };
   p.bytes += packed(l.x, l.m, l.x_stride) + packed(l.weight, l.n, l.weight_stride);
+  if (l.dtype == QV_DTYPE_F32) p.bytes += kChoiceBytes;
   p.bytes += p.product.partial_bytes[0];
   return p;
 }
@@ -1665,7 +1782,9 @@ void linear_forward(const qv_linear& l, void* workspace, size_t workspace_bytes,
     d.b = pack.rows(l.weight, l.n, l.k, l.weight_stride);
     d.ep = ep;
     const bool packed = pack.count() > 0;
-    run_products<T>(&d, 1, p.product, pack.run(false, st), SumsJob{}, packed, sms, st);
+    unsigned char* partial = pack.run(false, st);
+    d.wide = pack.wide();
+    run_products<T>(&d, 1, p.product, partial, SumsJob{}, packed, sms, st);
   });
 }
 

@@ -113,3 +113,76 @@ def test_wait_that_runs_out_over_many_units(embed, monkeypatch, m, k, n, t):
     assert lost > 0
     for c, v in zip(calls, want):
         assert all(torch.equal(p, q) for p, q in zip(c(), v))
+
+
+def product_bound(x, w):
+    """What a float32 product of k terms in any order and its parts may be off by, from sum |x||w|
+    alone: 2u a term where the accumulator cuts, and 2^-21 for parts that leave out up to 2^-22 and
+    2^-23 of a term."""
+    return (x.double().abs() @ w.double().abs().t()) * ((x.shape[1] + 8) * 2 * U + 2.0 ** -21) \
+        + TINY[torch.float32]
+
+
+def wide_inputs(kind, m, n, k):
+    g = gen(m + n + k)
+    x, w = normal(g, m, k), normal(g, n, k)
+    if kind == "column":  # one feature far above the others, its weights as far below
+        for i, p in enumerate((20, 25, 30, 60)):
+            x[:, i] *= 2.0 ** p
+            w[:, i] *= 2.0 ** -p
+    elif kind == "columns":  # every feature its own unit
+        e = torch.linspace(-40, 40, k, device="cuda").round()
+        x, w = x * 2.0 ** e, w * 2.0 ** -e
+    elif kind == "row":  # a single row of the batch, its large element without a weight
+        x[m // 2] = 1
+        x[m // 2, 0] = 2.0 ** 40
+        w[:, 0] = 0
+    elif kind == "weight":
+        w[n // 2] = 1
+        w[n // 2, k - 1] = 2.0 ** 45
+        x[:, k - 1] = 0
+    elif kind == "one-hot":
+        x.zero_()
+        x[:, 1] = 1
+        w[:, 0] = 2.0 ** 50
+    elif kind == "tiny":  # rows of subnormal elements and weights that bring them back
+        x = x * 2.0 ** -135
+        x[:, 0] = 2.0 ** -112
+        w = w * 2.0 ** 100
+        w[:, 0] = 2.0 ** 60
+    elif kind == "sparse":
+        x = x.clamp(min=0) * (torch.rand(m, k, generator=g, device="cuda") < 0.3)
+        w = w * 2.0 ** torch.randint(-30, 1, (1, k), generator=g, device="cuda")
+    return x, w
+
+
+@pytest.mark.parametrize("kind", ["plain", "column", "columns", "row", "weight", "one-hot", "tiny",
+                                  "sparse"])
+@pytest.mark.parametrize("m,k,n", [(300, 80, 72), (140, 129, 130), (6000, 512, 768),
+                                   (64, 8192, 128)])
+def test_linear_float32_wide_rows(embed, kind, m, k, n):
+    """Elements of very different magnitudes within a row keep float32's accuracy of the sum."""
+    x, w = wide_inputs(kind, m, n, k)
+    want = x.double() @ w.double().t()
+    got = embed.linear(x, w)
+    assert_within(got, want, product_bound(x, w), kind)
+    assert torch.equal(got, embed.linear(x, w))
+    y, z = embed.linear_preact(x, w, None, residual=got, activation="relu")
+    assert torch.equal(z, got)
+
+
+def test_linear_float32_wide_rows_alternate(embed):
+    """Batches that need the planes and batches that do not, in turn and from replayed graphs with
+    one workspace each: nothing of one call is left for the next."""
+    plain, wide = wide_inputs("plain", 300, 72, 80), wide_inputs("row", 300, 72, 80)
+    want = [embed.linear(*v) for v in (plain, wide)]
+    held = [v.clone() for v in plain]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = embed.linear(*held)
+    for i in (0, 1, 0, 1, 1, 0):
+        for h, v in zip(held, (plain, wide)[i]):
+            h.copy_(v)
+        graph.replay()
+        assert torch.equal(out, want[i])
+        assert torch.equal(embed.linear(*(plain, wide)[i]), want[i])
