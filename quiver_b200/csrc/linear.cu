@@ -98,11 +98,13 @@ struct PackJob {
 // S >= 2^-15 k X W, and the addition is at most 2^-23 S. Otherwise the call's product takes three
 // bfloat16 planes (choose_planes_kernel). Vectors of normally distributed elements have shares of
 // 0.9 and more, half of them zero (ReLU) about 0.45. Rows of zeros and rows that hold infinity or
-// NaN (whose results do not depend on the planes' last bits) tell 256.
+// NaN (whose results do not depend on the planes' last bits) tell 256. Three blocks an SM: counting
+// took the kernel to 126 registers and from 12.6 to 15.8 us for 10,000 + 768 rows of 768; held to 80
+// it takes 13.8.
 constexpr int kSplitHeld = 8, kSplitBlocks = 148 * 8;
 constexpr uint32_t kShareOne = 256, kSharesNeeded = kShareOne + kShareOne / 8;
 template <int kV>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 3)
     split_rows_kernel(const PackJob j0, const PackJob j1, uint32_t* __restrict__ shares) {
   dev::allow_next();
   const PackJob& j = blockIdx.y == 0 ? j0 : j1;
@@ -158,9 +160,9 @@ __global__ void __launch_bounds__(256)
 #pragma unroll 4
     for (int64_t c = kHeld + lane * kV; c < j.cols; c += 32 * kV)
       split(dev::load_pack<float, kV>(src + c), c);
-    large = __reduce_add_sync(dev::kFull, large);
+    const uint32_t count = __reduce_add_sync(dev::kFull, large);
     if (top != 0 && top < 0x7f800000u)
-      least = min(least, large * kShareOne / static_cast<uint32_t>(j.cols));
+      least = min(least, count * kShareOne / static_cast<uint32_t>(j.cols));
   }
   __shared__ uint32_t s_least[8];
   if (lane == 0) s_least[threadIdx.x >> 5] = least;
@@ -294,8 +296,18 @@ __device__ __forceinline__ float times_pow2(float v, int e) {
   return v * __int_as_float((127 + h) << 23) * __int_as_float((127 + e - h) << 23);
 }
 
+// Operands of a float32 product for sums outside the tensor core: element k of row r, B as the caller
+// has it, A too or (plane > 0) as three bfloat16 planes.
+struct Sources {
+  const void* a;
+  int64_t a_row, a_k, plane;  // strides
+  const float* b;
+  int64_t b_row, b_k;
+};
+
 struct ProductArgs {
-  int64_t m, n;
+  int64_t m, n, k;
+  Sources from;           // of float32 products
   int pairs;              // plane pairs: 1, or 3 or 6 for float32
   const int* exp_a;       // scaled rows of A and B: their exponents, or nullptr
   const int* exp_b;
@@ -321,6 +333,118 @@ struct ProductGroup {
 struct ProductMaps {
   CUtensorMap a[2], b[2], out[2], residual[2];
 };
+
+// The sum of an element in plain float32 arithmetic, by a warp whose lanes go along k until the sum is
+// NaN.
+template <bool kPlanes>
+__device__ __forceinline__ float plain_sum_of(const Sources& f, int64_t row, int64_t col, int64_t k,
+                                              int lane) {
+  const float* a = static_cast<const float*>(f.a) + row * f.a_row;
+  const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(f.a) + row * f.a_row;
+  const float* b = f.b + col * f.b_row;
+  float s = 0.0f;
+  for (int64_t i0 = 0; i0 < k; i0 += 8 * 32) {
+    float x[8], y[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int64_t i = i0 + u * 32 + lane, at = min(i, k - 1);
+      y[u] = b[at * f.b_k];
+      if constexpr (kPlanes) {
+        const __nv_bfloat16* q = p + at * f.a_k;
+        x[u] = __bfloat162float(q[0]) +
+               (__bfloat162float(q[f.plane]) + __bfloat162float(q[2 * f.plane]));
+      } else {
+        x[u] = a[at * f.a_k];
+      }
+      if (i >= k) x[u] = y[u] = 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s = fmaf(x[u], y[u], s);
+    if (__any_sync(dev::kFull, s != s)) return __uint_as_float(0x7fc00000u);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(dev::kFull, s, d);
+  return s;
+}
+// Whether row `row` of A holds NaN (its results are then NaN already).
+__device__ __noinline__ bool row_holds_nan(const Sources& f, int64_t row, int64_t k, int lane) {
+  bool nan = false;
+  for (int64_t i = lane; i < k; i += 32) {
+    const int64_t at = row * f.a_row + i * f.a_k;
+    const float x = f.plane > 0 ? __bfloat162float(static_cast<const __nv_bfloat16*>(f.a)[at])
+                                : static_cast<const float*>(f.a)[at];
+    nan |= x != x;
+  }
+  return __any_sync(dev::kFull, nan);
+}
+__device__ __noinline__ float plain_sum(const Sources& f, int64_t row, int64_t col, int64_t k,
+                                        int lane) {
+  return f.plane > 0 ? plain_sum_of<true>(f, row, col, k, lane)
+                     : plain_sum_of<false>(f, row, col, k, lane);
+}
+
+// A unit of work: product q, split, then tile row / column, columns fastest (a wave's CTAs share rows
+// of A and all of B in L2), and the split's blocks of k.
+struct Unit {
+  int q, split, tm, tn, b0, b1;
+};
+__device__ __forceinline__ Unit unit_of(const ProductGroup& g, int u) {
+  Unit w;
+  w.q = u >= g.units[0];
+  u -= w.q ? g.units[0] : 0;
+  const ProductArgs& a = g.p[w.q];
+  const int per = a.tiles_m * a.tiles_n;
+  w.split = u / per;
+  const int t = u - w.split * per;
+  w.tm = t / a.tiles_n;
+  w.tn = t - w.tm * a.tiles_n;
+  w.b0 = w.split * a.blocks_per_split;
+  w.b1 = min(a.k_blocks, w.b0 + a.blocks_per_split);
+  return w;
+}
+
+// A float32 product runs on parts of the values, where an infinity gives NaN: it meets a part that is
+// zero, or one of the other sign. So a warp that saw NaN or infinity among its sums comes back here
+// once its tiles are done: what is NaN becomes what plain float32 arithmetic says. Apart from the
+// epilogue, which only notes what it saw (inside it, these loops cost the kernel a fifth of its time
+// whether there was a NaN or not). row, col: of the warp's part of a tile.
+__device__ __noinline__ void finish_special(const ProductGroup& g, int first, int step, int kM,
+                                            int row, int kBN, int col, int cols, int lane) {
+  const int units = g.units[0] + g.units[1];
+  for (int u = first; u < units; u += step) {
+    const Unit w = unit_of(g, u);
+    const ProductArgs& a = g.p[w.q];
+    if (a.splits > 1) continue;  // the join's
+    const int64_t row0 = static_cast<int64_t>(w.tm) * kM + row;
+    const int64_t col0 = static_cast<int64_t>(w.tn) * kBN + col;
+    for (int64_t r = row0; r < min(row0 + 32, a.m); ++r) {
+      bool asked = false;
+      for (int64_t c0 = col0; c0 < min(col0 + cols, a.n); c0 += 32) {
+        const int64_t c = c0 + lane;
+        bool again = c < min(col0 + cols, a.n);
+        if (again) {
+          const float y = static_cast<const volatile float*>(a.ep.out)[r * a.ep.out_stride + c];
+          again = y != y;
+        }
+        if (again && a.ep.preact != nullptr) {  // else it is the residual's
+          const float z =
+              static_cast<const volatile float*>(a.ep.preact)[r * a.ep.preact_stride + c];
+          again = z != z;
+        }
+        uint32_t todo = __ballot_sync(dev::kFull, again);
+        if (todo != 0 && !asked) {
+          asked = true;
+          if (row_holds_nan(a.from, r, a.k, lane)) break;
+        }
+        for (; todo != 0; todo &= todo - 1) {
+          const int l = __ffs(todo) - 1;
+          const float s = plain_sum(a.from, r, c0 + l, a.k, lane);
+          if (lane == l) finish1<float>(a.ep, r, c, s);
+        }
+      }
+    }
+  }
+}
 
 // TMA loads; in a pair the bytes are counted on the leader's barrier (a shared::cluster address).
 template <bool kPair>
@@ -409,11 +533,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&r)[16]) 
 // One epilogue warp's piece of a tile: 32 rows (one a lane) x kCols columns of results of type Out,
 // out of tensor memory into shared memory in the tensor map's swizzle. exp_b: the columns'
 // exponents (exp_a: this lane's row's) where operands were scaled, or nullptr. residual: the piece
-// holds it, in type Out. preact: this lane's row, or nullptr.
+// holds it, in type Out. preact: this lane's row, or nullptr. special: float32 only, set where a sum
+// is NaN or infinite.
 template <class T, class Out, int kCols, int kAct>
 __device__ __forceinline__ void finish_piece(uint32_t taddr, const float* bias, const int* exp_b,
                                              int exp_a, T* preact, bool preact_wide,
-                                             bool residual, unsigned char* piece, int lane) {
+                                             bool residual, unsigned char* piece, int lane,
+                                             bool& special) {
   constexpr uint32_t kRow = kCols * sizeof(Out);
   constexpr uint32_t kSwizzle = kRow == 128 ? 7 : (kRow == 64 ? 3 : 1);
   constexpr int kPer = 16 / static_cast<int>(sizeof(Out));  // elements of 16 bytes
@@ -428,6 +554,10 @@ __device__ __forceinline__ void finish_piece(uint32_t taddr, const float* bias, 
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] = times_pow2(v[j], exp_a + exp_b[i + j]);
       }
+      float2 z = both(0.0f);  // NaN where an element is, or infinite
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) z = fma2(make_float2(v[j], v[j + 1]), both(0.0f), z);
+      special |= !(z.x + z.y == 0.0f);
     }
     if (bias != nullptr) {
 #pragma unroll
@@ -470,11 +600,13 @@ __device__ __forceinline__ void finish_piece(uint32_t taddr, const float* bias, 
   }
 }
 
-// NaN over a piece (this lane's row of it), where the pipeline gave up.
+// NaN over a piece (this lane's row of it), where the pipeline gave up; with bits of its own, since
+// splits of a sum that hold it are not computed anew.
+constexpr uint32_t kGivenUp = 0x7fc0dead;
 template <class Out, int kCols>
 __device__ __noinline__ void poison_piece(unsigned char* piece, int lane) {
   Out* row = reinterpret_cast<Out*>(piece) + lane * kCols;
-  for (int c = 0; c < kCols; ++c) row[c] = dev::from_f32<Out>(__uint_as_float(0x7fc00000u));
+  for (int c = 0; c < kCols; ++c) row[c] = dev::from_f32<Out>(__uint_as_float(kGivenUp));
 }
 
 // The preactivations of a piece's columns where they can neither be stored whole nor through the
@@ -558,25 +690,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   const int units = g.units[0] + g.units[1];
   const int worker = kPair ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
   const int workers = kPair ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
-  // Unit u: product q, split, then tile row / column, columns fastest (a wave's CTAs share rows of
-  // A and all of B in L2), and the split's blocks of k.
-  struct Unit {
-    int q, split, tm, tn, b0, b1;
-  };
-  auto unit = [&](int u) {
-    Unit w;
-    w.q = u >= g.units[0];
-    u -= w.q ? g.units[0] : 0;
-    const ProductArgs& a = g.p[w.q];
-    const int per = a.tiles_m * a.tiles_n;
-    w.split = u / per;
-    const int t = u - w.split * per;
-    w.tm = t / a.tiles_n;
-    w.tn = t - w.tm * a.tiles_n;
-    w.b0 = w.split * a.blocks_per_split;
-    w.b1 = min(a.k_blocks, w.b0 + a.blocks_per_split);
-    return w;
-  };
+  auto unit = [&](int u) { return unit_of(g, u); };
 
   // Ahead of the set-up's barrier: the first unit's parameters and tensor maps are on their way
   // while tensor memory is allocated.
@@ -799,6 +913,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     // results are NaN: a barrier that nobody advances would satisfy the wait after next with the
     // phase before, and arrivals out of turn would stand in for the other CTA's.
     bool alive = true;
+    bool special = false;
     int t = 0, parity = 0;  // chunks read so far; of units
     for (int u = worker; u < units; u += workers, parity ^= 1) {
       const Unit w = u == worker ? first : unit(u);
@@ -903,7 +1018,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         auto finish_f32 = [&](int act, T* preact, bool wide, bool residual) {
           by_act(act, [&](auto k) {
             finish_piece<T, float, kWide, decltype(k)::value>(taddr, b, e, exp_a, preact, wide,
-                                                              residual, piece, lane);
+                                                              residual, piece, lane, special);
           });
           if (!alive) poison_piece<float, kWide>(piece, lane);
           __syncwarp();
@@ -932,7 +1047,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             if (!a.ep.out_f32) {
               by_act(a.ep.act, [&](auto k) {
                 finish_piece<T, T, kCols, decltype(k)::value>(taddr, b, e, exp_a, preact, wide,
-                                                              res_tiles, piece, lane);
+                                                              res_tiles, piece, lane, special);
               });
               if (!alive) poison_piece<T, kCols>(piece, lane);
             }
@@ -970,6 +1085,15 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       }
       if (alive) release(slot);
     }
+    if constexpr (sizeof(T) == 4) {
+      if (alive && __any_sync(dev::kFull, special)) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // written
+        asm volatile("fence.proxy.async;" ::: "memory");
+        __syncwarp();
+        finish_special(g, worker, workers, S::kM, static_cast<int>(rank) * kBM + quarter * 32, kBN,
+                       group * kCols, kCols, lane);
+      }
+    }
     // The pieces stay until the last stores have read them.
     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
   }
@@ -1004,7 +1128,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
 struct SplitJob {
   const float* partial;
   int splits;  // 0: nothing to join
-  int64_t m, n;
+  int64_t m, n, k;
+  Sources from;
   Epilogue ep;
 };
 struct SumsJob {
@@ -1027,7 +1152,10 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinJ
     const int splits = j.splits;
     const float* partial = j.partial;
     const uint32_t per_row = static_cast<uint32_t>(j.n / kV);
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < size / kV; i += gridDim.x * 256ll) {
+    const int lane = threadIdx.x & 31;
+    const int64_t packs = size / kV;
+    for (int64_t i0 = blockIdx.x * 256ll + threadIdx.x - lane; i0 < packs; i0 += gridDim.x * 256ll) {
+      const int64_t i = min(i0 + lane, packs - 1);  // past the end the last again: whole warps
       float s[kV];
 #pragma unroll
       for (int v = 0; v < kV; ++v) s[v] = 0.0f;
@@ -1040,7 +1168,20 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinJ
       const int64_t row = i >> 32 ? i / per_row : static_cast<uint32_t>(i) / per_row;
       const int64_t col = (i - row * per_row) * kV;
 #pragma unroll
-      for (int v = 0; v < kV; ++v) finish1<T>(j.ep, row, col + v, s[v]);
+      for (int v = 0; v < kV; ++v) {
+        if constexpr (sizeof(T) == 4) {
+          bool again = s[v] != s[v];  // unless a split gave up
+          for (int k = 0; again && k < splits; ++k)
+            again = __float_as_uint(partial[k * size + i * kV + v]) != kGivenUp;
+          for (uint32_t todo = __ballot_sync(dev::kFull, again); todo != 0; todo &= todo - 1) {
+            const int l = __ffs(todo) - 1;
+            const float y = plain_sum(j.from, __shfl_sync(dev::kFull, row, l),
+                                      __shfl_sync(dev::kFull, col, l) + v, j.k, lane);
+            if (lane == l) s[v] = y;
+          }
+        }
+        if (i0 + lane < packs) finish1<T>(j.ep, row, col + v, s[v]);
+      }
     }
     return;
   }
@@ -1282,6 +1423,7 @@ struct Product {
   int64_t m, n, k;
   bool a_mn, b_mn;
   Stored a, b;
+  Sources from;  // of float32
   Epilogue ep;
   const int* wide = nullptr;  // scaled operands that may be three planes instead: which they are
 };
@@ -1444,6 +1586,8 @@ void run_products(const Product* p, int count, const ProductPlan& plan, unsigned
     ProductArgs& a = g.p[q];
     a.m = p[q].m;
     a.n = p[q].n;
+    a.k = p[q].k;
+    a.from = p[q].from;
     a.pairs = p[q].a.planes == 3 ? 6 : (p[q].a.planes == 2 ? 3 : 1);
     a.exp_a = p[q].a.exponents;
     a.exp_b = p[q].b.exponents;
@@ -1472,7 +1616,7 @@ void run_products(const Product* p, int count, const ProductPlan& plan, unsigned
     partial += plan.partial_bytes[q];
     g.units[q] = a.tiles_m * a.tiles_n * a.splits;
     if (a.splits > 1) {
-      jobs.split[q] = SplitJob{a.partial, a.splits, a.m, a.n, a.ep};
+      jobs.split[q] = SplitJob{a.partial, a.splits, a.m, a.n, a.k, a.from, a.ep};
       items = std::max(items, static_cast<size_t>(a.m) * a.n);
     }
   }
@@ -1780,6 +1924,8 @@ void linear_forward(const qv_linear& l, void* workspace, size_t workspace_bytes,
     d.k = static_cast<int64_t>(l.k);
     d.a = pack.rows(l.x, l.m, l.k, l.x_stride);
     d.b = pack.rows(l.weight, l.n, l.k, l.weight_stride);
+    d.from = Sources{l.x, static_cast<int64_t>(l.x_stride), 1, 0,
+                     static_cast<const float*>(l.weight), static_cast<int64_t>(l.weight_stride), 1};
     d.ep = ep;
     const bool packed = pack.count() > 0;
     unsigned char* partial = pack.run(false, st);
@@ -1963,12 +2109,17 @@ void linear_grad(const qv_linear_grad& g, void* workspace, size_t workspace_byte
       Product& d = L.products[q++];
       d.a = dz;
       d.b = pack.rows(g.x, g.m, g.k, g.x_stride);
+      d.from = Sources{dz.p, 1, dz.ld, m * dz.ld,
+                       static_cast<const float*>(g.x), 1, static_cast<int64_t>(g.x_stride)};
       d.ep = result(g.dweight, g.dweight_stride);
     }
     if (g.dx != nullptr) {
       Product& d = L.products[q++];
       d.a = dz;
       d.b = pack.rows(g.weight, g.n, g.k, g.weight_stride);
+      d.from = Sources{dz.p, dz.ld, 1, m * dz.ld,
+                       static_cast<const float*>(g.weight), 1,
+                       static_cast<int64_t>(g.weight_stride)};
       d.ep = result(g.dx, g.dx_stride);
     }
     const bool first = L.store_dz || sums != nullptr;  // the dz kernel ran

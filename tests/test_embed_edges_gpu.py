@@ -186,3 +186,72 @@ def test_linear_float32_wide_rows_alternate(embed):
         graph.replay()
         assert torch.equal(out, want[i])
         assert torch.equal(embed.linear(*(plain, wide)[i]), want[i])
+
+
+def same_special(got, want, what=""):
+    """Infinities and NaN exactly where the definition has them, and nowhere else."""
+    assert torch.equal(got.isnan(), want.isnan()), what
+    inf = want.isinf()
+    assert torch.equal(got.isinf(), inf), what
+    assert torch.equal(got[inf].double(), want[inf]), what
+
+
+def plain_product(x, w):
+    """x w^T in 64 bits with every term's own infinities (a library product may skip zeros)."""
+    return torch.cat([(p[:, None, :] * w.double()[None]).sum(-1) for p in x.double().split(64)])
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("m,k,n", [(3, 40, 50), (140, 72, 130), (40, 4096, 72), (700, 129, 257)])
+def test_linear_infinities(embed, t, m, k, n):
+    """Infinite elements of x and of the weights: alone, beside large finite ones, of both signs,
+    against zeros."""
+    t = TYPES[t]
+    g = gen(m + k)
+    x, w = normal(g, m, k, t=t), normal(g, n, k, t=t)
+    w[:, ::7] = 1  # values one part holds
+    clean = embed.linear(x, w)
+    inf = math.inf
+    x[0, 0] = inf
+    x[1, [3, 5]] = torch.tensor([-inf, -inf], device="cuda", dtype=t)
+    x[2, [2, 7]] = torch.tensor([inf, -inf], device="cuda", dtype=t)
+    if m > 8:
+        x[m - 1, 1], x[m - 1, 2] = inf, (1e6 if t != torch.float16 else 6e4)
+        x[5, 4], x[6, k - 1] = math.nan, inf
+        w[n - 1, 9] = -inf
+        w[n - 2, 11], w[n - 2, 12] = inf, 0
+        w[3, 0] = 0  # against x[0, 0]
+        x[7, 9] = 0
+    want = plain_product(x, w)
+    got = embed.linear(x, w)
+    same_special(got, want)
+    keep = torch.isfinite(x).all(1)[:, None] & torch.isfinite(w).all(1)[None] & (w[:, 0] != 0)
+    if m > 8:
+        keep[7] = False
+    assert torch.equal(got[keep], clean[keep])
+    # through bias, residual and preactivations, whole and unaligned rows
+    b, r = normal(g, n, t=t), normal(g, m, n, t=t)
+    z = want + b.double()
+    y, pre = embed.linear_preact(x, w, b, residual=r, activation="relu")
+    same_special(pre, z)
+    same_special(y, torch.where(z.isnan(), z, z.clamp(min=0)) + r.double())
+    # gradients: dz holds the infinities
+    dy = normal(g, m, n, t=t)
+    dy[0, 0] = inf
+    dy[1, 1], dy[1, 2] = -inf, -inf
+    fx, fw = normal(g, m, k, t=t), normal(g, n, k, t=t)
+    fx[0, 0] = 0
+    fw[:, ::5] = -1
+    dx, dw, db = embed.linear_grad(dy, fx, fw)
+    same_special(dx, plain_product(dy, fw.t()), "dx")
+    same_special(dw, plain_product(dy.t(), fx.t()), "dw")
+    same_special(db, dy.double().sum(0), "db")
+
+
+def test_linear_all_special(embed):
+    """Nothing but NaN, and nothing but infinities, at a size of many tiles."""
+    x, w = torch.full((3000, 256), math.nan, device="cuda"), normal(gen(1), 500, 256)
+    assert embed.linear(x, w).isnan().all()
+    x.fill_(math.inf)
+    assert embed.linear(x, w.abs() + 1).eq(math.inf).all()
+    same_special(embed.linear(x[:100], w), plain_product(x[:100], w))
