@@ -255,3 +255,39 @@ def test_linear_all_special(embed):
     x.fill_(math.inf)
     assert embed.linear(x, w.abs() + 1).eq(math.inf).all()
     same_special(embed.linear(x[:100], w), plain_product(x[:100], w))
+
+
+def act_ref(z, act):
+    if act == "relu":
+        return z.clamp(min=0)
+    if act == "gelu":  # by erfc, which keeps the tail
+        return z * 0.5 * torch.special.erfc(-z * math.sqrt(0.5))
+    if act == "gelu_tanh":  # z / (1 + exp(-2u)): the tanh form without its cancellation
+        return z * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))
+    if act == "silu":
+        return z * torch.sigmoid(z)
+    return z
+
+
+def activations_on_a_grid(embed, t, act, out_dtype, m, relative):
+    """act(z) by a layer of zero weights whose bias is z."""
+    z = torch.cat([torch.linspace(-90, 90, 24001), torch.linspace(-14, 14, 40001),
+                   torch.linspace(-0.01, 0.01, 2001)]).cuda().to(t)
+    for z in z.split(65536):
+        got = embed.linear(torch.zeros(m, 16, device="cuda", dtype=t),
+                           torch.zeros(len(z), 16, device="cuda", dtype=t), z, activation=act,
+                           out_dtype=out_dtype)
+        want = act_ref(z.double(), act).expand(m, len(z))
+        # factors below 2^-126 are flushed to zero: up to |z| 2^-126 <= 90 * 2^-126 < 2^-119
+        assert_within(got, want, want.abs() * relative + 2.0 ** -119 + TINY[got.dtype], act)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("m", [1, 200])
+def test_activation_tails(embed, t, act, m):
+    """16-bit activations to their own half step in the tails too. The exponents reach 126 in units
+    of log2, with up to three roundings of 2^-24: 1.6e-5; with the fitted tail's 4.3e-6 less than
+    2^-15 of the value."""
+    t = TYPES[t]
+    activations_on_a_grid(embed, t, act, None, m, half_step(t) + 2.0 ** -15)
