@@ -257,12 +257,14 @@ __global__ void __launch_bounds__(256)
 // ring of shared-memory stages with TMA, one thread issues the MMAs into one of two accumulators
 // in tensor memory, and sixteen warps finish the other accumulator's elements meanwhile.
 //
-// The tensor core's float32 sums are cut, not rounded, after each 16 terms: over k terms of one
-// sign the result falls short by about k / 32 * 1.7e-7 of itself (2.6e-5 measured at k = 4096), and
+// The tensor core's float32 sums are cut, not rounded, several times in 16 terms: over k terms of one
+// sign the result falls short by about k * 6.4e-9 of itself (2.6e-5 measured at k = 4096), and
 // sums of random signs lose a fifth of that. So no sum stays there for more than `chunk` blocks of
 // 64 terms: the epilogue warps then add it to one in their registers, rounding, while the next
-// chunk's MMAs fill the other accumulator. Float32 products take chunks of 2 blocks (7e-7), 16-bit
-// ones 128 (5e-5, a fortieth of bfloat16's half step and a tenth of float16's).
+// chunk's MMAs fill the other accumulator. Float32 products take chunks of 2 blocks (8e-7); 16-bit
+// operands chunks of 128 for 16-bit results (5e-5, a fortieth of bfloat16's half step and a tenth of
+// float16's), of 8 for float32 results (3.4e-6; chunks of 2 took 544 us for 32,768 x 1024 x 4096
+// where one of 16 takes 247).
 //
 // Large products run in CTA pairs (tcgen05 cta_group::2): 256 x 256 tiles, each CTA loading its
 // 128 rows of A and half of B. A CTA by itself would have to load 384 rows of operands for
@@ -534,8 +536,8 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&r)[16]) 
 // out of tensor memory into shared memory in the tensor map's swizzle. exp_b: the columns'
 // exponents (exp_a: this lane's row's) where operands were scaled, or nullptr. residual: the piece
 // holds it, in type Out. preact: this lane's row, or nullptr. special: float32 only, set where a sum
-// is NaN or infinite.
-template <class T, class Out, int kCols, int kAct>
+// is NaN or infinite. kFast: the activation for 16-bit results.
+template <class T, class Out, int kCols, int kAct, bool kFast>
 __device__ __forceinline__ void finish_piece(uint32_t taddr, const float* bias, const int* exp_b,
                                              int exp_a, T* preact, bool preact_wide,
                                              bool residual, unsigned char* piece, int lane,
@@ -574,7 +576,7 @@ __device__ __forceinline__ void finish_piece(uint32_t taddr, const float* bias, 
     if (preact != nullptr) put16<T>(preact + i, v, 16, preact_wide ? 32 : 16);
 #pragma unroll
     for (int j = 0; j < 16; j += 2) {
-      const float2 y = activate2<sizeof(T) == 2>(kAct, make_float2(v[j], v[j + 1]));
+      const float2 y = activate2<kFast>(kAct, make_float2(v[j], v[j + 1]));
       v[j] = y.x;
       v[j + 1] = y.y;
     }
@@ -661,11 +663,13 @@ __device__ __forceinline__ void store_piece(const unsigned char* piece, Out* out
   }
 }
 
-template <class T, int kBN, bool kPair, bool kChunked>
+// T: the operands' type, Out: the results' (T or float32).
+template <class T, class Out, int kBN, bool kPair, bool kChunked>
 __global__ void __launch_bounds__(kProductThreads, 1)
     product_kernel(const __grid_constant__ ProductMaps maps,
                    const __grid_constant__ ProductGroup g) {
   using S = Tile<kBN, kPair>;
+  constexpr bool kOutF32 = sizeof(Out) == 4;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* tiles = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -944,7 +948,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       // The piece's columns: 128 bytes at most, of the result or, where that is not stored as a
       // tile, of float32.
       constexpr int kWide = kCols < 32 ? kCols : 32;
-      const int per_piece = in_tiles && !a.ep.out_f32 ? kCols : kWide;
+      const int per_piece = in_tiles && !kOutF32 ? kCols : kWide;
 #pragma unroll 1
       for (int c = 0; c < kCols; c += per_piece) {
         const int64_t col = col0 + c;
@@ -954,7 +958,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           if (lane == 0) {
             asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the piece is free
             if (load) {
-              tc::mbar_expect_tx(res_bar, 32 * per_piece * (a.ep.out_f32 ? 4 : 2));
+              tc::mbar_expect_tx(res_bar, 32 * per_piece * sizeof(Out));
               tc::tma_load_2d(tc::smem_u32(piece), &maps.residual[w.q], static_cast<int>(col),
                               static_cast<int>(row0), res_bar);
             }
@@ -1017,8 +1021,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         };
         auto finish_f32 = [&](int act, T* preact, bool wide, bool residual) {
           by_act(act, [&](auto k) {
-            finish_piece<T, float, kWide, decltype(k)::value>(taddr, b, e, exp_a, preact, wide,
-                                                              residual, piece, lane, special);
+            finish_piece<T, float, kWide, decltype(k)::value, !kOutF32>(
+                taddr, b, e, exp_a, preact, wide, residual, piece, lane, special);
           });
           if (!alive) poison_piece<float, kWide>(piece, lane);
           __syncwarp();
@@ -1043,16 +1047,15 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           }
         }
         if (in_tiles) {
-          if constexpr (sizeof(T) == 2) {
-            if (!a.ep.out_f32) {
-              by_act(a.ep.act, [&](auto k) {
-                finish_piece<T, T, kCols, decltype(k)::value>(taddr, b, e, exp_a, preact, wide,
-                                                              res_tiles, piece, lane, special);
-              });
-              if (!alive) poison_piece<T, kCols>(piece, lane);
-            }
+          if constexpr (kOutF32) {
+            finish_f32(a.ep.act, preact, wide, res_tiles);
+          } else {
+            by_act(a.ep.act, [&](auto k) {
+              finish_piece<T, T, kCols, decltype(k)::value, true>(
+                  taddr, b, e, exp_a, preact, wide, res_tiles, piece, lane, special);
+            });
+            if (!alive) poison_piece<T, kCols>(piece, lane);
           }
-          if (sizeof(T) == 4 || a.ep.out_f32) finish_f32(a.ep.act, preact, wide, res_tiles);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0)
@@ -1071,15 +1074,9 @@ __global__ void __launch_bounds__(kProductThreads, 1)
                                   ? static_cast<const T*>(a.ep.residual) +
                                         row0 * a.ep.residual_stride + col
                                   : nullptr;
-          if (a.ep.out_f32)
-            store_piece<T, float, kWide>(
-                piece, static_cast<float*>(a.ep.out) + row0 * a.ep.out_stride + col,
-                a.ep.out_stride, residual, a.ep.residual_stride, rows, cols, lane);
-          else
-            store_piece<T, T, kWide>(piece,
-                                     static_cast<T*>(a.ep.out) + row0 * a.ep.out_stride + col,
-                                     a.ep.out_stride, residual, a.ep.residual_stride, rows, cols,
-                                     lane);
+          store_piece<T, Out, kWide>(
+              piece, static_cast<Out*>(a.ep.out) + row0 * a.ep.out_stride + col, a.ep.out_stride,
+              residual, a.ep.residual_stride, rows, cols, lane);
         }
         __syncwarp();
       }
@@ -1521,7 +1518,7 @@ ProductPlan plan_products(const Product* p, int count, int pairs, int sms) {
   return best;
 }
 
-template <class T, int kBN, bool kPair, bool kChunked>
+template <class T, class Out, int kBN, bool kPair, bool kChunked>
 void launch_products(const Product* p, int count, const ProductGroup& g, bool chained, int sms,
                      cudaStream_t st) {
   using S = Tile<kBN, kPair>;
@@ -1548,7 +1545,7 @@ void launch_products(const Product* p, int count, const ProductGroup& g, bool ch
   int device = 0;
   QV_CUDA(cudaGetDevice(&device));
   std::call_once(once[device & 15], [&] {
-    QV_CUDA(cudaFuncSetAttribute(product_kernel<T, kBN, kPair, kChunked>,
+    QV_CUDA(cudaFuncSetAttribute(product_kernel<T, Out, kBN, kPair, kChunked>,
                                  cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  static_cast<int>(S::kSmem)));
   });
@@ -1568,7 +1565,7 @@ void launch_products(const Product* p, int count, const ProductGroup& g, bool ch
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = kPair ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, product_kernel<T, kBN, kPair, kChunked>, maps, g);  // reported by check_launch
+  cudaLaunchKernelEx(&cfg, product_kernel<T, Out, kBN, kPair, kChunked>, maps, g);  // reported by check_launch
   check_launch("product_kernel");
 }
 
@@ -1596,7 +1593,7 @@ void run_products(const Product* p, int count, const ProductPlan& plan, unsigned
     a.tiles_n = static_cast<int>(ceil_div(a.n, plan.bn));
     a.splits = plan.splits[q];
     a.blocks_per_split = plan.blocks_per_split[q];
-    a.chunk = a.pairs > 1 ? 2 : 128;
+    a.chunk = a.pairs > 1 ? 2 : (p[q].ep.out_f32 ? 8 : 128);
     auto idesc = [&](bool bf16) {
       const uint32_t fmt = bf16 ? 1 : 0;
       return (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(p[q].a_mn) << 15) |
@@ -1623,25 +1620,29 @@ void run_products(const Product* p, int count, const ProductPlan& plan, unsigned
   g.wait_cycles = tc::wait_limit_cycles();
   g.drain_ns = tc::drain_limit_ns();
   if (count > 0) {
-    auto launch = [&](auto chunked) {
+    auto launch = [&](auto out, auto chunked) {
+      using Out = decltype(out);
       constexpr bool kChunked = decltype(chunked)::value;
       if (plan.pair)
-        launch_products<T, 256, true, kChunked>(p, count, g, chained, sms, st);
+        launch_products<T, Out, 256, true, kChunked>(p, count, g, chained, sms, st);
       else if (plan.bn == 128)
-        launch_products<T, 128, false, kChunked>(p, count, g, chained, sms, st);
+        launch_products<T, Out, 128, false, kChunked>(p, count, g, chained, sms, st);
       else
-        launch_products<T, 64, false, kChunked>(p, count, g, chained, sms, st);
+        launch_products<T, Out, 64, false, kChunked>(p, count, g, chained, sms, st);
     };
-    // Sums of one chunk (16-bit operands with k up to 8192) leave the adding out of the kernel,
-    // whose registers cost 4 % there.
+    // Sums of one chunk (16-bit operands and results with k up to 8192) leave the adding out of the
+    // kernel, whose registers cost 4 % there. Float32 results of 16-bit operands have kernels of
+    // their own: with both results in one, linear layers of 16-bit results took 14 % longer.
     bool chunked = std::is_same_v<T, float>;
     for (int q = 0; q < count; ++q) chunked |= plan.blocks_per_split[q] > g.p[q].chunk;
     if constexpr (std::is_same_v<T, float>)
-      launch(std::true_type{});
+      launch(float{}, std::true_type{});
+    else if (p[0].ep.out_f32)  // a forward product, by itself
+      launch(float{}, std::true_type{});
     else if (chunked)
-      launch(std::true_type{});
+      launch(T{}, std::true_type{});
     else
-      launch(std::false_type{});
+      launch(T{}, std::false_type{});
   }
   if (sums.sums != nullptr) items = std::max(items, static_cast<size_t>(sums.n) * 8);
   if (items > 0) {

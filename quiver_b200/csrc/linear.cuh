@@ -129,7 +129,8 @@ __device__ __forceinline__ float tanh_arg(float x) {
 }
 __device__ __forceinline__ float logistic(float x) { return 1.0f / (1.0f + expf(-x)); }
 
-// act(z) of two values: for 16-bit results (kFast) the formulas above, for float32 the math library.
+// act(z) of two values: for 16-bit results (kFast) the formulas above, for float32 results, of 16-bit
+// inputs too, the math library.
 template <bool kFast>
 __device__ __forceinline__ float2 activate2(int act, float2 z) {
   switch (act) {
@@ -242,7 +243,8 @@ __device__ __forceinline__ void finish1(const Epilogue& e, int64_t row, int64_t 
   if (e.bias != nullptr) s += dev::to_f32<T>(static_cast<const T*>(e.bias)[col]);
   if (e.preact != nullptr)
     static_cast<T*>(e.preact)[row * e.preact_stride + col] = dev::from_f32<T>(s);
-  float y = activate2<sizeof(T) == 2>(e.act, both(s)).x;
+  float y = sizeof(T) == 2 && !e.out_f32 ? activate2<true>(e.act, both(s)).x
+                                         : activate2<false>(e.act, both(s)).x;
   if (e.residual != nullptr)
     y += dev::to_f32<T>(static_cast<const T*>(e.residual)[row * e.residual_stride + col]);
   if (e.out_f32)

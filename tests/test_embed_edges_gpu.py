@@ -291,3 +291,45 @@ def test_activation_tails(embed, t, act, m):
     2^-15 of the value."""
     t = TYPES[t]
     activations_on_a_grid(embed, t, act, None, m, half_step(t) + 2.0 ** -15)
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("m", [1, 200])
+def test_activations_to_float32(embed, t, act, m):
+    """Float32 results, of 16-bit inputs too: the math library's few ulp (2^-21) and the exponents'
+    roundings, which grow with them: |x| <= 4 gelu_tanh's argument has at most 2^3.4 and three
+    roundings of 2^-24."""
+    t = TYPES[t]
+    z = torch.linspace(-4, 4, 40001).cuda().to(t)
+    got = embed.linear(torch.zeros(m, 16, device="cuda", dtype=t),
+                       torch.zeros(len(z), 16, device="cuda", dtype=t), z, activation=act,
+                       out_dtype=torch.float32)
+    want = act_ref(z.double(), act).expand(m, len(z))
+    assert_within(got, want, want.abs() * 2.0 ** -18.5 + 2.0 ** -140, act)
+    activations_on_a_grid(embed, t, act, torch.float32, m, 2.0 ** -15)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("m,k,n", [(3, 500, 70), (300, 1000, 96), (300, 4096, 1000),
+                                   (5000, 8192, 520), (260, 8190, 257)])
+def test_float32_results_of_16_bit_inputs(embed, t, m, k, n):
+    """Sums of one sign, with bias, activation and residual. The accumulator cuts its sum so far by
+    at most 2u, and at most once for every four terms (at 4096 terms it loses 436u, which are 1.7u
+    of the mean sum for every eight: cuts lose half of what they may at the mean). 512 terms stay
+    there: 128 cuts, at half of the last sum on average, 128u; then the sums are added, rounding."""
+    t = TYPES[t]
+    g = gen(m + n)
+    x, w = normal(g, m, k, t=t).abs(), normal(g, n, k, t=t, scale=1 / k).abs()
+    b, r = normal(g, n, t=t), normal(g, m, n, t=t)
+    mass = x.double() @ w.double().t()
+    sums = mass * (128 + k / 512 + 8) * U
+    got = embed.linear(x, w, out_dtype=torch.float32)
+    assert_within(got, mass, sums)
+    z = mass + b.double()
+    zerr = sums + z.abs() * U
+    for act in ("none", "silu"):
+        want = act_ref(z, act) + r.double()
+        err = 1.13 * zerr + (z.abs() + want.abs()) * (2.0 ** -21 + U)
+        got = embed.linear(x, w, b, residual=r, activation=act, out_dtype=torch.float32)
+        assert_within(got, want, err, act)
