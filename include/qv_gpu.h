@@ -351,7 +351,9 @@ qv_status qv_linear_device(int device, const qv_linear* args, void* workspace,
  * dz = grad * activation'(preact), dx = dz weight, dweight = dz^T x, dbias = the column sums of dz
  * (the residual's gradient is grad itself). Outputs that are NULL are not computed, inputs that no
  * output needs may be NULL (preact: QV_ACT_NONE; weight: no dx; x: no dweight). 16-bit dz is
- * rounded once to dtype before the products; dbias sums the unrounded values. */
+ * rounded once to dtype before the products; dbias sums the unrounded values. grad is float32 where
+ * dtype has QV_GRAD_F32 added (as the gradient of a float32 result is). */
+enum { QV_GRAD_F32 = 0x100 };
 typedef struct qv_linear_grad {
   uint32_t dtype, activation;
   size_t m, n, k;

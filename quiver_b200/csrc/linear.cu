@@ -1280,7 +1280,7 @@ __global__ void __launch_bounds__(128)
 // ---- dz and the bias gradient ----------------------------------------------------------------------
 
 // dz = dy * act'(z), rounded to the operand type (float32: three planes), and float32 column sums
-// of the unrounded dz over this block's rows. A block takes 32 pieces' columns and a range of rows:
+// of the unrounded dz; dy is of type G (T, or float32 as it comes from a float32 result) over this block's rows. A block takes 32 pieces' columns and a range of rows:
 // warp w walks rows w, w + 8, .. of it, and the warps' sums are added in order at the end, so the
 // sums have a fixed order. Bound by memory: dy and z read, dz written.
 constexpr int kDzWarps = 8, kDzRows = 4;  // rows in flight per warp
@@ -1288,9 +1288,9 @@ constexpr int dz_pieces(size_t piece_bytes) {  // 2-byte pieces: four a lane
   return piece_bytes == 2 ? 4 : 1;
 }
 
-template <class T, int kV, bool kStore, int kAct>
+template <class T, class G, int kV, bool kStore, int kAct>
 __global__ void __launch_bounds__(32 * kDzWarps)
-    dz_kernel(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ z,
+    dz_kernel(const G* __restrict__ dy, int64_t dy_stride, const T* __restrict__ z,
               int64_t z_stride, int64_t m, int64_t n, int64_t rows_per_block,
               typename Operand<T>::type* __restrict__ dz, int64_t ld, float* __restrict__ sums) {
   dev::allow_next();
@@ -1312,13 +1312,14 @@ __global__ void __launch_bounds__(32 * kDzWarps)
     for (int j = 0; j < kV; ++j) s[q][j] = 0.0f;
   }
   for (int64_t r = blockIdx.x * rows_per_block + warp; r < r1; r += kDzWarps * kDzRows) {
-    Pack<T, kV> g[kDzRows][kC], x[kDzRows][kC];
+    Pack<G, kV> g[kDzRows][kC];
+    Pack<T, kV> x[kDzRows][kC];
 #pragma unroll
     for (int u = 0; u < kDzRows; ++u) {
       const int64_t row = min(r + u * kDzWarps, r1 - 1);  // past the range its last row again
 #pragma unroll
       for (int q = 0; q < kC; ++q) {
-        g[u][q] = dev::load_pack<T, kV>(dy + row * dy_stride + col[q]);
+        g[u][q] = dev::load_pack<G, kV>(dy + row * dy_stride + col[q]);
         if (kAct != QV_ACT_NONE) x[u][q] = dev::load_pack<T, kV>(z + row * z_stride + col[q]);
       }
     }
@@ -1330,7 +1331,7 @@ __global__ void __launch_bounds__(32 * kDzWarps)
       for (int q = 0; q < kC; ++q) {
         float d[kV];
 #pragma unroll
-        for (int j = 0; j < kV; ++j) d[j] = dev::to_f32<T>(g[u][q].v[j]);
+        for (int j = 0; j < kV; ++j) d[j] = dev::to_f32<G>(g[u][q].v[j]);
         if constexpr (kAct != QV_ACT_NONE) {
 #pragma unroll
           for (int j = 0; j < kV; j += 2) {
@@ -1939,31 +1940,35 @@ void linear_forward(const qv_linear& l, void* workspace, size_t workspace_bytes,
 
 namespace {
 
+// The type of everything but the gradient, and whether that is float32.
+uint32_t grad_dtype(const qv_linear_grad& g) { return g.dtype & ~static_cast<uint32_t>(QV_GRAD_F32); }
+bool grad_f32(const qv_linear_grad& g) {
+  return (g.dtype & QV_GRAD_F32) != 0 || g.dtype == QV_DTYPE_F32;
+}
+
 void check_linear_grad(const qv_linear_grad& g) {
-  check_dtype(g.dtype);
+  const uint32_t dtype = grad_dtype(g);
+  check_dtype(dtype);
   QV_REQUIRE(g.activation <= QV_ACT_SILU, "unknown activation");
   QV_REQUIRE(g.k >= 1 && g.k <= kMaxDim && g.n >= 1 && g.n <= kMaxDim,
              "dimensions must be between 1 and 65536");
   QV_REQUIRE(g.m <= kMaxLinearRows, "too many rows");
   if (g.dweight != nullptr)
-    check_matrix("dweight", g.dtype, g.dweight, g.n, g.k, g.dweight_stride);
-  if (g.dbias != nullptr) check_matrix("dbias", g.dtype, g.dbias, 1, g.n, g.n);
+    check_matrix("dweight", dtype, g.dweight, g.n, g.k, g.dweight_stride);
+  if (g.dbias != nullptr) check_matrix("dbias", dtype, g.dbias, 1, g.n, g.n);
   if (g.m == 0) return;
-  check_matrix("grad", g.dtype, g.grad, g.m, g.n, g.grad_stride);
+  check_matrix("grad", grad_f32(g) ? QV_DTYPE_F32 : dtype, g.grad, g.m, g.n, g.grad_stride);
   if (g.activation != QV_ACT_NONE)
-    check_matrix("preact", g.dtype, g.preact, g.m, g.n, g.preact_stride);
+    check_matrix("preact", dtype, g.preact, g.m, g.n, g.preact_stride);
   if (g.dx != nullptr) {
-    check_matrix("weight", g.dtype, g.weight, g.n, g.k, g.weight_stride);
-    check_matrix("dx", g.dtype, g.dx, g.m, g.k, g.dx_stride);
+    check_matrix("weight", dtype, g.weight, g.n, g.k, g.weight_stride);
+    check_matrix("dx", dtype, g.dx, g.m, g.k, g.dx_stride);
   }
-  if (g.dweight != nullptr) check_matrix("x", g.dtype, g.x, g.m, g.k, g.x_stride);
+  if (g.dweight != nullptr) check_matrix("x", dtype, g.x, g.m, g.k, g.x_stride);
 }
 
-template <class T>
-constexpr int kWideDz = 16 / static_cast<int>(sizeof(T));
-
 struct GradLayout {
-  bool wide_dz = false;       // 16-byte pieces of the gradient and the preactivations
+  bool wide_dz = false;       // 16-byte pieces of the gradient, and as many preactivations
   bool store_dz = false;      // dz is not the caller's gradient itself
   size_t row_blocks = 0;      // row ranges of the column sums
   int64_t rows_per_block = 0;
@@ -1975,16 +1980,18 @@ struct GradLayout {
 GradLayout grad_layout(const qv_linear_grad& g, int sms) {
   GradLayout L;
   if (g.m == 0) return L;
-  const int pairs = g.dtype == QV_DTYPE_F32 ? 6 : 1;
+  const uint32_t dtype = grad_dtype(g);
+  const int pairs = dtype == QV_DTYPE_F32 ? 6 : 1;
   const bool products = g.dx != nullptr || g.dweight != nullptr;
-  L.store_dz = products && (g.activation != QV_ACT_NONE ||
-                            !in_place(g.dtype, g.grad, g.m, g.grad_stride));
-  const size_t e = dtype_size(g.dtype);
-  L.wide_dz = common_align({reinterpret_cast<uintptr_t>(g.grad),
-                            reinterpret_cast<uintptr_t>(g.preact), g.m > 1 ? g.grad_stride * e : 0,
-                            g.m > 1 ? g.preact_stride * e : 0, g.n * e}) == 16;
+  L.store_dz = products && (g.activation != QV_ACT_NONE || (grad_f32(g) && dtype != QV_DTYPE_F32) ||
+                            !in_place(dtype, g.grad, g.m, g.grad_stride));
+  const size_t e = dtype_size(dtype), ge = grad_f32(g) ? 4 : e;
+  L.wide_dz = common_align({reinterpret_cast<uintptr_t>(g.grad), g.m > 1 ? g.grad_stride * ge : 0,
+                            g.n * ge}) == 16 &&
+              common_align({reinterpret_cast<uintptr_t>(g.preact),
+                            g.m > 1 ? g.preact_stride * e : 0}) >= static_cast<int>(16 / ge * e);
   // About eight blocks an SM, each with at least one round of its warps.
-  const size_t col_blocks = ceil_div(g.n, L.wide_dz ? 32 * 16 / e : 32 * dz_pieces(e));
+  const size_t col_blocks = ceil_div(g.n, L.wide_dz ? 32 * 16 / ge : 32 * dz_pieces(e));
   L.row_blocks = std::min<size_t>(ceil_div(g.m, kDzWarps * kDzRows),
                                   std::max<size_t>(1, sms * 8 / col_blocks));
   L.rows_per_block = static_cast<int64_t>(ceil_div(g.m, L.row_blocks));
@@ -1995,7 +2002,7 @@ GradLayout grad_layout(const qv_linear_grad& g, int sms) {
     o += (bytes + 255) / 256 * 256;
     return at;
   };
-  L.off_dz = take(L.store_dz ? packed_bytes(g.dtype, g.m, g.n) : 0);
+  L.off_dz = take(L.store_dz ? packed_bytes(dtype, g.m, g.n) : 0);
   L.off_sums = take(g.dbias != nullptr ? L.row_blocks * g.n * sizeof(float) : 0);
   L.off_packed = o;
   // dweight first: its units are the longest where there are many rows.
@@ -2006,7 +2013,7 @@ GradLayout grad_layout(const qv_linear_grad& g, int sms) {
     d.n = static_cast<int64_t>(g.k);
     d.k = static_cast<int64_t>(g.m);
     d.a_mn = d.b_mn = true;
-    if (!in_place(g.dtype, g.x, g.m, g.x_stride)) take(packed_bytes(g.dtype, g.m, g.k));
+    if (!in_place(dtype, g.x, g.m, g.x_stride)) take(packed_bytes(dtype, g.m, g.k));
   }
   if (g.dx != nullptr) {
     Product& d = L.products[L.count++];
@@ -2015,7 +2022,7 @@ GradLayout grad_layout(const qv_linear_grad& g, int sms) {
     d.n = static_cast<int64_t>(g.k);
     d.k = static_cast<int64_t>(g.n);
     d.b_mn = true;
-    if (!in_place(g.dtype, g.weight, g.n, g.weight_stride)) take(packed_bytes(g.dtype, g.n, g.k));
+    if (!in_place(dtype, g.weight, g.n, g.weight_stride)) take(packed_bytes(dtype, g.n, g.k));
   }
   if (L.count > 0) L.plan = plan_products(L.products, L.count, pairs, sms);
   L.off_partial = take(L.plan.partial_bytes[0] + L.plan.partial_bytes[1]);
@@ -2033,7 +2040,8 @@ size_t linear_grad_workspace(const qv_linear_grad& g, int sms) {
 void linear_grad(const qv_linear_grad& g, void* workspace, size_t workspace_bytes, int sms,
                  cudaStream_t st) {
   check_linear_grad(g);
-  const size_t e = dtype_size(g.dtype);
+  const uint32_t dtype = grad_dtype(g);
+  const size_t e = dtype_size(dtype);
   if (g.m == 0) {  // no rows: the sums over them are zero
     if (g.dweight != nullptr)
       QV_CUDA(cudaMemset2DAsync(g.dweight, std::max(g.dweight_stride, g.k) * e, 0, g.k * e, g.n,
@@ -2047,7 +2055,7 @@ void linear_grad(const qv_linear_grad& g, void* workspace, size_t workspace_byte
   QV_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0 || L.bytes == 0,
              "workspace must be 256-byte aligned");
   unsigned char* ws = static_cast<unsigned char*>(workspace);
-  by_type(g.dtype, [&](auto t) {
+  by_type(dtype, [&](auto t) {
     using T = decltype(t);
     using O = typename Operand<T>::type;
     const int64_t m = g.m, n = g.n;
@@ -2055,23 +2063,30 @@ void linear_grad(const qv_linear_grad& g, void* workspace, size_t workspace_byte
     Stored dz;
     dz.inner = n;
     dz.outer = m;
-    dz.bf16 = g.dtype != QV_DTYPE_F16;
+    dz.bf16 = dtype != QV_DTYPE_F16;
     if (L.store_dz || sums != nullptr) {
       O* store = reinterpret_cast<O*>(ws + L.off_dz);
       const int64_t ld = static_cast<int64_t>(packed_ld(g.n));
-      auto go = [&](auto v, auto act) {
+      auto launch = [&](auto type, auto v, auto act) {
+        using G = decltype(type);
         constexpr int kV = decltype(v)::value;
         constexpr int kAct = decltype(act)::value;
         const dim3 grid(static_cast<unsigned>(L.row_blocks),
                         static_cast<unsigned>(ceil_div(g.n, 32 * kV * dz_pieces(sizeof(T) * kV))));
-        if (L.store_dz)
-          dz_kernel<T, kV, true, kAct><<<grid, 32 * kDzWarps, 0, st>>>(
-              static_cast<const T*>(g.grad), g.grad_stride, static_cast<const T*>(g.preact),
-              g.preact_stride, m, n, L.rows_per_block, store, ld, sums);
+        auto* kernel = L.store_dz ? dz_kernel<T, G, kV, true, kAct> : dz_kernel<T, G, kV, false, kAct>;
+        kernel<<<grid, 32 * kDzWarps, 0, st>>>(
+            static_cast<const G*>(g.grad), g.grad_stride, static_cast<const T*>(g.preact),
+            g.preact_stride, m, n, L.rows_per_block, store, ld, sums);
+      };
+      auto go = [&](auto wide, auto act) {
+        auto by_grad = [&](auto type) {
+          constexpr int kV = decltype(wide)::value ? 16 / static_cast<int>(sizeof(type)) : 1;
+          launch(type, std::integral_constant<int, kV>{}, act);
+        };
+        if (grad_f32(g))
+          by_grad(float{});
         else
-          dz_kernel<T, kV, false, kAct><<<grid, 32 * kDzWarps, 0, st>>>(
-              static_cast<const T*>(g.grad), g.grad_stride, static_cast<const T*>(g.preact),
-              g.preact_stride, m, n, L.rows_per_block, store, ld, sums);
+          by_grad(T{});
       };
       auto by_act = [&](auto v) {
         switch (g.activation) {
@@ -2083,9 +2098,9 @@ void linear_grad(const qv_linear_grad& g, void* workspace, size_t workspace_byte
         }
       };
       if (L.wide_dz)
-        by_act(std::integral_constant<int, kWideDz<T>>{});
+        by_act(std::true_type{});
       else
-        by_act(std::integral_constant<int, 1>{});
+        by_act(std::false_type{});
       check_launch("dz_kernel");
     }
     if (L.store_dz) {
@@ -2096,12 +2111,12 @@ void linear_grad(const qv_linear_grad& g, void* workspace, size_t workspace_byte
       dz.p = g.grad;
       dz.ld = static_cast<int64_t>(g.grad_stride);
     }
-    Packer<T> pack(g.dtype, false, ws + L.off_packed);
+    Packer<T> pack(dtype, false, ws + L.off_packed);
     auto result = [&](void* p, size_t stride) {
       Epilogue ep{};
       ep.out = p;
       ep.out_stride = static_cast<int64_t>(stride);
-      ep.out_f32 = g.dtype == QV_DTYPE_F32;
+      ep.out_f32 = dtype == QV_DTYPE_F32;
       ep.set_aligns(e);
       return ep;
     };

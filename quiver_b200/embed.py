@@ -36,6 +36,7 @@ __all__ = ["ACTIVATIONS", "Adapter", "embedding_grad", "embedding_lookup", "line
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _ID_TYPES = {torch.int32: 0, torch.int64: 1}
+_GRAD_F32 = 0x100  # QV_GRAD_F32
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 
@@ -275,11 +276,11 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, grad):
         x, weight, preact = ctx.saved_tensors
         need = ctx.needs_input_grad
-        g = grad if grad.dtype == x.dtype else grad.to(x.dtype)  # of a float32 result
         dx, dw, db = (None, None, None)
         if need[0] or need[1] or need[2]:  # what the forward pass checked
-            dx, dw, db = _linear_grad(g, x, weight, preact, ACTIVATIONS[ctx.activation], need)
-        return dx, dw, db, g if need[3] else None, None, None
+            dx, dw, db = _linear_grad(grad, x, weight, preact, ACTIVATIONS[ctx.activation], need)
+        # the residual's own type: the gradient of a float32 result is float32
+        return dx, dw, db, grad.to(x.dtype) if need[3] else None, None, None
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -307,8 +308,8 @@ def linear_preact(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
 def linear_grad(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
                 preact: Optional[torch.Tensor] = None, activation: str = "none", *,
                 need: Tuple[bool, bool, bool] = (True, True, True)):
-    """The gradients (dx, dweight, dbias) of :func:`linear` for ``grad`` = d loss / d result, in x's
-    type; those not asked for in ``need`` are None. ``preact`` (from :func:`linear_preact`) may be
+    """The gradients (dx, dweight, dbias) of :func:`linear` for ``grad`` = d loss / d result (in x's
+    type or float32), in x's type; those not asked for in ``need`` are None. ``preact`` (from :func:`linear_preact`) may be
     None without an activation. The residual's gradient is ``grad`` itself."""
     _dtype_code(x, "x")
     act = _activation_code(activation)
@@ -319,7 +320,11 @@ def linear_grad(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
     n, k = weight.shape
     _like(weight, x, "weight", (n, k))
     shape = (*x.shape[:-1], n)
-    _like(grad, x, "grad", shape)
+    if getattr(grad, "dtype", None) == torch.float32:
+        if grad.device != x.device or grad.shape != shape:
+            raise _bad("grad", f"{tuple(shape)} on {x.device}", f"{tuple(grad.shape)} on {grad.device}")
+    else:
+        _like(grad, x, "grad", shape)
     if act != 0:
         if preact is None:
             raise ValueError("preact: needed for the gradient of an activation")
@@ -341,7 +346,10 @@ def _linear_grad(grad, x, weight, preact, act, need):
     dx = x.new_empty(x.shape) if need[0] else None
     dw = x.new_empty((n, k)) if need[1] else None
     db = x.new_empty((n,)) if need[2] else None
-    a = _native.qv_linear_grad(_DTYPES[x.dtype], act, m, n, k, g.data_ptr(), max(g.stride(0), n),
+    code = _DTYPES[x.dtype]
+    if code and grad.dtype == torch.float32:
+        code |= _GRAD_F32
+    a = _native.qv_linear_grad(code, act, m, n, k, g.data_ptr(), max(g.stride(0), n),
                                x2.data_ptr(), max(x2.stride(0), k), w.data_ptr(),
                                max(w.stride(0), k), preact_ptr, preact_stride,
                                dx.data_ptr() if need[0] else None, k,

@@ -333,3 +333,70 @@ def test_float32_results_of_16_bit_inputs(embed, t, m, k, n):
         err = 1.13 * zerr + (z.abs() + want.abs()) * (2.0 ** -21 + U)
         got = embed.linear(x, w, b, residual=r, activation=act, out_dtype=torch.float32)
         assert_within(got, want, err, act)
+
+
+def act_slope(z, act):
+    """act'(z) and act in 64 bits, by autograd of the definition."""
+    z = z.clone().requires_grad_()
+    (d,) = torch.autograd.grad(act_ref(z, act).sum(), z)
+    return d
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
+@pytest.mark.parametrize("m,k,n", [(1, 16, 24), (40, 64, 72), (300, 40, 57), (2000, 96, 260)])
+def test_gradients_of_float32_results(embed, t, act, m, k, n):
+    """A float32 gradient is rounded once, with the derivative on it: values that the 16-bit type
+    cannot hold do not become infinite or zero ahead of it."""
+    t = TYPES[t]
+    h = half_step(t)
+    g = gen(m + n)
+    x, w = normal(g, m, k, t=t), normal(g, n, k, t=t, scale=k ** -0.5)
+    z = normal(g, m, n, t=t)
+    dy = normal(g, m, n)
+    if t == torch.float16:  # past the type's range where the derivative is small
+        z[:, ::3] = -4.0
+        dy[:, ::3] *= 1e5 / (1.0 if act in ("gelu", "silu") else 1e5)
+    dx, dw, db = embed.linear_grad(dy, x, w, z, act)
+    dz = dy.double() * act_slope(z.double(), act)
+    # the derivative to 2^-15 (+ as much of 1 where it crosses 0), one rounding of dz, the sums
+    off = dy.double().abs() * 2.0 ** -14 * (0 if act in ("none", "relu") else 1)
+    rounded = off + (dz.abs() + off) * (h + 2 * U) + TINY[t]
+
+    def check(got, a, b, err, what):
+        want = a @ b
+        bound = err @ b.abs() + (a.abs() + err) @ b.abs() * ((a.shape[1] + 8) * 2 * U)
+        held = (want.abs() + bound) < torch.finfo(t).max
+        bound = bound + (want.abs() + bound) * h + TINY[t]
+        assert_within(got[held], want[held], bound[held], what)
+
+    check(dx, dz, w.double(), rounded, "dx")
+    check(dw, dz.t(), x.double(), rounded.t(), "dw")
+    ones = torch.ones(m, 1, dtype=torch.float64, device="cuda")
+    check(db[:, None], dz.t(), ones, (off + dz.abs() * 2 * U).t(), "db")
+    # autograd takes the same way, also strided and broadcast
+    leaves = [v.clone().requires_grad_() for v in (x, w, normal(g, n, t=t), normal(g, m, n, t=t))]
+    y = embed.linear(*leaves[:3], residual=leaves[3], activation=act, out_dtype=torch.float32)
+    _, pre = embed.linear_preact(*[v.detach() for v in leaves[:3]], activation=act,
+                                 out_dtype=torch.float32)
+    dy = normal(g, m, n)  # in range for these preactivations: NaN would equal nothing
+    for up in (dy, dy[:1].expand(m, n), torch.cat([dy, dy], 1)[:, 1:n + 1]):
+        got = torch.autograd.grad(y, leaves, up, retain_graph=True)
+        want = embed.linear_grad(up.contiguous(), x, w, pre, act)
+        for p, q in zip(got, want):
+            assert torch.equal(p, q)
+        assert torch.equal(got[3], up.to(t))
+
+
+def test_gradients_of_float32_results_hold_the_range(embed):
+    """Upstream values outside float16's range whose gradients are inside it."""
+    x = torch.full((40, 16), 2.0 ** -8, device="cuda", dtype=torch.float16)
+    w = torch.full((24, 16), 2.0 ** -8, device="cuda", dtype=torch.float16)
+    z = torch.full((40, 24), -4.0, device="cuda", dtype=torch.float16)
+    dy = torch.full((40, 24), 2.0 ** 18, device="cuda")
+    dx, dw, db = embed.linear_grad(dy, x, w, z, "gelu")
+    d = float(act_slope(torch.tensor([-4.0], dtype=torch.float64), "gelu")) * 2.0 ** 18
+    for got, want in ((dx, d * 24 / 256), (dw, d * 40 / 256), (db, d * 40)):
+        assert ((got.double() / want - 1).abs() <= 2 * 2.0 ** -11 + 2.0 ** -13).all()
+    dx, dw, db = embed.linear_grad(dy * 2.0 ** -50, x, w, z, "gelu")
+    assert (db != 0).logical_or(torch.tensor(abs(d) * 40 * 2.0 ** -50 < 2.0 ** -25)).all()
