@@ -1070,13 +1070,20 @@ __global__ void __launch_bounds__(kProductThreads, 1)
               piece, a.partial + (static_cast<int64_t>(w.split) * a.m + row0) * a.n + col, a.n,
               nullptr, 0, rows, cols, lane);
         } else {
-          const T* residual = a.ep.residual != nullptr
-                                  ? static_cast<const T*>(a.ep.residual) +
-                                        row0 * a.ep.residual_stride + col
-                                  : nullptr;
-          store_piece<T, Out, kWide>(
-              piece, static_cast<Out*>(a.ep.out) + row0 * a.ep.out_stride + col, a.ep.out_stride,
-              residual, a.ep.residual_stride, rows, cols, lane);
+          auto store = [&](auto type) {
+            using R = decltype(type);
+            const R* residual = a.ep.residual != nullptr
+                                    ? static_cast<const R*>(a.ep.residual) +
+                                          row0 * a.ep.residual_stride + col
+                                    : nullptr;
+            store_piece<R, Out, kWide>(
+                piece, static_cast<Out*>(a.ep.out) + row0 * a.ep.out_stride + col, a.ep.out_stride,
+                residual, a.ep.residual_stride, rows, cols, lane);
+          };
+          if (kOutF32 && a.ep.residual_f32)
+            store(float{});
+          else
+            store(T{});
         }
         __syncwarp();
       }
@@ -1536,7 +1543,8 @@ void launch_products(const Product* p, int count, const ProductGroup& g, bool ch
                               ep.out_f32 ? QV_DTYPE_F32 : type, kBN / 4);
     if (g.p[q].splits == 1 && ep.residual_tiles)
       maps.residual[q] =
-          piece_map(ep.residual, p[q].m, p[q].n, ep.residual_stride, type, kBN / 4);
+          piece_map(ep.residual, p[q].m, p[q].n, ep.residual_stride,
+                    ep.residual_f32 ? QV_DTYPE_F32 : type, kBN / 4);
   }
   if (p[0].wide != nullptr) {  // along k, by itself
     maps.a[1] = operand_map(as_planes(p[0].a), kBM);
@@ -1799,22 +1807,31 @@ void check_matrix(const char* what, uint32_t dtype, const void* p, size_t rows, 
   QV_REQUIRE(stride < (size_t{1} << 36), std::string(what) + ": row stride too large");
 }
 
+uint32_t out_dtype(const qv_linear& l) {
+  return l.out_dtype & ~static_cast<uint32_t>(QV_RESIDUAL_F32);
+}
+bool residual_f32(const qv_linear& l) {
+  return l.dtype == QV_DTYPE_F32 || (l.out_dtype & QV_RESIDUAL_F32) != 0;
+}
+
 void check_linear(const qv_linear& l) {
   check_dtype(l.dtype);
   QV_REQUIRE(l.activation <= QV_ACT_SILU, "unknown activation");
   QV_REQUIRE(l.k >= 1 && l.k <= kMaxDim && l.n >= 1 && l.n <= kMaxDim,
              "dimensions must be between 1 and 65536");
   QV_REQUIRE(l.m <= kMaxLinearRows, "too many rows");
-  QV_REQUIRE(l.out_dtype == l.dtype || l.out_dtype == QV_DTYPE_F32,
+  QV_REQUIRE(out_dtype(l) == l.dtype || out_dtype(l) == QV_DTYPE_F32,
              "results have the inputs' type or float32");
+  QV_REQUIRE((l.out_dtype & QV_RESIDUAL_F32) == 0 || out_dtype(l) == QV_DTYPE_F32,
+             "a float32 residual goes with float32 results");
   if (l.m == 0) return;
   check_matrix("x", l.dtype, l.x, l.m, l.k, l.x_stride);
   check_matrix("weight", l.dtype, l.weight, l.n, l.k, l.weight_stride);
-  check_matrix("out", l.out_dtype, l.out, l.m, l.n, l.out_stride);
+  check_matrix("out", out_dtype(l), l.out, l.m, l.n, l.out_stride);
   if (l.bias != nullptr) check_matrix("bias", l.dtype, l.bias, 1, l.n, l.n);
   if (l.residual != nullptr) {
     // Stride 0 adds one row to every row of the result.
-    check_matrix("residual", l.dtype, l.residual, l.residual_stride == 0 ? 1 : l.m, l.n,
+    check_matrix("residual", residual_f32(l) ? QV_DTYPE_F32 : l.dtype, l.residual, l.residual_stride == 0 ? 1 : l.m, l.n,
                  l.residual_stride);
   }
   if (l.preact != nullptr) check_matrix("preact", l.dtype, l.preact, l.m, l.n, l.preact_stride);
@@ -1828,7 +1845,8 @@ Epilogue epilogue_of(const qv_linear& l) {
   e.residual_stride = static_cast<int64_t>(l.residual_stride);
   e.out = l.out;
   e.out_stride = static_cast<int64_t>(l.out_stride);
-  e.out_f32 = l.out_dtype == QV_DTYPE_F32;
+  e.out_f32 = out_dtype(l) == QV_DTYPE_F32;
+  e.residual_f32 = residual_f32(l);
   e.preact = l.preact;
   e.preact_stride = static_cast<int64_t>(l.preact_stride);
   e.set_aligns(dtype_size(l.dtype));

@@ -10,7 +10,7 @@ namespace qv {
 // preact when given), y = act(z) + residual[row][col], written to out.
 struct Epilogue {
   int act;
-  bool out_f32;
+  bool out_f32, residual_f32;
   const void* bias;
   const void* residual;
   int64_t residual_stride;
@@ -30,11 +30,11 @@ struct Epilogue {
   void set_aligns(size_t elem) {
     const int64_t e = static_cast<int64_t>(elem);
     out_align = align32(out, out_stride * (out_f32 ? 4 : e));
-    residual_align = align32(residual, residual_stride * e);
+    residual_align = align32(residual, residual_stride * (residual_f32 ? 4 : e));
     preact_align = align32(preact, preact_stride * e);
     out_tiles = out_align >= 16;
     residual_tiles = out_tiles && residual != nullptr && residual_align >= 16 &&
-                     residual_stride != 0 && (out_f32 ? 4 : e) == e;
+                     residual_stride != 0 && (out_f32 ? 4 : e) == (residual_f32 ? 4 : e);
   }
 };
 
@@ -245,8 +245,11 @@ __device__ __forceinline__ void finish1(const Epilogue& e, int64_t row, int64_t 
     static_cast<T*>(e.preact)[row * e.preact_stride + col] = dev::from_f32<T>(s);
   float y = sizeof(T) == 2 && !e.out_f32 ? activate2<true>(e.act, both(s)).x
                                          : activate2<false>(e.act, both(s)).x;
-  if (e.residual != nullptr)
-    y += dev::to_f32<T>(static_cast<const T*>(e.residual)[row * e.residual_stride + col]);
+  if (e.residual != nullptr) {
+    const int64_t at = row * e.residual_stride + col;
+    y += e.residual_f32 ? static_cast<const float*>(e.residual)[at]
+                        : dev::to_f32<T>(static_cast<const T*>(e.residual)[at]);
+  }
   if (e.out_f32)
     static_cast<float*>(e.out)[row * e.out_stride + col] = y;
   else

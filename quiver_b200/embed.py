@@ -37,6 +37,7 @@ __all__ = ["ACTIVATIONS", "Adapter", "embedding_grad", "embedding_lookup", "line
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _ID_TYPES = {torch.int32: 0, torch.int64: 1}
 _GRAD_F32 = 0x100  # QV_GRAD_F32
+_RESIDUAL_F32 = 0x100  # QV_RESIDUAL_F32
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 
@@ -229,16 +230,23 @@ def _linear(x, weight, bias, residual, activation, out_dtype, want_preact, out=N
     if bias is not None:
         bias = _like(bias, x, "bias", (n,)).contiguous()  # held until the call is enqueued
         bias_ptr = bias.data_ptr()
-    if residual is not None:
-        r = _like(residual, x, "residual", shape)
-        r = r if r.dim() == 2 else r.reshape(m, n)
-        if not (r.stride(0) == 0 and (r.stride(1) == 1 or n == 1)):
-            r = _rows(r)
-        residual_ptr, residual_stride = r.data_ptr(), r.stride(0) if m > 1 else n
     if out_dtype is None:
         out_dtype = x.dtype
     elif out_dtype != x.dtype and out_dtype != torch.float32:
         raise _bad("out_dtype", f"{x.dtype} or torch.float32", out_dtype)
+    out_code = _DTYPES[out_dtype]
+    if residual is not None:
+        r = residual
+        if out_code == 0 and code != 0 and getattr(r, "dtype", None) == torch.float32:
+            out_code |= _RESIDUAL_F32
+            if r.device != device or r.shape != shape:
+                raise _bad("residual", f"{tuple(shape)} on {device}", f"{tuple(r.shape)} on {r.device}")
+        else:
+            _like(r, x, "residual", shape)
+        r = r if r.dim() == 2 else r.reshape(m, n)
+        if not (r.stride(0) == 0 and (r.stride(1) == 1 or n == 1)):
+            r = _rows(r)
+        residual_ptr, residual_stride = r.data_ptr(), r.stride(0) if m > 1 else n
     if out is None:
         out = torch.empty(shape, dtype=out_dtype, device=device)
     else:
@@ -246,7 +254,7 @@ def _linear(x, weight, bias, residual, activation, out_dtype, want_preact, out=N
                residual=residual)
     if want_preact:
         preact = x.new_empty(shape)
-    a = _native.qv_linear(code, _DTYPES[out_dtype], act, m, n, k, x2.data_ptr(),
+    a = _native.qv_linear(code, out_code, act, m, n, k, x2.data_ptr(),
                           max(x2.stride(0), k), w.data_ptr(), max(w.stride(0), k), bias_ptr,
                           residual_ptr, residual_stride, out.data_ptr(), n,
                           preact.data_ptr() if want_preact else None, n)
@@ -269,6 +277,7 @@ class _Linear(torch.autograd.Function):
                             activation != "none")
         ctx.save_for_backward(x, weight, preact)
         ctx.activation = activation
+        ctx.residual_dtype = None if residual is None else residual.dtype
         return y
 
     @staticmethod
@@ -279,8 +288,7 @@ class _Linear(torch.autograd.Function):
         dx, dw, db = (None, None, None)
         if need[0] or need[1] or need[2]:  # what the forward pass checked
             dx, dw, db = _linear_grad(grad, x, weight, preact, ACTIVATIONS[ctx.activation], need)
-        # the residual's own type: the gradient of a float32 result is float32
-        return dx, dw, db, grad.to(x.dtype) if need[3] else None, None, None
+        return dx, dw, db, grad.to(ctx.residual_dtype) if need[3] else None, None, None
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -289,7 +297,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``activation(x @ weight.T + bias) + residual`` for x [..., k], weight [n, k], bias [n] and a
     residual of the result's shape [..., n] (an expanded one is not copied). ``activation`` is one of
-    :data:`ACTIVATIONS`; ``out_dtype`` may be torch.float32 to leave the result unrounded.
+    :data:`ACTIVATIONS`; ``out_dtype`` may be torch.float32 to leave the result unrounded (the residual
+    may then be float32 too). float32 products are off by at most 2^-21 of sum |x||w| beside a float32
+    sum's own roundings; float32 results of 16-bit inputs, whose sums the tensor core cuts, by up to
+    3.4e-6 of it.
     Differentiable in all four tensors (unless ``out`` is given)."""
     if out is None and torch.is_grad_enabled() and any(
             [isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, bias, residual)]):
@@ -366,7 +377,8 @@ def _linear_grad(grad, x, weight, preact, act, need):
 
 class Adapter:
     """One linear map for the vectors of an index: ``activation(v W^T + bias)``, plus v itself with
-    ``residual=True`` (W square). ``adapter(v)`` gives float32 vectors, ready for
+    ``residual=True`` (W square). The product takes v in the weight's type; what is added is v as it
+    is. ``adapter(v)`` gives float32 vectors, ready for
     :meth:`FlatIndex.add_device` and the device searches, which also take it as ``adapter=``. The same
     vector in batches of different sizes may differ in its last bits (sums run in another order)."""
 
@@ -386,8 +398,11 @@ class Adapter:
     def __call__(self, vectors: torch.Tensor) -> torch.Tensor:
         with torch.no_grad():
             x = vectors.to(self.weight.dtype)
-            return linear(x, self.weight, self.bias, residual=x if self.residual else None,
-                          activation=self.activation, out_dtype=torch.float32)
+            skip = None
+            if self.residual:
+                skip = x if vectors.dtype == x.dtype else vectors.to(torch.float32)
+            return linear(x, self.weight, self.bias, residual=skip, activation=self.activation,
+                          out_dtype=torch.float32)
 
     @property
     def in_dim(self) -> int:

@@ -400,3 +400,46 @@ def test_gradients_of_float32_results_hold_the_range(embed):
         assert ((got.double() / want - 1).abs() <= 2 * 2.0 ** -11 + 2.0 ** -13).all()
     dx, dw, db = embed.linear_grad(dy * 2.0 ** -50, x, w, z, "gelu")
     assert (db != 0).logical_or(torch.tensor(abs(d) * 40 * 2.0 ** -50 < 2.0 ** -25)).all()
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("m,k,n", [(1, 40, 40), (6, 64, 33), (300, 96, 96), (1000, 64, 257)])
+def test_float32_residual(embed, t, m, k, n):
+    """A 16-bit layer with a float32 result adds a float32 residual with all its bits: whole and
+    unaligned rows, one row for all, windows, with preactivations."""
+    t = TYPES[t]
+    g = gen(m + n)
+    x, w, b = normal(g, m, k, t=t), normal(g, n, k, t=t, scale=k ** -0.5), normal(g, n, t=t)
+    plain, z = embed.linear_preact(x, w, b, activation="silu", out_dtype=torch.float32)
+    wide = normal(g, m, n + 7)
+    for r in (normal(g, m, n), wide[:, 3:n + 3], wide[:1, :n].expand(m, n)):
+        got = embed.linear(x, w, b, residual=r, activation="silu", out_dtype=torch.float32)
+        assert torch.equal(got, plain + r)  # the same sum, one float32 addition
+        y, pre = embed.linear_preact(x, w, b, residual=r, activation="silu", out_dtype=torch.float32)
+        assert torch.equal(y, got) and torch.equal(pre, z)
+    leaf = normal(g, m, n).requires_grad_()
+    dy = normal(g, m, n)
+    (dr,) = torch.autograd.grad(embed.linear(x, w, b, residual=leaf, out_dtype=torch.float32), leaf,
+                                dy)
+    assert dr.dtype == torch.float32 and torch.equal(dr, dy)
+    for bad in (lambda: embed.linear(x, w, residual=leaf.detach()),  # a 16-bit result
+                lambda: embed.linear(x, w, residual=leaf.detach()[:, 1:], out_dtype=torch.float32),
+                lambda: embed.linear(x, w, residual=leaf.detach().double(),
+                                     out_dtype=torch.float32)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_adapter_adds_the_vector_itself(embed):
+    """A 16-bit adapter with a skip keeps the float32 vector's bits; zero weights give it back."""
+    for t in TYPES.values():
+        for m in (1, 500):
+            v = normal(gen(m), m, 96)
+            a = embed.Adapter(torch.zeros(96, 96, device="cuda", dtype=t), residual=True)
+            assert torch.equal(a(v), v)
+            w, b = normal(gen(1), 96, 96, t=t, scale=0.1), normal(gen(2), 96, t=t)
+            got = embed.Adapter(w, b, activation="gelu", residual=True)(v)
+            x = v.to(t)
+            assert torch.equal(got, embed.linear(x, w, b, activation="gelu",
+                                                 out_dtype=torch.float32) + v)
+            assert embed.Adapter(w, residual=True)(x).dtype == torch.float32
