@@ -315,7 +315,9 @@ qv_status qv_embedding_grad_device(int device, uint32_t dtype, const void* upstr
                                    size_t grad_stride, void* workspace, size_t workspace_bytes,
                                    void* stream);
 /* qv_embedding_lookup_device on a Flat index's stored float32 rows (as qv_flat_rows reports them,
- * normalized for cosine), by row number. */
+ * normalized for cosine), by row number (a search's keys, less the index's row offset; labels only
+ * where rows were added without any). A captured call keeps the rows' address: capture it again after
+ * an add. */
 qv_status qv_flat_lookup_device(const qv_flat* index, uint32_t id_type, const void* ids, size_t n,
                                 float scale, float* out, size_t out_stride, void* stream);
 

@@ -156,11 +156,14 @@ class FlatIndex:
         check(lib().qv_flat_add_device(self._h, vectors.data_ptr(), n, lp,
                                        C.c_void_p(stream) if stream else None))
 
-    def search_device(self, queries, k: int = 10, *, adapter=None):
+    def search_device(self, queries, k: int = 10, *, adapter=None, return_rows: bool = False):
         """k-NN search of queries in GPU memory on PyTorch's current stream, without waiting for
         it: ``queries`` a float32 CUDA tensor [nq, dim] on this index's device, or vectors that
         ``adapter`` (:class:`quiver_b200.embed.Adapter`) turns into them. Returns CUDA tensors
-        (distances float32 [nq, k], labels int64 [nq, k]; no counterpart in the reference)."""
+        (distances float32 [nq, k], labels int64 [nq, k]; no counterpart in the reference), with
+        ``return_rows`` also the results' row numbers (int64 [nq, k], -1 in unfilled slots), which
+        :meth:`lookup_device` takes; the labels are row numbers only where rows were added without
+        labels of their own."""
         import torch
         q = queries if adapter is None else _adapted(adapter, queries, None)
         if q.dim() != 2 or q.shape[1] != self.dim or q.dtype != torch.float32 or not q.is_cuda:
@@ -173,17 +176,20 @@ class FlatIndex:
         nq = int(q.shape[0])
         dists = torch.empty((nq, int(k)), dtype=torch.float32, device=q.device)
         labels = torch.empty((nq, int(k)), dtype=torch.int64, device=q.device)
+        rows = torch.empty_like(labels) if return_rows else None
         st = torch.cuda.current_stream(q.device).cuda_stream
         check(lib().qv_flat_search_device(self._h, q.data_ptr(), nq, int(k), None,
-                                          labels.data_ptr(), dists.data_ptr(), None,
+                                          labels.data_ptr(), dists.data_ptr(),
+                                          rows.data_ptr() if return_rows else None,
                                           C.c_void_p(st)))
-        return dists, labels
+        return (dists, labels, rows) if return_rows else (dists, labels)
 
     def lookup_device(self, rows, scale: float = 1.0):
         """Stored vectors by row number, times ``scale``, on PyTorch's current stream: ``rows`` an
         int32 or int64 CUDA tensor of any shape on this index's device; returns float32
         ``[*rows.shape, dim]``. A negative number (an unfilled result slot) gives zeros, one past
-        the last row NaN (no counterpart in the reference; :meth:`rows` copies to the host)."""
+        the last row NaN (no counterpart in the reference; :meth:`rows` copies to the host). A call
+        captured into a CUDA graph keeps the rows' address: capture it again after an add."""
         import torch
         codes = {torch.int32: 0, torch.int64: 1}
         if not rows.is_cuda or rows.dtype not in codes:

@@ -443,3 +443,28 @@ def test_adapter_adds_the_vector_itself(embed):
             assert torch.equal(got, embed.linear(x, w, b, activation="gelu",
                                                  out_dtype=torch.float32) + v)
             assert embed.Adapter(w, residual=True)(x).dtype == torch.float32
+
+
+def test_rows_of_answers(gpu, embed):
+    """From answers to their stored rows, with labels of one's own, unfilled slots and an adapter."""
+    base = normal(gen(1), 400, 48)
+    labels = torch.randperm(400, generator=torch.Generator().manual_seed(1)).cuda() + 10_000
+    ix = gpu.FlatIndex(48, "l2")
+    ix.add_device(base[:250], labels[:250])
+    ix.add_device(base[250:], labels[250:])
+    at = torch.tensor([7, 399, 250], device="cuda")
+    dist, label, rows = ix.search_device(base[at], 5, return_rows=True)
+    assert rows.dtype == torch.int64 and rows.shape == (3, 5)
+    assert torch.equal(rows[:, 0], at) and torch.equal(labels[rows], label)
+    assert torch.equal(ix.lookup_device(rows), base[rows])
+    d2, l2 = ix.search_device(base[at], 5)
+    assert torch.equal(dist, d2) and torch.equal(label, l2)
+    few = gpu.FlatIndex(48, "l2")
+    few.add_device(base[:3], labels[:3])
+    eye = embed.Adapter(torch.eye(48, device="cuda"))
+    dist, label, rows = few.search_device(base[:2], 7, adapter=eye, return_rows=True)
+    assert (rows[:, 3:] == -1).all() and (rows[:, :3].sort(1)[0] == torch.arange(3).cuda()).all()
+    near = few.lookup_device(rows)
+    assert (near[:, 3:] == 0).all() and torch.equal(near[:, :3], base[rows[:, :3]])
+    none = few.search_device(base[:0], 7, return_rows=True)
+    assert [tuple(v.shape) for v in none] == [(0, 7)] * 3
