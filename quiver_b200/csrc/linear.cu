@@ -87,8 +87,14 @@ struct PackJob {
   int* exponents;  // scaled rows: each row's scale was 2^-exponent
 };
 
-// float32 rows scaled and split into two float16 planes; one warp per row, which keeps up to
-// 32 * kSplitHeld pieces of it in registers and reads what is more a second time.
+// A row's exponent as three bfloat16 planes, from its exponent as two float16 planes. The planes end
+// at 2^-133, bfloat16's last bit, so that elements below 2^-110 would lose bits: rows whose largest
+// is below 2^-20 are brought up to that, which keeps every product with another row in range.
+__device__ __forceinline__ int lifted(int exponent) { return min(0, exponent + 34); }
+
+// float32 rows scaled and split into two float16 planes, or (kPlanes) lifted and split into three
+// bfloat16 ones; one warp per row, which keeps up to 32 * kSplitHeld pieces of it in registers and
+// reads what is more a second time.
 //
 // The planes hold an element to 2^-23 of itself or 2^-39 of the row's largest, X. The second part
 // adds up to 2^-39 (X sum|w| + W sum|x|) <= 2^-38 k X W to a result, which is nothing beside
@@ -103,7 +109,7 @@ struct PackJob {
 // it takes 13.8.
 constexpr int kSplitHeld = 8, kSplitBlocks = 148 * 8;
 constexpr uint32_t kShareOne = 256, kSharesNeeded = kShareOne + kShareOne / 8;
-template <int kV>
+template <int kV, bool kPlanes>
 __global__ void __launch_bounds__(256, 3)
     split_rows_kernel(const PackJob j0, const PackJob j1, uint32_t* __restrict__ shares) {
   dev::allow_next();
@@ -135,22 +141,30 @@ __global__ void __launch_bounds__(256, 3)
     // A row of zeros, or one that holds infinity or NaN, stays as it is.
     const int shift =
         top == 0 || top >= 0x7f800000u ? 0 : min(14 + 127 - static_cast<int>(top >> 23), 126);
-    const float scale = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
-    if (lane == 0) j.exponents[r] = -shift;
+    const int exponent = kPlanes ? lifted(-shift) : -shift;
+    const float scale = __uint_as_float(static_cast<uint32_t>(127 - exponent) << 23);
+    if (lane == 0) j.exponents[r] = exponent;
     const float from = __uint_as_float(top) * scale * 0x1p-6f;
     uint32_t large = 0;
     auto split = [&](const Pack<float, kV>& x, int64_t c) {
-      Pack<__half, kV> hi, lo;
+      if constexpr (kPlanes) {
+        float y[kV];
 #pragma unroll
-      for (int v = 0; v < kV; ++v) {
-        const float y = x.v[v] * scale;
-        large += fabsf(y) >= from;
-        hi.v[v] = __float2half_rn(y);
-        lo.v[v] = __hisinf(hi.v[v]) ? __float2half_rn(0.0f)
-                                    : __float2half_rn(y - __half2float(hi.v[v]));
+        for (int v = 0; v < kV; ++v) y[v] = x.v[v] * scale;
+        put_operand<float, kV>(y, static_cast<__nv_bfloat16*>(j.dst), plane, r * j.ld + c);
+      } else {
+        Pack<__half, kV> hi, lo;
+#pragma unroll
+        for (int v = 0; v < kV; ++v) {
+          const float y = x.v[v] * scale;
+          large += fabsf(y) >= from;
+          hi.v[v] = __float2half_rn(y);
+          lo.v[v] = __hisinf(hi.v[v]) ? __float2half_rn(0.0f)
+                                      : __float2half_rn(y - __half2float(hi.v[v]));
+        }
+        dev::store_pack<__half, kV>(dst + c, hi);
+        dev::store_pack<__half, kV>(dst + plane + c, lo);
       }
-      dev::store_pack<__half, kV>(dst + c, hi);
-      dev::store_pack<__half, kV>(dst + plane + c, lo);
     };
 #pragma unroll
     for (int h = 0; h < kSplitHeld; ++h) {
@@ -164,6 +178,10 @@ __global__ void __launch_bounds__(256, 3)
     if (top != 0 && top < 0x7f800000u)
       least = min(least, count * kShareOne / static_cast<uint32_t>(j.cols));
   }
+  if constexpr (kPlanes) {
+    dev::wait_previous();
+    return;
+  }
   __shared__ uint32_t s_least[8];
   if (lane == 0) s_least[threadIdx.x >> 5] = least;
   __syncthreads();
@@ -173,11 +191,6 @@ __global__ void __launch_bounds__(256, 3)
   }
   dev::wait_previous();
 }
-
-// A row's exponent as three bfloat16 planes, from its exponent as two float16 planes. The planes end
-// at 2^-133, bfloat16's last bit, so that elements below 2^-110 would lose bits: rows whose largest
-// is below 2^-20 are brought up to that, which keeps every product with another row in range.
-__device__ __forceinline__ int lifted(int exponent) { return min(0, exponent + 34); }
 
 // Up to two matrices in one launch (blockIdx.y). Bound by memory: every thread moves kV values of
 // kPackRows rows at a time.
@@ -1469,6 +1482,7 @@ struct ProductPlan {
   bool pair = false;
   int splits[2] = {1, 1}, blocks_per_split[2] = {1, 1}, k_blocks[2] = {1, 1};
   size_t partial_bytes[2] = {0, 0};
+  double cycles = 0;
 };
 
 // Tiles and splits of k with the least estimated time. In cycles: a 64-wide block of k takes the
@@ -1521,6 +1535,7 @@ ProductPlan plan_products(const Product* p, int count, int pairs, int sms) {
     if (t < best_t) {
       best_t = t;
       best = plan;
+      best.cycles = t;
     }
   }
   return best;
@@ -1686,9 +1701,10 @@ constexpr size_t kSharesBytes = (2 * kSplitBlocks * 4 + 255) / 256 * 256, kChoic
 template <class T>
 class Packer {
  public:
-  // scaled: float32 rows as two float16 planes, for products whose sums run along the rows.
-  Packer(uint32_t dtype, bool scaled, unsigned char* ws)
-      : dtype_(dtype), scaled_(scaled && sizeof(T) == 4), ws_(ws) {}
+  // scaled: rows with exponents, for products whose sums run along the rows; float32 ones as two
+  // float16 planes where those do, or (planes) three bfloat16 ones at once.
+  Packer(uint32_t dtype, bool scaled, bool planes, unsigned char* ws)
+      : dtype_(dtype), scaled_(scaled && sizeof(T) == 4), planes_(planes), ws_(ws) {}
   Stored rows(const void* src, size_t rows, size_t cols, size_t stride) {
     Stored s;
     s.inner = static_cast<int64_t>(cols);
@@ -1701,8 +1717,9 @@ class Packer {
     }
     s.p = ws_;
     s.ld = static_cast<int64_t>(packed_ld(cols));
-    s.planes = scaled_ ? 2 : Operand<T>::kPlanes;
-    s.bf16 = s.bf16 && !scaled_;
+    const bool halves = scaled_ && !planes_;
+    s.planes = halves ? 2 : Operand<T>::kPlanes;
+    s.bf16 = s.bf16 && !halves;
     int* exponents = nullptr;
     if (scaled_)
       exponents = reinterpret_cast<int*>(ws_ + scaled_bytes(rows, cols) -
@@ -1742,11 +1759,16 @@ class Packer {
         const size_t rows = static_cast<size_t>(std::max(jobs_[0].rows, jobs_[1].rows));
         const unsigned blocks =
             static_cast<unsigned>(std::min<size_t>(ceil_div(rows, 8), kSplitBlocks));
+        if (planes_) {
+          split_rows_kernel<kV, true><<<dim3(blocks, 2), 256, 0, st>>>(jobs_[0], jobs_[1], nullptr);
+          check_launch("split_rows_kernel");
+          return;
+        }
         uint32_t* shares = reinterpret_cast<uint32_t*>(ws_);
         int* wide = reinterpret_cast<int*>(ws_ + kSharesBytes);
         ws_ += kChoiceBytes;
         wide_ = wide;
-        split_rows_kernel<kV><<<dim3(blocks, 2), 256, 0, st>>>(jobs_[0], jobs_[1], shares);
+        split_rows_kernel<kV, false><<<dim3(blocks, 2), 256, 0, st>>>(jobs_[0], jobs_[1], shares);
         check_launch("split_rows_kernel");
         // Two blocks an SM in all: it rarely packs.
         launch_chained(choose_planes_kernel<kV>, dim3(std::min(blocks, 148u), 2), 256, 0, st,
@@ -1767,7 +1789,7 @@ class Packer {
     check_launch("pack_kernel");
   }
   uint32_t dtype_;
-  bool scaled_;
+  bool scaled_, planes_;
   unsigned char* ws_;
   PackJob jobs_[2];
   int count_ = 0, align_ = 16;
@@ -1855,6 +1877,7 @@ Epilogue epilogue_of(const qv_linear& l) {
 
 struct LinearPlan {
   bool few = false;
+  bool planes = false;  // float32: three bfloat16 planes whatever the elements
   ProductPlan product;
   size_t bytes = 0;
 };
@@ -1867,12 +1890,20 @@ LinearPlan linear_plan(const qv_linear& l, int sms) {
   d.n = static_cast<int64_t>(l.n);
   d.k = static_cast<int64_t>(l.k);
   p.product = plan_products(&d, 1, l.dtype == QV_DTYPE_F32 ? 3 : 1, sms);
+  if (l.dtype == QV_DTYPE_F32) {
+    // Scaled operands need one launch more (choose_planes_kernel, 2.5 us of the GPU and as much of the
+    // host), three planes twice the MMAs. Scaled and as planes, us on the GPU and a pass: 4097 x 100 x
+    // 100 14.0 and 13.9, 21.8 and 19.0; 1000 x 768 x 768 19.5 and 26.5, 22.1 and 28.8.
+    const ProductPlan six = plan_products(&d, 1, 6, sms);
+    p.planes = six.cycles <= p.product.cycles + 5000;
+    if (p.planes) p.product = six;
+  }
   auto packed = [&](const void* src, size_t rows, size_t stride) -> size_t {
     if (in_place(l.dtype, src, rows, stride)) return 0;
     return l.dtype == QV_DTYPE_F32 ? scaled_bytes(rows, l.k) : packed_bytes(l.dtype, rows, l.k);
   };
   p.bytes += packed(l.x, l.m, l.x_stride) + packed(l.weight, l.n, l.weight_stride);
-  if (l.dtype == QV_DTYPE_F32) p.bytes += kChoiceBytes;
+  if (l.dtype == QV_DTYPE_F32 && !p.planes) p.bytes += kChoiceBytes;
   p.bytes += p.product.partial_bytes[0];
   return p;
 }
@@ -1937,7 +1968,7 @@ void linear_forward(const qv_linear& l, void* workspace, size_t workspace_bytes,
       launch_few<T>(l, ep, st);
       return;
     }
-    Packer<T> pack(l.dtype, true, static_cast<unsigned char*>(workspace));
+    Packer<T> pack(l.dtype, true, p.planes, static_cast<unsigned char*>(workspace));
     Product d{};
     d.m = static_cast<int64_t>(l.m);
     d.n = static_cast<int64_t>(l.n);
@@ -2129,7 +2160,7 @@ void linear_grad(const qv_linear_grad& g, void* workspace, size_t workspace_byte
       dz.p = g.grad;
       dz.ld = static_cast<int64_t>(g.grad_stride);
     }
-    Packer<T> pack(dtype, false, ws + L.off_packed);
+    Packer<T> pack(dtype, false, false, ws + L.off_packed);
     auto result = [&](void* p, size_t stride) {
       Epilogue ep{};
       ep.out = p;

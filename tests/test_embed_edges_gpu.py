@@ -159,7 +159,7 @@ def wide_inputs(kind, m, n, k):
 @pytest.mark.parametrize("kind", ["plain", "column", "columns", "row", "weight", "one-hot", "tiny",
                                   "sparse"])
 @pytest.mark.parametrize("m,k,n", [(300, 80, 72), (140, 129, 130), (6000, 512, 768),
-                                   (64, 8192, 128)])
+                                   (1001, 1027, 515), (64, 8192, 128)])
 def test_linear_float32_wide_rows(embed, kind, m, k, n):
     """Elements of very different magnitudes within a row keep float32's accuracy of the sum."""
     x, w = wide_inputs(kind, m, n, k)
@@ -171,10 +171,11 @@ def test_linear_float32_wide_rows(embed, kind, m, k, n):
     assert torch.equal(z, got)
 
 
-def test_linear_float32_wide_rows_alternate(embed):
+@pytest.mark.parametrize("m,n,k", [(300, 72, 80), (1500, 520, 1024)])
+def test_linear_float32_wide_rows_alternate(embed, m, n, k):
     """Batches that need the planes and batches that do not, in turn and from replayed graphs with
     one workspace each: nothing of one call is left for the next."""
-    plain, wide = wide_inputs("plain", 300, 72, 80), wide_inputs("row", 300, 72, 80)
+    plain, wide = wide_inputs("plain", m, n, k), wide_inputs("row", m, n, k)
     want = [embed.linear(*v) for v in (plain, wide)]
     held = [v.clone() for v in plain]
     graph = torch.cuda.CUDAGraph()
