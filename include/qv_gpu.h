@@ -357,7 +357,7 @@ qv_status qv_linear_device(int device, const qv_linear* args, void* workspace,
  * output needs may be NULL (preact: QV_ACT_NONE; weight: no dx; x: no dweight). 16-bit dz is
  * rounded once to dtype before the products; dbias sums the unrounded values. grad is float32 where
  * dtype has QV_GRAD_F32 added (as the gradient of a float32 result is). */
-enum { QV_GRAD_F32 = 0x100 };
+enum { QV_GRAD_F32 = 0x100 }; /* float32 elements below 2^-110 keep 2^-134 in the gradients' products */
 typedef struct qv_linear_grad {
   uint32_t dtype, activation;
   size_t m, n, k;

@@ -13,7 +13,8 @@
 //   widely for that (split_rows_kernel) take the next form, with another scale (lifted).
 // * dz W and dz^T x, whose sums run across the rows: three bfloat16 planes (8 + 8 + 8 bits, the
 //   element itself down to the planes' last bit, 2^-133), six products; what is left out is at most
-//   2^-24 of a term.
+//   2^-24 of a term. Smallest products first: a sum next to float32's end is not passed on the way.
+// Sums that come out as NaN are taken again without parts (finish_special).
 // Batches of a few rows (single queries) take a kernel that reads the weights once with plain
 // loads.
 #include <algorithm>
@@ -454,7 +455,7 @@ __device__ __noinline__ void finish_special(const ProductGroup& g, int first, in
         for (; todo != 0; todo &= todo - 1) {
           const int l = __ffs(todo) - 1;
           const float s = plain_sum(a.from, r, c0 + l, a.k, lane);
-          if (lane == l) finish1<float>(a.ep, r, c, s);
+          if (lane == l) finish1<float, false>(a.ep, r, c, s);
         }
       }
     }
@@ -743,9 +744,10 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   tc::tc_fence_after();
   dev::wait_previous();  // what packed the operands
   const uint32_t tmem = s_tmem;
-  bool wide = false;  // a vote, so that what depends on it stays uniform
+  bool in_planes = false;  // a vote, so that what depends on it stays uniform
   if constexpr (sizeof(T) == 4)
-    wide = g.wide != nullptr && __any_sync(dev::kFull, *static_cast<const volatile int*>(g.wide) != 0);
+    in_planes = g.wide != nullptr &&
+                __any_sync(dev::kFull, *static_cast<const volatile int*>(g.wide) != 0);
   volatile int* abort_flag = &s_abort;
   // Bounded wait of a whole warp; false on timeout or abort, after which the CTA's remaining results
   // are NaN.
@@ -778,8 +780,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     bool ok = true;
     auto produce = [&](auto a_mn, auto b_mn, const Unit& w, int q) {
       const ProductArgs& a = g.p[q];
-      const int form = wide ? 1 : q;
-      const int pairs = wide ? 6 : a.pairs;
+      const int form = in_planes ? 1 : q;
+      const int pairs = in_planes ? 6 : a.pairs;
       const CUtensorMap* map_a = &maps.a[form];
       const CUtensorMap* map_b = &maps.b[form];
       const int row_a = w.tm * S::kM + static_cast<int>(rank) * kBM;
@@ -843,11 +845,11 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       for (int u = worker; u < units && ok; u += workers) {
         const Unit w = u == worker ? first : unit(u);
         const ProductArgs& a = g.p[w.q];
-        const uint32_t idesc = wide ? g.wide_idesc : a.idesc;
+        const uint32_t idesc = in_planes ? g.wide_idesc : a.idesc;
         const uint32_t a_step = a.a_mn ? 2048 >> 4 : 32 >> 4, b_step = a.b_mn ? 2048 >> 4 : 32 >> 4;
         const uint64_t ad0 = operand_desc(tiles_at, a.a_mn);
         const uint64_t bd0 = operand_desc(tiles_at + S::kABytes, a.b_mn);
-        const int pairs = wide ? 6 : a.pairs, chunk = a.chunk;
+        const int pairs = in_planes ? 6 : a.pairs, chunk = a.chunk;
         for (int c0 = w.b0; c0 < w.b1 && ok; c0 += chunk, ++t) {
           const int slot = t & 1;
           if (!wait(bar(ACC_EMPTY + slot), ((t >> 1) & 1) ^ 1)) {
@@ -949,7 +951,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       int exp_a = 0;
       if constexpr (sizeof(T) == 4) {
         if (a.exp_a != nullptr) {
-          auto form = [&](int e) { return wide ? lifted(e) : e; };
+          auto form = [&](int e) { return in_planes ? lifted(e) : e; };
           exp_a = row < a.m ? form(a.exp_a[row]) : 0;
           for (int j = lane; j < kCols; j += 32)
             exp_b[j] = col0 + j < a.n ? form(a.exp_b[col0 + j]) : 0;
@@ -983,7 +985,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           tc::tc_fence_after();
           slot = t & 1;
           ++t;
-          if (kChunked && alive && w.b1 - w.b0 > a.chunk) {  // chunks before the last, added up in registers
+          if (kChunked && alive && w.b1 - w.b0 > a.chunk) {
+            // Chunks before the last, added up in registers.
             const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
             float sum[kCols];
 #pragma unroll
@@ -1159,7 +1162,7 @@ struct JoinJobs {
   SplitJob split[2];
   SumsJob sums;
 };
-template <class T, int kV>
+template <class T, class Out, int kV>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinJobs jobs) {
   dev::wait_previous();
   if (blockIdx.y < 2) {
@@ -1169,11 +1172,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinJ
     const int splits = j.splits;
     const float* partial = j.partial;
     const uint32_t per_row = static_cast<uint32_t>(j.n / kV);
-    const int lane = threadIdx.x & 31;
     const int64_t packs = size / kV;
-    for (int64_t i0 = blockIdx.x * 256ll + threadIdx.x - lane; i0 < packs; i0 += gridDim.x * 256ll) {
-      const int64_t i = min(i0 + lane, packs - 1);  // past the end the last again: whole warps
-      float s[kV];
+    auto add_up = [&](int64_t i, float(&s)[kV]) {
 #pragma unroll
       for (int v = 0; v < kV; ++v) s[v] = 0.0f;
 #pragma unroll 8
@@ -1182,11 +1182,28 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinJ
 #pragma unroll
         for (int v = 0; v < kV; ++v) s[v] += x.v[v];
       }
-      const int64_t row = i >> 32 ? i / per_row : static_cast<uint32_t>(i) / per_row;
-      const int64_t col = (i - row * per_row) * kV;
+    };
+    auto row_of = [&](int64_t i) {
+      return i >> 32 ? i / per_row : static_cast<uint32_t>(i) / per_row;
+    };
+    if constexpr (sizeof(T) == 2) {
+      for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < packs; i += gridDim.x * 256ll) {
+        float s[kV];
+        add_up(i, s);
+        const int64_t row = row_of(i), col = (i - row * per_row) * kV;
 #pragma unroll
-      for (int v = 0; v < kV; ++v) {
-        if constexpr (sizeof(T) == 4) {
+        for (int v = 0; v < kV; ++v) finish1<T, sizeof(Out) == 2>(j.ep, row, col + v, s[v]);
+      }
+    } else {  // whole warps, for sums that have to be taken again
+      const int lane = threadIdx.x & 31;
+      for (int64_t i0 = blockIdx.x * 256ll + threadIdx.x - lane; i0 < packs;
+           i0 += gridDim.x * 256ll) {
+        const int64_t i = min(i0 + lane, packs - 1);  // past the end the last again
+        float s[kV];
+        add_up(i, s);
+        const int64_t row = row_of(i), col = (i - row * per_row) * kV;
+#pragma unroll
+        for (int v = 0; v < kV; ++v) {
           bool again = s[v] != s[v];  // unless a split gave up
           for (int k = 0; again && k < splits; ++k)
             again = __float_as_uint(partial[k * size + i * kV + v]) != kGivenUp;
@@ -1196,8 +1213,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinJ
                                       __shfl_sync(dev::kFull, col, l) + v, j.k, lane);
             if (lane == l) s[v] = y;
           }
+          if (i0 + lane < packs) finish1<T, false>(j.ep, row, col + v, s[v]);
         }
-        if (i0 + lane < packs) finish1<T>(j.ep, row, col + v, s[v]);
       }
     }
     return;
@@ -1292,7 +1309,12 @@ __global__ void __launch_bounds__(128)
       float s = acc[r][q].x + acc[r][q].y;
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(dev::kFull, s, d);
-      if (r < m && lane == r && col + q < n) finish1<T>(ep, row0 + r, col + q, s);
+      if (r < m && lane == r && col + q < n) {
+        if (sizeof(T) == 2 && !ep.out_f32)
+          finish1<T, true>(ep, row0 + r, col + q, s);
+        else
+          finish1<T, false>(ep, row0 + r, col + q, s);
+      }
     }
   }
 }
@@ -1673,7 +1695,10 @@ void run_products(const Product* p, int count, const ProductPlan& plan, unsigned
     bool four = true;
     for (int q = 0; q < count; ++q) four &= plan.splits[q] == 1 || p[q].n % 4 == 0;
     const size_t threads = four ? ceil_div(items, 4) : items;
-    launch_chained(four ? join_kernel<T, 4> : join_kernel<T, 1>,
+    const bool f32 = count > 0 && p[0].ep.out_f32;
+    auto* join = f32 ? (four ? join_kernel<T, float, 4> : join_kernel<T, float, 1>)
+                     : (four ? join_kernel<T, T, 4> : join_kernel<T, T, 1>);
+    launch_chained(join,
                    dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(threads, 256), 148 * 8)),
                         sums.sums != nullptr ? 3 : 2),
                    256, 0, st, jobs);

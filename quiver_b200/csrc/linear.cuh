@@ -237,20 +237,19 @@ __device__ __forceinline__ void put16(T* p, const float (&v)[16], int left, int 
       if (j < left) p[j] = u.t[j];
   }
 }
-// Finishes one element of a product with inputs of type T.
-template <class T>
+// Finishes one element of a product with inputs of type T; kFast: a 16-bit result.
+template <class T, bool kFast>
 __device__ __forceinline__ void finish1(const Epilogue& e, int64_t row, int64_t col, float s) {
   if (e.bias != nullptr) s += dev::to_f32<T>(static_cast<const T*>(e.bias)[col]);
   if (e.preact != nullptr)
     static_cast<T*>(e.preact)[row * e.preact_stride + col] = dev::from_f32<T>(s);
-  float y = sizeof(T) == 2 && !e.out_f32 ? activate2<true>(e.act, both(s)).x
-                                         : activate2<false>(e.act, both(s)).x;
+  float y = activate2<kFast>(e.act, both(s)).x;
   if (e.residual != nullptr) {
     const int64_t at = row * e.residual_stride + col;
-    y += e.residual_f32 ? static_cast<const float*>(e.residual)[at]
-                        : dev::to_f32<T>(static_cast<const T*>(e.residual)[at]);
+    y += !kFast && e.residual_f32 ? static_cast<const float*>(e.residual)[at]
+                                  : dev::to_f32<T>(static_cast<const T*>(e.residual)[at]);
   }
-  if (e.out_f32)
+  if (!kFast)
     static_cast<float*>(e.out)[row * e.out_stride + col] = y;
   else
     static_cast<T*>(e.out)[row * e.out_stride + col] = dev::from_f32<T>(y);

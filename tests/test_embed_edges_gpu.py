@@ -469,3 +469,31 @@ def test_rows_of_answers(gpu, embed):
     assert (near[:, 3:] == 0).all() and torch.equal(near[:, :3], base[rows[:, :3]])
     none = few.search_device(base[:0], 7, return_rows=True)
     assert [tuple(v.shape) for v in none] == [(0, 7)] * 3
+
+
+@pytest.mark.parametrize("m,k,n", [(20, 40, 50), (140, 72, 130), (3000, 512, 520), (64, 8192, 128)])
+def test_linear_float32_next_to_the_largest(embed, m, k, n):
+    """Products just below float32's end, whose operands' first parts multiply to infinity."""
+    v = 1.9995 * 2.0 ** 63  # v^2 = 1.999 * 2^127; bfloat16 rounds v up to 2^64
+    x, w = torch.zeros(m, k, device="cuda"), torch.zeros(n, k, device="cuda")
+    x[:, 3], w[:, 3] = v, v
+    x[1::3, 3] = -v
+    w[:, 5] = 2.0 ** -126
+    b = torch.full((n,), -2.0 ** 126, device="cuda")
+    want = x.double() @ w.double().t()
+    same = lambda got, want: assert_within(got, want, want.abs() * 2.0 ** -21)  # noqa: E731
+    same(embed.linear(x, w), want)
+    y, z = embed.linear_preact(x, w, b.abs() * torch.where(x[0, 3] > 0, -1, 1), activation="relu")
+    keep = x[:, 3] > 0
+    same(z[keep], want[keep] - 2.0 ** 126)
+    same(y[keep], want[keep] - 2.0 ** 126)
+    assert (y[~keep] == 0).all()
+    dy = torch.zeros(m, n, device="cuda")
+    dy[:, 3], w[3] = v, v
+    dx, _, _ = embed.linear_grad(dy, x, w, need=(True, False, False))
+    same(dx, dy.double() @ w.double())
+    dy.zero_()
+    dy[3] = v
+    x[3] = -v
+    _, dw, _ = embed.linear_grad(dy, x, w, need=(False, True, False))
+    same(dw, dy.double().t() @ x.double())
