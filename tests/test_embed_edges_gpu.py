@@ -497,3 +497,28 @@ def test_linear_float32_next_to_the_largest(embed, m, k, n):
     x[3] = -v
     _, dw, _ = embed.linear_grad(dy, x, w, need=(False, True, False))
     same(dw, dy.double().t() @ x.double())
+
+
+def test_float32_far_offsets(embed):
+    """Float32 operands, parts and results past 2^31 elements, infinities at their end, and their
+    gradients."""
+    m, k, n = 17_000_000, 136, 130
+    x = torch.zeros(m, k, device="cuda")
+    x[-300:] = normal(gen(1), 300, k)
+    w = normal(gen(2), n, k)
+    for wide in (False, True):
+        if wide:
+            x[-300:, 0], w[:, 0] = 2.0 ** 40, 0
+            x[-300:, 1:] = 1
+        y = embed.linear(x, w, activation="relu")
+        want = (x[-300:].double() @ w.double().t()).clamp(min=0)
+        assert_within(y[-300:], want, product_bound(x[-300:], w))
+        assert (y[:1000] == 0).all() and (y[m // 2:m // 2 + 1000] == 0).all()
+        del y
+    x[-7, 5] = math.inf
+    y = embed.linear(x, w)
+    same_special(y[-300:], plain_product(x[-300:], w))
+    dx, dw, db = embed.linear_grad(y, x, w)
+    assert dx[-7].isnan().any() and torch.isfinite(dx[-6:]).all() and (dx[:1000] == 0).all()
+    assert_within(dx[-6:], y[-6:].double() @ w.double(), product_bound(y[-6:], w.t()))
+    same_special(db, y[-300:].double().sum(0))
