@@ -325,13 +325,13 @@ qv_status qv_flat_lookup_device(const qv_flat* index, uint32_t id_type, const vo
  * residual (m x n; residual_stride 0 adds one row to every row) may be NULL. preact (may be NULL)
  * receives x weight^T + bias, which the gradient of an activation needs. out_dtype is dtype or
  * QV_DTYPE_F32; everything else has dtype, the residual float32 where QV_RESIDUAL_F32 is added to an
- * out_dtype of QV_DTYPE_F32. float32 products run on parts of the values; beside the
- * roundings of a float32 sum a result is off by at most 2^-21 of its sum of |x||w|, however the
- * elements differ in magnitude (those below both 2^-110 and 2^-90 of their row's largest keep 2^-134,
- * or 2^-114 of that). Infinities and NaN follow float32 arithmetic term by term.
- * Sums of 16-bit inputs fall short by up to 3.4e-6 of sum |x||w| in float32 results, 5e-5 in 16-bit
- * ones (the tensor core cuts its sums). Results that a pipeline
- * wait ran out on (QV_TC_WAIT_LIMIT_US) are NaN. */
+ * out_dtype of QV_DTYPE_F32. float32 products run on parts of the values; beside the roundings of a
+ * float32 sum a result is off by at most 2^-21 of its sum of |x||w|, however the elements differ in
+ * magnitude (those below both 2^-110 and 2^-90 of their row's largest keep 2^-134, or 2^-114 of that).
+ * Infinities and NaN follow float32 arithmetic, but for an infinity against an element below 2^-39 of
+ * its row's largest, which may give NaN. Sums of 16-bit inputs fall short by up to 3.4e-6 of
+ * sum |x||w| in float32 results, 5e-5 in 16-bit ones (the tensor core cuts its sums). Results that a
+ * pipeline wait ran out on (QV_TC_WAIT_LIMIT_US) are NaN. */
 enum { QV_RESIDUAL_F32 = 0x100 };
 typedef struct qv_linear {
   uint32_t dtype, out_dtype, activation;

@@ -14,7 +14,6 @@
 // * dz W and dz^T x, whose sums run across the rows: three bfloat16 planes (8 + 8 + 8 bits, the
 //   element itself down to the planes' last bit, 2^-133), six products; what is left out is at most
 //   2^-24 of a term. Smallest products first: a sum next to float32's end is not passed on the way.
-// Sums that come out as NaN are taken again without parts (finish_special).
 // Batches of a few rows (single queries) take a kernel that reads the weights once with plain
 // loads.
 #include <algorithm>
@@ -31,14 +30,28 @@ using dev::Pack;
 
 // ---- packing: operands TMA cannot read in place, and float32 as three bfloat16 planes ------------
 
+// Infinities in the parts of float32 values: the last part holds it and the first has 1 with its sign.
+// The last part of one operand meets only the first of the other, which is zero only where the value
+// is (bfloat16: tiny values round away from zero; float16: or is below 2^-39 of its row's largest): so
+// every infinite term comes out once, with its sign, or as NaN against a zero, and nothing else of the
+// sum is infinite.
+
 // x as a sum of three bfloat16: each is the rounded remainder of the ones before, and the last
 // remainder has at most 8 bits left, so that the sum is x itself. The largest finite values round
-// to infinity in the first plane and are cut there instead; infinity and NaN stay in the first.
+// to infinity in the first plane and are cut there instead; NaN stays in the first.
 __device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
   p[0] = __float2bfloat16_rn(x);
   p[1] = p[2] = __float2bfloat16_rn(0.0f);
-  if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) return;
+  if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) {
+    if (x == x) {
+      p[0] = __float2bfloat16_rn(copysignf(1.0f, x));
+      p[2] = __float2bfloat16_rn(x);
+    }
+    return;
+  }
   if (__hisinf(p[0])) p[0] = __float2bfloat16_rz(x);
+  if (x != 0.0f && __bfloat162float(p[0]) == 0.0f)
+    p[0] = __float2bfloat16_rn(copysignf(0x1p-133f, x));
   const float r = x - __bfloat162float(p[0]);
   p[1] = __float2bfloat16_rn(r);
   p[2] = __float2bfloat16_rn(r - __bfloat162float(p[1]));
@@ -105,9 +118,9 @@ __device__ __forceinline__ int lifted(int exponent) { return min(0, exponent + 3
 // S >= 2^-15 k X W, and the addition is at most 2^-23 S. Otherwise the call's product takes three
 // bfloat16 planes (choose_planes_kernel). Vectors of normally distributed elements have shares of
 // 0.9 and more, half of them zero (ReLU) about 0.45. Rows of zeros and rows that hold infinity or
-// NaN (whose results do not depend on the planes' last bits) tell 256. Three blocks an SM: counting
+// NaN (whose results are none but these) tell 256. Three blocks an SM: counting
 // took the kernel to 126 registers and from 12.6 to 15.8 us for 10,000 + 768 rows of 768; held to 80
-// it takes 13.8.
+// it takes 13.0.
 constexpr int kSplitHeld = 8, kSplitBlocks = 148 * 8;
 constexpr uint32_t kShareOne = 256, kSharesNeeded = kShareOne + kShareOne / 8;
 template <int kV, bool kPlanes>
@@ -139,9 +152,17 @@ __global__ void __launch_bounds__(256, 3)
     for (int64_t c = kHeld + lane * kV; c < j.cols; c += 32 * kV)
       see(dev::load_pack<float, kV>(src + c));
     top = __reduce_max_sync(dev::kFull, top);
-    // A row of zeros, or one that holds infinity or NaN, stays as it is.
-    const int shift =
-        top == 0 || top >= 0x7f800000u ? 0 : min(14 + 127 - static_cast<int>(top >> 23), 126);
+    const bool odd = top >= 0x7f800000u;  // infinity or NaN among them: the largest of the others
+    if (odd) {
+      top = 0;
+#pragma unroll 1
+      for (int64_t c = lane; c < j.cols; c += 32) {
+        const uint32_t bits = __float_as_uint(src[c]) & 0x7fffffffu;
+        top = max(top, bits < 0x7f800000u ? bits : 0u);
+      }
+      top = __reduce_max_sync(dev::kFull, top);
+    }
+    const int shift = top == 0 ? 0 : min(14 + 127 - static_cast<int>(top >> 23), 126);
     const int exponent = kPlanes ? lifted(-shift) : -shift;
     const float scale = __uint_as_float(static_cast<uint32_t>(127 - exponent) << 23);
     if (lane == 0) j.exponents[r] = exponent;
@@ -160,8 +181,7 @@ __global__ void __launch_bounds__(256, 3)
           const float y = x.v[v] * scale;
           large += fabsf(y) >= from;
           hi.v[v] = __float2half_rn(y);
-          lo.v[v] = __hisinf(hi.v[v]) ? __float2half_rn(0.0f)
-                                      : __float2half_rn(y - __half2float(hi.v[v]));
+          lo.v[v] = __float2half_rn(y - __half2float(hi.v[v]));
         }
         dev::store_pack<__half, kV>(dst + c, hi);
         dev::store_pack<__half, kV>(dst + plane + c, lo);
@@ -175,8 +195,17 @@ __global__ void __launch_bounds__(256, 3)
 #pragma unroll 4
     for (int64_t c = kHeld + lane * kV; c < j.cols; c += 32 * kV)
       split(dev::load_pack<float, kV>(src + c), c);
+    if (!kPlanes && odd) {  // infinities once more, in their own form
+      __syncwarp();
+#pragma unroll 1
+      for (int64_t c = lane; c < j.cols; c += 32) {
+        if ((__float_as_uint(src[c]) & 0x7fffffffu) != 0x7f800000u) continue;
+        dst[c] = __float2half_rn(copysignf(1.0f, src[c]));
+        dst[plane + c] = __float2half_rn(src[c]);
+      }
+    }
     const uint32_t count = __reduce_add_sync(dev::kFull, large);
-    if (top != 0 && top < 0x7f800000u)
+    if (top != 0 && !odd)
       least = min(least, count * kShareOne / static_cast<uint32_t>(j.cols));
   }
   if constexpr (kPlanes) {
@@ -312,18 +341,8 @@ __device__ __forceinline__ float times_pow2(float v, int e) {
   return v * __int_as_float((127 + h) << 23) * __int_as_float((127 + e - h) << 23);
 }
 
-// Operands of a float32 product for sums outside the tensor core: element k of row r, B as the caller
-// has it, A too or (plane > 0) as three bfloat16 planes.
-struct Sources {
-  const void* a;
-  int64_t a_row, a_k, plane;  // strides
-  const float* b;
-  int64_t b_row, b_k;
-};
-
 struct ProductArgs {
-  int64_t m, n, k;
-  Sources from;           // of float32 products
+  int64_t m, n;
   int pairs;              // plane pairs: 1, or 3 or 6 for float32
   const int* exp_a;       // scaled rows of A and B: their exponents, or nullptr
   const int* exp_b;
@@ -350,55 +369,6 @@ struct ProductMaps {
   CUtensorMap a[2], b[2], out[2], residual[2];
 };
 
-// The sum of an element in plain float32 arithmetic, by a warp whose lanes go along k until the sum is
-// NaN.
-template <bool kPlanes>
-__device__ __forceinline__ float plain_sum_of(const Sources& f, int64_t row, int64_t col, int64_t k,
-                                              int lane) {
-  const float* a = static_cast<const float*>(f.a) + row * f.a_row;
-  const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(f.a) + row * f.a_row;
-  const float* b = f.b + col * f.b_row;
-  float s = 0.0f;
-  for (int64_t i0 = 0; i0 < k; i0 += 8 * 32) {
-    float x[8], y[8];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int64_t i = i0 + u * 32 + lane, at = min(i, k - 1);
-      y[u] = b[at * f.b_k];
-      if constexpr (kPlanes) {
-        const __nv_bfloat16* q = p + at * f.a_k;
-        x[u] = __bfloat162float(q[0]) +
-               (__bfloat162float(q[f.plane]) + __bfloat162float(q[2 * f.plane]));
-      } else {
-        x[u] = a[at * f.a_k];
-      }
-      if (i >= k) x[u] = y[u] = 0.0f;
-    }
-#pragma unroll
-    for (int u = 0; u < 8; ++u) s = fmaf(x[u], y[u], s);
-    if (__any_sync(dev::kFull, s != s)) return __uint_as_float(0x7fc00000u);
-  }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(dev::kFull, s, d);
-  return s;
-}
-// Whether row `row` of A holds NaN (its results are then NaN already).
-__device__ __noinline__ bool row_holds_nan(const Sources& f, int64_t row, int64_t k, int lane) {
-  bool nan = false;
-  for (int64_t i = lane; i < k; i += 32) {
-    const int64_t at = row * f.a_row + i * f.a_k;
-    const float x = f.plane > 0 ? __bfloat162float(static_cast<const __nv_bfloat16*>(f.a)[at])
-                                : static_cast<const float*>(f.a)[at];
-    nan |= x != x;
-  }
-  return __any_sync(dev::kFull, nan);
-}
-__device__ __noinline__ float plain_sum(const Sources& f, int64_t row, int64_t col, int64_t k,
-                                        int lane) {
-  return f.plane > 0 ? plain_sum_of<true>(f, row, col, k, lane)
-                     : plain_sum_of<false>(f, row, col, k, lane);
-}
-
 // A unit of work: product q, split, then tile row / column, columns fastest (a wave's CTAs share rows
 // of A and all of B in L2), and the split's blocks of k.
 struct Unit {
@@ -417,49 +387,6 @@ __device__ __forceinline__ Unit unit_of(const ProductGroup& g, int u) {
   w.b0 = w.split * a.blocks_per_split;
   w.b1 = min(a.k_blocks, w.b0 + a.blocks_per_split);
   return w;
-}
-
-// A float32 product runs on parts of the values, where an infinity gives NaN: it meets a part that is
-// zero, or one of the other sign. So a warp that saw NaN or infinity among its sums comes back here
-// once its tiles are done: what is NaN becomes what plain float32 arithmetic says. Apart from the
-// epilogue, which only notes what it saw (inside it, these loops cost the kernel a fifth of its time
-// whether there was a NaN or not). row, col: of the warp's part of a tile.
-__device__ __noinline__ void finish_special(const ProductGroup& g, int first, int step, int kM,
-                                            int row, int kBN, int col, int cols, int lane) {
-  const int units = g.units[0] + g.units[1];
-  for (int u = first; u < units; u += step) {
-    const Unit w = unit_of(g, u);
-    const ProductArgs& a = g.p[w.q];
-    if (a.splits > 1) continue;  // the join's
-    const int64_t row0 = static_cast<int64_t>(w.tm) * kM + row;
-    const int64_t col0 = static_cast<int64_t>(w.tn) * kBN + col;
-    for (int64_t r = row0; r < min(row0 + 32, a.m); ++r) {
-      bool asked = false;
-      for (int64_t c0 = col0; c0 < min(col0 + cols, a.n); c0 += 32) {
-        const int64_t c = c0 + lane;
-        bool again = c < min(col0 + cols, a.n);
-        if (again) {
-          const float y = static_cast<const volatile float*>(a.ep.out)[r * a.ep.out_stride + c];
-          again = y != y;
-        }
-        if (again && a.ep.preact != nullptr) {  // else it is the residual's
-          const float z =
-              static_cast<const volatile float*>(a.ep.preact)[r * a.ep.preact_stride + c];
-          again = z != z;
-        }
-        uint32_t todo = __ballot_sync(dev::kFull, again);
-        if (todo != 0 && !asked) {
-          asked = true;
-          if (row_holds_nan(a.from, r, a.k, lane)) break;
-        }
-        for (; todo != 0; todo &= todo - 1) {
-          const int l = __ffs(todo) - 1;
-          const float s = plain_sum(a.from, r, c0 + l, a.k, lane);
-          if (lane == l) finish1<float, false>(a.ep, r, c, s);
-        }
-      }
-    }
-  }
 }
 
 // TMA loads; in a pair the bytes are counted on the leader's barrier (a shared::cluster address).
@@ -549,13 +476,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&r)[16]) 
 // One epilogue warp's piece of a tile: 32 rows (one a lane) x kCols columns of results of type Out,
 // out of tensor memory into shared memory in the tensor map's swizzle. exp_b: the columns'
 // exponents (exp_a: this lane's row's) where operands were scaled, or nullptr. residual: the piece
-// holds it, in type Out. preact: this lane's row, or nullptr. special: float32 only, set where a sum
-// is NaN or infinite. kFast: the activation for 16-bit results.
+// holds it, in type Out. preact: this lane's row, or nullptr. kFast: the activation for 16-bit
+// results.
 template <class T, class Out, int kCols, int kAct, bool kFast>
 __device__ __forceinline__ void finish_piece(uint32_t taddr, const float* bias, const int* exp_b,
                                              int exp_a, T* preact, bool preact_wide,
-                                             bool residual, unsigned char* piece, int lane,
-                                             bool& special) {
+                                             bool residual, unsigned char* piece, int lane) {
   constexpr uint32_t kRow = kCols * sizeof(Out);
   constexpr uint32_t kSwizzle = kRow == 128 ? 7 : (kRow == 64 ? 3 : 1);
   constexpr int kPer = 16 / static_cast<int>(sizeof(Out));  // elements of 16 bytes
@@ -570,10 +496,6 @@ __device__ __forceinline__ void finish_piece(uint32_t taddr, const float* bias, 
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] = times_pow2(v[j], exp_a + exp_b[i + j]);
       }
-      float2 z = both(0.0f);  // NaN where an element is, or infinite
-#pragma unroll
-      for (int j = 0; j < 16; j += 2) z = fma2(make_float2(v[j], v[j + 1]), both(0.0f), z);
-      special |= !(z.x + z.y == 0.0f);
     }
     if (bias != nullptr) {
 #pragma unroll
@@ -616,13 +538,11 @@ __device__ __forceinline__ void finish_piece(uint32_t taddr, const float* bias, 
   }
 }
 
-// NaN over a piece (this lane's row of it), where the pipeline gave up; with bits of its own, since
-// splits of a sum that hold it are not computed anew.
-constexpr uint32_t kGivenUp = 0x7fc0dead;
+// NaN over a piece (this lane's row of it), where the pipeline gave up.
 template <class Out, int kCols>
 __device__ __noinline__ void poison_piece(unsigned char* piece, int lane) {
   Out* row = reinterpret_cast<Out*>(piece) + lane * kCols;
-  for (int c = 0; c < kCols; ++c) row[c] = dev::from_f32<Out>(__uint_as_float(kGivenUp));
+  for (int c = 0; c < kCols; ++c) row[c] = dev::from_f32<Out>(__uint_as_float(0x7fc00000u));
 }
 
 // The preactivations of a piece's columns where they can neither be stored whole nor through the
@@ -932,7 +852,6 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     // results are NaN: a barrier that nobody advances would satisfy the wait after next with the
     // phase before, and arrivals out of turn would stand in for the other CTA's.
     bool alive = true;
-    bool special = false;
     int t = 0, parity = 0;  // chunks read so far; of units
     for (int u = worker; u < units; u += workers, parity ^= 1) {
       const Unit w = u == worker ? first : unit(u);
@@ -1038,7 +957,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         auto finish_f32 = [&](int act, T* preact, bool wide, bool residual) {
           by_act(act, [&](auto k) {
             finish_piece<T, float, kWide, decltype(k)::value, !kOutF32>(
-                taddr, b, e, exp_a, preact, wide, residual, piece, lane, special);
+                taddr, b, e, exp_a, preact, wide, residual, piece, lane);
           });
           if (!alive) poison_piece<float, kWide>(piece, lane);
           __syncwarp();
@@ -1068,7 +987,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           } else {
             by_act(a.ep.act, [&](auto k) {
               finish_piece<T, T, kCols, decltype(k)::value, true>(
-                  taddr, b, e, exp_a, preact, wide, res_tiles, piece, lane, special);
+                  taddr, b, e, exp_a, preact, wide, res_tiles, piece, lane);
             });
             if (!alive) poison_piece<T, kCols>(piece, lane);
           }
@@ -1105,15 +1024,6 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       }
       if (alive) release(slot);
     }
-    if constexpr (sizeof(T) == 4) {
-      if (alive && __any_sync(dev::kFull, special)) {
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // written
-        asm volatile("fence.proxy.async;" ::: "memory");
-        __syncwarp();
-        finish_special(g, worker, workers, S::kM, static_cast<int>(rank) * kBM + quarter * 32, kBN,
-                       group * kCols, kCols, lane);
-      }
-    }
     // The pieces stay until the last stores have read them.
     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
   }
@@ -1148,8 +1058,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
 struct SplitJob {
   const float* partial;
   int splits;  // 0: nothing to join
-  int64_t m, n, k;
-  Sources from;
+  int64_t m, n;
   Epilogue ep;
 };
 struct SumsJob {
@@ -1172,8 +1081,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinJ
     const int splits = j.splits;
     const float* partial = j.partial;
     const uint32_t per_row = static_cast<uint32_t>(j.n / kV);
-    const int64_t packs = size / kV;
-    auto add_up = [&](int64_t i, float(&s)[kV]) {
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < size / kV; i += gridDim.x * 256ll) {
+      float s[kV];
 #pragma unroll
       for (int v = 0; v < kV; ++v) s[v] = 0.0f;
 #pragma unroll 8
@@ -1182,40 +1091,10 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinJ
 #pragma unroll
         for (int v = 0; v < kV; ++v) s[v] += x.v[v];
       }
-    };
-    auto row_of = [&](int64_t i) {
-      return i >> 32 ? i / per_row : static_cast<uint32_t>(i) / per_row;
-    };
-    if constexpr (sizeof(T) == 2) {
-      for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < packs; i += gridDim.x * 256ll) {
-        float s[kV];
-        add_up(i, s);
-        const int64_t row = row_of(i), col = (i - row * per_row) * kV;
+      const int64_t row = i >> 32 ? i / per_row : static_cast<uint32_t>(i) / per_row;
+      const int64_t col = (i - row * per_row) * kV;
 #pragma unroll
-        for (int v = 0; v < kV; ++v) finish1<T, sizeof(Out) == 2>(j.ep, row, col + v, s[v]);
-      }
-    } else {  // whole warps, for sums that have to be taken again
-      const int lane = threadIdx.x & 31;
-      for (int64_t i0 = blockIdx.x * 256ll + threadIdx.x - lane; i0 < packs;
-           i0 += gridDim.x * 256ll) {
-        const int64_t i = min(i0 + lane, packs - 1);  // past the end the last again
-        float s[kV];
-        add_up(i, s);
-        const int64_t row = row_of(i), col = (i - row * per_row) * kV;
-#pragma unroll
-        for (int v = 0; v < kV; ++v) {
-          bool again = s[v] != s[v];  // unless a split gave up
-          for (int k = 0; again && k < splits; ++k)
-            again = __float_as_uint(partial[k * size + i * kV + v]) != kGivenUp;
-          for (uint32_t todo = __ballot_sync(dev::kFull, again); todo != 0; todo &= todo - 1) {
-            const int l = __ffs(todo) - 1;
-            const float y = plain_sum(j.from, __shfl_sync(dev::kFull, row, l),
-                                      __shfl_sync(dev::kFull, col, l) + v, j.k, lane);
-            if (lane == l) s[v] = y;
-          }
-          if (i0 + lane < packs) finish1<T, false>(j.ep, row, col + v, s[v]);
-        }
-      }
+      for (int v = 0; v < kV; ++v) finish1<T, sizeof(Out) == 2>(j.ep, row, col + v, s[v]);
     }
     return;
   }
@@ -1463,7 +1342,6 @@ struct Product {
   int64_t m, n, k;
   bool a_mn, b_mn;
   Stored a, b;
-  Sources from;  // of float32
   Epilogue ep;
   const int* wide = nullptr;  // scaled operands that may be three planes instead: which they are
 };
@@ -1629,8 +1507,6 @@ void run_products(const Product* p, int count, const ProductPlan& plan, unsigned
     ProductArgs& a = g.p[q];
     a.m = p[q].m;
     a.n = p[q].n;
-    a.k = p[q].k;
-    a.from = p[q].from;
     a.pairs = p[q].a.planes == 3 ? 6 : (p[q].a.planes == 2 ? 3 : 1);
     a.exp_a = p[q].a.exponents;
     a.exp_b = p[q].b.exponents;
@@ -1659,7 +1535,7 @@ void run_products(const Product* p, int count, const ProductPlan& plan, unsigned
     partial += plan.partial_bytes[q];
     g.units[q] = a.tiles_m * a.tiles_n * a.splits;
     if (a.splits > 1) {
-      jobs.split[q] = SplitJob{a.partial, a.splits, a.m, a.n, a.k, a.from, a.ep};
+      jobs.split[q] = SplitJob{a.partial, a.splits, a.m, a.n, a.ep};
       items = std::max(items, static_cast<size_t>(a.m) * a.n);
     }
   }
@@ -2000,8 +1876,6 @@ void linear_forward(const qv_linear& l, void* workspace, size_t workspace_bytes,
     d.k = static_cast<int64_t>(l.k);
     d.a = pack.rows(l.x, l.m, l.k, l.x_stride);
     d.b = pack.rows(l.weight, l.n, l.k, l.weight_stride);
-    d.from = Sources{l.x, static_cast<int64_t>(l.x_stride), 1, 0,
-                     static_cast<const float*>(l.weight), static_cast<int64_t>(l.weight_stride), 1};
     d.ep = ep;
     const bool packed = pack.count() > 0;
     unsigned char* partial = pack.run(false, st);
@@ -2199,17 +2073,12 @@ void linear_grad(const qv_linear_grad& g, void* workspace, size_t workspace_byte
       Product& d = L.products[q++];
       d.a = dz;
       d.b = pack.rows(g.x, g.m, g.k, g.x_stride);
-      d.from = Sources{dz.p, 1, dz.ld, m * dz.ld,
-                       static_cast<const float*>(g.x), 1, static_cast<int64_t>(g.x_stride)};
       d.ep = result(g.dweight, g.dweight_stride);
     }
     if (g.dx != nullptr) {
       Product& d = L.products[q++];
       d.a = dz;
       d.b = pack.rows(g.weight, g.n, g.k, g.weight_stride);
-      d.from = Sources{dz.p, dz.ld, 1, m * dz.ld,
-                       static_cast<const float*>(g.weight), 1,
-                       static_cast<int64_t>(g.weight_stride)};
       d.ep = result(g.dx, g.dx_stride);
     }
     const bool first = L.store_dz || sums != nullptr;  // the dz kernel ran
