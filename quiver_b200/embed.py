@@ -300,8 +300,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     :data:`ACTIVATIONS`; ``out_dtype`` may be torch.float32 to leave the result unrounded (the residual
     may then be float32 too). float32 products are off by at most 2^-21 of sum |x||w| beside a float32
     sum's own roundings; float32 results of 16-bit inputs, whose sums the tensor core cuts, by up to
-    3.4e-6 of it.
-    Differentiable in all four tensors (unless ``out`` is given)."""
+    3.4e-6 of it. Differentiable in all four tensors (unless ``out`` is given)."""
     if out is None and torch.is_grad_enabled() and any(
             [isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, bias, residual)]):
         return _Linear.apply(x, weight, bias, residual, activation, out_dtype)
@@ -320,8 +319,9 @@ def linear_grad(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
                 preact: Optional[torch.Tensor] = None, activation: str = "none", *,
                 need: Tuple[bool, bool, bool] = (True, True, True)):
     """The gradients (dx, dweight, dbias) of :func:`linear` for ``grad`` = d loss / d result (in x's
-    type or float32), in x's type; those not asked for in ``need`` are None. ``preact`` (from :func:`linear_preact`) may be
-    None without an activation. The residual's gradient is ``grad`` itself."""
+    type or float32), in x's type; those not asked for in ``need`` are None. ``preact`` (from
+    :func:`linear_preact`) may be None without an activation. The residual's gradient is ``grad``
+    itself."""
     _dtype_code(x, "x")
     act = _activation_code(activation)
     _dtype_code(weight, "weight")
@@ -380,7 +380,8 @@ class Adapter:
     ``residual=True`` (W square). The product takes v in the weight's type; what is added is v as it
     is. ``adapter(v)`` gives float32 vectors, ready for
     :meth:`FlatIndex.add_device` and the device searches, which also take it as ``adapter=``. The same
-    vector in batches of different sizes may differ in its last bits (sums run in another order)."""
+    vector in another batch may differ in its last bits (sums run in another order by the batch's
+    size, float32 ones on other parts where the batch holds rows of wide range)."""
 
     def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
                  activation: str = "none", residual: bool = False):

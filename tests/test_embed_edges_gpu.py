@@ -522,3 +522,31 @@ def test_float32_far_offsets(embed):
     assert dx[-7].isnan().any() and torch.isfinite(dx[-6:]).all() and (dx[:1000] == 0).all()
     assert_within(dx[-6:], y[-6:].double() @ w.double(), product_bound(y[-6:], w.t()))
     same_special(db, y[-300:].double().sum(0))
+
+
+def test_flags_of_the_c_interface(embed):
+    """QV_RESIDUAL_F32 goes with float32 results, QV_GRAD_F32 with every type; other bits are refused."""
+    import ctypes as C
+    from quiver_b200 import _native
+    lib, size = _native.lib(), C.c_size_t()
+    x, w, y = normal(gen(1), 20, 16), normal(gen(2), 24, 16), torch.empty(20, 24, device="cuda")
+    p = [v.data_ptr() for v in (x, w, y)]
+
+    def forward(dtype, out_dtype):
+        a = _native.qv_linear(dtype, out_dtype, 0, 20, 24, 16, p[0], 16, p[1], 16, None, p[2], 24, p[2],
+                              24, None, 24)
+        return lib.qv_linear_workspace(0, C.byref(a), C.byref(size))
+
+    def backward(dtype):
+        a = _native.qv_linear_grad(dtype, 0, 20, 24, 16, p[2], 24, p[0], 16, p[1], 16, None, 0, p[0],
+                                   16, p[1], 16, None)
+        return lib.qv_linear_grad_workspace(0, C.byref(a), C.byref(size))
+
+    for good in (lambda: forward(2, 0x100), lambda: forward(0, 0x100), lambda: forward(1, 0),
+                 lambda: backward(0x100), lambda: backward(0x102), lambda: backward(1)):
+        _native.check(good())
+    for bad in (lambda: forward(2, 0x102), lambda: forward(0x102, 2), lambda: forward(2, 0x200),
+                lambda: forward(2, 1), lambda: backward(0x202), lambda: backward(3),
+                lambda: backward(0x103)):
+        with pytest.raises(ValueError):
+            _native.check(bad())
